@@ -1,13 +1,15 @@
 """Build the native parts of carl_amd in-tree.
 
-    python carl_amd/build.py          # engine + Python binding
+    python carl_amd/build.py          # engine + Python bindings
     python carl_amd/build.py --oracle # also the CPU oracle (test infrastructure)
 
 (Run by path: importing the carl_amd package needs the extension built here.)
 
 Outputs (next to this file):
-  libcarl_amd.so   HIP engine for gfx950 + C-ABI (include/carl_amd.h)
+  libcarl_amd.so   HIP engine and learner's operators for gfx950 + C-ABI
+                   (include/carl_amd.h, include/carl_amd_ops.h)
   _carl*.so        pybind11 module exposing carl_amd._carl.Env
+  _ops*.so         torch extension: the operators on torch tensors
 """
 from __future__ import annotations
 
@@ -15,6 +17,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -32,6 +36,9 @@ HIP_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 
+ENGINE_SOURCES = ["engine.hip", "arena.cpp", "adamw.hip", "attention.hip", "attention_f32.hip",
+                  "attention_bf16.hip", "attention_f16.hip"]
+
 
 def _run(cmd: list[str]) -> None:
     print("+", " ".join(cmd), flush=True)
@@ -42,16 +49,19 @@ def engine_path() -> Path:
     return PKG / "libcarl_amd.so"
 
 
-def binding_path() -> Path:
+def binding_path(name: str = "_carl") -> Path:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    return PKG / f"_carl{suffix}"
+    return PKG / f"{name}{suffix}"
 
 
 def build_engine() -> Path:
     out = engine_path()
     hipcc = str(ROCM / "bin" / "hipcc")
-    _run([hipcc, *HIP_FLAGS, "-shared", "-o", str(out),
-          str(CSRC / "engine.hip"), str(CSRC / "arena.cpp")])
+    sources = [CSRC / name for name in ENGINE_SOURCES]
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(sources)) as pool:
+        objects = [Path(tmp) / f"{src.name}.o" for src in sources]
+        list(pool.map(lambda so: _run([hipcc, *HIP_FLAGS, "-c", str(so[0]), "-o", str(so[1])]), zip(sources, objects)))
+        _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(out), *map(str, objects)])
     return out
 
 
@@ -68,6 +78,24 @@ def build_binding() -> Path:
     return out
 
 
+def build_ops() -> Path:
+    import torch
+    from torch.utils import cpp_extension
+
+    out = binding_path("_ops")
+    py_inc = sysconfig.get_paths()["include"]
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-attributes",
+          "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_EXTENSION_NAME=_ops",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          f"-I{py_inc}", *(f"-isystem{d}" for d in cpp_extension.include_paths()),
+          f"-isystem{ROCM / 'include'}", str(CSRC / "ops_binding.cpp"),
+          f"-L{PKG}", "-lcarl_amd", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10",
+          "-lc10_hip", "-ltorch_python",
+          "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}", f"-Wl,-rpath,{ROCM / 'lib'}", "-o", str(out)])
+    return out
+
+
 def build_oracle() -> Path:
     _run(["make", "-C", str(ROOT / "oracle"), "-B"])
     return ROOT / "oracle" / "liboracle.so"
@@ -76,6 +104,7 @@ def build_oracle() -> Path:
 def main(argv: list[str]) -> None:
     build_engine()
     build_binding()
+    build_ops()
     if "--oracle" in argv:
         build_oracle()
 

@@ -1,0 +1,71 @@
+// attention.h - linear attention with a decay for each head, chunked form.
+//
+// One kernel runs every direction.  With queries a, keys b and values c,
+//   out_t = sum over s of w(t, s) (a_t . b_s) c_s        (+ carried memory)
+// is the forward pass for (q, k, v), and each gradient is the same sum with
+// the roles exchanged: dq from (dout, v, k), and, with time running backwards
+// (s >= t), dk from (v, dout, q) and dv from (k, q, dout).  w(t, s) is
+// decay^|t-s| where no episode starts between the two steps, else 0.
+//
+// In chunks of kC steps, with X the chunk's rows and M the memory before it:
+//   P = (A B^T) o w          [kC x kC], rounded to the rows' type
+//   out = P C + w_in A M     w_in(t) = decay^(steps since the chunk's edge)
+//   M  <- w_all M + B^T (w_out C)
+// Products run on the matrix cores as 16x16 tiles, k in groups of 16: a lane's
+// fragment of either operand is row or column lane%16 and k = 4 (lane/16) + j,
+// and its share of a result is column lane%16, rows 4 (lane/16) + i.  So the
+// transposed tile P^T leaves a lane four neighbouring s of one t, and the
+// memory's tile (rows: a's dimension, column: c's) is, as it stands, the
+// operand M^T of the next chunk: it never leaves the registers.  Each wave
+// owns 16-column tiles of c, all rows.
+//
+// Precision with 16-bit rows: P is rounded once (the error of one rounding of
+// the output); the memory meets A as two terms of that type, and w_out C meets
+// B as three, so that the memory itself stays within float32's error of sums.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/carl_amd_ops.h"
+#include "elem.h"
+
+namespace carl {
+
+struct Rows {
+    void* data;
+    int64_t batch, step, head;
+};
+
+// One direction of one pass.
+struct Role {
+    Rows a, b, c, out;
+    int32_t aHeads, bHeads, cHeads;         // query heads that share a row of each
+    int32_t aGrain, bGrain, cGrain;         // bytes that its rows' addresses are multiples of: 16, 8, 4 or 2
+    int32_t outWide;                        // out's rows take stores of four elements
+    int32_t outFloat;                       // out is float32 whatever the rows' type
+    int32_t dimA, dimC;
+    int32_t backwards;
+    float scaleP, scaleIn, scaleOut;        // of P, of the carried memory where it is read, of what enters the memory
+    const float* first;                     // the memory before the first chunk, or NULL
+    float* last;                            // after the last one, or NULL
+    int32_t firstSwapped, lastSwapped;      // stored as [dimC, dimA]
+    float* parts;                           // split passes: [segment, batch, head, dimA, dimC] and a factor for each
+    float* factors;
+};
+
+struct Pass {
+    Role role[3];
+    int64_t batch, steps;
+    int32_t heads, segments;
+    int64_t segmentSteps;
+    const float* logDecay;
+    const uint8_t* starts;
+    int64_t startsBatch, startsStep;
+};
+
+// kStates: only the memories that the segments leave, each from zero.
+int launchAttention(int type, const Pass& pass, int firstRole, int roles, bool states, hipStream_t stream);
+
+template <typename T> int launchAttentionOf(const Pass& pass, int firstRole, int roles, bool states, hipStream_t stream);
+
+}  // namespace carl

@@ -1,0 +1,418 @@
+// attention.hip - linear attention with a decay for each head: the C-ABI's
+// checks and passes, the joining of split sequences, the sums over query heads
+// that share a key head, and the recurrent form.  The chunked kernel is in
+// attention_kernel.h, its mathematics in attention.h.
+#include <algorithm>
+#include <cstring>
+
+#include "attention.h"
+#include "status.h"
+
+using namespace carl;
+
+int carl::launchAttention(int type, const Pass& pass, int firstRole, int roles, bool states, hipStream_t stream)
+{
+    if (type == CARL_OP_F32) return launchAttentionOf<float>(pass, firstRole, roles, states, stream);
+    if (type == CARL_OP_BF16) return launchAttentionOf<bf16>(pass, firstRole, roles, states, stream);
+    return launchAttentionOf<f16>(pass, firstRole, roles, states, stream);
+}
+
+namespace {
+
+// The memories before each segment from what each leaves, in the place of the
+// latter.  A thread for each element of a memory.
+__global__ __launch_bounds__(256) void joinKernel(const Pass pass)
+{
+    const Role& r = pass.role[blockIdx.z];
+    const int64_t size = (int64_t)r.dimA * r.dimC, units = pass.batch * pass.heads;
+    const int64_t unit = blockIdx.x;
+    for (int64_t e = threadIdx.x + (int64_t)blockIdx.y * 256; e < size; e += (int64_t)gridDim.y * 256) {
+        const int64_t swapped = e % r.dimC * r.dimA + e / r.dimC;
+        float m = r.first ? r.first[unit * size + (r.firstSwapped ? swapped : e)] : 0.0f;
+        for (int i = 0; i < pass.segments; i++) {
+            const int64_t at = (r.backwards ? pass.segments - 1 - i : i) * units + unit;
+            const float own = r.parts[at * size + e], f = r.factors[at];
+            r.parts[at * size + e] = m;
+            m = f == 0.0f ? own : m * f + own;        // nothing of a memory that an episode's start clears
+        }
+        if (r.last) r.last[unit * size + (r.lastSwapped ? swapped : e)] = m;
+    }
+}
+
+// Sums of `group` query heads' float32 rows into their shared head's row.
+template <typename T>
+__global__ __launch_bounds__(256) void groupKernel(const float* rows, Rows out, int64_t batch, int64_t steps, int heads,
+                                                   int group, int dim)
+{
+    const int64_t n = batch * steps * heads * dim;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+        const int64_t d = e % dim, h = e / dim % heads, t = e / dim / heads % steps, b = e / dim / heads / steps;
+        float sum = 0.0f;
+        for (int g = 0; g < group; g++) sum += rows[(((b * steps + t) * heads + h) * group + g) * dim + d];
+        static_cast<T*>(out.data)[b * out.batch + t * out.step + h * out.head + d] = (T)sum;
+    }
+}
+
+// ---- the recurrent form ------------------------------------------------------
+// Bound by the memory's bytes, read and written once: each wave takes a tile of
+// 32 columns (8 lanes of 16 bytes) of one head's memory and its rows 8 at a
+// time, so a wave's accesses are whole 128-byte lines and nothing has to be
+// exchanged but the 8 partial sums of an output.
+struct Step {
+    Rows q, k, v, out;
+    const float* logDecay;
+    const uint8_t* starts;
+    int64_t startsBatch;
+    float* state;
+    int64_t batch;
+    int32_t heads, group, dimK, dimV;
+    int32_t wide;
+    float scale;
+};
+
+template <typename T> __global__ __launch_bounds__(256) void stepKernel(const Step p, const int64_t waves, const int tiles)
+{
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= waves) return;
+    const int tile = (int)(w % tiles), head = (int)(w / tiles % p.heads);
+    const int64_t batch = w / tiles / p.heads;
+    const int lane = threadIdx.x & 63, y = tile * 32 + (lane & 7) * 4, first = lane >> 3;
+    const int have = y >= p.dimV ? 0 : p.dimV - y < 4 ? p.dimV - y : 4;
+    const bool fresh = p.starts && p.starts[batch * p.startsBatch] != 0;
+    const float decay = expf(p.logDecay[head]);
+    const T* q = static_cast<const T*>(p.q.data) + batch * p.q.batch + head * p.q.head;
+    const T* k = static_cast<const T*>(p.k.data) + batch * p.k.batch + head / p.group * p.k.head;
+    const T* v = static_cast<const T*>(p.v.data) + batch * p.v.batch + head / p.group * p.v.head;
+    float* state = p.state + (batch * p.heads + head) * (int64_t)p.dimK * p.dimV;
+    f32x4 value = { 0.f, 0.f, 0.f, 0.f }, out = { 0.f, 0.f, 0.f, 0.f };
+    for (int i = 0; i < 4; i++)
+        if (i < have) value[i] = (float)v[y + i];
+    for (int x0 = 0; x0 < p.dimK; x0 += 32) {
+        f32x4 m[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int x = x0 + u * 8 + first;
+            m[u] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+            if (fresh || x >= p.dimK) continue;
+            const float* s = state + (int64_t)x * p.dimV + y;
+            if (p.wide && have == 4) m[u] = *reinterpret_cast<const f32x4*>(s);
+            else
+                for (int i = 0; i < 4; i++)
+                    if (i < have) m[u][i] = s[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int x = x0 + u * 8 + first;
+            if (x >= p.dimK) continue;
+            const float key = (float)k[x], query = (float)q[x];
+            m[u] = fresh ? value * key : m[u] * decay + value * key;
+            out += m[u] * query;
+            float* s = state + (int64_t)x * p.dimV + y;
+            if (p.wide && have == 4) *reinterpret_cast<f32x4*>(s) = m[u];
+            else
+                for (int i = 0; i < 4; i++)
+                    if (i < have) s[i] = m[u][i];
+        }
+    }
+    for (int i = 0; i < 4; i++)
+        for (int d = 8; d < 64; d <<= 1) out[i] += __shfl_xor(out[i], d);
+    if (first != 0) return;
+    T* to = static_cast<T*>(p.out.data) + batch * p.out.batch + head * p.out.head + y;
+    for (int i = 0; i < 4; i++)
+        if (i < have) to[i] = (T)(out[i] * p.scale);
+}
+
+// ---- checks ------------------------------------------------------------------
+
+constexpr int64_t kMostUnits = (int64_t)1 << 23;     // workgroups of a launch (2^31 threads)
+
+int elementBytes(int type) { return type == CARL_OP_F32 ? 4 : 2; }
+
+bool empty(const carl_attention& a) { return a.batch == 0 || a.steps == 0; }
+
+int checkAttention(const carl_attention* a, bool backward, bool step)
+{
+    if (!a) return fail(CARL_ERR_VALUE, "null attention argument");
+    if (a->type != CARL_OP_F32 && a->type != CARL_OP_BF16 && a->type != CARL_OP_F16) return fail(CARL_ERR_TYPE, "unknown element type");
+    if (a->batch < 0 || a->steps < 0) return fail(CARL_ERR_VALUE, "batch and steps must be non-negative");
+    if (step && a->steps != 1) return fail(CARL_ERR_VALUE, "steps must be 1");
+    if (a->heads < 1 || a->heads > 65535) return fail(CARL_ERR_VALUE, "heads must be in [1, 65535]");
+    if (a->kv_heads < 1 || a->heads % a->kv_heads) return fail(CARL_ERR_VALUE, "heads must be a multiple of kv_heads");
+    if (a->key_dim < 1 || a->key_dim > CARL_ATTENTION_MAX_DIM) return fail(CARL_ERR_VALUE, "key_dim must be in [1, 128]");
+    if (a->value_dim < 1 || a->value_dim > CARL_ATTENTION_MAX_DIM) return fail(CARL_ERR_VALUE, "value_dim must be in [1, 128]");
+    if (a->batch > kMostUnits / a->heads) return fail(CARL_ERR_VALUE, "batch times heads must be at most 8,388,608");
+    if (a->steps > (int64_t)1 << 40) return fail(CARL_ERR_VALUE, "too many steps");
+    if (a->batch > 0 && !a->log_decay) return fail(CARL_ERR_VALUE, "null log_decay");
+    if (empty(*a)) return CARL_OK;
+    if (!a->q.data || !a->k.data || !a->v.data) return fail(CARL_ERR_VALUE, "null attention input");
+    if (!backward && !a->out.data) return fail(CARL_ERR_VALUE, "null attention output");
+    if (backward && (!a->d_out.data || !a->d_q.data || !a->d_k.data || !a->d_v.data))
+        return fail(CARL_ERR_VALUE, "null attention gradient");
+    return CARL_OK;
+}
+
+// ---- passes ------------------------------------------------------------------
+
+// Bytes that every row's address is a multiple of (at most 16): the row
+// strides that are taken more than once and the base.
+int grainOf(const Rows& r, int type, int64_t batch, int64_t steps, int heads)
+{
+    const int size = elementBytes(type);
+    uint64_t bits = reinterpret_cast<uintptr_t>(r.data) | 16;
+    if (batch > 1) bits |= (uint64_t)r.batch * size;
+    if (steps > 1) bits |= (uint64_t)r.step * size;
+    if (heads > 1) bits |= (uint64_t)r.head * size;
+    return (int)(bits & (~bits + 1));
+}
+
+Rows rowsOf(const carl_rows& r) { return Rows{ r.data, r.batch, r.step, r.head }; }
+
+// How a sequence is split.  One workgroup walks a whole sequence of one head
+// where batch times heads fill the GPU; with fewer, segments of at least 256
+// steps, so that about 1,024 workgroups run: they need the memories before
+// each segment, which a first launch sums up (reading keys and values once more).
+struct Split {
+    int segments;
+    int64_t steps;
+};
+
+Split splitOf(const carl_attention& a)
+{
+    const int64_t units = a.batch * a.heads;
+    if (units >= 512 || a.steps <= 256) return { 1, std::max<int64_t>(a.steps, 1) };
+    int64_t segments = std::min<int64_t>((1024 + units - 1) / units, (a.steps + 255) / 256);
+    int64_t steps = (a.steps + segments - 1) / segments;
+    steps = (steps + 63) / 64 * 64;
+    segments = (a.steps + steps - 1) / steps;
+    return { (int)segments, steps };
+}
+
+int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+struct Layout {
+    int64_t parts = 0, factors = 0;      // bytes of one role's
+    int64_t keyRows = 0, valueRows = 0;  // of the query heads' gradients
+    int64_t total = 0;
+};
+
+Layout layoutOf(const carl_attention& a, bool backward)
+{
+    Layout l;
+    const Split s = splitOf(a);
+    if (s.segments > 1) {
+        const int64_t units = a.batch * a.heads * s.segments;
+        l.parts = rounded(units * a.key_dim * a.value_dim * 4);
+        l.factors = rounded(units * 4);
+    }
+    if (backward && a.heads != a.kv_heads) {
+        l.keyRows = rounded(a.batch * a.steps * a.heads * a.key_dim * 4);
+        l.valueRows = rounded(a.batch * a.steps * a.heads * a.value_dim * 4);
+    }
+    l.total = (l.parts + l.factors) * (backward ? 3 : 1) + l.keyRows + l.valueRows;
+    return l;
+}
+
+int run(const carl_attention& a, Pass& pass, int roles, hipStream_t stream)
+{
+    // roles next to each other with the same widths share a launch
+    const auto launch = [&](bool states) {
+        for (int i = 0; i < roles;) {
+            int n = 1;
+            while (i + n < roles && pass.role[i + n].dimA == pass.role[i].dimA && pass.role[i + n].dimC == pass.role[i].dimC) n++;
+            if (int rc = launchAttention(a.type, pass, i, n, states, stream)) return rc;
+            i += n;
+        }
+        return (int)CARL_OK;
+    };
+    if (pass.segments > 1) {
+        if (int rc = launch(true)) return rc;
+        const int blocks = (int)std::min<int64_t>(16, ((int64_t)a.key_dim * a.value_dim + 255) / 256);
+        joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)roles), 256, 0, stream>>>(pass);
+        if (int rc = launched("joining of segments")) return rc;
+    }
+    return launch(false);
+}
+
+Pass passOf(const carl_attention& a)
+{
+    Pass pass{};
+    const Split s = splitOf(a);
+    pass.batch = a.batch;
+    pass.steps = a.steps;
+    pass.heads = a.heads;
+    pass.segments = s.segments;
+    pass.segmentSteps = s.steps;
+    pass.logDecay = a.log_decay;
+    pass.starts = a.starts;
+    pass.startsBatch = a.starts_batch;
+    pass.startsStep = a.starts_step;
+    return pass;
+}
+
+// which: 0 query-like rows [heads], 1 key or value rows [kv_heads]
+Role roleOf(const carl_attention& a, const carl_rows& x, bool xShared, const carl_rows& y, bool yShared, const carl_rows& z,
+            bool zShared, const Rows& out, int dimA, int dimC)
+{
+    Role r{};
+    const int group = a.heads / a.kv_heads;
+    r.a = rowsOf(x);
+    r.b = rowsOf(y);
+    r.c = rowsOf(z);
+    r.out = out;
+    r.aHeads = xShared ? group : 1;
+    r.bHeads = yShared ? group : 1;
+    r.cHeads = zShared ? group : 1;
+    r.aGrain = grainOf(r.a, a.type, a.batch, a.steps, xShared ? a.kv_heads : a.heads);
+    r.bGrain = grainOf(r.b, a.type, a.batch, a.steps, yShared ? a.kv_heads : a.heads);
+    r.cGrain = grainOf(r.c, a.type, a.batch, a.steps, zShared ? a.kv_heads : a.heads);
+    r.outWide = grainOf(out, a.type, a.batch, a.steps, a.heads) >= 4 * elementBytes(a.type);
+    r.dimA = dimA;
+    r.dimC = dimC;
+    r.scaleP = a.scale;
+    return r;
+}
+
+
+__global__ __launch_bounds__(256) void copyKernel(const float* from, float* to, int64_t n)
+{
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256)
+        to[e] = from ? from[e] : 0.0f;
+}
+
+// a sequence of no steps leaves the memory as it was
+int passMemory(const float* from, float* to, int64_t n, hipStream_t stream)
+{
+    if (!to || n == 0) return CARL_OK;
+    copyKernel<<<dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), 256, 0, stream>>>(from, to, n);
+    return launched("memory copy");
+}
+
+}  // namespace
+
+extern "C" {
+
+int carl_linear_attention_workspace(const carl_attention* a, int backward, int64_t* bytes)
+{
+    if (!a || !bytes) return fail(CARL_ERR_VALUE, "null attention argument");
+    carl_attention shape = *a;
+    // sizes only: pointers may not be there yet
+    static char some;
+    static const float none = 0.0f;
+    shape.log_decay = &none;
+    for (carl_rows* r : { &shape.q, &shape.k, &shape.v, &shape.out, &shape.d_out, &shape.d_q, &shape.d_k, &shape.d_v }) r->data = &some;
+    if (int rc = checkAttention(&shape, backward != 0, false)) return rc;
+    *bytes = empty(shape) ? 0 : layoutOf(shape, backward != 0).total;
+    return CARL_OK;
+}
+
+int carl_linear_attention(const carl_attention* a, void* stream)
+{
+    if (int rc = checkAttention(a, false, false)) return rc;
+    const int64_t memory = a->batch * a->heads * a->key_dim * a->value_dim;
+    if (empty(*a)) return passMemory(a->initial_state, a->final_state, memory, (hipStream_t)stream);
+    const Layout l = layoutOf(*a, false);
+    if (l.total > 0 && !a->workspace) return fail(CARL_ERR_VALUE, "null workspace");
+    Pass pass = passOf(*a);
+    Role& r = pass.role[0];
+    r = roleOf(*a, a->q, false, a->k, true, a->v, true, rowsOf(a->out), a->key_dim, a->value_dim);
+    r.scaleIn = a->scale;
+    r.scaleOut = 1.0f;
+    r.first = a->initial_state;
+    r.last = a->final_state;
+    r.parts = static_cast<float*>(a->workspace);
+    r.factors = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + l.parts);
+    return run(*a, pass, 1, (hipStream_t)stream);
+}
+
+int carl_linear_attention_backward(const carl_attention* a, void* stream)
+{
+    if (int rc = checkAttention(a, true, false)) return rc;
+    const int64_t memory = a->batch * a->heads * a->key_dim * a->value_dim;
+    if (empty(*a)) return passMemory(a->d_final_state, a->d_initial_state, memory, (hipStream_t)stream);
+    const Layout l = layoutOf(*a, true);
+    if (l.total > 0 && !a->workspace) return fail(CARL_ERR_VALUE, "null workspace");
+    Pass pass = passOf(*a);
+    char* work = static_cast<char*>(a->workspace);
+    const bool grouped = a->heads != a->kv_heads;
+    const auto queryRows = [&](int64_t at, int dim) {
+        return Rows{ work + at, a->steps * a->heads * dim, (int64_t)a->heads * dim, dim };
+    };
+    const int64_t rowsAt = (l.parts + l.factors) * 3;
+    const Rows keyRows = grouped ? queryRows(rowsAt, a->key_dim) : rowsOf(a->d_k);
+    const Rows valueRows = grouped ? queryRows(rowsAt + l.keyRows, a->value_dim) : rowsOf(a->d_v);
+
+    // dq: time forwards, the memory transposed
+    Role& dq = pass.role[0];
+    dq = roleOf(*a, a->d_out, false, a->v, true, a->k, true, rowsOf(a->d_q), a->value_dim, a->key_dim);
+    dq.scaleIn = a->scale;
+    dq.scaleOut = 1.0f;
+    dq.first = a->initial_state;
+    dq.firstSwapped = 1;
+    // dk and dv: time backwards, the gradient of the memory instead of it
+    Role& dk = pass.role[1];
+    dk = roleOf(*a, a->v, true, a->d_out, false, a->q, false, keyRows, a->value_dim, a->key_dim);
+    Role& dv = pass.role[2];
+    dv = roleOf(*a, a->k, true, a->q, false, a->d_out, false, valueRows, a->key_dim, a->value_dim);
+    for (Role* r : { &dk, &dv }) {
+        r->backwards = 1;
+        r->scaleIn = 1.0f;
+        r->scaleOut = a->scale;
+        r->first = a->d_final_state;
+        r->outFloat = grouped;
+        if (grouped) r->outWide = a->key_dim % 4 == 0 && a->value_dim % 4 == 0;
+    }
+    dk.firstSwapped = 1;
+    dv.last = a->d_initial_state;
+    for (int i = 0; i < 3; i++) {
+        pass.role[i].parts = reinterpret_cast<float*>(work + (l.parts + l.factors) * i);
+        pass.role[i].factors = reinterpret_cast<float*>(work + (l.parts + l.factors) * i + l.parts);
+    }
+    if (int rc = run(*a, pass, 3, (hipStream_t)stream)) return rc;
+    if (!grouped) return CARL_OK;
+    const auto sum = [&](const Rows& from, const carl_rows& to, int dim) {
+        const int64_t n = a->batch * a->steps * a->kv_heads * dim;
+        const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 8192));
+        const float* rows = static_cast<const float*>(from.data);
+        const int group = a->heads / a->kv_heads;
+        const hipStream_t s = (hipStream_t)stream;
+        if (a->type == CARL_OP_F32) groupKernel<float><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
+        else if (a->type == CARL_OP_BF16) groupKernel<bf16><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
+        else groupKernel<f16><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
+        return launched("sum over shared heads");
+    };
+    if (int rc = sum(keyRows, a->d_k, a->key_dim)) return rc;
+    return sum(valueRows, a->d_v, a->value_dim);
+}
+
+int carl_linear_attention_step(const carl_attention* a, float* state, void* stream)
+{
+    if (int rc = checkAttention(a, false, true)) return rc;
+    if (a->batch == 0) return CARL_OK;
+    if (!state) return fail(CARL_ERR_VALUE, "null state");
+    const int tiles = (a->value_dim + 31) / 32;
+    const int64_t waves = a->batch * a->heads * tiles;
+    Step p{};
+    p.q = rowsOf(a->q);
+    p.k = rowsOf(a->k);
+    p.v = rowsOf(a->v);
+    p.out = rowsOf(a->out);
+    p.logDecay = a->log_decay;
+    p.starts = a->starts;
+    p.startsBatch = a->starts_batch;
+    p.state = state;
+    p.batch = a->batch;
+    p.heads = a->heads;
+    p.group = a->heads / a->kv_heads;
+    p.dimK = a->key_dim;
+    p.dimV = a->value_dim;
+    p.wide = a->value_dim % 4 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0;
+    p.scale = a->scale;
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    const hipStream_t s = (hipStream_t)stream;
+    if (a->type == CARL_OP_F32) stepKernel<float><<<grid, 256, 0, s>>>(p, waves, tiles);
+    else if (a->type == CARL_OP_BF16) stepKernel<bf16><<<grid, 256, 0, s>>>(p, waves, tiles);
+    else stepKernel<f16><<<grid, 256, 0, s>>>(p, waves, tiles);
+    return launched("linear attention step");
+}
+
+}  // extern "C"

@@ -31,6 +31,7 @@
 #include "../../include/carl_amd.h"
 #include "arena.h"
 #include "envio.h"
+#include "status.h"
 #include "wave.h"
 
 using namespace carl;
@@ -39,11 +40,15 @@ namespace {
 
 thread_local std::string g_lastError;
 
-int fail(int code, const std::string& msg)
+}  // namespace
+
+int carl::fail(int code, const std::string& msg)
 {
     g_lastError = msg;
     return code;
 }
+
+namespace {
 
 #define HIP_TRY(expr)                                                                   \
     do {                                                                                \

@@ -1,0 +1,310 @@
+// ops_binding.cpp - the `carl_amd._ops` Python module: torch tensors to the
+// C-ABI of include/carl_amd_ops.h.
+//
+// Every tensor is checked (type, device, shape, strides) before anything is
+// queued, raising TypeError / ValueError like the environment's binding; work
+// is queued on torch's current stream, so it is ordered like any torch
+// operation; outputs and scratch memory come from torch's allocator.
+#include <torch/extension.h>
+
+#include <c10/hip/HIPStream.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "../../include/carl_amd_ops.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+namespace {
+
+void check(int rc)
+{
+    if (rc == CARL_OK) return;
+    const std::string msg = carl_last_error();
+    if (rc == CARL_ERR_TYPE) throw py::type_error(msg);
+    if (rc == CARL_ERR_VALUE) throw py::value_error(msg);
+    throw std::runtime_error(msg);
+}
+
+void* currentStream() { return c10::hip::getCurrentHIPStream(0).stream(); }
+
+void require(bool ok, const std::string& msg)
+{
+    if (!ok) throw py::value_error(msg);
+}
+
+void requireType(bool ok, const std::string& msg)
+{
+    if (!ok) throw py::type_error(msg);
+}
+
+void onDevice(const Tensor& t, const char* name)
+{
+    require(t.defined() && t.is_cuda() && t.get_device() == 0, std::string(name) + " must be on cuda:0");
+    require(t.layout() == at::kStrided, std::string(name) + " must be a dense tensor");
+}
+
+int elementType(const Tensor& t, const char* name)
+{
+    switch (t.scalar_type()) {
+    case at::kFloat: return CARL_OP_F32;
+    case at::kBFloat16: return CARL_OP_BF16;
+    case at::kHalf: return CARL_OP_F16;
+    default: throw py::type_error(std::string(name) + " must have dtype float32, bfloat16 or float16");
+    }
+}
+
+// ------------------------------------------------------- linear attention
+
+carl_rows rowsOf(const Tensor& t, bool steps = true)
+{
+    return steps ? carl_rows{ t.data_ptr(), t.stride(0), t.stride(1), t.stride(2) }
+                 : carl_rows{ t.data_ptr(), t.stride(0), 0, t.stride(1) };
+}
+
+// The checks of q, k, v, log_decay, starts and the memory; the sizes of the call.
+carl_attention attentionOf(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& logDecay,
+                           const OptTensor& starts, const OptTensor& memory, double scale, bool steps)
+{
+    const int dims = steps ? 4 : 3;
+    const char* lead = steps ? "[batch, steps, " : "[batch, ";
+    for (const auto& [t, name] : { std::pair{ &q, "q" }, { &k, "k" }, { &v, "v" } }) {
+        onDevice(*t, name);
+        require(t->dim() == dims, std::string(name) + " must have shape " + lead + "heads, width]");
+        require(t->stride(dims - 1) == 1 || t->size(dims - 1) <= 1, std::string(name) + " must be contiguous in its last dimension");
+        requireType(t->scalar_type() == q.scalar_type(), "q, k and v must have the same dtype");
+    }
+    carl_attention a{};
+    a.type = elementType(q, "q");
+    a.batch = q.size(0);
+    a.steps = steps ? q.size(1) : 1;
+    for (const Tensor* t : { &k, &v })
+        require(t->size(0) == a.batch && (!steps || t->size(1) == a.steps), "k and v must have q's batch and steps");
+    require(q.size(dims - 2) <= 65535, "heads must be in [1, 65535]");
+    a.heads = (int32_t)q.size(dims - 2);
+    require(k.size(dims - 2) == v.size(dims - 2), "k and v must have the same heads");
+    a.kv_heads = (int32_t)std::min<int64_t>(k.size(dims - 2), 65536);
+    require(k.size(dims - 1) == q.size(dims - 1), "q and k must have the same width");
+    a.key_dim = (int32_t)std::min<int64_t>(q.size(dims - 1), 1 << 20);
+    a.value_dim = (int32_t)std::min<int64_t>(v.size(dims - 1), 1 << 20);
+    a.scale = (float)scale;
+    a.q = rowsOf(q, steps);
+    a.k = rowsOf(k, steps);
+    a.v = rowsOf(v, steps);
+    onDevice(logDecay, "log_decay");
+    requireType(logDecay.scalar_type() == at::kFloat, "log_decay must have dtype float32");
+    require(logDecay.dim() == 1 && logDecay.size(0) == a.heads, "log_decay must have shape [heads]");
+    require(logDecay.is_contiguous(), "log_decay must be contiguous");
+    require(!logDecay.requires_grad(), "log_decay has no gradient: detach it");
+    a.log_decay = logDecay.data_ptr<float>();
+    if (starts) {
+        onDevice(*starts, "starts");
+        requireType(starts->scalar_type() == at::kBool, "starts must have dtype bool");
+        require(starts->dim() == dims - 2 && starts->size(0) == a.batch && (!steps || starts->size(1) == a.steps),
+                steps ? "starts must have shape [batch, steps]" : "starts must have shape [batch]");
+        a.starts = static_cast<const uint8_t*>(starts->data_ptr());
+        a.starts_batch = starts->stride(0);
+        a.starts_step = steps ? starts->stride(1) : 0;
+    }
+    if (memory) {
+        const char* name = steps ? "initial_state" : "state";
+        onDevice(*memory, name);
+        requireType(memory->scalar_type() == at::kFloat, std::string(name) + " must have dtype float32");
+        require(memory->dim() == 4 && memory->size(0) == a.batch && memory->size(1) == a.heads
+                    && memory->size(2) == a.key_dim && memory->size(3) == a.value_dim,
+                std::string(name) + " must have shape [batch, heads, key width, value width]");
+        require(memory->is_contiguous(), std::string(name) + " must be contiguous");
+    }
+    return a;
+}
+
+// Rows like q's but of the width of v, in q's order of batch and steps.
+Tensor rowsLike(const Tensor& q, int64_t width)
+{
+    if (q.stride(1) > q.stride(0) && q.size(0) > 1)
+        return at::empty({ q.size(1), q.size(0), q.size(2), width }, q.options()).transpose(0, 1);
+    return at::empty({ q.size(0), q.size(1), q.size(2), width }, q.options());
+}
+
+Tensor workspaceOf(const carl_attention& a, bool backward, const Tensor& like)
+{
+    int64_t bytes = 0;
+    check(carl_linear_attention_workspace(&a, backward, &bytes));
+    return bytes ? at::empty({ bytes }, like.options().dtype(at::kByte)) : Tensor();
+}
+
+struct LinearAttention : torch::autograd::Function<LinearAttention> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                  const Tensor& v, const Tensor& logDecay, const OptTensor& starts,
+                                                  const OptTensor& initial, double scale)
+    {
+        carl_attention a = attentionOf(q, k, v, logDecay, starts, initial, scale, true);
+        Tensor out = rowsLike(q, a.value_dim);
+        Tensor last = at::empty({ a.batch, a.heads, a.key_dim, a.value_dim }, logDecay.options());
+        a.out = rowsOf(out);
+        a.initial_state = initial ? initial->data_ptr<float>() : nullptr;
+        a.final_state = last.data_ptr<float>();
+        const Tensor work = workspaceOf(a, false, q);
+        a.workspace = work.defined() ? work.data_ptr() : nullptr;
+        check(carl_linear_attention(&a, currentStream()));
+        ctx->save_for_backward({ q, k, v, logDecay, starts ? *starts : Tensor(), initial ? *initial : Tensor() });
+        ctx->saved_data["scale"] = scale;
+        ctx->set_materialize_grads(false);
+        return { out, last };
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        if (at::GradMode::is_enabled()) throw std::runtime_error("linear_attention has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &logDecay = saved[3];
+        const OptTensor starts = saved[4].defined() ? OptTensor(saved[4]) : std::nullopt;
+        const OptTensor initial = saved[5].defined() ? OptTensor(saved[5]) : std::nullopt;
+        if (!grads[0].defined() && !grads[1].defined()) return { {}, {}, {}, {}, {}, {}, {} };
+        carl_attention a = attentionOf(q.detach(), k.detach(), v.detach(), logDecay, starts, initial, ctx->saved_data["scale"].toDouble(), true);
+        Tensor dOut = grads[0];
+        if (!dOut.defined()) dOut = at::zeros({ a.batch, a.steps, a.heads, a.value_dim }, q.options());
+        if (dOut.stride(3) != 1 && dOut.size(3) > 1) dOut = dOut.contiguous();
+        const Tensor dLast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+        // edges count the tensors that were given
+        const Tensor dFirst = initial && ctx->needs_input_grad(starts ? 5 : 4) ? at::empty_like(*initial) : Tensor();
+        a.initial_state = initial ? initial->data_ptr<float>() : nullptr;
+        a.d_out = rowsOf(dOut);
+        a.d_q = rowsOf(dq);
+        a.d_k = rowsOf(dk);
+        a.d_v = rowsOf(dv);
+        a.d_final_state = dLast.defined() ? dLast.data_ptr<float>() : nullptr;
+        a.d_initial_state = dFirst.defined() ? dFirst.data_ptr<float>() : nullptr;
+        const Tensor work = workspaceOf(a, true, q);
+        a.workspace = work.defined() ? work.data_ptr() : nullptr;
+        check(carl_linear_attention_backward(&a, currentStream()));
+        return { dq, dk, dv, {}, {}, dFirst, {} };
+    }
+};
+
+std::tuple<Tensor, Tensor> linearAttention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& logDecay,
+                                           const OptTensor& starts, const OptTensor& initial, std::optional<double> scale)
+{
+    const double s = scale ? *scale : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
+    auto out = LinearAttention::apply(q, k, v, logDecay, starts, initial, s);
+    return { out[0], out[1] };
+}
+
+Tensor linearAttentionStep(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& logDecay, const Tensor& state,
+                           const OptTensor& starts, std::optional<double> scale)
+{
+    const double s = scale ? *scale : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
+    if (at::GradMode::is_enabled())
+        for (const Tensor* t : { &q, &k, &v, &state })
+            require(!t->requires_grad(), "linear_attention_step has no gradient: call it under torch.no_grad()");
+    carl_attention a = attentionOf(q, k, v, logDecay, starts, state, s, false);
+    Tensor out = at::empty({ a.batch, a.heads, a.value_dim }, q.options());
+    a.out = rowsOf(out, false);
+    check(carl_linear_attention_step(&a, state.data_ptr<float>(), currentStream()));
+    state.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
+// ------------------------------------------------------------------- AdamW
+
+void adamwStep(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& first,
+               const std::vector<Tensor>& second, const std::vector<Tensor>& firstScale,
+               const std::vector<Tensor>& secondScale, int64_t step, double lr, double beta1, double beta2, double eps,
+               double weightDecay, const OptTensor& gradScale)
+{
+    const size_t n = params.size();
+    require(grads.size() == n && first.size() == n && second.size() == n,
+            "params, grads, exp_avg and exp_avg_sq must have the same length");
+    const bool eight = n > 0 && first[0].scalar_type() == at::kChar;
+    if (eight) require(firstScale.size() == n && secondScale.size() == n, "8-bit moments need exp_avg_scale and exp_avg_sq_scale");
+    else require(firstScale.empty() && secondScale.empty(), "float32 moments have no scales");
+    std::vector<carl_adamw_tensor> list(n);
+    for (size_t i = 0; i < n; i++) {
+        const Tensor &p = params[i], &g = grads[i], &m = first[i], &v = second[i];
+        onDevice(p, "params");
+        onDevice(g, "grads");
+        onDevice(m, "exp_avg");
+        onDevice(v, "exp_avg_sq");
+        require(g.sizes() == p.sizes(), "grads must have their parameters' shapes");
+        require(m.numel() == p.numel() && v.numel() == p.numel(), "moments must have their parameters' sizes");
+        require(p.is_contiguous(), "params must be contiguous");
+        require(g.is_contiguous(), "grads must be contiguous");
+        require(m.is_contiguous() && v.is_contiguous(), "moments must be contiguous");
+        requireType(m.scalar_type() == (eight ? at::kChar : at::kFloat), "exp_avg must all have dtype float32, or all int8");
+        requireType(v.scalar_type() == (eight ? at::kByte : at::kFloat), "exp_avg_sq must have dtype float32, or uint8 with an int8 exp_avg");
+        carl_adamw_tensor& t = list[i];
+        t = { p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, nullptr, p.numel(),
+              elementType(p, "params"), elementType(g, "grads") };
+        if (eight) {
+            const int64_t blocks = (p.numel() + CARL_ADAMW_BLOCK - 1) / CARL_ADAMW_BLOCK;
+            for (const Tensor* s : { &firstScale[i], &secondScale[i] }) {
+                onDevice(*s, "scales");
+                requireType(s->scalar_type() == at::kFloat, "scales must have dtype float32");
+                require(s->numel() == blocks && s->is_contiguous(), "scales must be contiguous with one value for each 256 elements");
+            }
+            t.exp_avg_scale = firstScale[i].data_ptr<float>();
+            t.exp_avg_sq_scale = secondScale[i].data_ptr<float>();
+        }
+    }
+    carl_adamw h{ lr, beta1, beta2, eps, weightDecay, step, eight ? 8 : 32, nullptr };
+    if (gradScale) {
+        onDevice(*gradScale, "grad_scale");
+        requireType(gradScale->scalar_type() == at::kFloat, "grad_scale must have dtype float32");
+        require(gradScale->numel() == 1, "grad_scale must hold one value");
+        h.grad_scale = gradScale->data_ptr<float>();
+    }
+    check(carl_adamw_step(list.data(), (int)n, &h, currentStream()));
+    for (const auto* tensors : { &params, &first, &second, &firstScale, &secondScale })
+        for (const Tensor& t : *tensors) t.unsafeGetTensorImpl()->bump_version();
+}
+
+int64_t momentBlocks(const Tensor& m) { return (m.numel() + CARL_ADAMW_BLOCK - 1) / CARL_ADAMW_BLOCK; }
+
+std::tuple<Tensor, Tensor> decodeMoments(const Tensor& m, const Tensor& ms, const Tensor& v, const Tensor& vs)
+{
+    for (const Tensor* t : { &m, &ms, &v, &vs }) {
+        onDevice(*t, "moments");
+        require(t->is_contiguous(), "moments must be contiguous");
+    }
+    requireType(m.scalar_type() == at::kChar && v.scalar_type() == at::kByte, "codes must have dtypes int8 and uint8");
+    requireType(ms.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat, "scales must have dtype float32");
+    require(m.sizes() == v.sizes(), "moments must have the same shape");
+    require(ms.numel() == momentBlocks(m) && vs.numel() == momentBlocks(m), "scales must have one value for each 256 elements");
+    Tensor mOut = at::empty(m.sizes(), ms.options()), vOut = at::empty(m.sizes(), ms.options());
+    check(carl_adamw_decode(m.data_ptr<int8_t>(), ms.data_ptr<float>(), v.data_ptr<uint8_t>(), vs.data_ptr<float>(),
+                            m.numel(), mOut.data_ptr<float>(), vOut.data_ptr<float>(), currentStream()));
+    return { mOut, vOut };
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> encodeMoments(const Tensor& m, const Tensor& v)
+{
+    for (const Tensor* t : { &m, &v }) {
+        onDevice(*t, "moments");
+        require(t->is_contiguous(), "moments must be contiguous");
+        requireType(t->scalar_type() == at::kFloat, "moments must have dtype float32");
+    }
+    require(m.sizes() == v.sizes(), "moments must have the same shape");
+    Tensor mOut = at::empty(m.sizes(), m.options().dtype(at::kChar)), vOut = at::empty(m.sizes(), m.options().dtype(at::kByte));
+    Tensor ms = at::empty({ momentBlocks(m) }, m.options()), vs = at::empty({ momentBlocks(m) }, m.options());
+    check(carl_adamw_encode(m.data_ptr<float>(), v.data_ptr<float>(), m.numel(), mOut.data_ptr<int8_t>(),
+                            ms.data_ptr<float>(), vOut.data_ptr<uint8_t>(), vs.data_ptr<float>(), currentStream()));
+    return { mOut, ms, vOut, vs };
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ops, m)
+{
+    m.doc() = "The learner's operators of the MI355X engine (C-ABI in include/carl_amd_ops.h).";
+    m.def("linear_attention", &linearAttention);
+    m.def("linear_attention_step", &linearAttentionStep);
+    m.def("adamw_step", &adamwStep);
+    m.def("decode_moments", &decodeMoments);
+    m.def("encode_moments", &encodeMoments);
+}
