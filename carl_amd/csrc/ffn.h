@@ -1,0 +1,88 @@
+// ffn.h - the gated feed-forward block's products on the matrix cores.
+//
+//   h = act(x Wg^T) o (x Wu^T)          y = h Wd^T
+//   dh = dy Wd      dg = dh o up o act'(gate)      du = dh o act(gate)
+//   dx = dg Wg + du Wu      dWg = dg^T x      dWu = du^T x      dWd = dy^T h
+// act(g) = g s(z(g)) with s the logistic function and z = g (SiLU) or
+// z = 2 sqrt(2/pi) (g + 0.044715 g^3) (GELU in its tanh form, since
+// (1 + tanh u) / 2 = s(2u)); act'(g) = s + g s (1 - s) z'(g).
+//
+// The backward pass recomputes gate and up in the kernel that forms dh, beside
+// it, so that dg, du and h come from float32 values with one rounding each:
+// kept from the forward pass in 16 bits they would be rounded twice, in 32
+// bits they would cost more traffic than the products take.
+//
+// Two kernels do all products.  `product` multiplies rows by rows (both
+// operands contiguous along the sum); `outer` sums over rows (both operands
+// contiguous across it), for the weights' gradients.  Both copy panels of 128
+// bytes along the sum straight into LDS, two stages, one barrier a stage.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/carl_amd_ops.h"
+#include "elem.h"
+
+namespace carl {
+
+struct Panel {
+    const void* data;      // 16-byte aligned, rows of `stride` elements, a multiple of 16 bytes
+    int64_t rows, stride;
+    int32_t width;         // elements along a row that count, rounded up to 16 bytes (the rest are zero)
+};
+
+enum { kProductPlain = 0, kProductGate = 1, kProductGrad = 2 };
+
+struct ProductArgs {
+    Panel a[2], b[3];      // plain: the sum of a[i] b[i]^T; gate: a[0] with b[0], b[1]; grad: those, and a[1] with b[2]
+    int32_t terms;
+    int32_t activation;
+    int64_t m;
+    int32_t n;
+    void* out[3];          // plain: out; gate: h; grad: h, dg, du
+    int64_t outStride;
+    int32_t outWidth;      // columns that are written (gate, grad: to the end of the padding)
+    int32_t outWide;       // rows are 16-byte aligned
+};
+
+struct OuterArgs {
+    Panel p[3], q[3];      // part[f][d] = sum over rows of p[row][f] q[row][d]
+    float* part[3];        // [split][m][n]
+    int32_t m[3], n[3];
+    int64_t k;             // rows
+    int64_t splitRows;     // of a split, a multiple of the stage
+    int32_t splits, jobs;
+};
+
+struct PackJob {
+    const void* from;
+    void* to;
+    int64_t rows, cols, fromStride, toStride;   // to: rows x toStride, zero past cols (transposed: cols x toStride, past rows)
+    int32_t transposed;
+};
+
+struct PackArgs {
+    PackJob job[8];
+    int32_t jobs;
+};
+
+struct SumJob {
+    const float* part;
+    void* out;
+    int64_t count;
+};
+
+struct SumArgs {
+    SumJob job[3];
+    int32_t splits, jobs;
+};
+
+template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream);
+template <typename T> int launchOuter(const OuterArgs& args, int tile, hipStream_t stream);
+template <typename T> int launchPack(const PackArgs& args, hipStream_t stream);
+template <typename T> int launchSum(const SumArgs& args, hipStream_t stream);
+
+// Columns and rows of an outer product's tile for these sizes.
+int outerTile(int m, int n);
+
+}  // namespace carl

@@ -1,0 +1,459 @@
+// ffn_kernel.h - the kernels of ffn.h, for one element type.
+#pragma once
+
+#include <algorithm>
+
+#include "ffn.h"
+#include "status.h"
+
+namespace carl {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+
+constexpr int kRowBytes = 128;      // of a panel's row in a stage
+constexpr int kOutside = (int)0x80000000u;
+
+// A lane's 16 bytes of either operand: row or column lane%16 of a 16x16 tile,
+// 16/size neighbouring steps of the sum from 16/size times lane/16 on.
+template <typename T> struct Mma;
+template <> struct Mma<float> {
+    static __device__ inline f32x4 run(uint4 a, uint4 b, f32x4 c)
+    {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mma<bf16> {
+    static __device__ inline f32x4 run(uint4 a, uint4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<f16> {
+    static __device__ inline f32x4 run(uint4 a, uint4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// A buffer descriptor of `records` bytes from `base`; accesses that do not lie
+// in them read zeros.
+__device__ inline i32x4 descriptor(const void* base, int records)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    return i32x4{ __builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff),
+                  __builtin_amdgcn_readfirstlane(records), 0x00027000 };
+}
+
+// 16 bytes a lane from memory to 16 x lane bytes past `lds` (the same for all
+// lanes of the wave), without a register.  Written out because the compiler
+// would have every later LDS read wait for it; the copies of a stage are
+// waited for once, by waitCopies() before the barrier that hands it over.
+__device__ inline void copyToLds(i32x4 from, int offset, int more, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(offset), "s"(from), "s"(more)
+                 : "memory");      // m0 is never live across statements of these kernels
+}
+
+__device__ inline void waitCopies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ inline uint32_t ldsAddress(const void* p)
+{
+    return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p);
+}
+
+// ---- product -------------------------------------------------------------------
+
+// Rows of a weights' panel sit in LDS with their eight 16-byte pieces permuted
+// by this, so that eight lanes reading one piece of eight rows meet all banks.
+// kRun: neighbouring columns of the result that a lane holds (below).
+template <int kRun> __device__ inline int swizzle(int row) { return (row & 3) | (row / kRun & 1) << 2; }
+
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN> struct ProductShape {
+    static constexpr int kNA = kKind == kProductGrad ? 2 : 1, kNB = kKind == kProductPlain ? 1 : kKind == kProductGate ? 2 : 3;
+    static constexpr int kThreads = kWM * kWN * 64;
+    static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
+    static constexpr int kRun = 4 * kTN;
+    static constexpr int kStage = (kNA * kBM + kNB * kBN) * kRowBytes;
+    static_assert((kBM * 8) % kThreads == 0 && (kBN * 8) % kThreads == 0, "whole loads");
+    // copies: a thread's rows differ by multiples of 8 and of 2 kRun
+    static_assert(kThreads / 8 % 8 == 0 && kThreads / 8 % (2 * kRun) == 0, "one permutation for a thread's pieces");
+};
+
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN>::kThreads)) void productKernel(const ProductArgs args)
+{
+    using S = ProductShape<T, kKind, kBM, kBN, kWM, kWN>;
+    constexpr int kE = 16 / sizeof(T), kStep = kRowBytes / sizeof(T);
+    constexpr int kNA = S::kNA, kNB = S::kNB, kTM = S::kTM, kTN = S::kTN, kRun = S::kRun, kThreads = S::kThreads;
+
+    __shared__ __align__(1024) char stages[2 * S::kStage];
+
+    // The tiles of one row of tiles run next to each other on one of the 8
+    // dies (blocks are dealt to them in turn), so that a's rows are read from
+    // memory once and b stays in that die's cache.
+    const int tilesN = (args.n + kBN - 1) / kBN;
+    const int64_t tilesM = (args.m + kBM - 1) / kBM;
+    const int die = blockIdx.x % 8;
+    const int64_t local = blockIdx.x / 8;
+    const int64_t tm = local / tilesN * 8 + die;
+    const int tn = (int)(local % tilesN);
+    if (tm >= tilesM) return;
+    const int64_t m0 = tm * kBM;
+    const int n0 = tn * kBN;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wm = wave / kWN, wn = wave % kWN;
+
+    f32x4 acc[kNB][kTN][kTM];
+#pragma unroll
+    for (int b = 0; b < kNB; b++)
+#pragma unroll
+        for (int j = 0; j < kTN; j++)
+#pragma unroll
+            for (int i = 0; i < kTM; i++) acc[b][j][i] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+
+    // Rows past the operand's end lie past the descriptor's, pieces past a
+    // row's width are sent there: both arrive as zeros.
+    const int copyRow = threadIdx.x >> 3;
+    const auto copyPanel = [&](const Panel& p, int64_t row0, int rows, int k0, uint32_t lds, bool weights) {
+        const T* base = static_cast<const T*>(p.data) + row0 * p.stride;
+        const int have = (int)(p.rows - row0 < rows ? p.rows - row0 : rows), strideBytes = (int)(p.stride * sizeof(T));
+        const i32x4 from = descriptor(base, have * strideBytes);
+        const int c = ((threadIdx.x & 7) ^ (weights ? swizzle<kRun>(copyRow) : copyRow & 7)) * 16;
+        const int at = c < (p.width - k0) * (int)sizeof(T) ? copyRow * strideBytes + c : kOutside;
+#pragma unroll
+        for (int i = 0; i < rows * 8 / kThreads; i++)
+            copyToLds(from, at + i * (kThreads / 8) * strideBytes, k0 * (int)sizeof(T), lds + (i * kThreads + wave * 64) * 16);
+    };
+    const int steps0 = (args.a[0].width + kStep - 1) / kStep;
+    const int steps = kKind == kProductPlain && args.terms == 2 ? steps0 + (args.a[1].width + kStep - 1) / kStep : steps0;
+    const auto copyStage = [&](int step, uint32_t lds) {
+        if constexpr (kKind == kProductPlain) {
+            const int term = step >= steps0, k0 = (term ? step - steps0 : step) * kStep;
+            copyPanel(args.a[term], m0, kBM, k0, lds, false);
+            copyPanel(args.b[term], n0, kBN, k0, lds + kBM * kRowBytes, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kNA; i++) copyPanel(args.a[i], m0, kBM, step * kStep, lds + i * kBM * kRowBytes, false);
+#pragma unroll
+            for (int i = 0; i < kNB; i++) copyPanel(args.b[i], n0, kBN, step * kStep, lds + (kNA * kBM + i * kBN) * kRowBytes, true);
+        }
+    };
+    // Tile i of a's: rows lane%16 of the tile.  Tile j of b's: row lane%16 is
+    // column (lane%16)/4 kRun + 4 j + lane%4 of the wave's, so that a lane's
+    // rows 4 quad + i of all tiles are kRun neighbouring columns of the result.
+    // swizzle() of that row is lane%8 as well.
+    const int aRow = (wm * kTM * 16 + col) * kRowBytes, piece0 = (quad ^ (col & 7)) * 16;
+    const int bRow = (wn * kTN * 16 + (col >> 2) * kRun + (col & 3)) * kRowBytes;
+    const auto multiply = [&](const char* lds) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            __builtin_amdgcn_sched_barrier(0);      // the fragments of one half at a time
+            const char* aAt = lds + (aRow + (piece0 ^ half * 64));
+            const char* bAt = lds + kNA * kBM * kRowBytes + (bRow + (piece0 ^ half * 64));
+            uint4 a[kNA][kTM];
+#pragma unroll
+            for (int p = 0; p < kNA; p++)
+#pragma unroll
+                for (int i = 0; i < kTM; i++) a[p][i] = *reinterpret_cast<const uint4*>(aAt + (p * kBM + i * 16) * kRowBytes);
+#pragma unroll
+            for (int p = 0; p < kNB; p++)
+#pragma unroll
+                for (int j = 0; j < kTN; j++) {
+                    const uint4 b = *reinterpret_cast<const uint4*>(bAt + (p * kBN + j * 4) * kRowBytes);
+#pragma unroll
+                    for (int i = 0; i < kTM; i++) acc[p][j][i] = Mma<T>::run(b, a[kNA == 2 && p == 2 ? 1 : 0][i], acc[p][j][i]);
+                }
+        }
+    };
+
+    const uint32_t lds = ldsAddress(stages);
+    copyStage(0, lds);
+    waitCopies();
+    __syncthreads();
+    for (int step = 0; step < steps; step++) {
+        if (step + 1 < steps) copyStage(step + 1, lds + ((step + 1) & 1) * S::kStage);
+        multiply(stages + (step & 1) * S::kStage);
+        waitCopies();
+        __syncthreads();
+    }
+
+    const auto store = [&](void* out, int64_t row, const float (&x)[kRun]) {
+        const int n = n0 + wn * kTN * 16 + quad * kRun;
+        T* to = static_cast<T*>(out) + row * args.outStride + n;
+        if (args.outWide && n + kRun <= args.outWidth) {
+            constexpr int kPiece = kRun < kE ? kRun : kE;
+#pragma unroll
+            for (int e = 0; e < kRun; e += kPiece) {
+                vec<T, kPiece> v;
+#pragma unroll
+                for (int i = 0; i < kPiece; i++) v[i] = (T)x[e + i];
+                *reinterpret_cast<vec<T, kPiece>*>(to + e) = v;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kRun; e++)
+                if (n + e < args.outWidth) to[e] = (T)x[e];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kTM; i++) {
+        const int64_t row = m0 + (wm * kTM + i) * 16 + col;
+        if (row >= args.m) continue;
+        float first[kRun], second[kRun], third[kRun];
+#pragma unroll
+        for (int j = 0; j < kTN; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int at = j * 4 + e;
+                if constexpr (kKind == kProductPlain) first[at] = acc[0][j][i][e];
+                else {
+                    const float g = acc[0][j][i][e], up = acc[1][j][i][e];
+                    float z = g, slope = 1.0f;
+                    if (args.activation == CARL_GELU) {
+                        const float c = 1.5957691216057308f, g2 = g * g;       // 2 sqrt(2 / pi)
+                        z = c * (g + 0.044715f * g2 * g);
+                        slope = c * (1.0f + 0.134145f * g2);
+                    }
+                    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+                    const float act = g * s;
+                    first[at] = act * up;
+                    if constexpr (kKind == kProductGrad) {
+                        const float dh = acc[kNB - 1][j][i][e];
+                        second[at] = dh * up * (s + act * (1.0f - s) * slope);
+                        third[at] = dh * act;
+                    }
+                }
+            }
+        store(args.out[0], row, first);
+        if constexpr (kKind == kProductGrad) {
+            store(args.out[1], row, second);
+            store(args.out[2], row, third);
+        }
+    }
+}
+
+// ---- outer ---------------------------------------------------------------------
+
+// A panel's stage is kStep rows of kB columns.  Its columns' 16-byte pieces are
+// permuted by the row so that the rows that one read touches meet other banks.
+template <typename T> __device__ inline int outerSwizzle(int row)
+{
+    if constexpr (sizeof(T) == 4) return (row >> 2 & 3) * 4;
+    else return ((row & 3) | (row >> 3 & 1) << 2) * 2;
+}
+
+template <typename T, int kB, int kWM, int kWN>
+__global__ __launch_bounds__(kWM* kWN * 64) void outerKernel(const OuterArgs args)
+{
+    constexpr int kThreads = kWM * kWN * 64, kE = 16 / sizeof(T), kStep = kRowBytes / sizeof(T);
+    constexpr int kTM = kB / kWM / 16, kTN = kB / kWN / 16;
+    constexpr int kPieces = kB / kE, kPanel = kStep * kB * (int)sizeof(T);
+    constexpr int kStage = 2 * kPanel;
+    __shared__ __align__(1024) char stages[2 * kStage];
+
+    const int job = blockIdx.y;
+    // splits in turn over the 8 dies: a split's rows are read through one cache
+    const int split = (int)(blockIdx.x % args.splits), tile = (int)(blockIdx.x / args.splits);
+    const int m = args.m[job], n = args.n[job], tilesN = (n + kB - 1) / kB;
+    if (tile >= tilesN * ((m + kB - 1) / kB)) return;
+    const int m0 = tile / tilesN * kB, n0 = tile % tilesN * kB;
+    const int64_t k0 = split * args.splitRows, k1 = k0 + args.splitRows < args.k ? k0 + args.splitRows : args.k;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wm = wave / kWN, wn = wave % kWN;
+    f32x4 acc[kTN][kTM];
+#pragma unroll
+    for (int j = 0; j < kTN; j++)
+#pragma unroll
+        for (int i = 0; i < kTM; i++) acc[j][i] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+
+    constexpr int kCopyRows = kThreads / kPieces;       // rows that the workgroup copies at once
+    const int copyRow = threadIdx.x / kPieces;
+    const auto copyPanel = [&](const Panel& p, int64_t row0, int col0, uint32_t lds) {
+        const T* base = static_cast<const T*>(p.data) + row0 * p.stride + col0;
+        const int have = (int)(k1 - row0 < kStep ? k1 - row0 : kStep), strideBytes = (int)(p.stride * sizeof(T));
+        // the last row ends with its width, not with its stride
+        const int records = (have - 1) * strideBytes + (p.width - col0) * (int)sizeof(T);
+        const i32x4 from = descriptor(base, records);
+#pragma unroll
+        for (int i = 0; i < kStep / kCopyRows; i++) {
+            const int row = i * kCopyRows + copyRow;
+            const int c = ((threadIdx.x % kPieces) ^ outerSwizzle<T>(row)) * 16;
+            const int at = row < have && c < (p.width - col0) * (int)sizeof(T) ? row * strideBytes + c : kOutside;
+            copyToLds(from, at, 0, lds + (i * kThreads + wave * 64) * 16);
+        }
+    };
+    const auto copyStage = [&](int64_t k, uint32_t lds) {
+        copyPanel(args.p[job], k, m0, lds);
+        copyPanel(args.q[job], k, n0, lds + kPanel);
+    };
+    // columns 16 c .. 16 c + 15 of the stage's rows, a lane's share of step `half`
+    const auto fragment = [&](const char* lds, int c, int half) {
+        if constexpr (sizeof(T) == 4) {
+            f32x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = half * 16 + quad * 4 + j, piece = c * 4 + (col >> 2);
+                x[j] = *reinterpret_cast<const float*>(lds + (row * kPieces + (piece ^ outerSwizzle<T>(row))) * 16 + (col & 3) * 4);
+            }
+            return __builtin_bit_cast(uint4, x);
+        } else {
+            // each read transposes 4 rows x 16 columns held by 16 lanes
+            i16x4 x[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = half * 32 + quad * 8 + j * 4 + (col >> 2), piece = c * 2 + (col >> 1 & 1);
+                x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LdsI16x4*)(lds + (row * kPieces + (piece ^ outerSwizzle<T>(row))) * 16 + (col & 1) * 8));
+            }
+            return __builtin_bit_cast(uint4, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+    const auto multiply = [&](const char* lds) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            __builtin_amdgcn_sched_barrier(0);
+            uint4 p[kTM];
+#pragma unroll
+            for (int i = 0; i < kTM; i++) p[i] = fragment(lds, wm * kTM + i, half);
+#pragma unroll
+            for (int j = 0; j < kTN; j++) {
+                const uint4 q = fragment(lds + kPanel, wn * kTN + j, half);
+#pragma unroll
+                for (int i = 0; i < kTM; i++) acc[j][i] = Mma<T>::run(q, p[i], acc[j][i]);
+            }
+        }
+    };
+
+    const uint32_t lds = ldsAddress(stages);
+    if (k0 < k1) copyStage(k0, lds);
+    waitCopies();
+    __syncthreads();
+    int stage = 0;
+    for (int64_t k = k0; k < k1; k += kStep) {
+        if (k + kStep < k1) copyStage(k + kStep, lds + (stage ^ 1) * kStage);
+        multiply(stages + stage * kStage);
+        waitCopies();
+        __syncthreads();
+        stage ^= 1;
+    }
+    float* part = args.part[job] + (int64_t)split * m * n;
+#pragma unroll
+    for (int i = 0; i < kTM; i++) {
+        const int f = m0 + (wm * kTM + i) * 16 + col;
+        if (f >= m) continue;
+#pragma unroll
+        for (int j = 0; j < kTN; j++) {
+            const int d = n0 + (wn * kTN + j) * 16 + quad * 4;
+            float* to = part + (int64_t)f * n + d;
+            if (n % 4 == 0 && d + 4 <= n) *reinterpret_cast<f32x4*>(to) = acc[j][i];
+            else
+                for (int e = 0; e < 4; e++)
+                    if (d + e < n) to[e] = acc[j][i][e];
+        }
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void sumKernel(const SumArgs args)
+{
+    const SumJob& job = args.job[blockIdx.y];
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < job.count; e += (int64_t)gridDim.x * 256) {
+        float x = 0.0f;
+        for (int s = 0; s < args.splits; s++) x += job.part[s * job.count + e];
+        static_cast<T*>(job.out)[e] = (T)x;
+    }
+}
+
+// Copies with rows padded by zeros, or transposes, tile by tile of 32 x 32.
+template <typename T> __global__ __launch_bounds__(256) void packKernel(const PackArgs args)
+{
+    __shared__ T tile[32][33];
+    const PackJob& job = args.job[blockIdx.y];
+    const T* from = static_cast<const T*>(job.from);
+    T* to = static_cast<T*>(job.to);
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    // of the destination
+    const int64_t rows = job.transposed ? job.cols : job.rows, across = (job.toStride + 31) / 32;
+    const int64_t tiles = (rows + 31) / 32 * across;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t r0 = t / across * 32, c0 = t % across * 32;
+        if (job.transposed) {
+            for (int i = y; i < 32; i += 8) {
+                const int64_t r = c0 + i, c = r0 + x;
+                tile[i][x] = r < job.rows && c < job.cols ? from[r * job.fromStride + c] : T(0);
+            }
+            __syncthreads();
+        }
+        for (int i = y; i < 32; i += 8) {
+            const int64_t r = r0 + i, c = c0 + x;
+            if (r >= rows || c >= job.toStride) continue;
+            to[r * job.toStride + c] = job.transposed ? tile[x][i] : c < job.cols ? from[r * job.fromStride + c] : T(0);
+        }
+        if (job.transposed) __syncthreads();
+    }
+}
+
+// ---- launches ------------------------------------------------------------------
+
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN>
+int launchProductShape(const ProductArgs& args, hipStream_t stream)
+{
+    const int64_t tilesM = (args.m + kBM - 1) / kBM, tilesN = (args.n + kBN - 1) / kBN;
+    const int64_t blocks = (tilesM + 7) / 8 * 8 * tilesN;
+    productKernel<T, kKind, kBM, kBN, kWM, kWN><<<dim3((unsigned)blocks), kWM * kWN * 64, 0, stream>>>(args);
+    return launched("feed-forward product");
+}
+
+template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream)
+{
+    // Few rows run in tiles small enough that the columns alone give work to
+    // many compute units.
+    const bool small = args.m <= 4096;
+    if (kind == kProductGate)
+        return small ? launchProductShape<T, kProductGate, 64, 32, 2, 2>(args, stream)
+                     : launchProductShape<T, kProductGate, 256, 128, 2, 4>(args, stream);
+    if (kind == kProductGrad)
+        return small ? launchProductShape<T, kProductGrad, 64, 32, 2, 2>(args, stream)
+                     : launchProductShape<T, kProductGrad, 128, 128, 2, 2>(args, stream);
+    return small ? launchProductShape<T, kProductPlain, 64, 32, 2, 2>(args, stream)
+                 : launchProductShape<T, kProductPlain, 256, 256, 2, 4>(args, stream);
+}
+
+template <typename T> int launchOuter(const OuterArgs& args, int tile, hipStream_t stream)
+{
+    int tiles = 0;
+    for (int j = 0; j < args.jobs; j++)
+        tiles = std::max(tiles, ((args.m[j] + tile - 1) / tile) * ((args.n[j] + tile - 1) / tile));
+    const dim3 grid((unsigned)(tiles * args.splits), (unsigned)args.jobs);
+    if (tile == 256) outerKernel<T, 256, 2, 4><<<grid, 512, 0, stream>>>(args);
+    else outerKernel<T, 128, 2, 2><<<grid, 256, 0, stream>>>(args);
+    return launched("weight gradient product");
+}
+
+template <typename T> int launchPack(const PackArgs& args, hipStream_t stream)
+{
+    int64_t tiles = 1;
+    for (int j = 0; j < args.jobs; j++) {
+        const PackJob& p = args.job[j];
+        tiles = std::max(tiles, ((p.transposed ? p.cols : p.rows) + 31) / 32 * ((p.toStride + 31) / 32));
+    }
+    packKernel<T><<<dim3((unsigned)std::min<int64_t>(tiles, 16384), (unsigned)args.jobs), 256, 0, stream>>>(args);
+    return launched("operand packing");
+}
+
+template <typename T> int launchSum(const SumArgs& args, hipStream_t stream)
+{
+    int64_t count = 1;
+    for (int j = 0; j < args.jobs; j++) count = std::max(count, args.job[j].count);
+    sumKernel<T><<<dim3((unsigned)std::min<int64_t>((count + 255) / 256, 8192), (unsigned)args.jobs), 256, 0, stream>>>(args);
+    return launched("weight gradient sum");
+}
+
+}  // namespace carl

@@ -211,6 +211,100 @@ Tensor linearAttentionStep(const Tensor& q, const Tensor& k, const Tensor& v, co
     return out;
 }
 
+// ------------------------------------------------- gated feed-forward block
+
+// x as rows of its last dimension, without a copy where its strides allow.
+Tensor asRows(const Tensor& x)
+{
+    const int64_t width = x.size(-1);
+    Tensor rows = x.dim() == 2 ? x : x.reshape({ width ? x.numel() / width : 0, width });
+    return rows.stride(1) == 1 || width <= 1 ? rows : rows.contiguous();
+}
+
+carl_ffn ffnOf(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation)
+{
+    for (const auto& [t, name] : { std::pair{ &x, "x" }, { &gate, "w_gate" }, { &up, "w_up" }, { &down, "w_down" } }) {
+        onDevice(*t, name);
+        requireType(t->scalar_type() == x.scalar_type(), "x and the weights must have the same dtype");
+    }
+    carl_ffn f{};
+    f.type = elementType(x, "x");
+    require(x.dim() >= 1, "x must have shape [..., width]");
+    const int64_t width = x.size(-1);
+    require(gate.dim() == 2 && gate.size(1) == width, "w_gate must have shape [inner, width]");
+    require(up.sizes() == gate.sizes(), "w_up must have shape [inner, width]");
+    require(down.dim() == 2 && down.size(0) == width && down.size(1) == gate.size(0), "w_down must have shape [width, inner]");
+    require(width >= 1 && width <= CARL_FFN_MAX_DIM, "width must be in [1, 65536]");
+    require(gate.size(0) >= 1 && gate.size(0) <= CARL_FFN_MAX_DIM, "inner must be in [1, 65536]");
+    f.rows = x.numel() / width;
+    f.width = (int32_t)width;
+    f.inner = (int32_t)gate.size(0);
+    f.activation = (int32_t)activation;
+    return f;
+}
+
+struct GatedFfn : torch::autograd::Function<GatedFfn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up,
+                          const Tensor& down, int64_t activation)
+    {
+        carl_ffn f = ffnOf(x, gate, up, down, activation);
+        const Tensor rows = asRows(x), g = gate.contiguous(), u = up.contiguous(), d = down.contiguous();
+        Tensor y = at::empty(x.sizes(), x.options());
+        f.x = rows.data_ptr();
+        f.x_row = rows.stride(0);
+        f.w_gate = g.data_ptr();
+        f.w_up = u.data_ptr();
+        f.w_down = d.data_ptr();
+        f.y = y.data_ptr();
+        int64_t bytes = 0;
+        check(carl_gated_ffn_workspace(&f, 0, &bytes));
+        const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
+        f.workspace = work.data_ptr();
+        check(carl_gated_ffn(&f, currentStream()));
+        ctx->save_for_backward({ x, gate, up, down });
+        ctx->saved_data["activation"] = activation;
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        if (at::GradMode::is_enabled()) throw std::runtime_error("gated_ffn has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &gate = saved[1], &up = saved[2], &down = saved[3];
+        if (!grads[0].defined()) return { {}, {}, {}, {}, {} };
+        carl_ffn f = ffnOf(x, gate, up, down, ctx->saved_data["activation"].toInt());
+        const Tensor rows = asRows(x.detach()), dy = asRows(grads[0]);
+        const Tensor g = gate.detach().contiguous(), u = up.detach().contiguous(), d = down.detach().contiguous();
+        f.x = rows.data_ptr();
+        f.x_row = rows.stride(0);
+        f.dy = dy.data_ptr();
+        f.dy_row = dy.stride(0);
+        f.w_gate = g.data_ptr();
+        f.w_up = u.data_ptr();
+        f.w_down = d.data_ptr();
+        const auto wanted = [&](int i, const Tensor& t) {
+            return ctx->needs_input_grad(i) ? at::empty(t.sizes(), t.options()) : Tensor();
+        };
+        const Tensor dx = wanted(0, x), dg = wanted(1, gate), du = wanted(2, up), dd = wanted(3, down);
+        f.dx = dx.defined() ? dx.data_ptr() : nullptr;
+        f.dw_gate = dg.defined() ? dg.data_ptr() : nullptr;
+        f.dw_up = du.defined() ? du.data_ptr() : nullptr;
+        f.dw_down = dd.defined() ? dd.data_ptr() : nullptr;
+        int64_t bytes = 0;
+        check(carl_gated_ffn_workspace(&f, 1, &bytes));
+        const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
+        f.workspace = work.data_ptr();
+        check(carl_gated_ffn_backward(&f, currentStream()));
+        return { dx, dg, du, dd, {} };
+    }
+};
+
+Tensor gatedFfn(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const std::string& activation)
+{
+    require(activation == "silu" || activation == "gelu", "activation must be 'silu' or 'gelu'");
+    return GatedFfn::apply(x, gate, up, down, activation == "silu" ? CARL_SILU : CARL_GELU);
+}
+
 // ------------------------------------------------------------------- AdamW
 
 void adamwStep(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& first,
@@ -304,6 +398,7 @@ PYBIND11_MODULE(_ops, m)
     m.doc() = "The learner's operators of the MI355X engine (C-ABI in include/carl_amd_ops.h).";
     m.def("linear_attention", &linearAttention);
     m.def("linear_attention_step", &linearAttentionStep);
+    m.def("gated_ffn", &gatedFfn);
     m.def("adamw_step", &adamwStep);
     m.def("decode_moments", &decodeMoments);
     m.def("encode_moments", &encodeMoments);

@@ -3,6 +3,7 @@
   linear_attention       linear attention with a decay for each head over
                          rollouts and replays, with gradients
   linear_attention_step  its recurrent form: one step of every agent
+  gated_ffn              a gated feed-forward block, with gradients
 
 Formulas are those of include/carl_amd_ops.h.  Tensors must be on cuda:0; work
 is queued on torch's current stream.  Unfitting arguments raise ValueError or
@@ -51,4 +52,20 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     return _ops.linear_attention_step(q, k, v, log_decay, state, starts, scale)
 
 
-__all__ = ["linear_attention", "linear_attention_step"]
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *,
+              activation: str = "silu") -> torch.Tensor:
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T
+
+    x               [..., width], float32, bfloat16 or float16
+    w_gate, w_up    [inner, width], as torch.nn.Linear keeps them
+    w_down          [width, inner]
+    activation      "silu", or "gelu" in its tanh form
+
+    All of one type; products are summed in float32.  Gradients reach x and the
+    weights, once; the backward pass computes both projections again instead of
+    keeping them.
+    """
+    return _ops.gated_ffn(x, w_gate, w_up, w_down, activation)
+
+
+__all__ = ["gated_ffn", "linear_attention", "linear_attention_step"]

@@ -73,6 +73,39 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream);
  * the memory `state` [batch, heads, key_dim, value_dim] is updated in place. */
 int carl_linear_attention_step(const carl_attention* a, float* state, void* stream);
 
+/* ---- gated feed-forward block -------------------------------------------------
+ *   h = act(x w_gate^T) * (x w_up^T)        y = h w_down^T
+ * and its gradients.  All matrices hold one element type; products are summed
+ * in float32, and h and the gradients of both projections are rounded to that
+ * type once, where the next product reads them.  The backward pass needs only
+ * the inputs: it computes both projections again. */
+enum { CARL_SILU = 0, CARL_GELU = 1 };  /* GELU in its tanh form */
+
+typedef struct carl_ffn {
+    int64_t rows;
+    int32_t width, inner;       /* 1 to CARL_FFN_MAX_DIM */
+    int32_t type, activation;
+    const void* x;              /* [rows, width], rows x_row elements apart */
+    int64_t x_row;
+    const void *w_gate, *w_up;  /* [inner, width] */
+    const void* w_down;         /* [width, inner] */
+    void* y;                    /* [rows, width] */
+    /* backward: dy is read; gradients that are NULL are left out */
+    const void* dy;             /* [rows, width], rows dy_row elements apart */
+    int64_t dy_row;
+    void* dx;                   /* [rows, width] */
+    void *dw_gate, *dw_up, *dw_down;
+    void* workspace;            /* carl_gated_ffn_workspace bytes */
+} carl_ffn;
+
+enum { CARL_FFN_MAX_DIM = 65536 };
+
+/* For the pointers and strides of the call to come (operands that are not
+ * aligned to 16 bytes are laid out anew in the workspace). */
+int carl_gated_ffn_workspace(const carl_ffn* f, int backward, int64_t* bytes);
+int carl_gated_ffn(const carl_ffn* f, void* stream);
+int carl_gated_ffn_backward(const carl_ffn* f, void* stream);
+
 /* ---- AdamW ----------------------------------------------------------------
  * For each element, in float32 and in this order of roundings:
  *   m = m beta1 + g (1 - beta1)
