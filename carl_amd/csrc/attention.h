@@ -20,8 +20,10 @@
 // owns 16-column tiles of c, all rows.
 //
 // Precision with 16-bit rows: P is rounded once (the error of one rounding of
-// the output); the memory meets A as two terms of that type, and w_out C meets
-// B as three, so that the memory itself stays within float32's error of sums.
+// the output).  With bfloat16 the memory meets A as two terms of that type, and
+// w_out C meets B as three, so that the memory itself stays within float32's
+// error of sums; float16's range does not hold such terms, and its products
+// with the memory run in float32.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -23,6 +23,18 @@ __device__ inline f32x4 mma(bf16x4 a, bf16x4 b, f32x4 c)
 
 __device__ inline f32x4 mma(f16x4 a, f16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 
+// How products with float32 factors run (the memory read by a, what enters it
+// from b): bfloat16 as terms of that type, two and three of them; float16
+// rows, whose terms would leave its range, and float32 as float32.
+template <typename T> struct Long {
+    using type = float;
+    static constexpr int kIn = 1, kOut = 1;
+};
+template <> struct Long<bf16> {
+    using type = bf16;
+    static constexpr int kIn = 2, kOut = 3;
+};
+
 // x as kTerms addends of type T, largest first.
 template <typename T, int kTerms> __device__ inline void split(f32x4 x, vec<T, 4> (&out)[kTerms])
 {
@@ -93,7 +105,7 @@ __global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads)) void attenti
     constexpr int kTilesA = kA / 16;                 // of the memory's rows
     constexpr int kOwn = kCd / 16 / kWaves;          // column tiles of a wave
     constexpr int kE = 16 / sizeof(T);
-    constexpr int kIn = sizeof(T) == 4 ? 1 : 2, kOut = sizeof(T) == 4 ? 1 : 3;      // terms of M and of w_out C
+    using L = Long<T>;
 
     __shared__ __align__(16) T sA[kStates ? 1 : kSteps * S::kStrideA];
     __shared__ __align__(16) T sB[kSteps * S::kStrideA];
@@ -243,10 +255,10 @@ __global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads)) void attenti
 #pragma unroll
                     for (int m = 0; m < kTilesA; m++) {
                         const auto a = *reinterpret_cast<const vec<T, 4>*>(sA + t * S::kStrideA + m * 16 + quad * 4);
-                        vec<T, 4> terms[kIn];
-                        split<T, kIn>(memory[o][m], terms);
+                        vec<typename L::type, 4> terms[L::kIn];
+                        split<typename L::type, L::kIn>(memory[o][m], terms);
 #pragma unroll
-                        for (int i = 0; i < kIn; i++) carried = mma(terms[i], a, carried);
+                        for (int i = 0; i < L::kIn; i++) carried = mma(terms[i], __builtin_convertvector(a, vec<typename L::type, 4>), carried);
                     }
                     // a closed step takes nothing from the memory, whatever that holds
                     f32x4 out = within;
@@ -301,13 +313,13 @@ __global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads)) void attenti
                     const bool leaves = s < have && episode(s) == (r.backwards ? 0 : all);
                     c[j] = leaves ? c[j] * (power(r.backwards ? s + 1 : have - 1 - s) * r.scaleOut) : 0.0f;
                 }
-                vec<T, 4> terms[kOut];
-                split<T, kOut>(c, terms);
+                vec<typename L::type, 4> terms[L::kOut];
+                split<typename L::type, L::kOut>(c, terms);
 #pragma unroll
                 for (int m = 0; m < kTilesA; m++) {
-                    const auto b = columns(sB, S::kStrideA, sb, m * 16 + col);
+                    const auto b = __builtin_convertvector(columns(sB, S::kStrideA, sb, m * 16 + col), vec<typename L::type, 4>);
 #pragma unroll
-                    for (int i = 0; i < kOut; i++) memory[o][m] = mma(b, terms[i], memory[o][m]);
+                    for (int i = 0; i < L::kOut; i++) memory[o][m] = mma(b, terms[i], memory[o][m]);
                 }
             }
         }
