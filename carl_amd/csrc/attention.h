@@ -42,11 +42,14 @@ struct Rows {
 struct Role {
     Rows a, b, c, out;
     int32_t aHeads, bHeads, cHeads;         // query heads that share a row of each
-    int32_t aGrain, bGrain, cGrain;         // bytes that its rows' addresses are multiples of: 16, 8, 4 or 2
+    int32_t aGrain, bGrain, cGrain;         // bytes that its rows' addresses and widths are multiples of: 16, 8, 4 or 2
+                                            // (2 too where a chunk's rows are too far apart for 32-bit offsets)
     int32_t outWide;                        // out's rows take stores of four elements
     int32_t outFloat;                       // out is float32 whatever the rows' type
     int32_t dimA, dimC;
     int32_t backwards;
+    int32_t inShift;                        // steps between the memory before a chunk and its first row (1; backwards 0,
+                                            // where the memory is the gradient of the one at the chunk's last step)
     float scaleP, scaleIn, scaleOut;        // of P, of the carried memory where it is read, of what enters the memory
     const float* first;                     // the memory before the first chunk, or NULL
     float* last;                            // after the last one, or NULL
@@ -59,6 +62,7 @@ struct Pass {
     Role role[3];
     int64_t batch, steps;
     int32_t heads, segments;
+    int32_t dealGroups;                     // whole sequences (or segments) are dealt to the dies, else heads are
     int64_t segmentSteps;
     const float* logDecay;
     const uint8_t* starts;

@@ -165,6 +165,16 @@ int grainOf(const Rows& r, int type, int64_t batch, int64_t steps, int heads)
     return (int)(bits & (~bits + 1));
 }
 
+// The same for rows of `dim` elements that are read: 2 where a chunk's rows do
+// not lie within the 32-bit offsets of a buffer descriptor.
+int readGrain(const Rows& r, int type, int64_t batch, int64_t steps, int heads, int dim)
+{
+    const int size = elementBytes(type);
+    if (r.step < 0 || r.step >= ((int64_t)1 << 31) / (64 * size) - 128) return size == 4 ? 0 : 2;
+    const int grain = grainOf(r, type, batch, steps, heads), width = dim * size & -(dim * size);
+    return grain < width ? grain : width;
+}
+
 Rows rowsOf(const carl_rows& r) { return Rows{ r.data, r.batch, r.step, r.head }; }
 
 // How a sequence is split.  One workgroup walks a whole sequence of one head
@@ -242,6 +252,7 @@ Pass passOf(const carl_attention& a)
     pass.heads = a.heads;
     pass.segments = s.segments;
     pass.segmentSteps = s.steps;
+    pass.dealGroups = a.batch * s.segments >= 64;
     pass.logDecay = a.log_decay;
     pass.starts = a.starts;
     pass.startsBatch = a.starts_batch;
@@ -262,13 +273,14 @@ Role roleOf(const carl_attention& a, const carl_rows& x, bool xShared, const car
     r.aHeads = xShared ? group : 1;
     r.bHeads = yShared ? group : 1;
     r.cHeads = zShared ? group : 1;
-    r.aGrain = grainOf(r.a, a.type, a.batch, a.steps, xShared ? a.kv_heads : a.heads);
-    r.bGrain = grainOf(r.b, a.type, a.batch, a.steps, yShared ? a.kv_heads : a.heads);
-    r.cGrain = grainOf(r.c, a.type, a.batch, a.steps, zShared ? a.kv_heads : a.heads);
+    r.aGrain = readGrain(r.a, a.type, a.batch, a.steps, xShared ? a.kv_heads : a.heads, dimA);
+    r.bGrain = readGrain(r.b, a.type, a.batch, a.steps, yShared ? a.kv_heads : a.heads, dimA);
+    r.cGrain = readGrain(r.c, a.type, a.batch, a.steps, zShared ? a.kv_heads : a.heads, dimC);
     r.outWide = grainOf(out, a.type, a.batch, a.steps, a.heads) >= 4 * elementBytes(a.type);
     r.dimA = dimA;
     r.dimC = dimC;
     r.scaleP = a.scale;
+    r.inShift = 1;
     return r;
 }
 
@@ -355,6 +367,7 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
     dv = roleOf(*a, a->k, true, a->q, false, a->d_out, false, valueRows, a->key_dim, a->value_dim);
     for (Role* r : { &dk, &dv }) {
         r->backwards = 1;
+        r->inShift = 0;
         r->scaleIn = 1.0f;
         r->scaleOut = a->scale;
         r->first = a->d_final_state;

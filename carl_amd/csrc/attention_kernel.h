@@ -6,22 +6,41 @@
 
 namespace carl {
 
-template <typename T> struct Frag {
-    using type = vec<T, 4>;
-};
-
+// One product of 16x16 tiles over one (x4: 16 steps of the sum) or two (x8: 32
+// steps) fragments of each operand.
 __device__ inline f32x4 mma(f32x4 a, f32x4 b, f32x4 c)
 {
+#pragma unroll
     for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
     return c;
 }
-
-__device__ inline f32x4 mma(bf16x4 a, bf16x4 b, f32x4 c)
+__device__ inline f32x4 mma(vec<float, 8> a, vec<float, 8> b, f32x4 c)
 {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
 }
+__device__ inline f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ inline f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-__device__ inline f32x4 mma(f16x4 a, f16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+template <typename V> __device__ inline auto both(V a, V b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// From column `at` on: of rows 4 quad .. 4 quad + 3 of a 16-row block of LDS,
+// the lane's column at + lane%16.
+__device__ inline f32x4 columns(const float* rows, int stride, int at, int col, int quad)
+{
+    f32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = rows[(quad * 4 + j) * stride + at + col];
+    return x;
+}
+typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+template <typename T> __device__ inline vec<T, 4> columns(const T* rows, int stride, int at, int col, int quad)
+{
+    // transposes 4 rows x 16 columns held by 16 lanes
+    return __builtin_bit_cast(vec<T, 4>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (LdsI16x4*)(rows + (quad * 4 + (col >> 2)) * stride + at + (col & 3) * 4)));
+}
 
 // How products with float32 factors run (the memory read by a, what enters it
 // from b): bfloat16 as terms of that type, two and three of them; float16
@@ -45,21 +64,10 @@ template <typename T, int kTerms> __device__ inline void split(f32x4 x, vec<T, 4
     }
 }
 
-// kBytes of a row from address p, in pieces that its alignment allows; zero past `have` elements.
-template <typename T> __device__ inline uint4 loadPiece(const T* p, int have, int grain)
+// 16 bytes of a row from address p, element by element; zero past `have`.
+template <typename T> __device__ inline uint4 loadPiece(const T* p, int have)
 {
     constexpr int kE = 16 / sizeof(T);
-    if (have >= kE) {
-        if (grain == 16) return *reinterpret_cast<const uint4*>(p);
-        if (grain == 8) {
-            const uint2 x = reinterpret_cast<const uint2*>(p)[0], y = reinterpret_cast<const uint2*>(p)[1];
-            return make_uint4(x.x, x.y, y.x, y.y);
-        }
-        if (grain == 4) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
     vec<T, kE> r;
 #pragma unroll
     for (int j = 0; j < kE; j++) r[j] = j < have ? p[j] : T(0);
@@ -93,54 +101,66 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static constexpr int kStrideA = kA + kPad, kStrideC = kC_ + kPad, kStrideP = kSteps + kPad;
     static constexpr int kPieceA = kA * (int)sizeof(T) / 16, kPieceC = kC_ * (int)sizeof(T) / 16;   // 16-byte pieces of a row
     static constexpr int kLoadsA = kSteps * kPieceA / kThreads, kLoadsC = kSteps * kPieceC / kThreads;
+    // waves of a SIMD that the registers leave room for
+    static constexpr int kResident = kA * kC_ <= 64 * 64 ? (sizeof(T) == 2 ? 3 : 2) : kA * kC_ <= 64 * 128 && sizeof(T) == 2 ? 2 : 1;
     static_assert(kSteps * kPieceA % kThreads == 0 && kSteps * kPieceC % kThreads == 0, "whole loads");
 };
 
 template <typename T, int kA, int kCd, int kSteps, bool kStates>
-__global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads)) void attentionKernel(const Pass pass, const int firstRole)
+__global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads), (Shape<T, kA, kCd, kSteps>::kResident))
+void attentionKernel(const Pass pass, const int firstRole, const int roles)
 {
     using S = Shape<T, kA, kCd, kSteps>;
     constexpr int kWaves = S::kWaves, kThreads = S::kThreads;
-    constexpr int kBlocks = kSteps / 16;             // 16-step blocks of a chunk
-    constexpr int kTilesA = kA / 16;                 // of the memory's rows
+    constexpr int kBlocks = kSteps / 16;             // 16-step blocks of a chunk, an even number
+    constexpr int kTilesA = kA / 16;                 // of the memory's rows, an even number
     constexpr int kOwn = kCd / 16 / kWaves;          // column tiles of a wave
     constexpr int kE = 16 / sizeof(T);
     using L = Long<T>;
+    using LT = typename L::type;
 
     __shared__ __align__(16) T sA[kStates ? 1 : kSteps * S::kStrideA];
     __shared__ __align__(16) T sB[kSteps * S::kStrideA];
     __shared__ __align__(16) T sC[kSteps * S::kStrideC];
     __shared__ __align__(16) T sP[kStates ? 1 : kSteps * S::kStrideP];
 
-    const Role& r = pass.role[firstRole + blockIdx.y];
-    const int64_t unit = blockIdx.x;
-    const int head = (int)(unit % pass.heads);
-    const int64_t batch = unit / pass.heads % pass.batch, segment = unit / pass.heads / pass.batch;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    // Blocks are dealt to the 8 dies in turn.  The roles of one unit and the
+    // heads of one sequence, which read the same rows or lines, run on one.
+    const int die = blockIdx.x % 8, local = blockIdx.x / 8;
+    const int64_t groups = pass.batch * pass.segments;
+    int64_t group;
+    int head;
+    if (pass.dealGroups) {
+        group = (int64_t)(local / roles / pass.heads) * 8 + die;
+        head = local / roles % pass.heads;
+    } else {
+        const int64_t unit = (int64_t)(local / roles) * 8 + die;
+        group = unit / pass.heads;
+        head = (int)(unit % pass.heads);
+    }
+    if (group >= groups) return;
+    const Role& r = pass.role[firstRole + local % roles];
+    const int64_t batch = group % pass.batch, segment = group / pass.batch;
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool backwards = r.backwards != 0;
 
     const int64_t begin = segment * pass.segmentSteps;
     const int64_t end = begin + pass.segmentSteps < pass.steps ? begin + pass.segmentSteps : pass.steps;
-    const int64_t chunks = (end - begin + kSteps - 1) / kSteps;
+    const int chunks = (int)((end - begin + kSteps - 1) / kSteps);
     const T* aRows = static_cast<const T*>(r.a.data) + batch * r.a.batch + head / r.aHeads * r.a.head;
     const T* bRows = static_cast<const T*>(r.b.data) + batch * r.b.batch + head / r.bHeads * r.b.head;
     const T* cRows = static_cast<const T*>(r.c.data) + batch * r.c.batch + head / r.cHeads * r.c.head;
 
     // -infinity times zero steps is no NaN
     const float decay2 = fmaxf(pass.logDecay[head] * 1.44269504088896341f, -1e30f);
-    const auto power = [&](int steps) { return exp2f(decay2 * (float)steps); };
+    const auto power = [&](int steps) { return __builtin_amdgcn_exp2f(decay2 * (float)steps); };
 
+    const int64_t size = (int64_t)r.dimA * r.dimC, unitState = batch * pass.heads + head;
+    const int64_t partState = segment * pass.batch * pass.heads + unitState;
+    // a lane's elements of the memory: rows 16 m + 4 quad + i, column 16 (wave's tile) + col
     f32x4 memory[kOwn][kTilesA];
-    {
-        const int64_t size = (int64_t)r.dimA * r.dimC, unitState = batch * pass.heads + head;
-        const float* from = nullptr;
-        bool swapped = false;
-        if (!kStates) {
-            if (pass.segments > 1) from = r.parts + (segment * pass.batch * pass.heads + unitState) * size;
-            else if (r.first) {
-                from = r.first + unitState * size;
-                swapped = r.firstSwapped != 0;
-            }
-        }
+    const auto eachMemory = [&](bool swapped, auto visit) {
 #pragma unroll
         for (int o = 0; o < kOwn; o++)
 #pragma unroll
@@ -148,205 +168,296 @@ __global__ __launch_bounds__((Shape<T, kA, kCd, kSteps>::kThreads)) void attenti
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int x = m * 16 + quad * 4 + i, y = (wave * kOwn + o) * 16 + col;
-                    const bool in = from && x < r.dimA && y < r.dimC;
-                    memory[o][m][i] = in ? from[swapped ? (int64_t)y * r.dimA + x : (int64_t)x * r.dimC + y] : 0.0f;
+                    memory[o][m][i] = visit(memory[o][m][i], swapped ? y * r.dimA + x : x * r.dimC + y, x < r.dimA && y < r.dimC);
                 }
+    };
+    {
+        const float* from = nullptr;
+        bool swapped = false;
+        if (!kStates) {
+            if (pass.segments > 1) from = r.parts + partState * size;
+            else if (r.first) {
+                from = r.first + unitState * size;
+                swapped = r.firstSwapped != 0;
+            }
+        }
+        if (from) eachMemory(swapped, [&](float, int at, bool in) { return in ? from[at] : 0.0f; });
+        else eachMemory(false, [&](float, int, bool) { return 0.0f; });
     }
 
+    // Chunks follow time in the pass's direction, and so do the rows of a chunk
+    // in LDS: what comes first is in row 0.
+    const auto chunkStart = [&](int n) { return begin + (int64_t)(backwards ? chunks - 1 - n : n) * kSteps; };
+
+    // Rows on the way to LDS: 16-byte pieces through a descriptor that gives
+    // zeros past the chunk's rows.  Pieces need addresses of 4 bytes; rows of
+    // other addresses are copied element by element when they are due.
     uint4 nextA[kStates ? 1 : S::kLoadsA], nextB[S::kLoadsA], nextC[S::kLoadsC];
-    const auto chunkStart = [&](int64_t n) { return begin + (r.backwards ? chunks - 1 - n : n) * kSteps; };
-    const auto fetchRows = [&](auto& next, const T* rows, int64_t step, int64_t t0, int pieces, int dim, int grain) {
+    const auto fetchRows = [&](auto& next, const T* rows, int64_t step, int64_t t0, int pieces, int dim) {
+        const int have = (int)(end - t0 < kSteps ? end - t0 : kSteps), stepBytes = (int)step * (int)sizeof(T);
+        const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(rows + t0 * step), 0,
+                                                           (have - 1) * stepBytes + dim * (int)sizeof(T), 0x00027000);
+        const int row = threadIdx.x / pieces, at = threadIdx.x % pieces * kE, rowsAtOnce = kThreads / pieces;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            const int piece = i * kThreads + threadIdx.x;
-            const int row = piece / pieces, at = piece % pieces * kE;
-            const int64_t t = t0 + row;
-            next[i] = t < end && at < dim ? loadPiece<T>(rows + t * step + at, dim - at, grain) : make_uint4(0, 0, 0, 0);
+            const int mine = row + i * rowsAtOnce, t = backwards ? have - 1 - mine : mine;
+            const int offset = mine < have && at < dim ? t * stepBytes + at * (int)sizeof(T) : (int)0x80000000u;
+            next[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
         }
     };
-    const auto fetch = [&](int64_t n) {
+    const auto fetch = [&](int n) {
         const int64_t t0 = chunkStart(n);
-        if constexpr (!kStates) fetchRows(nextA, aRows, r.a.step, t0, S::kPieceA, r.dimA, r.aGrain);
-        fetchRows(nextB, bRows, r.b.step, t0, S::kPieceA, r.dimA, r.bGrain);
-        fetchRows(nextC, cRows, r.c.step, t0, S::kPieceC, r.dimC, r.cGrain);
+        if constexpr (!kStates)
+            if (r.aGrain >= 4) fetchRows(nextA, aRows, r.a.step, t0, S::kPieceA, r.dimA);
+        if (r.bGrain >= 4) fetchRows(nextB, bRows, r.b.step, t0, S::kPieceA, r.dimA);
+        if (r.cGrain >= 4) fetchRows(nextC, cRows, r.c.step, t0, S::kPieceC, r.dimC);
     };
     uint32_t odd = 0;         // carry bits of non-finite values in this chunk's b and c
-    const auto put = [&](const auto& next, T* rows, int stride, int pieces) {
+    const auto put = [&](auto& next, T* lds, int stride, int pieces, bool look, int grain, int dim, const T* rows, int64_t step,
+                         int64_t t0, int have) {
+        const int at = threadIdx.x % pieces * kE;
+        T* to = lds + threadIdx.x / pieces * stride + at;
+        if (grain < 4) {
+            for (int row = threadIdx.x / pieces; row < kSteps; row += kThreads / pieces) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row < have) x = loadPiece<T>(rows + (t0 + (backwards ? have - 1 - row : row)) * step + at, dim - at);
+                *reinterpret_cast<uint4*>(lds + row * stride + at) = x;
+                if (look) odd |= nonFinite<T>(x);
+            }
+            return;
+        }
+        // words of the piece past the row's end hold what follows it
+        const int words = (dim - at) * (int)sizeof(T) / 4;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            const int piece = i * kThreads + threadIdx.x;
-            *reinterpret_cast<uint4*>(rows + piece / pieces * stride + piece % pieces * kE) = next[i];
-            odd |= nonFinite<T>(next[i]);
+            if (dim % kE) {
+                next[i].y = words > 1 ? next[i].y : 0;
+                next[i].z = words > 2 ? next[i].z : 0;
+                next[i].w = words > 3 ? next[i].w : 0;
+            }
+            *reinterpret_cast<uint4*>(to + i * (kThreads / pieces) * stride) = next[i];
+            if (look) odd |= nonFinite<T>(next[i]);
         }
-    };
-    // column `at` of rows 4 quad .. 4 quad + 3 of the 16-row block
-    const auto columns = [&](const T* rows, int stride, int block, int at) {
-        vec<T, 4> x;
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = rows[(block * 16 + quad * 4 + j) * stride + at];
-        return x;
     };
 
     float factor = 1.0f;      // of the memory over the whole segment
     if (chunks > 0) fetch(0);
-    for (int64_t n = 0; n < chunks; n++) {
+    for (int n = 0; n < chunks; n++) {
         const int64_t t0 = chunkStart(n);
         const int have = end - t0 < kSteps ? (int)(end - t0) : kSteps;
         __syncthreads();
-        if constexpr (!kStates) put(nextA, sA, S::kStrideA, S::kPieceA);
         odd = 0;
-        put(nextB, sB, S::kStrideA, S::kPieceA);
-        put(nextC, sC, S::kStrideC, S::kPieceC);
+        if constexpr (!kStates) put(nextA, sA, S::kStrideA, S::kPieceA, false, r.aGrain, r.dimA, aRows, r.a.step, t0, have);
+        put(nextB, sB, S::kStrideA, S::kPieceA, true, r.bGrain, r.dimA, bRows, r.b.step, t0, have);
+        put(nextC, sC, S::kStrideC, S::kPieceC, true, r.cGrain, r.dimC, cRows, r.c.step, t0, have);
+        // Bit t of `cuts`: row t sees nothing of the rows before it.  Forwards
+        // that is where an episode starts; backwards, where the step after
+        // (row t - 1) does, and a start at the chunk's first step, its last
+        // row, closes the way out instead (bit 0: the way in).
+        uint64_t cuts = 0;
+        bool shut = false;
+        if (pass.starts) {
+            const uint64_t starts = __ballot(
+                lane < have && pass.starts[batch * pass.startsBatch + (t0 + (backwards ? have - 1 - lane : lane)) * pass.startsStep] != 0);
+            cuts = backwards ? starts << 1 & (~0ull >> (64 - have)) : starts;
+            shut = backwards && (starts >> (have - 1) & 1);
+        }
         // A weight of zero takes a finite row out of a product, but not an
         // infinity or a NaN: a chunk whose b or c hold one is summed step by
         // step, leaving out the steps that are not seen.
         const bool careful = __syncthreads_or((odd & Exponent<T>::kCarry) != 0) != 0;
         if (n + 1 < chunks) fetch(n + 1);
 
-        // bit t: step t of the chunk starts an episode
-        uint64_t starts = 0;
-        if (pass.starts)
-            starts = __ballot(lane < have && pass.starts[batch * pass.startsBatch + (t0 + lane) * pass.startsStep] != 0);
-        const int all = __popcll(starts);
-        const auto episode = [&](int t) { return __popcll(starts & (~0ull >> (63 - t))); };
+        // Rows [low(t), t] are what row t sees of the chunk.
+        const auto low = [&](int t) {
+            const uint64_t before = cuts & (~0ull >> (63 - t));
+            return before ? 63 - __builtin_clzll(before) : 0;
+        };
+        // Rows [leave, have) are what the memory after the chunk sees.
+        const int leave = shut ? have : cuts ? 63 - __builtin_clzll(cuts) : 0;
+        const bool closed = cuts != 0 || shut;
 
+        f32x4 acc[kOwn][kBlocks];
         if constexpr (!kStates) {
-            for (int tile = wave; tile < kBlocks * kBlocks; tile += kWaves) {
-                const int tb = tile / kBlocks, sb = tile % kBlocks;
-                const int t = tb * 16 + col, mine = episode(t);
-                f32x4 p = { 0.f, 0.f, 0.f, 0.f };
-                if (r.backwards ? sb >= tb : sb <= tb) {
+            // P^T, tile by tile: rows s, column t
+            for (int tb = wave; tb < kBlocks; tb += kWaves) {
+                const int t = tb * 16 + col, from = low(t);
+                vec<T, 4> a[kTilesA];
 #pragma unroll
-                    for (int k = 0; k < kTilesA; k++) {
-                        const auto b = *reinterpret_cast<const vec<T, 4>*>(sB + (sb * 16 + col) * S::kStrideA + k * 16 + quad * 4);
-                        const auto a = *reinterpret_cast<const vec<T, 4>*>(sA + t * S::kStrideA + k * 16 + quad * 4);
-                        p = mma(b, a, p);
-                    }
+                for (int k = 0; k < kTilesA; k++) a[k] = *reinterpret_cast<const vec<T, 4>*>(sA + t * S::kStrideA + k * 16 + quad * 4);
+                for (int sb = 0; sb <= tb; sb++) {
+                    f32x4 p = { 0.f, 0.f, 0.f, 0.f };
+                    const T* rows = sB + (sb * 16 + col) * S::kStrideA + quad * 4;
+#pragma unroll
+                    for (int k = 0; k < kTilesA; k += 2)
+                        p = mma(both(*reinterpret_cast<const vec<T, 4>*>(rows + k * 16), *reinterpret_cast<const vec<T, 4>*>(rows + k * 16 + 16)),
+                                both(a[k], a[k + 1]), p);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int s = sb * 16 + quad * 4 + i, gap = r.backwards ? s - t : t - s;
-                        p[i] = gap >= 0 && episode(s) == mine ? p[i] * (power(gap) * r.scaleP) : 0.0f;
+                        const int s = sb * 16 + quad * 4 + i;
+                        const float w = p[i] * (power(t - s) * r.scaleP);
+                        p[i] = s >= from && s <= t ? w : 0.0f;
                     }
+                    *reinterpret_cast<vec<T, 4>*>(sP + t * S::kStrideP + sb * 16 + quad * 4) = fromFloat<T, 4>(p);
                 }
-                *reinterpret_cast<vec<T, 4>*>(sP + t * S::kStrideP + sb * 16 + quad * 4) = fromFloat<T, 4>(p);
+                // blocks of s are met in pairs below
+                if (tb % 2 == 0)
+                    *reinterpret_cast<vec<T, 4>*>(sP + t * S::kStrideP + (tb + 1) * 16 + quad * 4) = vec<T, 4>{ T(0), T(0), T(0), T(0) };
             }
-            __syncthreads();
-            for (int tb = 0; tb < kBlocks; tb++) {
-                const int t = tb * 16 + col, mine = episode(t);
-                const bool open = r.backwards ? mine == all : mine == 0;
-                const float in = open ? power(r.backwards ? have - 1 - t : t + 1) * r.scaleIn : 0.0f;
+            // what the carried memory gives
+#pragma unroll
+            for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                for (int tb = 0; tb < kBlocks; tb++) acc[o][tb] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int m = 0; m < kTilesA; m += 2) {
+                vec<LT, 4> lo[kOwn][L::kIn], hi[kOwn][L::kIn];
 #pragma unroll
                 for (int o = 0; o < kOwn; o++) {
-                    const int at = (wave * kOwn + o) * 16;
-                    f32x4 within = { 0.f, 0.f, 0.f, 0.f }, carried = { 0.f, 0.f, 0.f, 0.f };
-                    if (careful) {
-                        for (int s = r.backwards ? t : 0; s < (r.backwards ? have : t + 1); s++)
-                            if (episode(s) == mine)
-                                for (int i = 0; i < 4; i++)
-                                    within[i] += (float)sP[t * S::kStrideP + s] * (float)sC[s * S::kStrideC + at + quad * 4 + i];
-                    } else {
+                    split<LT, L::kIn>(memory[o][m], lo[o]);
+                    split<LT, L::kIn>(memory[o][m + 1], hi[o]);
+                }
 #pragma unroll
-                    for (int sb = 0; sb < kBlocks; sb++) {
-                        if (r.backwards ? sb < tb : sb > tb) continue;
-                        const auto p = *reinterpret_cast<const vec<T, 4>*>(sP + t * S::kStrideP + sb * 16 + quad * 4);
-                        within = mma(columns(sC, S::kStrideC, sb, at + col), p, within);
-                    }
-                    }
+                for (int tb = 0; tb < kBlocks; tb++) {
+                    const T* rows = sA + (tb * 16 + col) * S::kStrideA + m * 16 + quad * 4;
+                    const auto a = both(__builtin_convertvector(*reinterpret_cast<const vec<T, 4>*>(rows), vec<LT, 4>),
+                                        __builtin_convertvector(*reinterpret_cast<const vec<T, 4>*>(rows + 16), vec<LT, 4>));
 #pragma unroll
-                    for (int m = 0; m < kTilesA; m++) {
-                        const auto a = *reinterpret_cast<const vec<T, 4>*>(sA + t * S::kStrideA + m * 16 + quad * 4);
-                        vec<typename L::type, 4> terms[L::kIn];
-                        split<typename L::type, L::kIn>(memory[o][m], terms);
+                    for (int o = 0; o < kOwn; o++)
 #pragma unroll
-                        for (int i = 0; i < L::kIn; i++) carried = mma(terms[i], __builtin_convertvector(a, vec<typename L::type, 4>), carried);
+                        for (int i = 0; i < L::kIn; i++) acc[o][tb] = mma(both(lo[o][i], hi[o][i]), a, acc[o][tb]);
+                }
+            }
+#pragma unroll
+            for (int tb = 0; tb < kBlocks; tb++) {
+                const int t = tb * 16 + col;
+                const bool open = (cuts & (~0ull >> (63 - t))) == 0;
+                const float in = power(t + r.inShift) * r.scaleIn;
+                // a closed row takes nothing from the memory, whatever that holds
+#pragma unroll
+                for (int o = 0; o < kOwn; o++) acc[o][tb] = open ? acc[o][tb] * in : f32x4{ 0.f, 0.f, 0.f, 0.f };
+            }
+            __syncthreads();
+        }
+
+        const float keep = closed ? 0.0f : power(have);
+        factor *= keep;
+        // what row s weighs in the memory after the chunk
+        const auto weightOut = [&](int s) {
+            return s >= leave && s < have ? power(have - 1 - s + 1 - r.inShift) * r.scaleOut : 0.0f;
+        };
+        if (!careful) {
+            vec<T, 4> c[kOwn][kBlocks];
+#pragma unroll
+            for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                for (int sb = 0; sb < kBlocks; sb++)
+                    c[o][sb] = columns(sC + sb * 16 * S::kStrideC, S::kStrideC, (wave * kOwn + o) * 16, col, quad);
+            if constexpr (!kStates) {
+#pragma unroll
+                for (int tb = 0; tb < kBlocks; tb++)
+#pragma unroll
+                    for (int sb = 0; sb <= tb; sb += 2) {
+                        const T* row = sP + (tb * 16 + col) * S::kStrideP + sb * 16 + quad * 4;
+                        const auto p = both(*reinterpret_cast<const vec<T, 4>*>(row), *reinterpret_cast<const vec<T, 4>*>(row + 16));
+#pragma unroll
+                        for (int o = 0; o < kOwn; o++) acc[o][tb] = mma(both(c[o][sb], c[o][sb + 1]), p, acc[o][tb]);
                     }
-                    // a closed step takes nothing from the memory, whatever that holds
-                    f32x4 out = within;
-                    if (open) out += carried * in;
-                    const int y = at + quad * 4;
-                    if (t >= have || y >= r.dimC) continue;
-                    const int64_t to = batch * r.out.batch + (t0 + t) * r.out.step + head * r.out.head + y;
-                    if (r.outFloat) {
-                        float* x = static_cast<float*>(r.out.data) + to;
-                        if (r.outWide && y + 4 <= r.dimC) *reinterpret_cast<f32x4*>(x) = out;
-                        else
+            }
+#pragma unroll
+            for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                for (int m = 0; m < kTilesA; m++) memory[o][m] = closed ? f32x4{ 0.f, 0.f, 0.f, 0.f } : memory[o][m] * keep;
+#pragma unroll
+            for (int sb = 0; sb < kBlocks; sb += 2) {
+                f32x4 w[2];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    w[0][j] = weightOut(sb * 16 + quad * 4 + j);
+                    w[1][j] = weightOut(sb * 16 + 16 + quad * 4 + j);
+                }
+                vec<LT, 4> lo[kOwn][L::kOut], hi[kOwn][L::kOut];
+#pragma unroll
+                for (int o = 0; o < kOwn; o++) {
+                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb]) * w[0], lo[o]);
+                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb + 1]) * w[1], hi[o]);
+                }
+                const T* rows = sB + sb * 16 * S::kStrideA;
+#pragma unroll
+                for (int m = 0; m < kTilesA; m++) {
+                    const auto b = both(__builtin_convertvector(columns(rows, S::kStrideA, m * 16, col, quad), vec<LT, 4>),
+                                        __builtin_convertvector(columns(rows + 16 * S::kStrideA, S::kStrideA, m * 16, col, quad), vec<LT, 4>));
+#pragma unroll
+                    for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                        for (int i = 0; i < L::kOut; i++) memory[o][m] = mma(b, both(lo[o][i], hi[o][i]), memory[o][m]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int o = 0; o < kOwn; o++) {
+                const int tile = (wave * kOwn + o) * 16;
+                if constexpr (!kStates) {
+#pragma unroll
+                    for (int tb = 0; tb < kBlocks; tb++) {
+                        const int t = tb * 16 + col;
+#pragma unroll 1
+                        for (int s = low(t); s <= t && s < have; s++)
+#pragma unroll
                             for (int i = 0; i < 4; i++)
-                                if (y + i < r.dimC) x[i] = out[i];
-                    } else {
-                        T* x = static_cast<T*>(r.out.data) + to;
-                        if (r.outWide && y + 4 <= r.dimC) *reinterpret_cast<vec<T, 4>*>(x) = fromFloat<T, 4>(out);
-                        else
-                            for (int i = 0; i < 4; i++)
-                                if (y + i < r.dimC) x[i] = (T)out[i];
+                                acc[o][tb][i] += (float)sP[t * S::kStrideP + s] * (float)sC[s * S::kStrideC + tile + quad * 4 + i];
                     }
+                }
+#pragma unroll
+                for (int m = 0; m < kTilesA; m++) memory[o][m] = closed ? f32x4{ 0.f, 0.f, 0.f, 0.f } : memory[o][m] * keep;
+#pragma unroll 1
+                for (int s = leave; s < have; s++) {
+                    const float x = (float)sC[s * S::kStrideC + tile + col] * weightOut(s);
+#pragma unroll
+                    for (int m = 0; m < kTilesA; m++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) memory[o][m][i] += (float)sB[s * S::kStrideA + m * 16 + quad * 4 + i] * x;
                 }
             }
         }
 
-        // the memory: kept where no episode starts in the chunk, and what the chunk adds
-        const float keep = all == 0 ? power(have) : 0.0f;
-        factor *= keep;
+        if constexpr (!kStates) {
 #pragma unroll
-        for (int o = 0; o < kOwn; o++) {
+            for (int tb = 0; tb < kBlocks; tb++) {
+                const int t = tb * 16 + col;
+                if (t >= have) continue;
+                const int64_t row = batch * r.out.batch + (t0 + (backwards ? have - 1 - t : t)) * r.out.step + head * r.out.head;
 #pragma unroll
-            for (int m = 0; m < kTilesA; m++)
-                memory[o][m] = all == 0 ? memory[o][m] * keep : f32x4{ 0.f, 0.f, 0.f, 0.f };
-            if (careful) {
-                for (int s = 0; s < have; s++) {
-                    if (episode(s) != (r.backwards ? 0 : all)) continue;
-                    const float c = (float)sC[s * S::kStrideC + (wave * kOwn + o) * 16 + col]
-                                  * (power(r.backwards ? s + 1 : have - 1 - s) * r.scaleOut);
+                for (int o = 0; o < kOwn; o++) {
+                    const int y = (wave * kOwn + o) * 16 + quad * 4;
+                    if (r.outWide && !r.outFloat) {
+                        if (y + 4 <= r.dimC) *reinterpret_cast<vec<T, 4>*>(static_cast<T*>(r.out.data) + row + y) = fromFloat<T, 4>(acc[o][tb]);
+                        continue;
+                    }
 #pragma unroll
-                    for (int m = 0; m < kTilesA; m++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            memory[o][m][i] += (float)sB[s * S::kStrideA + m * 16 + quad * 4 + i] * c;
-                }
-                continue;
-            }
-#pragma unroll
-            for (int sb = 0; sb < kBlocks; sb++) {
-                f32x4 c = toFloat<T, 4>(columns(sC, S::kStrideC, sb, (wave * kOwn + o) * 16 + col));
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int s = sb * 16 + quad * 4 + j;
-                    const bool leaves = s < have && episode(s) == (r.backwards ? 0 : all);
-                    c[j] = leaves ? c[j] * (power(r.backwards ? s + 1 : have - 1 - s) * r.scaleOut) : 0.0f;
-                }
-                vec<typename L::type, 4> terms[L::kOut];
-                split<typename L::type, L::kOut>(c, terms);
-#pragma unroll
-                for (int m = 0; m < kTilesA; m++) {
-                    const auto b = __builtin_convertvector(columns(sB, S::kStrideA, sb, m * 16 + col), vec<typename L::type, 4>);
-#pragma unroll
-                    for (int i = 0; i < L::kOut; i++) memory[o][m] = mma(b, terms[i], memory[o][m]);
+                    for (int i = 0; i < 4; i++) {
+                        if (y + i >= r.dimC) continue;
+                        if (r.outFloat) static_cast<float*>(r.out.data)[row + y + i] = acc[o][tb][i];
+                        else static_cast<T*>(r.out.data)[row + y + i] = (T)acc[o][tb][i];
+                    }
                 }
             }
         }
     }
 
-    const int64_t size = (int64_t)r.dimA * r.dimC, unitState = batch * pass.heads + head;
     float* to = nullptr;
     bool swapped = false;
     if (kStates) {
-        to = r.parts + (segment * pass.batch * pass.heads + unitState) * size;
-        if (threadIdx.x == 0) r.factors[segment * pass.batch * pass.heads + unitState] = factor;
+        to = r.parts + partState * size;
+        if (threadIdx.x == 0) r.factors[partState] = factor;
     } else if (pass.segments == 1 && r.last) {
         to = r.last + unitState * size;
         swapped = r.lastSwapped != 0;
     }
-    if (to) {
-#pragma unroll
-        for (int o = 0; o < kOwn; o++)
-#pragma unroll
-            for (int m = 0; m < kTilesA; m++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int x = m * 16 + quad * 4 + i, y = (wave * kOwn + o) * 16 + col;
-                    if (x < r.dimA && y < r.dimC)
-                        to[swapped ? (int64_t)y * r.dimA + x : (int64_t)x * r.dimC + y] = memory[o][m][i];
-                }
-    }
+    if (to) eachMemory(swapped, [&](float x, int at, bool in) {
+        if (in) to[at] = x;
+        return x;
+    });
 }
 
 template <typename T, int kA, int kCd, bool kStates>
@@ -354,9 +465,10 @@ void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_
 {
     // float32 rows of 128 leave room for chunks of 32 steps
     constexpr int kSteps = sizeof(T) == 4 && (kA > 64 || kCd > 64) ? 32 : 64;
-    const int64_t units = pass.batch * pass.heads * pass.segments;
+    const int64_t groups = pass.batch * pass.segments;
+    const int64_t blocks = (pass.dealGroups ? (groups + 7) / 8 * pass.heads : (groups * pass.heads + 7) / 8) * 8 * roles;
     attentionKernel<T, kA, kCd, kSteps, kStates>
-        <<<dim3((unsigned)units, (unsigned)roles), Shape<T, kA, kCd, kSteps>::kThreads, 0, stream>>>(pass, firstRole);
+        <<<dim3((unsigned)blocks), Shape<T, kA, kCd, kSteps>::kThreads, 0, stream>>>(pass, firstRole, roles);
 }
 
 template <typename T, int kA, bool kStates>
