@@ -165,12 +165,10 @@ int grainOf(const Rows& r, int type, int64_t batch, int64_t steps, int heads)
     return (int)(bits & (~bits + 1));
 }
 
-// The same for rows of `dim` elements that are read: 2 where a chunk's rows do
-// not lie within the 32-bit offsets of a buffer descriptor.
+// The same for rows of `dim` elements that are read.
 int readGrain(const Rows& r, int type, int64_t batch, int64_t steps, int heads, int dim)
 {
     const int size = elementBytes(type);
-    if (r.step < 0 || r.step >= ((int64_t)1 << 31) / (64 * size) - 128) return size == 4 ? 0 : 2;
     const int grain = grainOf(r, type, batch, steps, heads), width = dim * size & -(dim * size);
     return grain < width ? grain : width;
 }

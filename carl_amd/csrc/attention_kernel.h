@@ -102,7 +102,7 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static constexpr int kPieceA = kA * (int)sizeof(T) / 16, kPieceC = kC_ * (int)sizeof(T) / 16;   // 16-byte pieces of a row
     static constexpr int kLoadsA = kSteps * kPieceA / kThreads, kLoadsC = kSteps * kPieceC / kThreads;
     // waves of a SIMD that the registers leave room for
-    static constexpr int kResident = kA * kC_ <= 64 * 64 ? (sizeof(T) == 2 ? 3 : 2) : kA * kC_ <= 64 * 128 && sizeof(T) == 2 ? 2 : 1;
+    static constexpr int kResident = kA * kC_ <= 64 * 128 && sizeof(T) == 2 || kA * kC_ <= 64 * 64 ? 2 : 1;
     static_assert(kSteps * kPieceA % kThreads == 0 && kSteps * kPieceC % kThreads == 0, "whole loads");
 };
 
@@ -158,18 +158,13 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
 
     const int64_t size = (int64_t)r.dimA * r.dimC, unitState = batch * pass.heads + head;
     const int64_t partState = segment * pass.batch * pass.heads + unitState;
-    // a lane's elements of the memory: rows 16 m + 4 quad + i, column 16 (wave's tile) + col
+    // A lane's elements of the memory: rows 16 m + 4 quad + i, column 16 (wave's
+    // tile) + col.  Through a descriptor, past whose end lies what the padding
+    // would hold: read as zero, written nowhere.
     f32x4 memory[kOwn][kTilesA];
-    const auto eachMemory = [&](bool swapped, auto visit) {
-#pragma unroll
-        for (int o = 0; o < kOwn; o++)
-#pragma unroll
-            for (int m = 0; m < kTilesA; m++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int x = m * 16 + quad * 4 + i, y = (wave * kOwn + o) * 16 + col;
-                    memory[o][m][i] = visit(memory[o][m][i], swapped ? y * r.dimA + x : x * r.dimC + y, x < r.dimA && y < r.dimC);
-                }
+    const auto memoryAt = [&](bool swapped, int o, int m, int i) {
+        const int x = m * 16 + quad * 4 + i, y = (wave * kOwn + o) * 16 + col;
+        return x < r.dimA && y < r.dimC ? (swapped ? y * r.dimA + x : x * r.dimC + y) * 4 : (int)0x80000000u;
     };
     {
         const float* from = nullptr;
@@ -181,28 +176,40 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 swapped = r.firstSwapped != 0;
             }
         }
-        if (from) eachMemory(swapped, [&](float, int at, bool in) { return in ? from[at] : 0.0f; });
-        else eachMemory(false, [&](float, int, bool) { return 0.0f; });
+        const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, from ? (int)size * 4 : 0, 0x00027000);
+#pragma unroll
+        for (int o = 0; o < kOwn; o++)
+#pragma unroll
+            for (int m = 0; m < kTilesA; m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    memory[o][m][i] = from ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(d, memoryAt(swapped, o, m, i), 0, 0)) : 0.0f;
     }
 
     // Chunks follow time in the pass's direction, and so do the rows of a chunk
     // in LDS: what comes first is in row 0.
     const auto chunkStart = [&](int n) { return begin + (int64_t)(backwards ? chunks - 1 - n : n) * kSteps; };
 
-    // Rows on the way to LDS: 16-byte pieces through a descriptor that gives
-    // zeros past the chunk's rows.  Pieces need addresses of 4 bytes; rows of
-    // other addresses are copied element by element when they are due.
+    // Rows on the way to LDS, in 16-byte pieces.  Past the chunk's last row that
+    // row is read again, and cleared when it is put down.  Pieces need addresses
+    // of 4 bytes, and are read word by word where a row ends within one; rows
+    // of other addresses are copied element by element when they are due.
     uint4 nextA[kStates ? 1 : S::kLoadsA], nextB[S::kLoadsA], nextC[S::kLoadsC];
     const auto fetchRows = [&](auto& next, const T* rows, int64_t step, int64_t t0, int pieces, int dim) {
-        const int have = (int)(end - t0 < kSteps ? end - t0 : kSteps), stepBytes = (int)step * (int)sizeof(T);
-        const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(rows + t0 * step), 0,
-                                                           (have - 1) * stepBytes + dim * (int)sizeof(T), 0x00027000);
+        const int have = (int)(end - t0 < kSteps ? end - t0 : kSteps);
         const int row = threadIdx.x / pieces, at = threadIdx.x % pieces * kE, rowsAtOnce = kThreads / pieces;
+        const char* base = reinterpret_cast<const char*>(rows + t0 * step + (at < dim ? at : 0));
+        const bool whole = dim % kE == 0;
+        const int words = at < dim ? (dim - at) * (int)sizeof(T) / 4 : 0;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            const int mine = row + i * rowsAtOnce, t = backwards ? have - 1 - mine : mine;
-            const int offset = mine < have && at < dim ? t * stepBytes + at * (int)sizeof(T) : (int)0x80000000u;
-            next[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
+            const int mine = row + i * rowsAtOnce, within = mine < have ? mine : have - 1;
+            const char* from = base + (backwards ? have - 1 - within : within) * (step * (int64_t)sizeof(T));
+            if (whole) next[i] = *reinterpret_cast<const uint4*>(from);
+            else {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(from);
+                next[i] = make_uint4(w[0], w[words > 1 ? 1 : 0], w[words > 2 ? 2 : 0], w[words > 3 ? 3 : 0]);
+            }
         }
     };
     const auto fetch = [&](int n) {
@@ -226,17 +233,17 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             }
             return;
         }
-        // words of the piece past the row's end hold what follows it
-        const int words = (dim - at) * (int)sizeof(T) / 4;
+        const int words = at < dim ? (dim - at) * (int)sizeof(T) / 4 : 0;
+        const bool whole = have == kSteps && pieces * kE == dim;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            if (dim % kE) {
-                next[i].y = words > 1 ? next[i].y : 0;
-                next[i].z = words > 2 ? next[i].z : 0;
-                next[i].w = words > 3 ? next[i].w : 0;
+            uint4 x = next[i];
+            if (!whole) {
+                const int left = threadIdx.x / pieces + i * (kThreads / pieces) < have ? words : 0;
+                x = make_uint4(left > 0 ? x.x : 0, left > 1 ? x.y : 0, left > 2 ? x.z : 0, left > 3 ? x.w : 0);
             }
-            *reinterpret_cast<uint4*>(to + i * (kThreads / pieces) * stride) = next[i];
-            if (look) odd |= nonFinite<T>(next[i]);
+            *reinterpret_cast<uint4*>(to + i * (kThreads / pieces) * stride) = x;
+            if (look) odd |= nonFinite<T>(x);
         }
     };
 
@@ -422,16 +429,19 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         }
 
         if constexpr (!kStates) {
+            const int64_t row0 = batch * r.out.batch + (t0 + (backwards ? have - 1 : 0)) * r.out.step + head * r.out.head;
+            const int64_t ahead = backwards ? -r.out.step : r.out.step;
+            const bool quick = r.outWide && !r.outFloat && r.dimC % 4 == 0;
 #pragma unroll
             for (int tb = 0; tb < kBlocks; tb++) {
                 const int t = tb * 16 + col;
                 if (t >= have) continue;
-                const int64_t row = batch * r.out.batch + (t0 + (backwards ? have - 1 - t : t)) * r.out.step + head * r.out.head;
+                const int64_t row = row0 + t * ahead;
 #pragma unroll
                 for (int o = 0; o < kOwn; o++) {
                     const int y = (wave * kOwn + o) * 16 + quad * 4;
-                    if (r.outWide && !r.outFloat) {
-                        if (y + 4 <= r.dimC) *reinterpret_cast<vec<T, 4>*>(static_cast<T*>(r.out.data) + row + y) = fromFloat<T, 4>(acc[o][tb]);
+                    if (quick) {
+                        if (y < r.dimC) *reinterpret_cast<vec<T, 4>*>(static_cast<T*>(r.out.data) + row + y) = fromFloat<T, 4>(acc[o][tb]);
                         continue;
                     }
 #pragma unroll
@@ -454,10 +464,15 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         to = r.last + unitState * size;
         swapped = r.lastSwapped != 0;
     }
-    if (to) eachMemory(swapped, [&](float x, int at, bool in) {
-        if (in) to[at] = x;
-        return x;
-    });
+    if (!to) return;
+    const auto d = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)size * 4, 0x00027000);
+#pragma unroll
+    for (int o = 0; o < kOwn; o++)
+#pragma unroll
+        for (int m = 0; m < kTilesA; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(memory[o][m][i]), d, memoryAt(swapped, o, m, i), 0, 0);
 }
 
 template <typename T, int kA, int kCd, bool kStates>
