@@ -43,7 +43,8 @@ struct Role {
     Rows a, b, c, out;
     int32_t aHeads, bHeads, cHeads;         // query heads that share a row of each
     int32_t aGrain, bGrain, cGrain;         // bytes that its rows' addresses and widths are multiples of: 16, 8, 4 or 2
-    int32_t outWide;                        // out's rows take stores of four elements
+                                            // (0 where a chunk's rows do not lie within 32 bits)
+    int32_t outWide;                        // out's rows take stores of four elements, and are whole ones
     int32_t outFloat;                       // out is float32 whatever the rows' type
     int32_t dimA, dimC;
     int32_t backwards;

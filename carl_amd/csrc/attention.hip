@@ -165,10 +165,12 @@ int grainOf(const Rows& r, int type, int64_t batch, int64_t steps, int heads)
     return (int)(bits & (~bits + 1));
 }
 
-// The same for rows of `dim` elements that are read.
+// The same for rows of `dim` elements that are read; 0 where 64 of them do not
+// lie within 32 bits.
 int readGrain(const Rows& r, int type, int64_t batch, int64_t steps, int heads, int dim)
 {
     const int size = elementBytes(type);
+    if (r.step < 0 || 63 * r.step * size + dim * size > 0xffffff00ll) return 0;
     const int grain = grainOf(r, type, batch, steps, heads), width = dim * size & -(dim * size);
     return grain < width ? grain : width;
 }
@@ -274,7 +276,7 @@ Role roleOf(const carl_attention& a, const carl_rows& x, bool xShared, const car
     r.aGrain = readGrain(r.a, a.type, a.batch, a.steps, xShared ? a.kv_heads : a.heads, dimA);
     r.bGrain = readGrain(r.b, a.type, a.batch, a.steps, yShared ? a.kv_heads : a.heads, dimA);
     r.cGrain = readGrain(r.c, a.type, a.batch, a.steps, zShared ? a.kv_heads : a.heads, dimC);
-    r.outWide = grainOf(out, a.type, a.batch, a.steps, a.heads) >= 4 * elementBytes(a.type);
+    r.outWide = dimC % 4 == 0 && grainOf(out, a.type, a.batch, a.steps, a.heads) >= 4 * elementBytes(a.type);
     r.dimA = dimA;
     r.dimC = dimC;
     r.scaleP = a.scale;
@@ -370,7 +372,6 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
         r->scaleOut = a->scale;
         r->first = a->d_final_state;
         r->outFloat = grouped;
-        if (grouped) r->outWide = a->key_dim % 4 == 0 && a->value_dim % 4 == 0;
     }
     dk.firstSwapped = 1;
     dv.last = a->d_initial_state;

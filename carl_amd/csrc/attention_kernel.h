@@ -2,6 +2,7 @@
 #pragma once
 
 #include "attention.h"
+#include "lds.h"
 #include "status.h"
 
 namespace carl {
@@ -25,22 +26,48 @@ __device__ inline f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn
 
 template <typename V> __device__ inline auto both(V a, V b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// From column `at` on: of rows 4 quad .. 4 quad + 3 of a 16-row block of LDS,
-// the lane's column at + lane%16.
-__device__ inline f32x4 columns(const float* rows, int stride, int at, int col, int quad)
-{
-    f32x4 x;
+// A tile of rows in LDS: rows of kPieces 16-byte pieces, each row's permuted by
+// its number so that the reads below meet all banks.
+template <typename T, int kWidth> struct Tile {
+    static constexpr int kBytes = kWidth * (int)sizeof(T), kPieces = kBytes / 16, kE = 16 / (int)sizeof(T);
+
+    static __device__ inline int permuted(int row, int piece)
+    {
+        if constexpr (sizeof(T) == 4) return piece ^ (((row & 3) | (row >> 2 & 3) << 2) & (kPieces - 1));
+        else if constexpr (kPieces == 4) return piece ^ (row >> 2 & 1) << 1;
+        else return piece ^ ((row & 3) << 1 | (row >> 2 & 1));
+    }
+    static __device__ inline int at(int row, int element)
+    {
+        return row * kBytes + permuted(row, element / kE) * 16 + element % kE * (int)sizeof(T);
+    }
+    static __device__ inline float element(const char* tile, int row, int i) { return (float)*reinterpret_cast<const T*>(tile + at(row, i)); }
+
+    // Row lane%16 of a 16-row block, elements 16 k + 4 quad + j; `lane` is
+    // at(lane%16, 4 quad), and the block's rows come before `tile`.
+    static __device__ inline vec<T, 4> row(const char* tile, int lane, int k)
+    {
+        return *reinterpret_cast<const vec<T, 4>*>(tile + (lane ^ k * 16 * (int)sizeof(T)));
+    }
+
+    // Column 16 m + lane%16 of rows 4 quad + j of a 16-row block; `lane` from columnLane().
+    static __device__ inline int columnLane(int col, int quad)
+    {
+        return sizeof(T) == 4 ? at(quad * 4, col) : at(quad * 4 + (col >> 2), (col & 3) * 4);
+    }
+    static __device__ inline vec<T, 4> column(const char* tile, int lane, int m)
+    {
+        if constexpr (sizeof(T) == 4) {
+            f32x4 x;
 #pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = rows[(quad * 4 + j) * stride + at + col];
-    return x;
-}
-typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
-template <typename T> __device__ inline vec<T, 4> columns(const T* rows, int stride, int at, int col, int quad)
-{
-    // transposes 4 rows x 16 columns held by 16 lanes
-    return __builtin_bit_cast(vec<T, 4>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (LdsI16x4*)(rows + (quad * 4 + (col >> 2)) * stride + at + (col & 3) * 4)));
-}
+            for (int j = 0; j < 4; j++)
+                x[j] = *reinterpret_cast<const float*>(tile + ((lane ^ m * 64 ^ j * 16) + j * kBytes));
+            return x;
+        } else      // transposes 4 rows x 16 columns held by 16 lanes
+            return __builtin_bit_cast(vec<T, 4>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) i16x4*)(tile + (lane ^ m * 32))));
+    }
+};
 
 // How products with float32 factors run (the memory read by a, what enters it
 // from b): bfloat16 as terms of that type, two and three of them; float16
@@ -97,13 +124,13 @@ template <typename T> __device__ inline uint32_t nonFinite(uint4 x)
 template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static constexpr int kWaves = kC_ / 16 < 4 ? kC_ / 16 : 4;
     static constexpr int kThreads = kWaves * 64;
-    static constexpr int kPad = 16 / sizeof(T);
-    static constexpr int kStrideA = kA + kPad, kStrideC = kC_ + kPad, kStrideP = kSteps + kPad;
-    static constexpr int kPieceA = kA * (int)sizeof(T) / 16, kPieceC = kC_ * (int)sizeof(T) / 16;   // 16-byte pieces of a row
-    static constexpr int kLoadsA = kSteps * kPieceA / kThreads, kLoadsC = kSteps * kPieceC / kThreads;
-    // waves of a SIMD that the registers leave room for
-    static constexpr int kResident = kA * kC_ <= 64 * 128 && sizeof(T) == 2 || kA * kC_ <= 64 * 64 ? 2 : 1;
-    static_assert(kSteps * kPieceA % kThreads == 0 && kSteps * kPieceC % kThreads == 0, "whole loads");
+    static constexpr int kStrideP = kSteps + 16 / (int)sizeof(T);
+    static constexpr int kTileA = kSteps * Tile<T, kA>::kBytes, kTileC = kSteps * Tile<T, kC_>::kBytes;
+    static constexpr int kLoadsA = kTileA / 16 / kThreads, kLoadsC = kTileC / 16 / kThreads;
+    static_assert(kTileA % (16 * kThreads) == 0 && kTileC % (16 * kThreads) == 0, "whole copies");
+    // workgroups that LDS holds at once, as waves of a SIMD that the registers leave room for
+    static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(T);
+    static constexpr int kResident = kLds * 4 <= 160 * 1024 ? 4 : kLds * 3 <= 160 * 1024 ? 3 : 2;
 };
 
 template <typename T, int kA, int kCd, int kSteps, bool kStates>
@@ -115,13 +142,14 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     constexpr int kBlocks = kSteps / 16;             // 16-step blocks of a chunk, an even number
     constexpr int kTilesA = kA / 16;                 // of the memory's rows, an even number
     constexpr int kOwn = kCd / 16 / kWaves;          // column tiles of a wave
-    constexpr int kE = 16 / sizeof(T);
     using L = Long<T>;
     using LT = typename L::type;
+    using TileA = Tile<T, kA>;
+    using TileC = Tile<T, kCd>;
 
-    __shared__ __align__(16) T sA[kStates ? 1 : kSteps * S::kStrideA];
-    __shared__ __align__(16) T sB[kSteps * S::kStrideA];
-    __shared__ __align__(16) T sC[kSteps * S::kStrideC];
+    __shared__ __align__(1024) char sA[kStates ? 16 : S::kTileA];
+    __shared__ __align__(1024) char sB[S::kTileA];
+    __shared__ __align__(1024) char sC[S::kTileC];
     __shared__ __align__(16) T sP[kStates ? 1 : kSteps * S::kStrideP];
 
     // Blocks are dealt to the 8 dies in turn.  The roles of one unit and the
@@ -144,6 +172,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool backwards = r.backwards != 0;
+    const int dimA = r.dimA, dimC = r.dimC, inShift = r.inShift;
 
     const int64_t begin = segment * pass.segmentSteps;
     const int64_t end = begin + pass.segmentSteps < pass.steps ? begin + pass.segmentSteps : pass.steps;
@@ -151,20 +180,38 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     const T* aRows = static_cast<const T*>(r.a.data) + batch * r.a.batch + head / r.aHeads * r.a.head;
     const T* bRows = static_cast<const T*>(r.b.data) + batch * r.b.batch + head / r.bHeads * r.b.head;
     const T* cRows = static_cast<const T*>(r.c.data) + batch * r.c.batch + head / r.cHeads * r.c.head;
+    const int64_t aStep = r.a.step, bStep = r.b.step, cStep = r.c.step;
+    const int aGrain = r.aGrain, bGrain = r.bGrain, cGrain = r.cGrain;
 
     // -infinity times zero steps is no NaN
     const float decay2 = fmaxf(pass.logDecay[head] * 1.44269504088896341f, -1e30f);
-    const auto power = [&](int steps) { return __builtin_amdgcn_exp2f(decay2 * (float)steps); };
+    const auto power = [&](float steps) { return __builtin_amdgcn_exp2f(decay2 * steps); };
 
-    const int64_t size = (int64_t)r.dimA * r.dimC, unitState = batch * pass.heads + head;
-    const int64_t partState = segment * pass.batch * pass.heads + unitState;
     // A lane's elements of the memory: rows 16 m + 4 quad + i, column 16 (wave's
     // tile) + col.  Through a descriptor, past whose end lies what the padding
     // would hold: read as zero, written nowhere.
+    const int64_t unitState = batch * pass.heads + head, partState = segment * pass.batch * pass.heads + unitState;
+    const int size = dimA * dimC;
     f32x4 memory[kOwn][kTilesA];
-    const auto memoryAt = [&](bool swapped, int o, int m, int i) {
-        const int x = m * 16 + quad * 4 + i, y = (wave * kOwn + o) * 16 + col;
-        return x < r.dimA && y < r.dimC ? (swapped ? y * r.dimA + x : x * r.dimC + y) * 4 : (int)0x80000000u;
+    const auto eachMemory = [&](bool swapped, auto one, auto four) {
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const int y = (wave * kOwn + o) * 16 + col;
+            const int base = y >= dimC ? kOutside : swapped ? (y * dimA + quad * 4) * 4 : (quad * 4 * dimC + y) * 4;
+            if (swapped && dimA % 4 == 0) {
+#pragma unroll
+                for (int m = 0; m < kTilesA; m++)
+                    four(o, m, y >= dimC || m * 16 + quad * 4 >= dimA ? kOutside : base + m * 64);
+                continue;
+            }
+#pragma unroll
+            for (int m = 0; m < kTilesA; m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int at = base + (m * 16 + i) * (swapped ? 4 : dimC * 4);
+                    one(o, m, i, y >= dimC || m * 16 + quad * 4 + i >= dimA ? kOutside : at);
+                }
+        }
     };
     {
         const float* from = nullptr;
@@ -176,87 +223,84 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 swapped = r.firstSwapped != 0;
             }
         }
-        const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, from ? (int)size * 4 : 0, 0x00027000);
+        if (from) {
+            const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, size * 4, 0x00027000);
+            eachMemory(
+                swapped,
+                [&](int o, int m, int i, int at) { memory[o][m][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(d, at, 0, 0)); },
+                [&](int o, int m, int at) { memory[o][m] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at, 0, 0)); });
+        } else {
 #pragma unroll
-        for (int o = 0; o < kOwn; o++)
+            for (int o = 0; o < kOwn; o++)
 #pragma unroll
-            for (int m = 0; m < kTilesA; m++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    memory[o][m][i] = from ? __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(d, memoryAt(swapped, o, m, i), 0, 0)) : 0.0f;
+                for (int m = 0; m < kTilesA; m++) memory[o][m] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+        }
     }
 
     // Chunks follow time in the pass's direction, and so do the rows of a chunk
     // in LDS: what comes first is in row 0.
     const auto chunkStart = [&](int n) { return begin + (int64_t)(backwards ? chunks - 1 - n : n) * kSteps; };
 
-    // Rows on the way to LDS, in 16-byte pieces.  Past the chunk's last row that
-    // row is read again, and cleared when it is put down.  Pieces need addresses
-    // of 4 bytes, and are read word by word where a row ends within one; rows
-    // of other addresses are copied element by element when they are due.
-    uint4 nextA[kStates ? 1 : S::kLoadsA], nextB[S::kLoadsA], nextC[S::kLoadsC];
-    const auto fetchRows = [&](auto& next, const T* rows, int64_t step, int64_t t0, int pieces, int dim) {
-        const int have = (int)(end - t0 < kSteps ? end - t0 : kSteps);
-        const int row = threadIdx.x / pieces, at = threadIdx.x % pieces * kE, rowsAtOnce = kThreads / pieces;
-        const char* base = reinterpret_cast<const char*>(rows + t0 * step + (at < dim ? at : 0));
-        const bool whole = dim % kE == 0;
-        const int words = at < dim ? (dim - at) * (int)sizeof(T) / 4 : 0;
+    // A chunk's rows to LDS, by copies that a descriptor ends at the chunk's
+    // last row (rows and pieces past it arrive as zeros).  They need addresses
+    // of 4 bytes within 32 bits of the chunk's first; others go element by
+    // element.  waitRows() waits for this thread's pieces, clears what lies
+    // past the row's end in the last one, and looks for non-finite values.
+    const auto copyRows = [&](auto tile, int loads, int thread, char* lds, const T* rows, int64_t step, int64_t t0, int have, int dim, int grain) {
+        using Rows = decltype(tile);
+        constexpr int kPieces = Rows::kPieces;
+        const T* base = rows + t0 * step;
+        if (grain >= 4) {
+            const int stepBytes = (int)step * (int)sizeof(T);
+            const i32x4 from = descriptor(base, (have - 1) * stepBytes + dim * (int)sizeof(T));
+            const uint32_t to = ldsAddress(lds) + wave * 1024;
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            const int mine = row + i * rowsAtOnce, within = mine < have ? mine : have - 1;
-            const char* from = base + (backwards ? have - 1 - within : within) * (step * (int64_t)sizeof(T));
-            if (whole) next[i] = *reinterpret_cast<const uint4*>(from);
-            else {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(from);
-                next[i] = make_uint4(w[0], w[words > 1 ? 1 : 0], w[words > 2 ? 2 : 0], w[words > 3 ? 3 : 0]);
-            }
-        }
-    };
-    const auto fetch = [&](int n) {
-        const int64_t t0 = chunkStart(n);
-        if constexpr (!kStates)
-            if (r.aGrain >= 4) fetchRows(nextA, aRows, r.a.step, t0, S::kPieceA, r.dimA);
-        if (r.bGrain >= 4) fetchRows(nextB, bRows, r.b.step, t0, S::kPieceA, r.dimA);
-        if (r.cGrain >= 4) fetchRows(nextC, cRows, r.c.step, t0, S::kPieceC, r.dimC);
-    };
-    uint32_t odd = 0;         // carry bits of non-finite values in this chunk's b and c
-    const auto put = [&](auto& next, T* lds, int stride, int pieces, bool look, int grain, int dim, const T* rows, int64_t step,
-                         int64_t t0, int have) {
-        const int at = threadIdx.x % pieces * kE;
-        T* to = lds + threadIdx.x / pieces * stride + at;
-        if (grain < 4) {
-            for (int row = threadIdx.x / pieces; row < kSteps; row += kThreads / pieces) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (row < have) x = loadPiece<T>(rows + (t0 + (backwards ? have - 1 - row : row)) * step + at, dim - at);
-                *reinterpret_cast<uint4*>(lds + row * stride + at) = x;
-                if (look) odd |= nonFinite<T>(x);
+            for (int i = 0; i < loads; i++) {
+                const int piece = i * kThreads + thread, row = piece / kPieces, at = Rows::permuted(row, piece % kPieces) * 16;
+                const int t = backwards ? have - 1 - row : row;
+                copyToLds(from, row < have && at < dim * (int)sizeof(T) ? t * stepBytes + at : kOutside, 0, to + i * kThreads * 16);
             }
             return;
         }
-        const int words = at < dim ? (dim - at) * (int)sizeof(T) / 4 : 0;
-        const bool whole = have == kSteps && pieces * kE == dim;
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(next) / sizeof(next[0])); i++) {
-            uint4 x = next[i];
-            if (!whole) {
-                const int left = threadIdx.x / pieces + i * (kThreads / pieces) < have ? words : 0;
-                x = make_uint4(left > 0 ? x.x : 0, left > 1 ? x.y : 0, left > 2 ? x.z : 0, left > 3 ? x.w : 0);
-            }
-            *reinterpret_cast<uint4*>(to + i * (kThreads / pieces) * stride) = x;
-            if (look) odd |= nonFinite<T>(x);
+#pragma unroll 1
+        for (int i = 0; i < loads; i++) {
+            const int piece = i * kThreads + thread, row = piece / kPieces, at = Rows::permuted(row, piece % kPieces) * Rows::kE;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < have) x = loadPiece<T>(base + (backwards ? have - 1 - row : row) * step + at, dim - at);
+            *reinterpret_cast<uint4*>(lds + piece * 16) = x;
         }
+    };
+    const auto waitRows = [&](auto tile, int loads, int thread, char* lds, int dim, bool look) {
+        using Rows = decltype(tile);
+        uint32_t odd = 0;         // carry bits of non-finite values
+        if (dim % Rows::kE) {
+#pragma unroll 1
+            for (int i = 0; i < loads; i++) {
+                const int piece = i * kThreads + thread;
+                if (Rows::permuted(piece / Rows::kPieces, piece % Rows::kPieces) != dim / Rows::kE) continue;
+                for (int e = dim % Rows::kE; e < Rows::kE; e++) reinterpret_cast<T*>(lds + piece * 16)[e] = T(0);
+            }
+        }
+        if (look)
+#pragma unroll
+            for (int i = 0; i < loads; i++) odd |= nonFinite<T>(*reinterpret_cast<const uint4*>(lds + (i * kThreads + thread) * 16));
+        return odd;
     };
 
     float factor = 1.0f;      // of the memory over the whole segment
-    if (chunks > 0) fetch(0);
+#pragma unroll 1
     for (int n = 0; n < chunks; n++) {
         const int64_t t0 = chunkStart(n);
         const int have = end - t0 < kSteps ? (int)(end - t0) : kSteps;
+        // Opaque, so that the many addresses made of it are made again for each
+        // chunk and not kept (spilled) from before the loop.
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        const int lane = thread & 63, col = lane & 15, quad = lane >> 4;
         __syncthreads();
-        odd = 0;
-        if constexpr (!kStates) put(nextA, sA, S::kStrideA, S::kPieceA, false, r.aGrain, r.dimA, aRows, r.a.step, t0, have);
-        put(nextB, sB, S::kStrideA, S::kPieceA, true, r.bGrain, r.dimA, bRows, r.b.step, t0, have);
-        put(nextC, sC, S::kStrideC, S::kPieceC, true, r.cGrain, r.dimC, cRows, r.c.step, t0, have);
+        if constexpr (!kStates) copyRows(TileA{}, S::kLoadsA, thread, sA, aRows, aStep, t0, have, dimA, aGrain);
+        copyRows(TileA{}, S::kLoadsA, thread, sB, bRows, bStep, t0, have, dimA, bGrain);
+        copyRows(TileC{}, S::kLoadsC, thread, sC, cRows, cStep, t0, have, dimC, cGrain);
         // Bit t of `cuts`: row t sees nothing of the rows before it.  Forwards
         // that is where an episode starts; backwards, where the step after
         // (row t - 1) does, and a start at the chunk's first step, its last
@@ -272,8 +316,19 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         // A weight of zero takes a finite row out of a product, but not an
         // infinity or a NaN: a chunk whose b or c hold one is summed step by
         // step, leaving out the steps that are not seen.
+        waitCopies();
+        uint32_t odd = 0;
+        if constexpr (!kStates) waitRows(TileA{}, S::kLoadsA, thread, sA, dimA, false);
+        odd |= waitRows(TileA{}, S::kLoadsA, thread, sB, dimA, true);
+        odd |= waitRows(TileC{}, S::kLoadsC, thread, sC, dimC, true);
         const bool careful = __syncthreads_or((odd & Exponent<T>::kCarry) != 0) != 0;
-        if (n + 1 < chunks) fetch(n + 1);
+
+        // where a lane's fragments lie: a row's neighbouring elements, columns of
+        // rows, and the results' rows of P
+        const int rowLane = TileA::at(col, quad * 4);
+        const int columnLaneA = TileA::columnLane(col, quad), columnLaneC = TileC::columnLane(col, quad);
+        T* const pLane = sP + col * S::kStrideP + quad * 4;
+        const float quadSteps = (float)(quad * 4), colSteps = (float)col;
 
         // Rows [low(t), t] are what row t sees of the chunk.
         const auto low = [&](int t) {
@@ -288,28 +343,29 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         if constexpr (!kStates) {
             // P^T, tile by tile: rows s, column t
             for (int tb = wave; tb < kBlocks; tb += kWaves) {
-                const int t = tb * 16 + col, from = low(t);
+                const int t = tb * 16 + col, from = cuts ? low(t) : 0;
                 vec<T, 4> a[kTilesA];
 #pragma unroll
-                for (int k = 0; k < kTilesA; k++) a[k] = *reinterpret_cast<const vec<T, 4>*>(sA + t * S::kStrideA + k * 16 + quad * 4);
-                for (int sb = 0; sb <= tb; sb++) {
+                for (int k = 0; k < kTilesA; k++) a[k] = TileA::row(sA + tb * 16 * TileA::kBytes, rowLane, k);
+                float gap = (float)(tb * 16) + colSteps - quadSteps;      // to the tile's first row of the lane
+#pragma unroll 1
+                for (int sb = 0; sb <= tb; sb++, gap -= 16.0f) {
                     f32x4 p = { 0.f, 0.f, 0.f, 0.f };
-                    const T* rows = sB + (sb * 16 + col) * S::kStrideA + quad * 4;
+                    const char* rows = sB + sb * 16 * TileA::kBytes;
 #pragma unroll
                     for (int k = 0; k < kTilesA; k += 2)
-                        p = mma(both(*reinterpret_cast<const vec<T, 4>*>(rows + k * 16), *reinterpret_cast<const vec<T, 4>*>(rows + k * 16 + 16)),
-                                both(a[k], a[k + 1]), p);
+                        p = mma(both(TileA::row(rows, rowLane, k), TileA::row(rows, rowLane, k + 1)), both(a[k], a[k + 1]), p);
+                    const int s = sb * 16 + quad * 4;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int s = sb * 16 + quad * 4 + i;
-                        const float w = p[i] * (power(t - s) * r.scaleP);
-                        p[i] = s >= from && s <= t ? w : 0.0f;
+                        const float w = p[i] * (power(gap - (float)i) * r.scaleP);
+                        p[i] = s + i >= from && s + i <= t ? w : 0.0f;
                     }
-                    *reinterpret_cast<vec<T, 4>*>(sP + t * S::kStrideP + sb * 16 + quad * 4) = fromFloat<T, 4>(p);
+                    *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + sb * 16) = fromFloat<T, 4>(p);
                 }
                 // blocks of s are met in pairs below
                 if (tb % 2 == 0)
-                    *reinterpret_cast<vec<T, 4>*>(sP + t * S::kStrideP + (tb + 1) * 16 + quad * 4) = vec<T, 4>{ T(0), T(0), T(0), T(0) };
+                    *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + (tb + 1) * 16) = vec<T, 4>{ T(0), T(0), T(0), T(0) };
             }
             // what the carried memory gives
 #pragma unroll
@@ -326,20 +382,20 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 }
 #pragma unroll
                 for (int tb = 0; tb < kBlocks; tb++) {
-                    const T* rows = sA + (tb * 16 + col) * S::kStrideA + m * 16 + quad * 4;
-                    const auto a = both(__builtin_convertvector(*reinterpret_cast<const vec<T, 4>*>(rows), vec<LT, 4>),
-                                        __builtin_convertvector(*reinterpret_cast<const vec<T, 4>*>(rows + 16), vec<LT, 4>));
+                    const char* rows = sA + tb * 16 * TileA::kBytes;
+                    const auto a = both(__builtin_convertvector(TileA::row(rows, rowLane, m), vec<LT, 4>),
+                                        __builtin_convertvector(TileA::row(rows, rowLane, m + 1), vec<LT, 4>));
 #pragma unroll
                     for (int o = 0; o < kOwn; o++)
 #pragma unroll
                         for (int i = 0; i < L::kIn; i++) acc[o][tb] = mma(both(lo[o][i], hi[o][i]), a, acc[o][tb]);
                 }
             }
+            const int firstCut = cuts ? __builtin_ctzll(cuts) : 64;
 #pragma unroll
             for (int tb = 0; tb < kBlocks; tb++) {
-                const int t = tb * 16 + col;
-                const bool open = (cuts & (~0ull >> (63 - t))) == 0;
-                const float in = power(t + r.inShift) * r.scaleIn;
+                const bool open = tb * 16 + col < firstCut;
+                const float in = power(colSteps + (float)(tb * 16 + inShift)) * r.scaleIn;
                 // a closed row takes nothing from the memory, whatever that holds
 #pragma unroll
                 for (int o = 0; o < kOwn; o++) acc[o][tb] = open ? acc[o][tb] * in : f32x4{ 0.f, 0.f, 0.f, 0.f };
@@ -347,11 +403,13 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             __syncthreads();
         }
 
-        const float keep = closed ? 0.0f : power(have);
+        const float keep = closed ? 0.0f : power((float)have);
         factor *= keep;
         // what row s weighs in the memory after the chunk
-        const auto weightOut = [&](int s) {
-            return s >= leave && s < have ? power(have - 1 - s + 1 - r.inShift) * r.scaleOut : 0.0f;
+        const float rest = (float)(have - inShift) - quadSteps;
+        const auto weightOut = [&](int block, int j) {
+            const int s = block * 16 + quad * 4 + j;
+            return s >= leave && s < have ? power(rest - (float)(block * 16 + j)) * r.scaleOut : 0.0f;
         };
         if (!careful) {
             vec<T, 4> c[kOwn][kBlocks];
@@ -359,13 +417,13 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             for (int o = 0; o < kOwn; o++)
 #pragma unroll
                 for (int sb = 0; sb < kBlocks; sb++)
-                    c[o][sb] = columns(sC + sb * 16 * S::kStrideC, S::kStrideC, (wave * kOwn + o) * 16, col, quad);
+                    c[o][sb] = TileC::column(sC + sb * 16 * TileC::kBytes, columnLaneC, wave * kOwn + o);
             if constexpr (!kStates) {
 #pragma unroll
                 for (int tb = 0; tb < kBlocks; tb++)
 #pragma unroll
                     for (int sb = 0; sb <= tb; sb += 2) {
-                        const T* row = sP + (tb * 16 + col) * S::kStrideP + sb * 16 + quad * 4;
+                        const T* row = pLane + tb * 16 * S::kStrideP + sb * 16;
                         const auto p = both(*reinterpret_cast<const vec<T, 4>*>(row), *reinterpret_cast<const vec<T, 4>*>(row + 16));
 #pragma unroll
                         for (int o = 0; o < kOwn; o++) acc[o][tb] = mma(both(c[o][sb], c[o][sb + 1]), p, acc[o][tb]);
@@ -380,8 +438,8 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 f32x4 w[2];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    w[0][j] = weightOut(sb * 16 + quad * 4 + j);
-                    w[1][j] = weightOut(sb * 16 + 16 + quad * 4 + j);
+                    w[0][j] = weightOut(sb, j);
+                    w[1][j] = weightOut(sb + 1, j);
                 }
                 vec<LT, 4> lo[kOwn][L::kOut], hi[kOwn][L::kOut];
 #pragma unroll
@@ -389,11 +447,11 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                     split<LT, L::kOut>(toFloat<T, 4>(c[o][sb]) * w[0], lo[o]);
                     split<LT, L::kOut>(toFloat<T, 4>(c[o][sb + 1]) * w[1], hi[o]);
                 }
-                const T* rows = sB + sb * 16 * S::kStrideA;
+                const char* rows = sB + sb * 16 * TileA::kBytes;
 #pragma unroll
                 for (int m = 0; m < kTilesA; m++) {
-                    const auto b = both(__builtin_convertvector(columns(rows, S::kStrideA, m * 16, col, quad), vec<LT, 4>),
-                                        __builtin_convertvector(columns(rows + 16 * S::kStrideA, S::kStrideA, m * 16, col, quad), vec<LT, 4>));
+                    const auto b = both(__builtin_convertvector(TileA::column(rows, columnLaneA, m), vec<LT, 4>),
+                                        __builtin_convertvector(TileA::column(rows + 16 * TileA::kBytes, columnLaneA, m), vec<LT, 4>));
 #pragma unroll
                     for (int o = 0; o < kOwn; o++)
 #pragma unroll
@@ -412,44 +470,50 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                         for (int s = low(t); s <= t && s < have; s++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                acc[o][tb][i] += (float)sP[t * S::kStrideP + s] * (float)sC[s * S::kStrideC + tile + quad * 4 + i];
+                                acc[o][tb][i] += (float)sP[t * S::kStrideP + s] * TileC::element(sC, s, tile + quad * 4 + i);
                     }
                 }
 #pragma unroll
                 for (int m = 0; m < kTilesA; m++) memory[o][m] = closed ? f32x4{ 0.f, 0.f, 0.f, 0.f } : memory[o][m] * keep;
 #pragma unroll 1
                 for (int s = leave; s < have; s++) {
-                    const float x = (float)sC[s * S::kStrideC + tile + col] * weightOut(s);
+                    const float x = TileC::element(sC, s, tile + col) * (power((float)(have - inShift - s)) * r.scaleOut);
 #pragma unroll
                     for (int m = 0; m < kTilesA; m++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) memory[o][m][i] += (float)sB[s * S::kStrideA + m * 16 + quad * 4 + i] * x;
+                        for (int i = 0; i < 4; i++) memory[o][m][i] += TileA::element(sB, s, m * 16 + quad * 4 + i) * x;
                 }
             }
         }
 
         if constexpr (!kStates) {
-            const int64_t row0 = batch * r.out.batch + (t0 + (backwards ? have - 1 : 0)) * r.out.step + head * r.out.head;
-            const int64_t ahead = backwards ? -r.out.step : r.out.step;
-            const bool quick = r.outWide && !r.outFloat && r.dimC % 4 == 0;
+            const int64_t outStep = r.out.step;
+            const int64_t row0 = batch * r.out.batch + (t0 + (backwards ? have - 1 : 0)) * outStep + head * r.out.head;
+            if (r.outWide && !r.outFloat) {
+                const int y = wave * kOwn * 16 + quad * 4;
+                T* const lane0 = static_cast<T*>(r.out.data) + row0 + (backwards ? -(int64_t)col : (int64_t)col) * outStep + y;
+                const int64_t ahead = (backwards ? -16 : 16) * outStep;
 #pragma unroll
-            for (int tb = 0; tb < kBlocks; tb++) {
-                const int t = tb * 16 + col;
-                if (t >= have) continue;
-                const int64_t row = row0 + t * ahead;
+                for (int tb = 0; tb < kBlocks; tb++)
 #pragma unroll
-                for (int o = 0; o < kOwn; o++) {
-                    const int y = (wave * kOwn + o) * 16 + quad * 4;
-                    if (quick) {
-                        if (y < r.dimC) *reinterpret_cast<vec<T, 4>*>(static_cast<T*>(r.out.data) + row + y) = fromFloat<T, 4>(acc[o][tb]);
-                        continue;
-                    }
+                    for (int o = 0; o < kOwn; o++)
+                        if (tb * 16 + col < have && y + o * 16 < dimC)
+                            *reinterpret_cast<vec<T, 4>*>(lane0 + tb * ahead + o * 16) = fromFloat<T, 4>(acc[o][tb]);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (y + i >= r.dimC) continue;
-                        if (r.outFloat) static_cast<float*>(r.out.data)[row + y + i] = acc[o][tb][i];
-                        else static_cast<T*>(r.out.data)[row + y + i] = (T)acc[o][tb][i];
-                    }
+                for (int tb = 0; tb < kBlocks; tb++) {
+                    const int t = tb * 16 + col;
+                    if (t >= have) continue;
+                    const int64_t row = row0 + (backwards ? -t : t) * outStep;
+#pragma unroll
+                    for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int y = (wave * kOwn + o) * 16 + quad * 4 + i;
+                            if (y >= dimC) continue;
+                            if (r.outFloat) static_cast<float*>(r.out.data)[row + y] = acc[o][tb][i];
+                            else static_cast<T*>(r.out.data)[row + y] = (T)acc[o][tb][i];
+                        }
                 }
             }
         }
@@ -465,14 +529,13 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         swapped = r.lastSwapped != 0;
     }
     if (!to) return;
-    const auto d = __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)size * 4, 0x00027000);
-#pragma unroll
-    for (int o = 0; o < kOwn; o++)
-#pragma unroll
-        for (int m = 0; m < kTilesA; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(memory[o][m][i]), d, memoryAt(swapped, o, m, i), 0, 0);
+    const auto d = __builtin_amdgcn_make_buffer_rsrc(to, 0, size * 4, 0x00027000);
+    eachMemory(
+        swapped,
+        [&](int o, int m, int i, int at) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(memory[o][m][i]), d, at, 0, 0); },
+        [&](int o, int m, int at) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vec<uint32_t, 4>, memory[o][m]), d, at, 0, 0);
+        });
 }
 
 template <typename T, int kA, int kCd, bool kStates>

@@ -4,15 +4,14 @@
 #include <algorithm>
 
 #include "ffn.h"
+#include "lds.h"
 #include "status.h"
 
 namespace carl {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
 
 constexpr int kRowBytes = 128;      // of a panel's row in a stage
-constexpr int kOutside = (int)0x80000000u;
 
 // A lane's 16 bytes of either operand: row or column lane%16 of a 16x16 tile,
 // 16/size neighbouring steps of the sum from 16/size times lane/16 on.
@@ -38,34 +37,6 @@ template <> struct Mma<f16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 };
-
-// A buffer descriptor of `records` bytes from `base`; accesses that do not lie
-// in them read zeros.
-__device__ inline i32x4 descriptor(const void* base, int records)
-{
-    const uint64_t at = reinterpret_cast<uint64_t>(base);
-    return i32x4{ __builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff),
-                  __builtin_amdgcn_readfirstlane(records), 0x00027000 };
-}
-
-// 16 bytes a lane from memory to 16 x lane bytes past `lds` (the same for all
-// lanes of the wave), without a register.  Written out because the compiler
-// would have every later LDS read wait for it; the copies of a stage are
-// waited for once, by waitCopies() before the barrier that hands it over.
-__device__ inline void copyToLds(i32x4 from, int offset, int more, uint32_t lds)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :
-                 : "s"(lds), "v"(offset), "s"(from), "s"(more)
-                 : "memory");      // m0 is never live across statements of these kernels
-}
-
-__device__ inline void waitCopies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-__device__ inline uint32_t ldsAddress(const void* p)
-{
-    return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p);
-}
 
 // ---- product -------------------------------------------------------------------
 
