@@ -97,10 +97,11 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN>::kThrea
         const int have = (int)(p.rows - row0 < rows ? p.rows - row0 : rows), strideBytes = (int)(p.stride * sizeof(T));
         const i32x4 from = descriptor(base, have * strideBytes);
         const int c = ((threadIdx.x & 7) ^ (weights ? swizzle<kRun>(copyRow) : copyRow & 7)) * 16;
-        const int at = c < (p.width - k0) * (int)sizeof(T) ? copyRow * strideBytes + c : kOutside;
+        const bool within = c < (p.width - k0) * (int)sizeof(T);
+        const int at = copyRow * strideBytes + c;
 #pragma unroll
         for (int i = 0; i < rows * 8 / kThreads; i++)
-            copyToLds(from, at + i * (kThreads / 8) * strideBytes, k0 * (int)sizeof(T), lds + (i * kThreads + wave * 64) * 16);
+            copyToLds(from, within ? at + i * (kThreads / 8) * strideBytes : kOutside, k0 * (int)sizeof(T), lds + (i * kThreads + wave * 64) * 16);
     };
     const int steps0 = (args.a[0].width + kStep - 1) / kStep;
     const int steps = kKind == kProductPlain && args.terms == 2 ? steps0 + (args.a[1].width + kStep - 1) / kStep : steps0;
