@@ -11,7 +11,6 @@ namespace carl {
 
 typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
 
-constexpr int kRowBytes = 128;      // of a panel's row in a stage
 
 // A lane's 16 bytes of either operand: row or column lane%16 of a 16x16 tile,
 // 16/size neighbouring steps of the sum from 16/size times lane/16 on.
@@ -40,26 +39,29 @@ template <> struct Mma<f16> {
 
 // ---- product -------------------------------------------------------------------
 
-// Rows of a weights' panel sit in LDS with their eight 16-byte pieces permuted
-// by this, so that eight lanes reading one piece of eight rows meet all banks.
-// kRun: neighbouring columns of the result that a lane holds (below).
-template <int kRun> __device__ inline int swizzle(int row) { return (row & 3) | (row / kRun & 1) << 2; }
+// Rows of a panel sit in LDS with their 16-byte pieces permuted, so that eight
+// lanes reading one piece of eight rows meet all banks: by the lane's number
+// mod 8 that reads the row, halved where a row has but four pieces.  That is
+// the row mod 8 in a's panels, and in b's, whose rows the lanes read in runs
+// of kRun (below), what bReader() says.
+template <int kRun> __device__ inline int bReader(int row) { return (row & 3) | (row / kRun & 1) << 2; }
 
-template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN> struct ProductShape {
+// kRowBytes: of a panel's row in a stage, 128 or 64.
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN, int kRowBytes> struct ProductShape {
     static constexpr int kNA = kKind == kProductGrad ? 2 : 1, kNB = kKind == kProductPlain ? 1 : kKind == kProductGate ? 2 : 3;
     static constexpr int kThreads = kWM * kWN * 64;
     static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
     static constexpr int kRun = 4 * kTN;
     static constexpr int kStage = (kNA * kBM + kNB * kBN) * kRowBytes;
-    static_assert((kBM * 8) % kThreads == 0 && (kBN * 8) % kThreads == 0, "whole loads");
-    // copies: a thread's rows differ by multiples of 8 and of 2 kRun
-    static_assert(kThreads / 8 % 8 == 0 && kThreads / 8 % (2 * kRun) == 0, "one permutation for a thread's pieces");
+    static constexpr int kPieces = kRowBytes / 16, kCopyRows = kThreads / kPieces;      // rows that the workgroup copies at once
+    static_assert(kBM % kCopyRows == 0 && kBN % kCopyRows == 0, "whole copies");
+    static_assert(kCopyRows % 8 == 0 && kCopyRows % (2 * kRun) == 0, "one permutation for a thread's pieces");
 };
 
-template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN>::kThreads)) void productKernel(const ProductArgs args)
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN, int kRowBytes>
+__global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowBytes>::kThreads)) void productKernel(const ProductArgs args)
 {
-    using S = ProductShape<T, kKind, kBM, kBN, kWM, kWN>;
+    using S = ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowBytes>;
     constexpr int kE = 16 / sizeof(T), kStep = kRowBytes / sizeof(T);
     constexpr int kNA = S::kNA, kNB = S::kNB, kTM = S::kTM, kTN = S::kTN, kRun = S::kRun, kThreads = S::kThreads;
 
@@ -91,17 +93,18 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN>::kThrea
 
     // Rows past the operand's end lie past the descriptor's, pieces past a
     // row's width are sent there: both arrive as zeros.
-    const int copyRow = threadIdx.x >> 3;
+    const int copyRow = threadIdx.x / S::kPieces;
     const auto copyPanel = [&](const Panel& p, int64_t row0, int rows, int k0, uint32_t lds, bool weights) {
         const T* base = static_cast<const T*>(p.data) + row0 * p.stride;
         const int have = (int)(p.rows - row0 < rows ? p.rows - row0 : rows), strideBytes = (int)(p.stride * sizeof(T));
         const i32x4 from = descriptor(base, have * strideBytes);
-        const int c = ((threadIdx.x & 7) ^ (weights ? swizzle<kRun>(copyRow) : copyRow & 7)) * 16;
+        const int reader = weights ? bReader<kRun>(copyRow) : copyRow & 7;
+        const int c = (threadIdx.x % S::kPieces ^ (kRowBytes == 128 ? reader : reader >> 1)) * 16;
         const bool within = c < (p.width - k0) * (int)sizeof(T);
         const int at = copyRow * strideBytes + c;
 #pragma unroll
-        for (int i = 0; i < rows * 8 / kThreads; i++)
-            copyToLds(from, within ? at + i * (kThreads / 8) * strideBytes : kOutside, k0 * (int)sizeof(T), lds + (i * kThreads + wave * 64) * 16);
+        for (int i = 0; i < rows / S::kCopyRows; i++)
+            copyToLds(from, within ? at + i * S::kCopyRows * strideBytes : kOutside, k0 * (int)sizeof(T), lds + (i * kThreads + wave * 64) * 16);
     };
     const int steps0 = (args.a[0].width + kStep - 1) / kStep;
     const int steps = kKind == kProductPlain && args.terms == 2 ? steps0 + (args.a[1].width + kStep - 1) / kStep : steps0;
@@ -120,12 +123,11 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN>::kThrea
     // Tile i of a's: rows lane%16 of the tile.  Tile j of b's: row lane%16 is
     // column (lane%16)/4 kRun + 4 j + lane%4 of the wave's, so that a lane's
     // rows 4 quad + i of all tiles are kRun neighbouring columns of the result.
-    // swizzle() of that row is lane%8 as well.
-    const int aRow = (wm * kTM * 16 + col) * kRowBytes, piece0 = (quad ^ (col & 7)) * 16;
+    const int aRow = (wm * kTM * 16 + col) * kRowBytes, piece0 = (quad ^ (kRowBytes == 128 ? col & 7 : (col & 7) >> 1)) * 16;
     const int bRow = (wn * kTN * 16 + (col >> 2) * kRun + (col & 3)) * kRowBytes;
     const auto multiply = [&](const char* lds) {
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
+        for (int half = 0; half < kRowBytes / 64; half++) {
             __builtin_amdgcn_sched_barrier(0);      // the fragments of one half at a time
             const char* aAt = lds + (aRow + (piece0 ^ half * 64));
             const char* bAt = lds + kNA * kBM * kRowBytes + (bRow + (piece0 ^ half * 64));
@@ -224,7 +226,7 @@ template <typename T> __device__ inline int outerSwizzle(int row)
 template <typename T, int kB, int kWM, int kWN>
 __global__ __launch_bounds__(kWM* kWN * 64) void outerKernel(const OuterArgs args)
 {
-    constexpr int kThreads = kWM * kWN * 64, kE = 16 / sizeof(T), kStep = kRowBytes / sizeof(T);
+    constexpr int kThreads = kWM * kWN * 64, kE = 16 / sizeof(T), kStep = 128 / sizeof(T);
     constexpr int kTM = kB / kWM / 16, kTN = kB / kWN / 16;
     constexpr int kPieces = kB / kE, kPanel = kStep * kB * (int)sizeof(T);
     constexpr int kStage = 2 * kPanel;
@@ -374,28 +376,44 @@ template <typename T> __global__ __launch_bounds__(256) void packKernel(const Pa
 
 // ---- launches ------------------------------------------------------------------
 
-template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN>
+template <typename T, int kKind, int kBM, int kBN, int kWM, int kWN, int kRowBytes>
 int launchProductShape(const ProductArgs& args, hipStream_t stream)
 {
     const int64_t tilesM = (args.m + kBM - 1) / kBM, tilesN = (args.n + kBN - 1) / kBN;
     const int64_t blocks = (tilesM + 7) / 8 * 8 * tilesN;
-    productKernel<T, kKind, kBM, kBN, kWM, kWN><<<dim3((unsigned)blocks), kWM * kWN * 64, 0, stream>>>(args);
+    productKernel<T, kKind, kBM, kBN, kWM, kWN, kRowBytes><<<dim3((unsigned)blocks), kWM * kWN * 64, 0, stream>>>(args);
     return launched("feed-forward product");
 }
 
+// Tiles of the three products of many rows, each the best of those tried at
+// 262,144 rows of 512 by 1,408 in bfloat16 (at 62,000 of 256 by 684 in float32):
+//   gate   128 x 128 of both, 64-byte rows      908 us, 833 TFLOP/s (256 x 128, 128-byte rows: 1,005 us;
+//          float32 128 x 64                     382 us, 114 TFLOP/s (256 x 128: 434 us)
+//   grad   128 x 128 of the three               1,790 us, 634 TFLOP/s (2 x 2 waves: 2,149 us; 128 x 64: 1,939 us;
+//          float32 128 x 64, 64-byte rows       578 us, 113 TFLOP/s (128 x 128: 662 us)
+//   plain  256 x 256, sum over 2,816            687 us, 1,101 TFLOP/s (over 1,408, 128 x 128: 471 us, 256 x 256: 375 us;
+//          float32 128 x 128, 64-byte rows      188 us, 115 TFLOP/s (256 x 256: 194 us)
+// float32 is bound by its matrix instructions (154 TFLOP/s in a large library
+// product) and by the last tiles; 16-bit gate and grad by their tiles' short
+// sums (512), under which the copies' latency and the stores of h, dg and du
+// (2.2 GB: 440 us of grad's time) do not disappear.
 template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream)
 {
     // Few rows run in tiles small enough that the columns alone give work to
     // many compute units.
     const bool small = args.m <= 4096;
+    constexpr bool wide = sizeof(T) == 4;
     if (kind == kProductGate)
-        return small ? launchProductShape<T, kProductGate, 64, 32, 2, 2>(args, stream)
-                     : launchProductShape<T, kProductGate, 256, 128, 2, 4>(args, stream);
+        return small ? launchProductShape<T, kProductGate, 64, 32, 2, 2, 128>(args, stream)
+             : wide  ? launchProductShape<T, kProductGate, 128, 64, 2, 2, 64>(args, stream)
+                     : launchProductShape<T, kProductGate, 128, 128, 2, 4, 64>(args, stream);
     if (kind == kProductGrad)
-        return small ? launchProductShape<T, kProductGrad, 64, 32, 2, 2>(args, stream)
-                     : launchProductShape<T, kProductGrad, 128, 128, 2, 2>(args, stream);
-    return small ? launchProductShape<T, kProductPlain, 64, 32, 2, 2>(args, stream)
-                 : launchProductShape<T, kProductPlain, 256, 256, 2, 4>(args, stream);
+        return small ? launchProductShape<T, kProductGrad, 64, 32, 2, 2, 128>(args, stream)
+             : wide  ? launchProductShape<T, kProductGrad, 128, 64, 2, 2, 64>(args, stream)
+                     : launchProductShape<T, kProductGrad, 128, 128, 2, 4, 128>(args, stream);
+    return small ? launchProductShape<T, kProductPlain, 64, 32, 2, 2, 128>(args, stream)
+         : wide  ? launchProductShape<T, kProductPlain, 128, 128, 2, 2, 64>(args, stream)
+                 : launchProductShape<T, kProductPlain, 256, 256, 2, 4, 128>(args, stream);
 }
 
 template <typename T> int launchOuter(const OuterArgs& args, int tile, hipStream_t stream)
