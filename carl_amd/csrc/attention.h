@@ -56,6 +56,7 @@ struct Role {
     int32_t firstSwapped, lastSwapped;      // stored as [dimC, dimA]
     float* parts;                           // split passes: [segment, batch, head, dimA, dimC] and a factor for each
     float* factors;
+    int32_t partsSwapped;                   // read from the parts of a role whose memory is this one's transpose
 };
 
 struct Pass {

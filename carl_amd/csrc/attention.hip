@@ -178,19 +178,25 @@ int readGrain(const Rows& r, int type, int64_t batch, int64_t steps, int heads, 
 Rows rowsOf(const carl_rows& r) { return Rows{ r.data, r.batch, r.step, r.head }; }
 
 // How a sequence is split.  One workgroup walks a whole sequence of one head
-// where batch times heads fill the GPU; with fewer, segments of at least 256
-// steps, so that about 1,024 workgroups run: they need the memories before
-// each segment, which a first launch sums up (reading keys and values once more).
+// where those and the pass's directions fill the GPU; with fewer, segments of
+// at least 256 steps, as many as run at once (two workgroups a compute unit
+// with the widest rows, three or four with others).  They need the memories
+// before each segment, which a first launch sums up (reading keys and values
+// once more) and a second joins.  6 sequences of 4,603 steps, 8 heads of 128:
+// 18 segments both ways, as 1,024 workgroups would have them, 855 us with
+// gradients.
 struct Split {
     int segments;
     int64_t steps;
 };
 
-Split splitOf(const carl_attention& a)
+Split splitOf(const carl_attention& a, bool backward)
 {
-    const int64_t units = a.batch * a.heads;
-    if (units >= 512 || a.steps <= 256) return { 1, std::max<int64_t>(a.steps, 1) };
-    int64_t segments = std::min<int64_t>((1024 + units - 1) / units, (a.steps + 255) / 256);
+    const int64_t units = a.batch * a.heads * (backward ? 3 : 1);
+    const int widest = std::max(a.key_dim, a.value_dim), other = std::min(a.key_dim, a.value_dim);
+    const int64_t resident = 256 * (other > 64 ? 2 : widest > 64 ? 3 : a.type == CARL_OP_F32 ? 2 : 4);
+    if (units > resident / 2 || a.steps <= 256) return { 1, std::max<int64_t>(a.steps, 1) };
+    int64_t segments = std::min<int64_t>(resident / units, (a.steps + 255) / 256);
     int64_t steps = (a.steps + segments - 1) / segments;
     steps = (steps + 63) / 64 * 64;
     segments = (a.steps + steps - 1) / steps;
@@ -208,7 +214,7 @@ struct Layout {
 Layout layoutOf(const carl_attention& a, bool backward)
 {
     Layout l;
-    const Split s = splitOf(a);
+    const Split s = splitOf(a, backward);
     if (s.segments > 1) {
         const int64_t units = a.batch * a.heads * s.segments;
         l.parts = rounded(units * a.key_dim * a.value_dim * 4);
@@ -218,14 +224,15 @@ Layout layoutOf(const carl_attention& a, bool backward)
         l.keyRows = rounded(a.batch * a.steps * a.heads * a.key_dim * 4);
         l.valueRows = rounded(a.batch * a.steps * a.heads * a.value_dim * 4);
     }
-    l.total = (l.parts + l.factors) * (backward ? 3 : 1) + l.keyRows + l.valueRows;
+    l.total = (l.parts + l.factors) * (backward ? 2 : 1) + l.keyRows + l.valueRows;
     return l;
 }
 
-int run(const carl_attention& a, Pass& pass, int roles, hipStream_t stream)
+// `summed`: the first roles, which have parts of their own.
+int run(const carl_attention& a, Pass& pass, int summed, int roles, hipStream_t stream)
 {
     // roles next to each other with the same widths share a launch
-    const auto launch = [&](bool states) {
+    const auto launch = [&](bool states, int roles) {
         for (int i = 0; i < roles;) {
             int n = 1;
             while (i + n < roles && pass.role[i + n].dimA == pass.role[i].dimA && pass.role[i + n].dimC == pass.role[i].dimC) n++;
@@ -235,18 +242,18 @@ int run(const carl_attention& a, Pass& pass, int roles, hipStream_t stream)
         return (int)CARL_OK;
     };
     if (pass.segments > 1) {
-        if (int rc = launch(true)) return rc;
+        if (int rc = launch(true, summed)) return rc;
         const int blocks = (int)std::min<int64_t>(16, ((int64_t)a.key_dim * a.value_dim + 255) / 256);
-        joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)roles), 256, 0, stream>>>(pass);
+        joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)summed), 256, 0, stream>>>(pass);
         if (int rc = launched("joining of segments")) return rc;
     }
-    return launch(false);
+    return launch(false, roles);
 }
 
-Pass passOf(const carl_attention& a)
+Pass passOf(const carl_attention& a, bool backward)
 {
     Pass pass{};
-    const Split s = splitOf(a);
+    const Split s = splitOf(a, backward);
     pass.batch = a.batch;
     pass.steps = a.steps;
     pass.heads = a.heads;
@@ -324,7 +331,7 @@ int carl_linear_attention(const carl_attention* a, void* stream)
     if (empty(*a)) return passMemory(a->initial_state, a->final_state, memory, (hipStream_t)stream);
     const Layout l = layoutOf(*a, false);
     if (l.total > 0 && !a->workspace) return fail(CARL_ERR_VALUE, "null workspace");
-    Pass pass = passOf(*a);
+    Pass pass = passOf(*a, false);
     Role& r = pass.role[0];
     r = roleOf(*a, a->q, false, a->k, true, a->v, true, rowsOf(a->out), a->key_dim, a->value_dim);
     r.scaleIn = a->scale;
@@ -333,7 +340,7 @@ int carl_linear_attention(const carl_attention* a, void* stream)
     r.last = a->final_state;
     r.parts = static_cast<float*>(a->workspace);
     r.factors = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + l.parts);
-    return run(*a, pass, 1, (hipStream_t)stream);
+    return run(*a, pass, 1, 1, (hipStream_t)stream);
 }
 
 int carl_linear_attention_backward(const carl_attention* a, void* stream)
@@ -343,13 +350,13 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
     if (empty(*a)) return passMemory(a->d_final_state, a->d_initial_state, memory, (hipStream_t)stream);
     const Layout l = layoutOf(*a, true);
     if (l.total > 0 && !a->workspace) return fail(CARL_ERR_VALUE, "null workspace");
-    Pass pass = passOf(*a);
+    Pass pass = passOf(*a, true);
     char* work = static_cast<char*>(a->workspace);
     const bool grouped = a->heads != a->kv_heads;
     const auto queryRows = [&](int64_t at, int dim) {
         return Rows{ work + at, a->steps * a->heads * dim, (int64_t)a->heads * dim, dim };
     };
-    const int64_t rowsAt = (l.parts + l.factors) * 3;
+    const int64_t rowsAt = (l.parts + l.factors) * 2;
     const Rows keyRows = grouped ? queryRows(rowsAt, a->key_dim) : rowsOf(a->d_k);
     const Rows valueRows = grouped ? queryRows(rowsAt + l.keyRows, a->value_dim) : rowsOf(a->d_v);
 
@@ -361,9 +368,9 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
     dq.first = a->initial_state;
     dq.firstSwapped = 1;
     // dk and dv: time backwards, the gradient of the memory instead of it
-    Role& dk = pass.role[1];
+    Role& dk = pass.role[2];
     dk = roleOf(*a, a->v, true, a->d_out, false, a->q, false, keyRows, a->value_dim, a->key_dim);
-    Role& dv = pass.role[2];
+    Role& dv = pass.role[1];
     dv = roleOf(*a, a->k, true, a->q, false, a->d_out, false, valueRows, a->key_dim, a->value_dim);
     for (Role* r : { &dk, &dv }) {
         r->backwards = 1;
@@ -375,11 +382,13 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
     }
     dk.firstSwapped = 1;
     dv.last = a->d_initial_state;
-    for (int i = 0; i < 3; i++) {
+    for (int i = 0; i < 2; i++) {
         pass.role[i].parts = reinterpret_cast<float*>(work + (l.parts + l.factors) * i);
         pass.role[i].factors = reinterpret_cast<float*>(work + (l.parts + l.factors) * i + l.parts);
     }
-    if (int rc = run(*a, pass, 3, (hipStream_t)stream)) return rc;
+    dk.parts = dv.parts;        // dk's memory is dv's, transposed
+    dk.partsSwapped = 1;
+    if (int rc = run(*a, pass, 2, 3, (hipStream_t)stream)) return rc;
     if (!grouped) return CARL_OK;
     const auto sum = [&](const Rows& from, const carl_rows& to, int dim) {
         const int64_t n = a->batch * a->steps * a->kv_heads * dim;

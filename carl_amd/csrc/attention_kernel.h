@@ -126,8 +126,8 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kStrideP = kSteps + 16 / (int)sizeof(T);
     static constexpr int kTileA = kSteps * Tile<T, kA>::kBytes, kTileC = kSteps * Tile<T, kC_>::kBytes;
-    static constexpr int kLoadsA = kTileA / 16 / kThreads, kLoadsC = kTileC / 16 / kThreads;
-    static_assert(kTileA % (16 * kThreads) == 0 && kTileC % (16 * kThreads) == 0, "whole copies");
+    static constexpr int kLoadsA = (kTileA / 16 + kThreads - 1) / kThreads, kLoadsC = (kTileC / 16 + kThreads - 1) / kThreads;
+    static_assert(kTileA % 1024 == 0 && kTileC % 1024 == 0, "whole copies of a wave");
     // workgroups that LDS holds at once, as waves of a SIMD that the registers leave room for
     static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(T);
     static constexpr int kResident = kLds * 4 <= 160 * 1024 ? 4 : kLds * 3 <= 160 * 1024 ? 3 : 2;
@@ -217,8 +217,10 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         const float* from = nullptr;
         bool swapped = false;
         if (!kStates) {
-            if (pass.segments > 1) from = r.parts + partState * size;
-            else if (r.first) {
+            if (pass.segments > 1) {
+                from = r.parts + partState * size;
+                swapped = r.partsSwapped != 0;
+            } else if (r.first) {
                 from = r.first + unitState * size;
                 swapped = r.firstSwapped != 0;
             }
@@ -256,6 +258,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             const uint32_t to = ldsAddress(lds) + wave * 1024;
 #pragma unroll
             for (int i = 0; i < loads; i++) {
+                if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
                 const int piece = i * kThreads + thread, row = piece / kPieces, at = Rows::permuted(row, piece % kPieces) * 16;
                 const int t = backwards ? have - 1 - row : row;
                 copyToLds(from, row < have && at < dim * (int)sizeof(T) ? t * stepBytes + at : kOutside, 0, to + i * kThreads * 16);
@@ -264,6 +267,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         }
 #pragma unroll 1
         for (int i = 0; i < loads; i++) {
+            if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
             const int piece = i * kThreads + thread, row = piece / kPieces, at = Rows::permuted(row, piece % kPieces) * Rows::kE;
             uint4 x = make_uint4(0, 0, 0, 0);
             if (row < have) x = loadPiece<T>(base + (backwards ? have - 1 - row : row) * step + at, dim - at);
@@ -276,6 +280,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         if (dim % Rows::kE) {
 #pragma unroll 1
             for (int i = 0; i < loads; i++) {
+                if (i * kThreads + wave * 64 >= kSteps * Rows::kPieces) break;
                 const int piece = i * kThreads + thread;
                 if (Rows::permuted(piece / Rows::kPieces, piece % Rows::kPieces) != dim / Rows::kE) continue;
                 for (int e = dim % Rows::kE; e < Rows::kE; e++) reinterpret_cast<T*>(lds + piece * 16)[e] = T(0);
@@ -283,7 +288,10 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         }
         if (look)
 #pragma unroll
-            for (int i = 0; i < loads; i++) odd |= nonFinite<T>(*reinterpret_cast<const uint4*>(lds + (i * kThreads + thread) * 16));
+            for (int i = 0; i < loads; i++) {
+                if (i * kThreads + wave * 64 >= kSteps * Rows::kPieces) break;
+                odd |= nonFinite<T>(*reinterpret_cast<const uint4*>(lds + (i * kThreads + thread) * 16));
+            }
         return odd;
     };
 
@@ -538,15 +546,26 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         });
 }
 
-template <typename T, int kA, int kCd, bool kStates>
-void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_t stream)
+template <typename T, int kA, int kCd, int kSteps, bool kStates>
+void launchAttentionSteps(const Pass& pass, int firstRole, int roles, hipStream_t stream)
 {
-    // float32 rows of 128 leave room for chunks of 32 steps
-    constexpr int kSteps = sizeof(T) == 4 && (kA > 64 || kCd > 64) ? 32 : 64;
     const int64_t groups = pass.batch * pass.segments;
     const int64_t blocks = (pass.dealGroups ? (groups + 7) / 8 * pass.heads : (groups * pass.heads + 7) / 8) * 8 * roles;
     attentionKernel<T, kA, kCd, kSteps, kStates>
         <<<dim3((unsigned)blocks), Shape<T, kA, kCd, kSteps>::kThreads, 0, stream>>>(pass, firstRole, roles);
+}
+
+template <typename T, int kA, int kCd, bool kStates>
+void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_t stream)
+{
+    // Chunks of 64 steps; of 32 where no sequence is longer, and for float32
+    // rows of 128, of which LDS would hold but one workgroup's.
+    constexpr bool large = sizeof(T) == 4 && (kA > 64 || kCd > 64);
+    if constexpr (!kStates && !large) {
+        if (pass.segmentSteps > 32) launchAttentionSteps<T, kA, kCd, 64, kStates>(pass, firstRole, roles, stream);
+        else launchAttentionSteps<T, kA, kCd, 32, kStates>(pass, firstRole, roles, stream);
+    } else
+        launchAttentionSteps<T, kA, kCd, large ? 32 : 64, kStates>(pass, firstRole, roles, stream);
 }
 
 template <typename T, int kA, bool kStates>
