@@ -130,7 +130,8 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static_assert(kTileA % 1024 == 0 && kTileC % 1024 == 0, "whole copies of a wave");
     // workgroups that LDS holds at once, as waves of a SIMD that the registers leave room for
     static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(T);
-    static constexpr int kResident = kLds * 4 <= 160 * 1024 ? 4 : kLds * 3 <= 160 * 1024 ? 3 : 2;
+    static constexpr int kMost = kA * kC_ > 64 * 128 ? 2 : kA * kC_ > 64 * 64 ? 3 : 4;
+    static constexpr int kResident = kLds * 4 <= 160 * 1024 && kMost >= 4 ? 4 : kLds * 3 <= 160 * 1024 && kMost >= 3 ? 3 : 2;
 };
 
 template <typename T, int kA, int kCd, int kSteps, bool kStates>
@@ -560,7 +561,7 @@ void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_
 {
     // Chunks of 64 steps; of 32 where no sequence is longer, and for float32
     // rows of 128, of which LDS would hold but one workgroup's.
-    constexpr bool large = sizeof(T) == 4 && (kA > 64 || kCd > 64);
+    constexpr bool large = sizeof(T) == 4;
     if constexpr (!kStates && !large) {
         if (pass.segmentSteps > 32) launchAttentionSteps<T, kA, kCd, 64, kStates>(pass, firstRole, roles, stream);
         else launchAttentionSteps<T, kA, kCd, 32, kStates>(pass, firstRole, roles, stream);
