@@ -134,6 +134,12 @@ __device__ inline f32x4 decodeSecond(uint32_t codes, float scale)
 
 // The largest magnitude over the wave's block; NaN where any is not finite.
 // Bit patterns of magnitudes order as unsigned numbers, infinity and NaN last.
+template <int kPattern> __device__ inline uint32_t maxOver(uint32_t x)
+{
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kPattern, 0xf, 0xf, false);
+    return o > x ? o : x;
+}
+
 __device__ inline float blockScale(f32x4 x)
 {
     uint32_t most = 0;
@@ -141,18 +147,37 @@ __device__ inline float blockScale(f32x4 x)
         const uint32_t u = __float_as_uint(x[j]) & 0x7fffffffu;
         most = u > most ? u : most;
     }
-    for (int d = 32; d; d >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)most, d);
-        most = o > most ? o : most;
+    // within each row of 16 lanes, then over the four rows
+    most = maxOver<0xb1>(most);      // quad_perm: 1 0 3 2
+    most = maxOver<0x4e>(most);      // quad_perm: 2 3 0 1
+    most = maxOver<0x141>(most);     // row_half_mirror
+    most = maxOver<0x140>(most);     // row_mirror
+    uint32_t all = 0;
+    for (int r = 0; r < 64; r += 16) {
+        const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)most, r);
+        all = row > all ? row : all;
     }
-    return __uint_as_float(most >= 0x7f800000u ? 0x7fc00000u : most);
+    return __uint_as_float(all >= 0x7f800000u ? 0x7fc00000u : all);
 }
+
+// Codes are defined by divisions and square roots that are correctly rounded,
+// about 25 operations for a first and 40 for a second moment.  The quick ones
+// here are good to a unit in the last place each: together they move 127 (255)
+// times the root by less than 5e-5 (1e-4), so only a value that close to the
+// border between two codes needs the others.  Scales far from 1, whose
+// reciprocals would leave the normal numbers, always take them.
+__device__ inline bool plainScale(float scale) { return scale > 0x1p-100f && scale < 0x1p100f; }
+
+__device__ inline float byBorder(float y) { return fabsf(fabsf(y - rintf(y)) - 0.5f); }      // distance from half way
 
 __device__ inline uint32_t encodeFirst(f32x4 x, float scale)
 {
     uint32_t r = 0;
+    const float inverse = __builtin_amdgcn_rcpf(scale);
     for (int j = 0; j < 4; j++) {
-        const float c = rintf(127.0f * sqrtf(fabsf(x[j]) / scale));
+        float y = 127.0f * __builtin_amdgcn_sqrtf(fabsf(x[j]) * inverse);
+        if (!plainScale(scale) || byBorder(y) < 2e-4f) y = 127.0f * sqrtf(fabsf(x[j]) / scale);
+        const float c = rintf(y);
         const int code = scale > 0.0f ? (x[j] < 0.0f ? -(int)c : (int)c) : 0;
         r |= (uint32_t)(code & 0xff) << (8 * j);
     }
@@ -162,8 +187,11 @@ __device__ inline uint32_t encodeFirst(f32x4 x, float scale)
 __device__ inline uint32_t encodeSecond(f32x4 x, float scale)
 {
     uint32_t r = 0;
+    const float inverse = __builtin_amdgcn_rcpf(scale);
     for (int j = 0; j < 4; j++) {
-        const float c = fmaxf(rintf(255.0f * sqrtf(sqrtf(x[j] / scale))), 1.0f);
+        float y = 255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(x[j] * inverse));
+        if (!plainScale(scale) || byBorder(y) < 4e-4f) y = 255.0f * sqrtf(sqrtf(x[j] / scale));
+        const float c = fmaxf(rintf(y), 1.0f);
         const uint32_t code = x[j] > 0.0f && scale > 0.0f ? (uint32_t)c : 0u;
         r |= code << (8 * j);
     }

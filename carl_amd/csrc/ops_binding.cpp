@@ -33,20 +33,28 @@ void check(int rc)
 
 void* currentStream() { return c10::hip::getCurrentHIPStream(0).stream(); }
 
-void require(bool ok, const std::string& msg)
+// The message is made of its parts only where it is thrown.
+template <typename... Parts> std::string message(const Parts&... parts)
 {
-    if (!ok) throw py::value_error(msg);
+    std::string s;
+    (s.append(parts), ...);
+    return s;
 }
 
-void requireType(bool ok, const std::string& msg)
+template <typename... Parts> void require(bool ok, const Parts&... parts)
 {
-    if (!ok) throw py::type_error(msg);
+    if (!ok) throw py::value_error(message(parts...));
+}
+
+template <typename... Parts> void requireType(bool ok, const Parts&... parts)
+{
+    if (!ok) throw py::type_error(message(parts...));
 }
 
 void onDevice(const Tensor& t, const char* name)
 {
-    require(t.defined() && t.is_cuda() && t.get_device() == 0, std::string(name) + " must be on cuda:0");
-    require(t.layout() == at::kStrided, std::string(name) + " must be a dense tensor");
+    require(t.defined() && t.is_cuda() && t.get_device() == 0, name, " must be on cuda:0");
+    require(t.layout() == at::kStrided, name, " must be a dense tensor");
 }
 
 int elementType(const Tensor& t, const char* name)
@@ -55,7 +63,7 @@ int elementType(const Tensor& t, const char* name)
     case at::kFloat: return CARL_OP_F32;
     case at::kBFloat16: return CARL_OP_BF16;
     case at::kHalf: return CARL_OP_F16;
-    default: throw py::type_error(std::string(name) + " must have dtype float32, bfloat16 or float16");
+    default: throw py::type_error(message(name, " must have dtype float32, bfloat16 or float16"));
     }
 }
 
@@ -75,8 +83,8 @@ carl_attention attentionOf(const Tensor& q, const Tensor& k, const Tensor& v, co
     const char* lead = steps ? "[batch, steps, " : "[batch, ";
     for (const auto& [t, name] : { std::pair{ &q, "q" }, { &k, "k" }, { &v, "v" } }) {
         onDevice(*t, name);
-        require(t->dim() == dims, std::string(name) + " must have shape " + lead + "heads, width]");
-        require(t->stride(dims - 1) == 1 || t->size(dims - 1) <= 1, std::string(name) + " must be contiguous in its last dimension");
+        require(t->dim() == dims, name, " must have shape ", lead, "heads, width]");
+        require(t->stride(dims - 1) == 1 || t->size(dims - 1) <= 1, name, " must be contiguous in its last dimension");
         requireType(t->scalar_type() == q.scalar_type(), "q, k and v must have the same dtype");
     }
     carl_attention a{};
@@ -114,11 +122,11 @@ carl_attention attentionOf(const Tensor& q, const Tensor& k, const Tensor& v, co
     if (memory) {
         const char* name = steps ? "initial_state" : "state";
         onDevice(*memory, name);
-        requireType(memory->scalar_type() == at::kFloat, std::string(name) + " must have dtype float32");
+        requireType(memory->scalar_type() == at::kFloat, name, " must have dtype float32");
         require(memory->dim() == 4 && memory->size(0) == a.batch && memory->size(1) == a.heads
                     && memory->size(2) == a.key_dim && memory->size(3) == a.value_dim,
-                std::string(name) + " must have shape [batch, heads, key width, value width]");
-        require(memory->is_contiguous(), std::string(name) + " must be contiguous");
+                name, " must have shape [batch, heads, key width, value width]");
+        require(memory->is_contiguous(), name, " must be contiguous");
     }
     return a;
 }
@@ -307,17 +315,42 @@ Tensor gatedFfn(const Tensor& x, const Tensor& gate, const Tensor& up, const Ten
 
 // ------------------------------------------------------------------- AdamW
 
-void adamwStep(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& first,
-               const std::vector<Tensor>& second, const std::vector<Tensor>& firstScale,
-               const std::vector<Tensor>& secondScale, int64_t step, double lr, double beta1, double beta2, double eps,
-               double weightDecay, const OptTensor& gradScale)
+// A sequence of tensors, looked at in place: a step's six lists of a policy's
+// tensors would take longer to convert than the step (35 tensors: 20 us).
+class TensorList {
+    py::object held_;
+    std::vector<const Tensor*> items_;
+
+public:
+    TensorList(const py::object& sequence, const char* name)
+    {
+        if (sequence.is_none()) return;
+        held_ = py::reinterpret_steal<py::object>(PySequence_Fast(sequence.ptr(), "sequences of tensors expected"));
+        if (!held_) throw py::error_already_set();
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(held_.ptr());
+        items_.reserve(n);
+        for (Py_ssize_t i = 0; i < n; i++) {
+            PyObject* const item = PySequence_Fast_GET_ITEM(held_.ptr(), i);
+            requireType(THPVariable_Check(item), name, " must be tensors");
+            items_.push_back(&THPVariable_Unpack(item));
+        }
+    }
+    size_t size() const { return items_.size(); }
+    const Tensor& operator[](size_t i) const { return *items_[i]; }
+};
+
+void adamwStep(const py::object& paramList, const py::object& gradList, const py::object& firstList, const py::object& secondList,
+               const py::object& firstScaleList, const py::object& secondScaleList, int64_t step, double lr, double beta1,
+               double beta2, double eps, double weightDecay, const OptTensor& gradScale)
 {
+    const TensorList params(paramList, "params"), grads(gradList, "grads"), first(firstList, "exp_avg"),
+        second(secondList, "exp_avg_sq"), firstScale(firstScaleList, "exp_avg_scale"), secondScale(secondScaleList, "exp_avg_sq_scale");
     const size_t n = params.size();
     require(grads.size() == n && first.size() == n && second.size() == n,
             "params, grads, exp_avg and exp_avg_sq must have the same length");
     const bool eight = n > 0 && first[0].scalar_type() == at::kChar;
     if (eight) require(firstScale.size() == n && secondScale.size() == n, "8-bit moments need exp_avg_scale and exp_avg_sq_scale");
-    else require(firstScale.empty() && secondScale.empty(), "float32 moments have no scales");
+    else require(firstScale.size() == 0 && secondScale.size() == 0, "float32 moments have no scales");
     std::vector<carl_adamw_tensor> list(n);
     for (size_t i = 0; i < n; i++) {
         const Tensor &p = params[i], &g = grads[i], &m = first[i], &v = second[i];
@@ -354,8 +387,8 @@ void adamwStep(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
         h.grad_scale = gradScale->data_ptr<float>();
     }
     check(carl_adamw_step(list.data(), (int)n, &h, currentStream()));
-    for (const auto* tensors : { &params, &first, &second, &firstScale, &secondScale })
-        for (const Tensor& t : *tensors) t.unsafeGetTensorImpl()->bump_version();
+    for (const TensorList* tensors : { &params, &first, &second, &firstScale, &secondScale })
+        for (size_t i = 0; i < tensors->size(); i++) (*tensors)[i].unsafeGetTensorImpl()->bump_version();
 }
 
 int64_t momentBlocks(const Tensor& m) { return (m.numel() + CARL_ADAMW_BLOCK - 1) / CARL_ADAMW_BLOCK; }

@@ -36,8 +36,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     grad_scale      a float32 tensor of one value on the GPU, multiplied onto
                     every gradient (a clipping factor that never reaches the host)
     """
-    _ops.adamw_step(list(params), list(grads), list(exp_avg), list(exp_avg_sq), list(exp_avg_scale or ()),
-                    list(exp_avg_sq_scale or ()), step, lr, betas[0], betas[1], eps, weight_decay, grad_scale)
+    _ops.adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, betas[0], betas[1], eps,
+                    weight_decay, grad_scale)
 
 
 def decode_moments(exp_avg: torch.Tensor, exp_avg_scale: torch.Tensor, exp_avg_sq: torch.Tensor,
