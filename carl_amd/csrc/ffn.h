@@ -45,6 +45,15 @@ struct ProductArgs {
     int32_t outWide;       // rows are 16-byte aligned
 };
 
+// The forward pass of a few rows: operands as they lie, whatever their addresses.
+struct ThinArgs {
+    const void* a;                // [m, k], rows aStride apart
+    const void *b0, *b1;          // [n, k]; b1 for gate
+    void* out;                    // [m, n], rows outStride apart
+    int64_t aStride, outStride;
+    int32_t m, n, k, activation;
+};
+
 struct OuterArgs {
     Panel p[3], q[3];      // part[f][d] = sum over rows of p[row][f] q[row][d]
     float* part[3];        // [split][m][n]
@@ -78,6 +87,7 @@ struct SumArgs {
 };
 
 template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream);
+template <typename T> int launchThin(bool gate, const ThinArgs& args, hipStream_t stream);
 template <typename T> int launchOuter(const OuterArgs& args, int tile, hipStream_t stream);
 template <typename T> int launchPack(const PackArgs& args, hipStream_t stream);
 template <typename T> int launchSum(const SumArgs& args, hipStream_t stream);

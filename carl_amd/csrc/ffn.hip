@@ -82,10 +82,17 @@ private:
     PackArgs packs_{};
 };
 
+// Up to so many rows the forward pass is a matter of latency.
+constexpr int kThinRows = 128;
+
 struct Forward {
-    Panel x, gate, up, down, h;
+    Panel x{}, gate{}, up{}, down{}, h;
     explicit Forward(const carl_ffn& f, Plan& plan)
     {
+        if (f.rows <= kThinRows) {
+            h = plan.scratch(f.rows, f.inner);
+            return;
+        }
         x = plan.rows(f.x, f.rows, f.width, f.x_row);
         gate = plan.rows(f.w_gate, f.inner, f.width, f.width);
         up = plan.rows(f.w_up, f.inner, f.width, f.width);
@@ -139,6 +146,13 @@ int product(int type, int kind, const ProductArgs& a, hipStream_t s)
     if (type == CARL_OP_F32) return launchProduct<float>(kind, a, s);
     if (type == CARL_OP_BF16) return launchProduct<bf16>(kind, a, s);
     return launchProduct<f16>(kind, a, s);
+}
+
+int thin(int type, bool gate, const ThinArgs& a, hipStream_t s)
+{
+    if (type == CARL_OP_F32) return launchThin<float>(gate, a, s);
+    if (type == CARL_OP_BF16) return launchThin<bf16>(gate, a, s);
+    return launchThin<f16>(gate, a, s);
 }
 
 int pack(int type, const PackArgs& a, hipStream_t s)
@@ -200,6 +214,13 @@ int carl_gated_ffn(const carl_ffn* f, void* stream)
     const hipStream_t s = (hipStream_t)stream;
     Plan plan(f->type, static_cast<char*>(f->workspace));
     const Forward p(*f, plan);
+    if (f->rows <= kThinRows) {
+        const ThinArgs up{ f->x, f->w_gate, f->w_up, const_cast<void*>(p.h.data), f->x_row, p.h.stride, (int32_t)f->rows, f->inner,
+                           f->width, f->activation };
+        if (int rc = thin(f->type, true, up, s)) return rc;
+        const ThinArgs down{ p.h.data, f->w_down, nullptr, f->y, p.h.stride, f->width, (int32_t)f->rows, f->width, f->inner, 0 };
+        return thin(f->type, false, down, s);
+    }
     if (int rc = pack(f->type, plan.packs(), s)) return rc;
     ProductArgs a{};
     a.a[0] = p.x;

@@ -37,6 +37,22 @@ template <> struct Mma<f16> {
     }
 };
 
+// act(g), and its slope where asked for.  The hardware's exponential and
+// reciprocal are good to a unit in the last place each.
+__device__ inline float activate(float g, int activation, float* slopeOut = nullptr)
+{
+    float z = g, slope = 1.0f;
+    if (activation == CARL_GELU) {
+        const float c = 1.5957691216057308f, g2 = g * g;       // 2 sqrt(2 / pi)
+        z = c * (g + 0.044715f * g2 * g);
+        slope = c * (1.0f + 0.134145f * g2);
+    }
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+    const float act = g * s;
+    if (slopeOut) *slopeOut = s + act * (1.0f - s) * slope;
+    return act;
+}
+
 // ---- product -------------------------------------------------------------------
 
 // Rows of a panel sit in LDS with their 16-byte pieces permuted, so that eight
@@ -188,19 +204,13 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
                 const int at = j * 4 + e;
                 if constexpr (kKind == kProductPlain) first[at] = acc[0][j][i][e];
                 else {
-                    const float g = acc[0][j][i][e], up = acc[1][j][i][e];
-                    float z = g, slope = 1.0f;
-                    if (args.activation == CARL_GELU) {
-                        const float c = 1.5957691216057308f, g2 = g * g;       // 2 sqrt(2 / pi)
-                        z = c * (g + 0.044715f * g2 * g);
-                        slope = c * (1.0f + 0.134145f * g2);
-                    }
-                    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
-                    const float act = g * s;
+                    const float up = acc[1][j][i][e];
+                    float slope;
+                    const float act = activate(acc[0][j][i][e], args.activation, &slope);
                     first[at] = act * up;
                     if constexpr (kKind == kProductGrad) {
                         const float dh = acc[kNB - 1][j][i][e];
-                        second[at] = dh * up * (s + act * (1.0f - s) * slope);
+                        second[at] = dh * up * slope;
                         third[at] = dh * act;
                     }
                 }
@@ -210,6 +220,83 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
             store(args.out[1], row, second);
             store(args.out[2], row, third);
         }
+    }
+}
+
+// ---- thin ----------------------------------------------------------------------
+
+// A product of at most 64 rows a workgroup (16 kTM), which is a matter of
+// latency: 16 columns a workgroup, its eight waves taking the sum's blocks in
+// turn, fragments straight from memory to registers, one exchange at the end.
+// Addresses may be any (the hardware takes 16 bytes from each), so weights
+// that the large products would lay out anew are read as they lie.  34 rows of
+// 256 by 683: the block's two launches 14.0 us before, laid out and in tiles
+// of 64 rows.
+template <typename T> __device__ inline uint4 loadAny(const T* p, int have)
+{
+    constexpr int kE = 16 / sizeof(T);
+    vec<T, kE> r;
+    if (have >= kE) __builtin_memcpy(&r, p, 16);
+    else
+#pragma unroll
+        for (int j = 0; j < kE; j++) r[j] = j < have ? p[j] : T(0);
+    return __builtin_bit_cast(uint4, r);
+}
+
+template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) void thinKernel(const ThinArgs args)
+{
+    constexpr int kE = 16 / sizeof(T), kBlock = 4 * kE, kWaves = 8, kNB = kGate ? 2 : 1;
+    __shared__ f32x4 parts[kWaves][kNB][kTM][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * kTM;
+    // rows past the end are the last one again; their results are not stored
+    const int n = n0 + col < args.n ? n0 + col : args.n - 1;
+    const T* b[kNB];
+    b[0] = static_cast<const T*>(args.b0) + (int64_t)n * args.k;
+    if constexpr (kGate) b[1] = static_cast<const T*>(args.b1) + (int64_t)n * args.k;
+    const T* a[kTM];
+#pragma unroll
+    for (int i = 0; i < kTM; i++) {
+        const int m = m0 + i * 16 + col;
+        a[i] = static_cast<const T*>(args.a) + (int64_t)(m < args.m ? m : args.m - 1) * args.aStride;
+    }
+    f32x4 acc[kNB][kTM];
+#pragma unroll
+    for (int p = 0; p < kNB; p++)
+#pragma unroll
+        for (int i = 0; i < kTM; i++) acc[p][i] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll 2
+    for (int k = wave * kBlock + quad * kE; k - quad * kE < args.k; k += kWaves * kBlock) {
+        const int have = args.k - k;
+        uint4 w[kNB], x[kTM];
+#pragma unroll
+        for (int p = 0; p < kNB; p++) w[p] = loadAny(b[p] + k, have);
+#pragma unroll
+        for (int i = 0; i < kTM; i++) x[i] = loadAny(a[i] + k, have);
+#pragma unroll
+        for (int p = 0; p < kNB; p++)
+#pragma unroll
+            for (int i = 0; i < kTM; i++) acc[p][i] = Mma<T>::run(w[p], x[i], acc[p][i]);
+    }
+#pragma unroll
+    for (int p = 0; p < kNB; p++)
+#pragma unroll
+        for (int i = 0; i < kTM; i++) parts[wave][p][i][lane] = acc[p][i];
+    __syncthreads();
+    if (wave >= kTM) return;
+    f32x4 sum[kNB];
+#pragma unroll
+    for (int p = 0; p < kNB; p++) {
+        sum[p] = parts[0][p][wave][lane];
+        for (int w = 1; w < kWaves; w++) sum[p] += parts[w][p][wave][lane];
+    }
+    const int m = m0 + wave * 16 + col;
+    if (m >= args.m) return;
+    T* out = static_cast<T*>(args.out) + m * args.outStride + n0 + quad * 4;
+    for (int e = 0; e < 4; e++) {
+        if (n0 + quad * 4 + e >= args.n) continue;
+        if constexpr (kGate) out[e] = (T)(activate(sum[0][e], args.activation) * sum[1][e]);
+        else out[e] = (T)sum[0][e];
     }
 }
 
@@ -414,6 +501,21 @@ template <typename T> int launchProduct(int kind, const ProductArgs& args, hipSt
     return small ? launchProductShape<T, kProductPlain, 64, 32, 2, 2, 128>(args, stream)
          : wide  ? launchProductShape<T, kProductPlain, 128, 128, 2, 2, 64>(args, stream)
                  : launchProductShape<T, kProductPlain, 256, 256, 2, 4, 128>(args, stream);
+}
+
+template <typename T, bool kGate> void launchThinRows(const ThinArgs& args, hipStream_t stream)
+{
+    const unsigned columns = (unsigned)((args.n + 15) / 16);
+    if (args.m <= 16) thinKernel<T, kGate, 1><<<dim3(columns), 512, 0, stream>>>(args);
+    else if (args.m <= 32) thinKernel<T, kGate, 2><<<dim3(columns), 512, 0, stream>>>(args);
+    else thinKernel<T, kGate, 4><<<dim3(columns, (unsigned)((args.m + 63) / 64)), 512, 0, stream>>>(args);
+}
+
+template <typename T> int launchThin(bool gate, const ThinArgs& args, hipStream_t stream)
+{
+    if (gate) launchThinRows<T, true>(args, stream);
+    else launchThinRows<T, false>(args, stream);
+    return launched("feed-forward product of few rows");
 }
 
 template <typename T> int launchOuter(const OuterArgs& args, int tile, hipStream_t stream)
