@@ -472,35 +472,52 @@ int launchProductShape(const ProductArgs& args, hipStream_t stream)
     return launched("feed-forward product");
 }
 
-// Tiles of the three products of many rows, each the best of those tried at
-// 262,144 rows of 512 by 1,408 in bfloat16 (at 62,000 of 256 by 684 in float32):
-//   gate   128 x 128 of both, 64-byte rows      908 us, 833 TFLOP/s (256 x 128, 128-byte rows: 1,005 us;
-//          float32 128 x 64                     382 us, 114 TFLOP/s (256 x 128: 434 us)
-//   grad   128 x 128 of the three               1,790 us, 634 TFLOP/s (2 x 2 waves: 2,149 us; 128 x 64: 1,939 us;
-//          float32 128 x 64, 64-byte rows       578 us, 113 TFLOP/s (128 x 128: 662 us)
-//   plain  256 x 256, sum over 2,816            687 us, 1,101 TFLOP/s (over 1,408, 128 x 128: 471 us, 256 x 256: 375 us;
-//          float32 128 x 128, 64-byte rows      188 us, 115 TFLOP/s (256 x 256: 194 us)
-// float32 is bound by its matrix instructions (154 TFLOP/s in a large library
-// product) and by the last tiles; 16-bit gate and grad by their tiles' short
-// sums (512), under which the copies' latency and the stores of h, dg and du
-// (2.2 GB: 440 us of grad's time) do not disappear.
+// The largest tiles whose number still keeps the 256 compute units busy, by a
+// sweep over 2,048 to 262,144 rows of 256 to 1,024 by 688 to 2,816 (us):
+//   16 bits  gate   2,048 x 256 x 688   64 x 32 5.8   128 x 128 7.8      8,192 x 512 x 1,408   40.6 and 34.4
+//                   8,192 x 1,024 x 2,816   128 x 128 113   256 x 128 97.7      262,144 x 512 x 1,408   908 and 1,005
+//            grad   2,048 x 256 x 688   64 x 32 10.1   128 x 128 12.3     8,192 x 512 x 1,408   96.5 and 56.4
+//            plain  2,048 x 1,408 to 512   64 x 64 12.0   128 x 128 18.6     8,192 x 2,816 to 1,024   86.2 and 49.7
+//                   32,768 x 1,408 to 512   128 x 128 52.9   256 x 256 45.9  8,192 x 2,816 to 1,024   49.7 and 69.4
+//   float32  gate   2,048 x 512 x 1,408   64 x 32 56.5   128 x 64 69.7    32,768 x 512 x 1,408   883 and 742
+//            grad   2,048 x 512 x 1,408   64 x 64 84   128 x 64 107       32,768 x 512 x 1,408   1,153 and 1,102
+//            plain  2,048 x 1,408 to 512   64 x 64 36.9   128 x 64 56.9     8,192 x 2,816 to 1,024   402 and 379
+//                   62,000 x 684 to 256   128 x 128 188   256 x 256 194
+// At 262,144 rows of 512 by 1,408 in bfloat16 gate runs at 830 TFLOP/s, grad at
+// 630 and plain at 1,010 to 1,100 (a large library product: 1,300; one of
+// gate's sizes: 770).  gate and grad are bound by their tiles' short sums
+// (512), under which the copies' latency and the stores of h, dg and du (2.2
+// GB: 440 us of grad's 1,790) do not disappear; float32 by its matrix
+// instructions (110 to 117 TFLOP/s; the library's product 154).
 template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream)
 {
-    // Few rows run in tiles small enough that the columns alone give work to
-    // many compute units.
-    const bool small = args.m <= 4096;
     constexpr bool wide = sizeof(T) == 4;
-    if (kind == kProductGate)
-        return small ? launchProductShape<T, kProductGate, 64, 32, 2, 2, 128>(args, stream)
-             : wide  ? launchProductShape<T, kProductGate, 128, 64, 2, 2, 64>(args, stream)
-                     : launchProductShape<T, kProductGate, 128, 128, 2, 4, 64>(args, stream);
-    if (kind == kProductGrad)
-        return small ? launchProductShape<T, kProductGrad, 64, 32, 2, 2, 128>(args, stream)
-             : wide  ? launchProductShape<T, kProductGrad, 128, 64, 2, 2, 64>(args, stream)
-                     : launchProductShape<T, kProductGrad, 128, 128, 2, 4, 128>(args, stream);
-    return small ? launchProductShape<T, kProductPlain, 64, 32, 2, 2, 128>(args, stream)
-         : wide  ? launchProductShape<T, kProductPlain, 128, 128, 2, 2, 64>(args, stream)
-                 : launchProductShape<T, kProductPlain, 256, 256, 2, 4, 128>(args, stream);
+    const auto tiles = [&](int rows, int columns) { return (args.m + rows - 1) / rows * ((args.n + columns - 1) / columns); };
+    if (kind == kProductGate) {
+        if constexpr (wide) {
+            if (tiles(128, 64) >= 1536) return launchProductShape<T, kProductGate, 128, 64, 2, 2, 64>(args, stream);
+        } else {
+            if (tiles(128, 128) >= 256 && args.a[0].width >= 1024) return launchProductShape<T, kProductGate, 256, 128, 2, 4, 128>(args, stream);
+            if (tiles(128, 128) >= 128) return launchProductShape<T, kProductGate, 128, 128, 2, 4, 64>(args, stream);
+        }
+        return launchProductShape<T, kProductGate, 64, 32, 2, 2, 128>(args, stream);
+    }
+    if (kind == kProductGrad) {
+        if constexpr (wide) {
+            if (tiles(128, 64) >= 1536) return launchProductShape<T, kProductGrad, 128, 64, 2, 2, 64>(args, stream);
+            if (tiles(64, 64) >= 512) return launchProductShape<T, kProductGrad, 64, 64, 2, 2, 64>(args, stream);
+        } else if (tiles(128, 128) >= 128) return launchProductShape<T, kProductGrad, 128, 128, 2, 4, 128>(args, stream);
+        return launchProductShape<T, kProductGrad, 64, 32, 2, 2, 128>(args, stream);
+    }
+    if constexpr (wide) {
+        if (tiles(128, 128) >= 512) return launchProductShape<T, kProductPlain, 128, 128, 2, 2, 64>(args, stream);
+        if (tiles(128, 64) >= 256) return launchProductShape<T, kProductPlain, 128, 64, 2, 2, 128>(args, stream);
+    } else {
+        if (tiles(256, 256) >= 256) return launchProductShape<T, kProductPlain, 256, 256, 2, 4, 128>(args, stream);
+        if (tiles(128, 128) >= 256) return launchProductShape<T, kProductPlain, 128, 128, 2, 2, 128>(args, stream);
+    }
+    if (tiles(64, 64) >= 256) return launchProductShape<T, kProductPlain, 64, 64, 2, 2, 128>(args, stream);
+    return launchProductShape<T, kProductPlain, 64, 32, 2, 2, 128>(args, stream);
 }
 
 template <typename T, bool kGate> void launchThinRows(const ThinArgs& args, hipStream_t stream)

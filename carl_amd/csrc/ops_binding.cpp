@@ -146,20 +146,36 @@ Tensor workspaceOf(const carl_attention& a, bool backward, const Tensor& like)
     return bytes ? at::empty({ bytes }, like.options().dtype(at::kByte)) : Tensor();
 }
 
+std::tuple<Tensor, Tensor> linearAttentionForward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& logDecay,
+                                                  const OptTensor& starts, const OptTensor& initial, double scale)
+{
+    carl_attention a = attentionOf(q, k, v, logDecay, starts, initial, scale, true);
+    Tensor out = rowsLike(q, a.value_dim);
+    Tensor last = at::empty({ a.batch, a.heads, a.key_dim, a.value_dim }, logDecay.options());
+    a.out = rowsOf(out);
+    a.initial_state = initial ? initial->data_ptr<float>() : nullptr;
+    a.final_state = last.data_ptr<float>();
+    const Tensor work = workspaceOf(a, false, q);
+    a.workspace = work.defined() ? work.data_ptr() : nullptr;
+    check(carl_linear_attention(&a, currentStream()));
+    return { out, last };
+}
+
+// Autograd's own bookkeeping is worth skipping where nothing asks for it (5 us a call).
+bool wantsGradient(std::initializer_list<const Tensor*> tensors)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->requires_grad()) return true;
+    return false;
+}
+
 struct LinearAttention : torch::autograd::Function<LinearAttention> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
                                                   const Tensor& v, const Tensor& logDecay, const OptTensor& starts,
                                                   const OptTensor& initial, double scale)
     {
-        carl_attention a = attentionOf(q, k, v, logDecay, starts, initial, scale, true);
-        Tensor out = rowsLike(q, a.value_dim);
-        Tensor last = at::empty({ a.batch, a.heads, a.key_dim, a.value_dim }, logDecay.options());
-        a.out = rowsOf(out);
-        a.initial_state = initial ? initial->data_ptr<float>() : nullptr;
-        a.final_state = last.data_ptr<float>();
-        const Tensor work = workspaceOf(a, false, q);
-        a.workspace = work.defined() ? work.data_ptr() : nullptr;
-        check(carl_linear_attention(&a, currentStream()));
+        auto [out, last] = linearAttentionForward(q, k, v, logDecay, starts, initial, scale);
         ctx->save_for_backward({ q, k, v, logDecay, starts ? *starts : Tensor(), initial ? *initial : Tensor() });
         ctx->saved_data["scale"] = scale;
         ctx->set_materialize_grads(false);
@@ -200,6 +216,7 @@ std::tuple<Tensor, Tensor> linearAttention(const Tensor& q, const Tensor& k, con
                                            const OptTensor& starts, const OptTensor& initial, std::optional<double> scale)
 {
     const double s = scale ? *scale : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
+    if (!wantsGradient({ &q, &k, &v, initial ? &*initial : &q })) return linearAttentionForward(q, k, v, logDecay, starts, initial, s);
     auto out = LinearAttention::apply(q, k, v, logDecay, starts, initial, s);
     return { out[0], out[1] };
 }
@@ -251,24 +268,30 @@ carl_ffn ffnOf(const Tensor& x, const Tensor& gate, const Tensor& up, const Tens
     return f;
 }
 
+Tensor gatedFfnForward(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation)
+{
+    carl_ffn f = ffnOf(x, gate, up, down, activation);
+    const Tensor rows = asRows(x), g = gate.contiguous(), u = up.contiguous(), d = down.contiguous();
+    Tensor y = at::empty(x.sizes(), x.options());
+    f.x = rows.data_ptr();
+    f.x_row = rows.stride(0);
+    f.w_gate = g.data_ptr();
+    f.w_up = u.data_ptr();
+    f.w_down = d.data_ptr();
+    f.y = y.data_ptr();
+    int64_t bytes = 0;
+    check(carl_gated_ffn_workspace(&f, 0, &bytes));
+    const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
+    f.workspace = work.data_ptr();
+    check(carl_gated_ffn(&f, currentStream()));
+    return y;
+}
+
 struct GatedFfn : torch::autograd::Function<GatedFfn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up,
                           const Tensor& down, int64_t activation)
     {
-        carl_ffn f = ffnOf(x, gate, up, down, activation);
-        const Tensor rows = asRows(x), g = gate.contiguous(), u = up.contiguous(), d = down.contiguous();
-        Tensor y = at::empty(x.sizes(), x.options());
-        f.x = rows.data_ptr();
-        f.x_row = rows.stride(0);
-        f.w_gate = g.data_ptr();
-        f.w_up = u.data_ptr();
-        f.w_down = d.data_ptr();
-        f.y = y.data_ptr();
-        int64_t bytes = 0;
-        check(carl_gated_ffn_workspace(&f, 0, &bytes));
-        const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
-        f.workspace = work.data_ptr();
-        check(carl_gated_ffn(&f, currentStream()));
+        const Tensor y = gatedFfnForward(x, gate, up, down, activation);
         ctx->save_for_backward({ x, gate, up, down });
         ctx->saved_data["activation"] = activation;
         return y;
@@ -310,7 +333,9 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 Tensor gatedFfn(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const std::string& activation)
 {
     require(activation == "silu" || activation == "gelu", "activation must be 'silu' or 'gelu'");
-    return GatedFfn::apply(x, gate, up, down, activation == "silu" ? CARL_SILU : CARL_GELU);
+    const int64_t which = activation == "silu" ? CARL_SILU : CARL_GELU;
+    if (!wantsGradient({ &x, &gate, &up, &down })) return gatedFfnForward(x, gate, up, down, which);
+    return GatedFfn::apply(x, gate, up, down, which);
 }
 
 // ------------------------------------------------------------------- AdamW
