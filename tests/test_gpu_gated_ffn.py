@@ -42,7 +42,7 @@ def _check(x, w_gate, w_up, w_down, dy, activation="silu"):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
-@pytest.mark.parametrize("N", [1, 2, 34, 63, 65, 257, 1000])
+@pytest.mark.parametrize("N", [1, 2, 16, 17, 33, 34, 63, 65, 128, 129, 257, 1000])
 def test_rows(N, activation, dtype):
     _check(*_inputs(N, 64, 136, dtype, seed=N), activation)
 
@@ -58,6 +58,14 @@ def test_widths(D, F, dtype):
 def test_many_rows(N, D, F, dtype):
     """Large tiles, and sums over rows split over workgroups."""
     _check(*_inputs(N, D, F, dtype, seed=N), "gelu")
+
+
+@pytest.mark.parametrize("dtype,N,D,F", [
+    (torch.bfloat16, 33_000, 512, 70), (torch.bfloat16, 8_192, 1024, 600), (torch.float16, 2_000, 1024, 2049),
+    (torch.float32, 25_000, 300, 520), (torch.float32, 8_000, 200, 300), (torch.float32, 9_001, 256, 96)])
+def test_every_tile(dtype, N, D, F):
+    """Sizes on both sides of each rule that chooses a product's tiles."""
+    _check(*_inputs(N, D, F, dtype, seed=N))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
