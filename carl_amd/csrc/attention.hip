@@ -259,7 +259,8 @@ Pass passOf(const carl_attention& a, bool backward)
     pass.heads = a.heads;
     pass.segments = s.segments;
     pass.segmentSteps = s.steps;
-    pass.dealGroups = a.batch * s.segments >= 64;
+    // (the grid's second dimension holds 65,535)
+    pass.dealGroups = a.batch * s.segments >= 64 && a.batch * s.segments <= 8 * 65535;
     pass.logDecay = a.log_decay;
     pass.starts = a.starts;
     pass.startsBatch = a.starts_batch;

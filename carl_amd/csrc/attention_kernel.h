@@ -154,22 +154,33 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     __shared__ __align__(16) T sP[kStates ? 1 : kSteps * S::kStrideP];
 
     // Blocks are dealt to the 8 dies in turn.  The roles of one unit and the
-    // heads of one sequence, which read the same rows or lines, run on one.
-    const int die = blockIdx.x % 8, local = blockIdx.x / 8;
-    const int64_t groups = pass.batch * pass.segments;
-    int64_t group;
-    int head;
-    if (pass.dealGroups) {
-        group = (int64_t)(local / roles / pass.heads) * 8 + die;
-        head = local / roles % pass.heads;
-    } else {
-        const int64_t unit = (int64_t)(local / roles) * 8 + die;
-        group = unit / pass.heads;
-        head = (int)(unit % pass.heads);
+    // heads of one sequence, which read the same rows or lines, run on one:
+    // the grid is (8 x heads x roles, groups / 8).  With few groups (sequences
+    // and their segments) units of one head are dealt instead.
+    const int die = blockIdx.x % 8, batches = (int)pass.batch, groups = batches * pass.segments;
+    int group, head, role = 0;
+    {
+        int unit = blockIdx.x / 8;
+        if (roles == 2) {
+            role = unit & 1;
+            unit >>= 1;
+        } else if (roles == 3) {
+            role = unit % 3;
+            unit /= 3;
+        }
+        if (pass.dealGroups) {
+            group = blockIdx.y * 8 + die;
+            head = unit;
+        } else {
+            unit = unit * 8 + die;
+            group = unit / pass.heads;
+            head = unit - group * pass.heads;
+        }
     }
     if (group >= groups) return;
-    const Role& r = pass.role[firstRole + local % roles];
-    const int64_t batch = group % pass.batch, segment = group / pass.batch;
+    const int segmentOf = pass.segments == 1 ? 0 : group / batches;
+    const Role& r = pass.role[firstRole + role];
+    const int64_t segment = segmentOf, batch = group - segmentOf * batches;
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool backwards = r.backwards != 0;
@@ -194,23 +205,26 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     const int64_t unitState = batch * pass.heads + head, partState = segment * pass.batch * pass.heads + unitState;
     const int size = dimA * dimC;
     f32x4 memory[kOwn][kTilesA];
+    // visits with a lane's offset and, of the whole wave, what is added to it
     const auto eachMemory = [&](bool swapped, auto one, auto four) {
+        const bool full = dimA == kA && dimC == kCd;
 #pragma unroll
         for (int o = 0; o < kOwn; o++) {
             const int y = (wave * kOwn + o) * 16 + col;
-            const int base = y >= dimC ? kOutside : swapped ? (y * dimA + quad * 4) * 4 : (quad * 4 * dimC + y) * 4;
+            const int base = swapped ? (y * dimA + quad * 4) * 4 : (quad * 4 * dimC + y) * 4;
             if (swapped && dimA % 4 == 0) {
 #pragma unroll
                 for (int m = 0; m < kTilesA; m++)
-                    four(o, m, y >= dimC || m * 16 + quad * 4 >= dimA ? kOutside : base + m * 64);
+                    four(o, m, full ? base : y < dimC && m * 16 + quad * 4 < dimA ? base + m * 64 : kOutside, full ? m * 64 : 0);
                 continue;
             }
+            const int row = swapped ? 4 : dimC * 4;
 #pragma unroll
             for (int m = 0; m < kTilesA; m++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int at = base + (m * 16 + i) * (swapped ? 4 : dimC * 4);
-                    one(o, m, i, y >= dimC || m * 16 + quad * 4 + i >= dimA ? kOutside : at);
+                    if (full) one(o, m, i, base, (m * 16 + i) * row);
+                    else one(o, m, i, y < dimC && m * 16 + quad * 4 + i < dimA ? base + (m * 16 + i) * row : kOutside, 0);
                 }
         }
     };
@@ -230,8 +244,12 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, size * 4, 0x00027000);
             eachMemory(
                 swapped,
-                [&](int o, int m, int i, int at) { memory[o][m][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(d, at, 0, 0)); },
-                [&](int o, int m, int at) { memory[o][m] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at, 0, 0)); });
+                [&](int o, int m, int i, int at, int more) {
+                    memory[o][m][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(d, at, more, 0));
+                },
+                [&](int o, int m, int at, int more) {
+                    memory[o][m] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at, more, 0));
+                });
         } else {
 #pragma unroll
             for (int o = 0; o < kOwn; o++)
@@ -257,6 +275,19 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             const int stepBytes = (int)step * (int)sizeof(T);
             const i32x4 from = descriptor(base, (have - 1) * stepBytes + dim * (int)sizeof(T));
             const uint32_t to = ldsAddress(lds) + wave * 1024;
+            // rows that a thread copies, 16 or a multiple apart, are permuted alike
+            constexpr int kAtOnce = kThreads / kPieces;
+            if (kAtOnce % 16 == 0 && have == kSteps) {
+                const int row = thread / kPieces, at = Rows::permuted(row, thread % kPieces) * 16;
+                const int first = (backwards ? kSteps - 1 - row : row) * stepBytes + at, ahead = (backwards ? -kAtOnce : kAtOnce) * stepBytes;
+                const bool within = at < dim * (int)sizeof(T);
+#pragma unroll
+                for (int i = 0; i < loads; i++) {
+                    if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
+                    copyToLds(from, within ? first + i * ahead : kOutside, 0, to + i * kThreads * 16);
+                }
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < loads; i++) {
                 if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
@@ -401,10 +432,11 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 }
             }
             const int firstCut = cuts ? __builtin_ctzll(cuts) : 64;
+            const float past16 = power(16.0f);
+            float in = power(colSteps + (float)inShift) * r.scaleIn;
 #pragma unroll
-            for (int tb = 0; tb < kBlocks; tb++) {
+            for (int tb = 0; tb < kBlocks; tb++, in *= past16) {
                 const bool open = tb * 16 + col < firstCut;
-                const float in = power(colSteps + (float)(tb * 16 + inShift)) * r.scaleIn;
                 // a closed row takes nothing from the memory, whatever that holds
 #pragma unroll
                 for (int o = 0; o < kOwn; o++) acc[o][tb] = open ? acc[o][tb] * in : f32x4{ 0.f, 0.f, 0.f, 0.f };
@@ -414,12 +446,6 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
 
         const float keep = closed ? 0.0f : power((float)have);
         factor *= keep;
-        // what row s weighs in the memory after the chunk
-        const float rest = (float)(have - inShift) - quadSteps;
-        const auto weightOut = [&](int block, int j) {
-            const int s = block * 16 + quad * 4 + j;
-            return s >= leave && s < have ? power(rest - (float)(block * 16 + j)) * r.scaleOut : 0.0f;
-        };
         if (!careful) {
             vec<T, 4> c[kOwn][kBlocks];
 #pragma unroll
@@ -438,23 +464,46 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                         for (int o = 0; o < kOwn; o++) acc[o][tb] = mma(both(c[o][sb], c[o][sb + 1]), p, acc[o][tb]);
                     }
             }
+            if (closed) {
 #pragma unroll
-            for (int o = 0; o < kOwn; o++)
+                for (int o = 0; o < kOwn; o++)
 #pragma unroll
-                for (int m = 0; m < kTilesA; m++) memory[o][m] = closed ? f32x4{ 0.f, 0.f, 0.f, 0.f } : memory[o][m] * keep;
+                    for (int m = 0; m < kTilesA; m++) memory[o][m] = f32x4{ 0.f, 0.f, 0.f, 0.f };
+            } else {
+#pragma unroll
+                for (int o = 0; o < kOwn; o++)
+#pragma unroll
+                    for (int m = 0; m < kTilesA; m++) memory[o][m] *= keep;
+            }
+            // What a row weighs in the memory after the chunk: of a full chunk
+            // without cuts one power of the last row's and the decay from row to
+            // row and block to block; of others each row's, and zero for those
+            // that it does not see.
+            f32x4 w[kBlocks];
+            const float rest = (float)(have - inShift) - quadSteps;
+            if (!closed && have == kSteps) {
+                const float once = power(1.0f), past16 = power(16.0f);
+                w[kBlocks - 1][3] = power(rest - (float)(kSteps - 13)) * r.scaleOut;
+#pragma unroll
+                for (int j = 2; j >= 0; j--) w[kBlocks - 1][j] = w[kBlocks - 1][j + 1] * once;
+#pragma unroll
+                for (int sb = kBlocks - 2; sb >= 0; sb--) w[sb] = w[sb + 1] * past16;
+            } else {
+#pragma unroll
+                for (int sb = 0; sb < kBlocks; sb++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int s = sb * 16 + quad * 4 + j;
+                        w[sb][j] = s >= leave && s < have ? power(rest - (float)(sb * 16 + j)) * r.scaleOut : 0.0f;
+                    }
+            }
 #pragma unroll
             for (int sb = 0; sb < kBlocks; sb += 2) {
-                f32x4 w[2];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    w[0][j] = weightOut(sb, j);
-                    w[1][j] = weightOut(sb + 1, j);
-                }
                 vec<LT, 4> lo[kOwn][L::kOut], hi[kOwn][L::kOut];
 #pragma unroll
                 for (int o = 0; o < kOwn; o++) {
-                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb]) * w[0], lo[o]);
-                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb + 1]) * w[1], hi[o]);
+                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb]) * w[sb], lo[o]);
+                    split<LT, L::kOut>(toFloat<T, 4>(c[o][sb + 1]) * w[sb + 1], hi[o]);
                 }
                 const char* rows = sB + sb * 16 * TileA::kBytes;
 #pragma unroll
@@ -541,19 +590,21 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     const auto d = __builtin_amdgcn_make_buffer_rsrc(to, 0, size * 4, 0x00027000);
     eachMemory(
         swapped,
-        [&](int o, int m, int i, int at) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(memory[o][m][i]), d, at, 0, 0); },
-        [&](int o, int m, int at) {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vec<uint32_t, 4>, memory[o][m]), d, at, 0, 0);
+        [&](int o, int m, int i, int at, int more) {
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(memory[o][m][i]), d, at, more, 0);
+        },
+        [&](int o, int m, int at, int more) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vec<uint32_t, 4>, memory[o][m]), d, at, more, 0);
         });
 }
 
 template <typename T, int kA, int kCd, int kSteps, bool kStates>
 void launchAttentionSteps(const Pass& pass, int firstRole, int roles, hipStream_t stream)
 {
-    const int64_t groups = pass.batch * pass.segments;
-    const int64_t blocks = (pass.dealGroups ? (groups + 7) / 8 * pass.heads : (groups * pass.heads + 7) / 8) * 8 * roles;
+    const unsigned groups = (unsigned)(pass.batch * pass.segments), heads = (unsigned)pass.heads;
+    const dim3 grid = pass.dealGroups ? dim3(8 * heads * roles, (groups + 7) / 8) : dim3((groups * heads + 7) / 8 * 8 * roles);
     attentionKernel<T, kA, kCd, kSteps, kStates>
-        <<<dim3((unsigned)blocks), Shape<T, kA, kCd, kSteps>::kThreads, 0, stream>>>(pass, firstRole, roles);
+        <<<grid, Shape<T, kA, kCd, kSteps>::kThreads, 0, stream>>>(pass, firstRole, roles);
 }
 
 template <typename T, int kA, int kCd, bool kStates>
