@@ -19,11 +19,12 @@
 // operand M^T of the next chunk: it never leaves the registers.  Each wave
 // owns 16-column tiles of c, all rows.
 //
-// Precision with 16-bit rows: P is rounded once (the error of one rounding of
-// the output).  With bfloat16 the memory meets A as two terms of that type, and
-// w_out C meets B as three, so that the memory itself stays within float32's
-// error of sums; float16's range does not hold such terms, and its products
-// with the memory run in float32.
+// Precision with 16-bit rows: P is rounded once, and so is the memory where a
+// reads it with bfloat16 (each the error of one rounding of its part of the
+// output).  w_out C meets B as terms of bfloat16, three where the memory is
+// handed to the caller, which keeps that within float32's error of sums;
+// float16's range does not hold such terms, and its products with the memory
+// run in float32.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -69,16 +69,18 @@ template <typename T, int kWidth> struct Tile {
     }
 };
 
-// How products with float32 factors run (the memory read by a, what enters it
-// from b): bfloat16 as terms of that type, two and three of them; float16
-// rows, whose terms would leave its range, and float32 as float32.
+// How products with float32 factors run.  bfloat16: the memory as it is read
+// by a rounded once, like the weights within a chunk, so that an output's two
+// parts are each as exact as the other; what enters the memory from c as three
+// terms where the memory is handed to the caller, else as two.  float16 rows,
+// whose terms would leave its range, and float32: as float32.
 template <typename T> struct Long {
     using type = float;
     static constexpr int kIn = 1, kOut = 1;
 };
 template <> struct Long<bf16> {
     using type = bf16;
-    static constexpr int kIn = 2, kOut = 3;
+    static constexpr int kIn = 1, kOut = 3;
 };
 
 // x as kTerms addends of type T, largest first.
@@ -327,6 +329,8 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         return odd;
     };
 
+    // the memory after the last chunk goes to the caller (or to the sums that do)
+    const bool handed = r.last && (kStates || pass.segments == 1);
     float factor = 1.0f;      // of the memory over the whole segment
 #pragma unroll 1
     for (int n = 0; n < chunks; n++) {
@@ -513,7 +517,8 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
 #pragma unroll
                     for (int o = 0; o < kOwn; o++)
 #pragma unroll
-                        for (int i = 0; i < L::kOut; i++) memory[o][m] = mma(b, both(lo[o][i], hi[o][i]), memory[o][m]);
+                        for (int i = 0; i < L::kOut; i++)
+                            if (i < 2 || handed) memory[o][m] = mma(b, both(lo[o][i], hi[o][i]), memory[o][m]);
                 }
             }
         } else {
