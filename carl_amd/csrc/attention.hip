@@ -39,17 +39,42 @@ __global__ __launch_bounds__(256) void joinKernel(const Pass pass)
     }
 }
 
-// Sums of `group` query heads' float32 rows into their shared head's row.
-template <typename T>
-__global__ __launch_bounds__(256) void groupKernel(const float* rows, Rows out, int64_t batch, int64_t steps, int heads,
-                                                   int group, int dim)
+// Sums of `group` query heads' float32 rows into their shared head's row, of
+// the keys' and of the values' gradients.  A workgroup for each step of a
+// sequence; four elements a thread where all rows allow it.
+struct GroupSum {
+    const float* rows;          // [batch, steps, heads * group, dim]
+    Rows out;
+    int32_t dim, wide;
+};
+struct GroupSums {
+    GroupSum sum[2];
+    int64_t steps;
+    int32_t heads, group;
+};
+
+template <typename T> __global__ __launch_bounds__(256) void groupKernel(const GroupSums args)
 {
-    const int64_t n = batch * steps * heads * dim;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-        const int64_t d = e % dim, h = e / dim % heads, t = e / dim / heads % steps, b = e / dim / heads / steps;
-        float sum = 0.0f;
-        for (int g = 0; g < group; g++) sum += rows[(((b * steps + t) * heads + h) * group + g) * dim + d];
-        static_cast<T*>(out.data)[b * out.batch + t * out.step + h * out.head + d] = (T)sum;
+    const GroupSum& s = args.sum[blockIdx.z];
+    const int64_t batch = blockIdx.y;
+    const int width = s.wide ? 4 : 1, each = s.dim / width;
+    for (int64_t step = blockIdx.x; step < args.steps; step += gridDim.x) {
+        const float* rows = s.rows + (batch * args.steps + step) * args.heads * args.group * s.dim;
+        T* out = static_cast<T*>(s.out.data) + batch * s.out.batch + step * s.out.step;
+        for (int e = threadIdx.x; e < args.heads * each; e += 256) {
+            const int head = e / each, d = (e - head * each) * width;
+            const float* from = rows + (int64_t)head * args.group * s.dim + d;
+            T* to = out + head * s.out.head + d;
+            if (s.wide) {
+                f32x4 sum = *reinterpret_cast<const f32x4*>(from);
+                for (int g = 1; g < args.group; g++) sum += *reinterpret_cast<const f32x4*>(from + g * s.dim);
+                *reinterpret_cast<vec<T, 4>*>(to) = fromFloat<T, 4>(sum);
+            } else {
+                float sum = *from;
+                for (int g = 1; g < args.group; g++) sum += from[g * s.dim];
+                *to = (T)sum;
+            }
+        }
     }
 }
 
@@ -124,7 +149,7 @@ template <typename T> __global__ __launch_bounds__(256) void stepKernel(const St
 
 // ---- checks ------------------------------------------------------------------
 
-constexpr int64_t kMostUnits = (int64_t)1 << 23;     // workgroups of a launch (2^31 threads)
+constexpr int64_t kMostUnits = (int64_t)1 << 22;     // three workgroups each: 3 x 2^30 threads a launch
 
 int elementBytes(int type) { return type == CARL_OP_F32 ? 4 : 2; }
 
@@ -140,7 +165,7 @@ int checkAttention(const carl_attention* a, bool backward, bool step)
     if (a->kv_heads < 1 || a->heads % a->kv_heads) return fail(CARL_ERR_VALUE, "heads must be a multiple of kv_heads");
     if (a->key_dim < 1 || a->key_dim > CARL_ATTENTION_MAX_DIM) return fail(CARL_ERR_VALUE, "key_dim must be in [1, 128]");
     if (a->value_dim < 1 || a->value_dim > CARL_ATTENTION_MAX_DIM) return fail(CARL_ERR_VALUE, "value_dim must be in [1, 128]");
-    if (a->batch > kMostUnits / a->heads) return fail(CARL_ERR_VALUE, "batch times heads must be at most 8,388,608");
+    if (a->batch > kMostUnits / a->heads) return fail(CARL_ERR_VALUE, "batch times heads must be at most 4,194,304");
     if (a->steps > (int64_t)1 << 40) return fail(CARL_ERR_VALUE, "too many steps");
     if (a->batch > 0 && !a->log_decay) return fail(CARL_ERR_VALUE, "null log_decay");
     if (empty(*a)) return CARL_OK;
@@ -391,19 +416,32 @@ int carl_linear_attention_backward(const carl_attention* a, void* stream)
     dk.partsSwapped = 1;
     if (int rc = run(*a, pass, 2, 3, (hipStream_t)stream)) return rc;
     if (!grouped) return CARL_OK;
-    const auto sum = [&](const Rows& from, const carl_rows& to, int dim) {
-        const int64_t n = a->batch * a->steps * a->kv_heads * dim;
-        const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 8192));
-        const float* rows = static_cast<const float*>(from.data);
-        const int group = a->heads / a->kv_heads;
-        const hipStream_t s = (hipStream_t)stream;
-        if (a->type == CARL_OP_F32) groupKernel<float><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
-        else if (a->type == CARL_OP_BF16) groupKernel<bf16><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
-        else groupKernel<f16><<<grid, 256, 0, s>>>(rows, rowsOf(to), a->batch, a->steps, a->kv_heads, group, dim);
-        return launched("sum over shared heads");
+    GroupSums sums{};
+    sums.steps = a->steps;
+    sums.heads = a->kv_heads;
+    sums.group = a->heads / a->kv_heads;
+    const auto sumOf = [&](const Rows& from, const carl_rows& to, int dim) {
+        const Rows out = rowsOf(to);
+        const bool wide = dim % 4 == 0 && grainOf(out, a->type, a->batch, a->steps, a->kv_heads) >= 4 * elementBytes(a->type);
+        return GroupSum{ static_cast<const float*>(from.data), out, dim, wide };
     };
-    if (int rc = sum(keyRows, a->d_k, a->key_dim)) return rc;
-    return sum(valueRows, a->d_v, a->value_dim);
+    sums.sum[0] = sumOf(keyRows, a->d_k, a->key_dim);
+    sums.sum[1] = sumOf(valueRows, a->d_v, a->value_dim);
+    // (65,535 sequences at a time: the grid's second dimension)
+    for (int64_t first = 0; first < a->batch; first += 65535) {
+        GroupSums some = sums;
+        for (GroupSum& s : some.sum) {
+            s.rows += first * a->steps * a->heads * s.dim;
+            s.out.data = static_cast<char*>(s.out.data) + first * s.out.batch * elementBytes(a->type);
+        }
+        const dim3 grid((unsigned)std::min<int64_t>(a->steps, 1 << 20), (unsigned)std::min<int64_t>(a->batch - first, 65535), 2);
+        const hipStream_t s = (hipStream_t)stream;
+        if (a->type == CARL_OP_F32) groupKernel<float><<<grid, 256, 0, s>>>(some);
+        else if (a->type == CARL_OP_BF16) groupKernel<bf16><<<grid, 256, 0, s>>>(some);
+        else groupKernel<f16><<<grid, 256, 0, s>>>(some);
+        if (int rc = launched("sum over shared heads")) return rc;
+    }
+    return CARL_OK;
 }
 
 int carl_linear_attention_step(const carl_attention* a, float* state, void* stream)

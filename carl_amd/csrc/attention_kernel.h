@@ -124,6 +124,9 @@ template <typename T> __device__ inline uint32_t nonFinite(uint4 x)
 }
 
 template <typename T, int kA, int kC_, int kSteps> struct Shape {
+    // A wave for each column tile of the memory, two tiles each of 128 columns:
+    // eight waves would leave room for one workgroup (or spill) where four
+    // leave it for two (2,048 x 64 of 128 bf16, gradients: 1.94 and 1.27 ms).
     static constexpr int kWaves = kC_ / 16 < 4 ? kC_ / 16 : 4;
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kStrideP = kSteps + 16 / (int)sizeof(T);
@@ -132,8 +135,9 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     static_assert(kTileA % 1024 == 0 && kTileC % 1024 == 0, "whole copies of a wave");
     // workgroups that LDS holds at once, as waves of a SIMD that the registers leave room for
     static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(T);
-    static constexpr int kMost = kA * kC_ > 64 * 128 ? 2 : kA * kC_ > 64 * 64 ? 3 : 4;
-    static constexpr int kResident = kLds * 4 <= 160 * 1024 && kMost >= 4 ? 4 : kLds * 3 <= 160 * 1024 && kMost >= 3 ? 3 : 2;
+    static constexpr int kFit = 160 * 1024 / kLds, kMost = kA * kC_ > 64 * 128 ? 2 : kA * kC_ > 64 * 64 ? 3 : 4;
+    static constexpr int kResident = kFit < kMost ? kFit : kMost;
+    static_assert(kFit >= 1, "one workgroup");
 };
 
 template <typename T, int kA, int kCd, int kSteps, bool kStates>
@@ -386,14 +390,17 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         f32x4 acc[kOwn][kBlocks];
         if constexpr (!kStates) {
             // P^T, tile by tile: rows s, column t
-            for (int tb = wave; tb < kBlocks; tb += kWaves) {
+            // (several waves share a column where there are more of them than columns)
+            constexpr int kShare = kWaves > kBlocks ? kWaves / kBlocks : 1;
+            for (int tb = wave % kBlocks; tb < kBlocks; tb += kWaves) {
                 const int t = tb * 16 + col, from = cuts ? low(t) : 0;
                 vec<T, 4> a[kTilesA];
 #pragma unroll
                 for (int k = 0; k < kTilesA; k++) a[k] = TileA::row(sA + tb * 16 * TileA::kBytes, rowLane, k);
-                float gap = (float)(tb * 16) + colSteps - quadSteps;      // to the tile's first row of the lane
+                const int share = kShare > 1 ? wave / kBlocks : 0;
+                float gap = (float)((tb - share) * 16) + colSteps - quadSteps;      // to the tile's first row of the lane
 #pragma unroll 1
-                for (int sb = 0; sb <= tb; sb++, gap -= 16.0f) {
+                for (int sb = share; sb <= tb; sb += kShare, gap -= 16.0f * kShare) {
                     f32x4 p = { 0.f, 0.f, 0.f, 0.f };
                     const char* rows = sB + sb * 16 * TileA::kBytes;
 #pragma unroll
@@ -408,7 +415,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                     *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + sb * 16) = fromFloat<T, 4>(p);
                 }
                 // blocks of s are met in pairs below
-                if (tb % 2 == 0)
+                if (tb % 2 == 0 && share == 0)
                     *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + (tb + 1) * 16) = vec<T, 4>{ T(0), T(0), T(0), T(0) };
             }
             // what the carried memory gives

@@ -47,7 +47,7 @@ typedef struct carl_rows {
 } carl_rows;
 
 typedef struct carl_attention {
-    int64_t batch, steps;       /* may be 0 */
+    int64_t batch, steps;       /* may be 0; batch times heads at most 4,194,304 */
     int32_t heads, kv_heads;    /* heads is a multiple of kv_heads, at most 65535 */
     int32_t key_dim, value_dim; /* 1 to CARL_ATTENTION_MAX_DIM */
     int32_t type;               /* of q, k, v, out and their gradients */

@@ -95,7 +95,7 @@ NONE = Rows(None, 0, 0, 0)
     ({"key_dim": 129}, VALUE, b"key_dim must be in [1, 128]"),
     ({"value_dim": 0}, VALUE, b"value_dim must be in [1, 128]"),
     ({"value_dim": 129}, VALUE, b"value_dim must be in [1, 128]"),
-    ({"batch": 1 << 23}, VALUE, b"batch times heads must be at most 8,388,608"),
+    ({"batch": (1 << 21) + 1}, VALUE, b"batch times heads must be at most 4,194,304"),
     ({"steps": (1 << 40) + 1}, VALUE, b"too many steps"),
     ({"log_decay": None}, VALUE, b"null log_decay"),
     ({"q": NONE}, VALUE, b"null attention input"),
