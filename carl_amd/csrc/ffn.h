@@ -47,9 +47,9 @@ struct ProductArgs {
 
 // The forward pass of a few rows: operands as they lie, whatever their addresses.
 struct ThinArgs {
-    const void* a;                // [m, k], rows aStride apart
+    const void* a;                // [m, k], rows aStride apart: x, or h
     const void *b0, *b1;          // [n, k]; b1 for gate
-    void* out;                    // [m, n], rows outStride apart
+    void* out;                    // [m, n], rows outStride apart: h (of up to 16 rows in float32), or y
     int64_t aStride, outStride;
     int32_t m, n, k, activation;
 };

@@ -90,7 +90,8 @@ struct Forward {
     explicit Forward(const carl_ffn& f, Plan& plan)
     {
         if (f.rows <= kThinRows) {
-            h = plan.scratch(f.rows, f.inner);
+            const int64_t stride = upTo(f.inner, 64);
+            h = Panel{ plan.take(f.rows * stride * 4), f.rows, stride, f.inner };
             return;
         }
         x = plan.rows(f.x, f.rows, f.width, f.x_row);

@@ -231,7 +231,10 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
 // Addresses may be any (the hardware takes 16 bytes from each), so weights
 // that the large products would lay out anew are read as they lie.  34 rows of
 // 256 by 683: the block's two launches 14.0 us before, laid out and in tiles
-// of 64 rows.
+// of 64 rows, now 9.5 us.  Up to 16 rows h goes from one launch to the other
+// in float32 and meets w_down as two terms of the elements' type (8.0 us for 16
+// rows either way; for 34 it would be 12.3 us).  h's rows are padded with
+// zeros to multiples of 64.
 template <typename T> __device__ inline uint4 loadAny(const T* p, int have)
 {
     constexpr int kE = 16 / sizeof(T);
@@ -251,14 +254,16 @@ template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) voi
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * kTM;
     // rows past the end are the last one again; their results are not stored
     const int n = n0 + col < args.n ? n0 + col : args.n - 1;
+    using H = std::conditional_t<kTM == 1, float, T>;
+    using A = std::conditional_t<kGate, T, H>;
     const T* b[kNB];
     b[0] = static_cast<const T*>(args.b0) + (int64_t)n * args.k;
     if constexpr (kGate) b[1] = static_cast<const T*>(args.b1) + (int64_t)n * args.k;
-    const T* a[kTM];
+    const A* a[kTM];
 #pragma unroll
     for (int i = 0; i < kTM; i++) {
         const int m = m0 + i * 16 + col;
-        a[i] = static_cast<const T*>(args.a) + (int64_t)(m < args.m ? m : args.m - 1) * args.aStride;
+        a[i] = static_cast<const A*>(args.a) + (int64_t)(m < args.m ? m : args.m - 1) * args.aStride;
     }
     f32x4 acc[kNB][kTM];
 #pragma unroll
@@ -268,15 +273,23 @@ template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) voi
 #pragma unroll 2
     for (int k = wave * kBlock + quad * kE; k - quad * kE < args.k; k += kWaves * kBlock) {
         const int have = args.k - k;
-        uint4 w[kNB], x[kTM];
+        uint4 w[kNB];
 #pragma unroll
         for (int p = 0; p < kNB; p++) w[p] = loadAny(b[p] + k, have);
 #pragma unroll
-        for (int i = 0; i < kTM; i++) x[i] = loadAny(a[i] + k, have);
+        for (int i = 0; i < kTM; i++) {
+            if constexpr (kGate || std::is_same_v<H, T>) {
+                const uint4 x = kGate ? loadAny(a[i] + k, have) : *reinterpret_cast<const uint4*>(a[i] + k);
 #pragma unroll
-        for (int p = 0; p < kNB; p++)
-#pragma unroll
-            for (int i = 0; i < kTM; i++) acc[p][i] = Mma<T>::run(w[p], x[i], acc[p][i]);
+                for (int p = 0; p < kNB; p++) acc[p][i] = Mma<T>::run(w[p], x, acc[p][i]);
+            } else {
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(a[i] + k), hi = *reinterpret_cast<const f32x4*>(a[i] + k + 4);
+                const auto h = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                const auto first = fromFloat<T, 8>(h), second = fromFloat<T, 8>(h - toFloat<T, 8>(first));
+                acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, first), acc[0][i]);
+                acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, second), acc[0][i]);
+            }
+        }
     }
 #pragma unroll
     for (int p = 0; p < kNB; p++)
@@ -292,11 +305,12 @@ template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) voi
     }
     const int m = m0 + wave * 16 + col;
     if (m >= args.m) return;
-    T* out = static_cast<T*>(args.out) + m * args.outStride + n0 + quad * 4;
+    using Out = std::conditional_t<kGate, H, T>;
+    Out* out = static_cast<Out*>(args.out) + m * args.outStride + n0 + quad * 4;
     for (int e = 0; e < 4; e++) {
-        if (n0 + quad * 4 + e >= args.n) continue;
-        if constexpr (kGate) out[e] = (T)(activate(sum[0][e], args.activation) * sum[1][e]);
-        else out[e] = (T)sum[0][e];
+        const bool in = n0 + quad * 4 + e < args.n;
+        if constexpr (kGate) out[e] = (Out)(in ? activate(sum[0][e], args.activation) * sum[1][e] : 0.0f);
+        else if (in) out[e] = (T)sum[0][e];
     }
 }
 
@@ -522,7 +536,8 @@ template <typename T> int launchProduct(int kind, const ProductArgs& args, hipSt
 
 template <typename T, bool kGate> void launchThinRows(const ThinArgs& args, hipStream_t stream)
 {
-    const unsigned columns = (unsigned)((args.n + 15) / 16);
+    // h's padding is written too, as zeros
+    const unsigned columns = (unsigned)(kGate ? args.outStride / 16 : (args.n + 15) / 16);
     if (args.m <= 16) thinKernel<T, kGate, 1><<<dim3(columns), 512, 0, stream>>>(args);
     else if (args.m <= 32) thinKernel<T, kGate, 2><<<dim3(columns), 512, 0, stream>>>(args);
     else thinKernel<T, kGate, 4><<<dim3(columns, (unsigned)((args.m + 63) / 64)), 512, 0, stream>>>(args);

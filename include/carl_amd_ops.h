@@ -77,8 +77,8 @@ int carl_linear_attention_step(const carl_attention* a, float* state, void* stre
 /* ---- gated feed-forward block -------------------------------------------------
  *   h = act(x w_gate^T) * (x w_up^T)        y = h w_down^T
  * and its gradients.  All matrices hold one element type; products are summed
- * in float32, and h and the gradients of both projections are rounded to that
- * type once, where the next product reads them.  The backward pass needs only
+ * in float32, and h (of more than 16 rows) and the gradients of both
+ * projections are rounded to that type once, where the next product reads them.  The backward pass needs only
  * the inputs: it computes both projections again. */
 enum { CARL_SILU = 0, CARL_GELU = 1 };  /* GELU in its tanh form */
 
