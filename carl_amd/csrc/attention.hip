@@ -20,20 +20,34 @@ int carl::launchAttention(int type, const Pass& pass, int firstRole, int roles, 
 namespace {
 
 // The memories before each segment from what each leaves, in the place of the
-// latter.  A thread for each element of a memory.
+// latter.  A thread for each element of a memory; eight segments' loads are on
+// their way at once, since each one's store would hold back the next one's
+// (36 segments of 64 x 128, 16 units: 25 us one by one).
 __global__ __launch_bounds__(256) void joinKernel(const Pass pass)
 {
+    constexpr int kAtOnce = 8;
     const Role& r = pass.role[blockIdx.z];
     const int64_t size = (int64_t)r.dimA * r.dimC, units = pass.batch * pass.heads;
     const int64_t unit = blockIdx.x;
     for (int64_t e = threadIdx.x + (int64_t)blockIdx.y * 256; e < size; e += (int64_t)gridDim.y * 256) {
         const int64_t swapped = e % r.dimC * r.dimA + e / r.dimC;
         float m = r.first ? r.first[unit * size + (r.firstSwapped ? swapped : e)] : 0.0f;
-        for (int i = 0; i < pass.segments; i++) {
-            const int64_t at = (r.backwards ? pass.segments - 1 - i : i) * units + unit;
-            const float own = r.parts[at * size + e], f = r.factors[at];
-            r.parts[at * size + e] = m;
-            m = f == 0.0f ? own : m * f + own;        // nothing of a memory that an episode's start clears
+        for (int i0 = 0; i0 < pass.segments; i0 += kAtOnce) {
+            float own[kAtOnce], f[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                const int i = i0 + j < pass.segments ? i0 + j : pass.segments - 1;
+                const int64_t at = (r.backwards ? pass.segments - 1 - i : i) * units + unit;
+                own[j] = r.parts[at * size + e];
+                f[j] = r.factors[at];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                const int i = i0 + j;
+                if (i >= pass.segments) break;
+                r.parts[((r.backwards ? pass.segments - 1 - i : i) * units + unit) * size + e] = m;
+                m = f[j] == 0.0f ? own[j] : m * f[j] + own[j];        // nothing of a memory that an episode's start clears
+            }
         }
         if (r.last) r.last[unit * size + (r.lastSwapped ? swapped : e)] = m;
     }
@@ -268,7 +282,7 @@ int run(const carl_attention& a, Pass& pass, int summed, int roles, hipStream_t 
     };
     if (pass.segments > 1) {
         if (int rc = launch(true, summed)) return rc;
-        const int blocks = (int)std::min<int64_t>(16, ((int64_t)a.key_dim * a.value_dim + 255) / 256);
+        const int blocks = (int)(((int64_t)a.key_dim * a.value_dim + 255) / 256);
         joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)summed), 256, 0, stream>>>(pass);
         if (int rc = launched("joining of segments")) return rc;
     }

@@ -278,19 +278,20 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         constexpr int kPieces = Rows::kPieces;
         const T* base = rows + t0 * step;
         if (grain >= 4) {
-            const int stepBytes = (int)step * (int)sizeof(T);
-            const i32x4 from = descriptor(base, (have - 1) * stepBytes + dim * (int)sizeof(T));
+            const uint32_t stepBytes = (uint32_t)step * (uint32_t)sizeof(T), rowBytes = (uint32_t)dim * (uint32_t)sizeof(T);
+            const i32x4 from = descriptor(base, (int)((uint32_t)(have - 1) * stepBytes + rowBytes));
             const uint32_t to = ldsAddress(lds) + wave * 1024;
             // rows that a thread copies, 16 or a multiple apart, are permuted alike
             constexpr int kAtOnce = kThreads / kPieces;
             if (kAtOnce % 16 == 0 && have == kSteps) {
-                const int row = thread / kPieces, at = Rows::permuted(row, thread % kPieces) * 16;
-                const int first = (backwards ? kSteps - 1 - row : row) * stepBytes + at, ahead = (backwards ? -kAtOnce : kAtOnce) * stepBytes;
-                const bool within = at < dim * (int)sizeof(T);
+                const uint32_t row = thread / kPieces, at = Rows::permuted(row, thread % kPieces) * 16;
+                const uint32_t first = (backwards ? kSteps - 1 - row : row) * stepBytes + at;
+                const uint32_t ahead = (backwards ? 0u - kAtOnce : kAtOnce) * stepBytes;
+                const bool within = at < rowBytes;
 #pragma unroll
                 for (int i = 0; i < loads; i++) {
                     if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
-                    copyToLds(from, within ? first + i * ahead : kOutside, 0, to + i * kThreads * 16);
+                    copyToLds(from, within ? (int)(first + i * ahead) : kOutside, 0, to + i * kThreads * 16);
                 }
                 return;
             }
@@ -298,8 +299,8 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
             for (int i = 0; i < loads; i++) {
                 if (i * kThreads + wave * 64 >= kSteps * kPieces) break;
                 const int piece = i * kThreads + thread, row = piece / kPieces, at = Rows::permuted(row, piece % kPieces) * 16;
-                const int t = backwards ? have - 1 - row : row;
-                copyToLds(from, row < have && at < dim * (int)sizeof(T) ? t * stepBytes + at : kOutside, 0, to + i * kThreads * 16);
+                const uint32_t t = backwards ? have - 1 - row : row;
+                copyToLds(from, row < have && at < (int)rowBytes ? (int)(t * stepBytes + at) : kOutside, 0, to + i * kThreads * 16);
             }
             return;
         }
