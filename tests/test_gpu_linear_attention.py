@@ -284,6 +284,28 @@ def test_rows_past_two_to_the_31():
     ref.assert_within(final, ref.wide(last), 2 * ref.memory_bound(last_size, tail), "memory")
 
 
+@pytest.mark.parametrize("backwards", [False, True])
+@pytest.mark.parametrize("apart", [1 << 25, (1 << 26) + 8])
+def test_steps_far_apart(apart, backwards):
+    """Steps whose rows lie up to 4 GiB (the last that 32 bits reach) and 8 GiB apart over a chunk."""
+    T, D = 70, 32
+    gen = torch.Generator().manual_seed(0)
+    rows = [torch.randn(1, T, 1, D, generator=gen).bfloat16().cuda() for _ in range(4)]
+    q, k, v, dout = rows
+    far = torch.empty((T - 1) * apart + D, device="cuda", dtype=torch.bfloat16).as_strided((1, T, 1, D), (1, apart, 1, 1)).copy_(q if backwards else k)
+    log_decay = torch.tensor([-0.05], device="cuda")
+    if backwards:
+        _check(far, k, v, log_decay, None, None, dout, None)
+    else:
+        _check(q, far, v, log_decay, None, None, dout, None)
+
+
+def test_one_row_for_every_step():
+    """Keys expanded over time: rows past a short chunk's end are not that row again."""
+    q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(2, 90, 2, 2, 32, 32, torch.bfloat16)
+    _check(q, k[:, :1].expand(2, 90, 2, 32), v, log_decay, starts, memory, dout, dfinal)
+
+
 # ------------------------------------------------------------------ streams and graphs
 
 def test_another_stream_and_a_graph():
