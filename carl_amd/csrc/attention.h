@@ -64,6 +64,7 @@ struct Pass {
     Role role[3];
     int64_t batch, steps;
     int32_t heads, segments;
+    int32_t finer;                          // memories in the parts for each segment: those that its parts leave
     int32_t dealGroups;                     // whole sequences (or segments) are dealt to the dies, else heads are
     int64_t segmentSteps;
     const float* logDecay;

@@ -224,9 +224,16 @@ Rows rowsOf(const carl_rows& r) { return Rows{ r.data, r.batch, r.step, r.head }
 // once more) and a second joins.  6 sequences of 4,603 steps, 8 heads of 128:
 // 18 segments both ways, as 1,024 workgroups would have them, 855 us with
 // gradients.
+//
+// Backwards fewer directions are summed up than run, and the first launch would
+// leave compute units with one workgroup: it takes the segments in two halves
+// where all of them run at once (three workgroups a compute unit, or as many
+// as of the others): 6 x 4,603 with gradients 636 us with whole segments, 601
+// with halves.
 struct Split {
     int segments;
     int64_t steps;
+    int finer;
 };
 
 Split splitOf(const carl_attention& a, bool backward)
@@ -234,12 +241,14 @@ Split splitOf(const carl_attention& a, bool backward)
     const int64_t units = a.batch * a.heads * (backward ? 3 : 1);
     const int widest = std::max(a.key_dim, a.value_dim), other = std::min(a.key_dim, a.value_dim);
     const int64_t resident = 256 * (other > 64 ? 2 : widest > 64 ? 3 : a.type == CARL_OP_F32 ? 2 : 4);
-    if (units > resident / 2 || a.steps <= 256) return { 1, std::max<int64_t>(a.steps, 1) };
+    if (units > resident / 2 || a.steps <= 256) return { 1, std::max<int64_t>(a.steps, 1), 1 };
     int64_t segments = std::min<int64_t>(resident / units, (a.steps + 255) / 256);
     int64_t steps = (a.steps + segments - 1) / segments;
     steps = (steps + 63) / 64 * 64;
     segments = (a.steps + steps - 1) / steps;
-    return { (int)segments, steps };
+    const int64_t summed = a.batch * a.heads * (backward ? 2 : 1) * segments;
+    const bool halves = steps % 128 == 0 && steps >= 512 && summed * 2 <= std::max<int64_t>(resident, 256 * 3);
+    return { (int)segments, steps, halves ? 2 : 1 };
 }
 
 int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -255,7 +264,7 @@ Layout layoutOf(const carl_attention& a, bool backward)
     Layout l;
     const Split s = splitOf(a, backward);
     if (s.segments > 1) {
-        const int64_t units = a.batch * a.heads * s.segments;
+        const int64_t units = a.batch * a.heads * s.segments * s.finer;
         l.parts = rounded(units * a.key_dim * a.value_dim * 4);
         l.factors = rounded(units * 4);
     }
@@ -267,11 +276,18 @@ Layout layoutOf(const carl_attention& a, bool backward)
     return l;
 }
 
+void dealUnits(Pass& pass)
+{
+    // (the grid's second dimension holds 65,535)
+    const int64_t groups = pass.batch * pass.segments;
+    pass.dealGroups = groups >= 64 && groups <= 8 * 65535;
+}
+
 // `summed`: the first roles, which have parts of their own.
 int run(const carl_attention& a, Pass& pass, int summed, int roles, hipStream_t stream)
 {
     // roles next to each other with the same widths share a launch
-    const auto launch = [&](bool states, int roles) {
+    const auto launch = [&](const Pass& pass, bool states, int roles) {
         for (int i = 0; i < roles;) {
             int n = 1;
             while (i + n < roles && pass.role[i + n].dimA == pass.role[i].dimA && pass.role[i + n].dimC == pass.role[i].dimC) n++;
@@ -281,12 +297,16 @@ int run(const carl_attention& a, Pass& pass, int summed, int roles, hipStream_t 
         return (int)CARL_OK;
     };
     if (pass.segments > 1) {
-        if (int rc = launch(true, summed)) return rc;
+        Pass sums = pass;       // an empty last half leaves a memory of zeros and a factor of one
+        sums.segments *= pass.finer;
+        sums.segmentSteps /= pass.finer;
+        dealUnits(sums);
+        if (int rc = launch(sums, true, summed)) return rc;
         const int blocks = (int)(((int64_t)a.key_dim * a.value_dim + 255) / 256);
-        joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)summed), 256, 0, stream>>>(pass);
+        joinKernel<<<dim3((unsigned)(a.batch * a.heads), (unsigned)blocks, (unsigned)summed), 256, 0, stream>>>(sums);
         if (int rc = launched("joining of segments")) return rc;
     }
-    return launch(false, roles);
+    return launch(pass, false, roles);
 }
 
 Pass passOf(const carl_attention& a, bool backward)
@@ -298,8 +318,8 @@ Pass passOf(const carl_attention& a, bool backward)
     pass.heads = a.heads;
     pass.segments = s.segments;
     pass.segmentSteps = s.steps;
-    // (the grid's second dimension holds 65,535)
-    pass.dealGroups = a.batch * s.segments >= 64 && a.batch * s.segments <= 8 * 65535;
+    pass.finer = s.finer;
+    dealUnits(pass);
     pass.logDecay = a.log_decay;
     pass.starts = a.starts;
     pass.startsBatch = a.starts_batch;

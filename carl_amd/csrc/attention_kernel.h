@@ -239,7 +239,8 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         bool swapped = false;
         if (!kStates) {
             if (pass.segments > 1) {
-                from = r.parts + partState * size;
+                const int64_t part = segment * pass.finer + (backwards ? pass.finer - 1 : 0);
+                from = r.parts + (part * pass.batch * pass.heads + unitState) * size;
                 swapped = r.partsSwapped != 0;
             } else if (r.first) {
                 from = r.first + unitState * size;

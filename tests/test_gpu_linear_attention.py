@@ -88,6 +88,11 @@ def test_sequences_split_over_workgroups(T, dk, dv, starts, dtype):
     _check(*_inputs(2, T, 2, 1, dk, dv, dtype, seed=T, starts=starts))
 
 
+@pytest.mark.parametrize("T", [2248, 2560])       # five segments of 512 steps; of the last one 200, its second half empty
+def test_segments_summed_in_halves(T):
+    _check(*_inputs(1, T, 32, 4, 72, 66, torch.bfloat16, seed=T, starts=0.002))
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("starts,carry", [(None, False), (None, True), (1.0, True), (0.5, False)])
 def test_masks_and_memories(starts, carry, dtype):
