@@ -139,6 +139,15 @@ Tensor rowsLike(const Tensor& q, int64_t width)
     return at::empty({ q.size(0), q.size(1), q.size(2), width }, q.options());
 }
 
+// For the gradient of t: its order of dimensions, but the last one contiguous
+// whatever t's is.  (Of a t that overlaps itself empty_like keeps the order of
+// the strides, which may put the last dimension anywhere.)
+Tensor gradientLike(const Tensor& t)
+{
+    Tensor g = at::empty_like(t);
+    return g.stride(3) == 1 || g.size(3) <= 1 ? g : rowsLike(t, t.size(3));
+}
+
 Tensor workspaceOf(const carl_attention& a, bool backward, const Tensor& like)
 {
     int64_t bytes = 0;
@@ -195,7 +204,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         if (!dOut.defined()) dOut = at::zeros({ a.batch, a.steps, a.heads, a.value_dim }, q.options());
         if (dOut.stride(3) != 1 && dOut.size(3) > 1) dOut = dOut.contiguous();
         const Tensor dLast = grads[1].defined() ? grads[1].contiguous() : Tensor();
-        const Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+        const Tensor dq = gradientLike(q), dk = gradientLike(k), dv = gradientLike(v);
         // edges count the tensors that were given
         const Tensor dFirst = initial && ctx->needs_input_grad(starts ? 5 : 4) ? at::empty_like(*initial) : Tensor();
         a.initial_state = initial ? initial->data_ptr<float>() : nullptr;

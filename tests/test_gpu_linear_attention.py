@@ -311,6 +311,18 @@ def test_one_row_for_every_step():
     _check(q, k[:, :1].expand(2, 90, 2, 32), v, log_decay, starts, memory, dout, dfinal)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shared", [False, True])
+def test_windows_that_slide_over_one_row(shared, dtype):
+    """Rows one element apart (and heads that are the same rows): the inputs overlap themselves, their gradients do not."""
+    B, T, H, D = 2, 31, 2 if shared else 1, 64
+    gen = torch.Generator().manual_seed(8)
+    q, k, v = (torch.randn(B, T + D - 1, generator=gen).to(dtype).cuda().unfold(1, D, 1)[:, :, None].expand(B, T, H, D) for _ in range(3))
+    assert q.stride(1) == q.stride(3) == 1
+    _, _, _, log_decay, starts, memory, dout, dfinal = _inputs(B, T, H, H, D, D, dtype)
+    _check(q, k, v, log_decay, starts, memory, dout, dfinal)
+
+
 # ------------------------------------------------------------------ streams and graphs
 
 def test_another_stream_and_a_graph():
