@@ -232,9 +232,12 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
 // that the large products would lay out anew are read as they lie.  34 rows of
 // 256 by 683: the block's two launches 14.0 us before, laid out and in tiles
 // of 64 rows, now 9.5 us.  Up to 16 rows h goes from one launch to the other
-// in float32 and meets w_down as two terms of the elements' type (8.0 us for 16
-// rows either way; for 34 it would be 12.3 us).  h's rows are padded with
-// zeros to multiples of 64.
+// in float32 and meets w_down as two terms of bfloat16 (8.0 us for 16 rows
+// either way; for 34 it would be 12.3 us); float16, whose range does not hold
+// such terms, runs that product in float32.  h's rows are padded with zeros to
+// multiples of 64.
+constexpr float kMostBf16 = 0x1.fep127f;
+
 template <typename T> __device__ inline uint4 loadAny(const T* p, int have)
 {
     constexpr int kE = 16 / sizeof(T);
@@ -284,10 +287,22 @@ template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) voi
                 for (int p = 0; p < kNB; p++) acc[p][i] = Mma<T>::run(w[p], x, acc[p][i]);
             } else {
                 const f32x4 lo = *reinterpret_cast<const f32x4*>(a[i] + k), hi = *reinterpret_cast<const f32x4*>(a[i] + k + 4);
-                const auto h = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                const auto first = fromFloat<T, 8>(h), second = fromFloat<T, 8>(h - toFloat<T, 8>(first));
-                acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, first), acc[0][i]);
-                acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, second), acc[0][i]);
+                if constexpr (std::is_same_v<T, bf16>) {
+                    const auto h = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    // a first term that is never infinite: the second takes what passes it
+                    auto near = h;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) near[j] = __builtin_amdgcn_fmed3f(h[j], -kMostBf16, kMostBf16);
+                    const auto first = fromFloat<T, 8>(near), second = fromFloat<T, 8>(h - toFloat<T, 8>(first));
+                    acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, first), acc[0][i]);
+                    acc[0][i] = Mma<T>::run(w[0], __builtin_bit_cast(uint4, second), acc[0][i]);
+                } else {
+                    const auto weights = toFloat<T, 8>(__builtin_bit_cast(vec<T, 8>, w[0]));
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[0][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(weights[j], lo[j], acc[0][i], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[0][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(weights[4 + j], hi[j], acc[0][i], 0, 0, 0);
+                }
             }
         }
     }

@@ -136,6 +136,39 @@ def test_a_non_finite_row_stays_its_own():
     assert torch.isnan(got[33]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("N", [1, 16])
+def test_inner_values_of_few_rows_past_the_types_range(N, dtype):
+    """h of up to 16 rows is not rounded to the elements' type: 90,000 of it meet weights of 0.01."""
+    gen = torch.Generator().manual_seed(N)
+
+    def around(middle, off, *shape):
+        return (middle + off * torch.randn(*shape, generator=gen)).to(dtype).cuda()
+
+    x, w_gate, w_up, w_down = around(1, 0.1, N, 8), around(37.5, 3.75, 24, 8), around(37.5, 3.75, 24, 8), around(0, 0.01, 8, 24)
+    value, bound = ref.ffn(x, w_gate, w_up, w_down, "silu")
+    ref.assert_within(_ops().gated_ffn(x, w_gate, w_up, w_down), value["y"], bound["y"], "y")
+
+
+def test_an_inner_value_between_bfloat16s_and_float32s_largest():
+    """gate = 2^64 (1 - 2^-10), up = 2^64 (1 - 2^-11): h is finite in float32 and would be infinite in bfloat16."""
+    x, w_down = torch.ones(1, 2), torch.full((2, 1), 2.0 ** -10)
+    w_gate, w_up = torch.tensor([[2.0 ** 64, -2.0 ** 54]]), torch.tensor([[2.0 ** 64, -2.0 ** 53]])
+    y = _ops().gated_ffn(*(t.bfloat16().cuda() for t in (x, w_gate, w_up, w_down)))
+    # 2^118 (1 - 2^-10) (1 - 2^-11), rounded to 8 bits
+    assert torch.equal(y.float().cpu(), torch.full((1, 2), 2.0 ** 118))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N,F", [(1, 24), (16, 24), (16, 683), (40, 24), (40, 683)])
+def test_an_infinity_of_few_rows_is_no_nan(N, F, dtype):
+    """With weights above zero an infinite input makes its row's outputs infinite, and no other's."""
+    x, w_gate, w_up, w_down, _ = _inputs(N, 40, F, dtype)
+    x[N - 1, 3] = math.inf
+    y = _ops().gated_ffn(x, w_gate.abs(), w_up.abs(), w_down.abs())
+    assert torch.isposinf(y[N - 1]).all() and torch.isfinite(y[: N - 1]).all()
+
+
 def test_gradients_against_differences():
     x, w_gate, w_up, w_down, dy = _inputs(20, 24, 40, torch.float32)
     leaves = [t.requires_grad_() for t in (x, w_gate, w_up, w_down)]
