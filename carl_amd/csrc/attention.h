@@ -8,7 +8,7 @@
 // decay^|t-s| where no episode starts between the two steps, else 0.
 //
 // In chunks of kC steps, with X the chunk's rows and M the memory before it:
-//   P = (A B^T) o w          [kC x kC], rounded to the rows' type
+//   P = (A B^T) o w          [kC x kC]
 //   out = P C + w_in A M     w_in(t) = decay^(steps since the chunk's edge)
 //   M  <- w_all M + B^T (w_out C)
 // Products run on the matrix cores as 16x16 tiles, k in groups of 16: a lane's
@@ -19,12 +19,13 @@
 // operand M^T of the next chunk: it never leaves the registers.  Each wave
 // owns 16-column tiles of c, all rows.
 //
-// Precision with 16-bit rows: P is rounded once, and so is the memory where a
-// reads it with bfloat16 (each the error of one rounding of its part of the
-// output).  w_out C meets B as terms of bfloat16, three where the memory is
-// handed to the caller, which keeps that within float32's error of sums;
-// float16's range does not hold such terms, and its products with the memory
-// run in float32.
+// Precision with bfloat16 rows: P is rounded once, and so is the memory where a
+// reads it (each the error of one rounding of its part of the output).  w_out C
+// meets B as terms of bfloat16: three where the memory is handed to the caller,
+// which keeps that within float32's error of sums, else two (2^-16 of each
+// addend, little beside the rounding that follows).  float16's range holds
+// neither P nor the memory nor such terms: all its products but A B^T run in
+// float32, and only outputs are rounded.
 //
 // What bounds it: no unit throughout, but the chain from a chunk's copies over
 // P to its outputs, which only other workgroups of the compute unit hide.

@@ -72,8 +72,9 @@ template <typename T, int kWidth> struct Tile {
 // How products with float32 factors run.  bfloat16: the memory as it is read
 // by a rounded once, like the weights within a chunk, so that an output's two
 // parts are each as exact as the other; what enters the memory from c as three
-// terms where the memory is handed to the caller, else as two.  float16 rows,
-// whose terms would leave its range, and float32: as float32.
+// terms where the memory is handed to the caller, else as two.  float16, whose
+// range holds neither (a . b passes 65,504 where each is 100 in 64 dimensions,
+// and of a small gradient little is left above 2^-24), and float32: as float32.
 template <typename T> struct Long {
     using type = float;
     static constexpr int kIn = 1, kOut = 1;
@@ -129,12 +130,13 @@ template <typename T, int kA, int kC_, int kSteps> struct Shape {
     // leave it for two (2,048 x 64 of 128 bf16, gradients: 1.94 and 1.27 ms).
     static constexpr int kWaves = kC_ / 16 < 4 ? kC_ / 16 : 4;
     static constexpr int kThreads = kWaves * 64;
-    static constexpr int kStrideP = kSteps + 16 / (int)sizeof(T);
+    using P = typename Long<T>::type;                // of the weights within a chunk
+    static constexpr int kStrideP = kSteps + 16 / (int)sizeof(P);
     static constexpr int kTileA = kSteps * Tile<T, kA>::kBytes, kTileC = kSteps * Tile<T, kC_>::kBytes;
     static constexpr int kLoadsA = (kTileA / 16 + kThreads - 1) / kThreads, kLoadsC = (kTileC / 16 + kThreads - 1) / kThreads;
     static_assert(kTileA % 1024 == 0 && kTileC % 1024 == 0, "whole copies of a wave");
     // workgroups that LDS holds at once, as waves of a SIMD that the registers leave room for
-    static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(T);
+    static constexpr int kLds = 2 * kTileA + kTileC + kSteps * kStrideP * (int)sizeof(P);
     static constexpr int kFit = 160 * 1024 / kLds, kMost = kA * kC_ > 64 * 128 ? 2 : kA * kC_ > 64 * 64 ? 3 : 4;
     static constexpr int kResident = kFit < kMost ? kFit : kMost;
     static_assert(kFit >= 1, "one workgroup");
@@ -157,7 +159,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     __shared__ __align__(1024) char sA[kStates ? 16 : S::kTileA];
     __shared__ __align__(1024) char sB[S::kTileA];
     __shared__ __align__(1024) char sC[S::kTileC];
-    __shared__ __align__(16) T sP[kStates ? 1 : kSteps * S::kStrideP];
+    __shared__ __align__(16) LT sP[kStates ? 1 : kSteps * S::kStrideP];
 
     // Blocks are dealt to the 8 dies in turn.  The roles of one unit and the
     // heads of one sequence, which read the same rows or lines, run on one:
@@ -377,7 +379,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         // rows, and the results' rows of P
         const int rowLane = TileA::at(col, quad * 4);
         const int columnLaneA = TileA::columnLane(col, quad), columnLaneC = TileC::columnLane(col, quad);
-        T* const pLane = sP + col * S::kStrideP + quad * 4;
+        LT* const pLane = sP + col * S::kStrideP + quad * 4;
         const float quadSteps = (float)(quad * 4), colSteps = (float)col;
 
         // Rows [low(t), t] are what row t sees of the chunk.
@@ -414,11 +416,11 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                         const float w = p[i] * (power(gap - (float)i) * r.scaleP);
                         p[i] = s + i >= from && s + i <= t ? w : 0.0f;
                     }
-                    *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + sb * 16) = fromFloat<T, 4>(p);
+                    *reinterpret_cast<vec<LT, 4>*>(pLane + tb * 16 * S::kStrideP + sb * 16) = fromFloat<LT, 4>(p);
                 }
                 // blocks of s are met in pairs below
                 if (tb % 2 == 0 && share == 0)
-                    *reinterpret_cast<vec<T, 4>*>(pLane + tb * 16 * S::kStrideP + (tb + 1) * 16) = vec<T, 4>{ T(0), T(0), T(0), T(0) };
+                    *reinterpret_cast<vec<LT, 4>*>(pLane + tb * 16 * S::kStrideP + (tb + 1) * 16) = vec<LT, 4>{ LT(0), LT(0), LT(0), LT(0) };
             }
             // what the carried memory gives
 #pragma unroll
@@ -471,10 +473,12 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
                 for (int tb = 0; tb < kBlocks; tb++)
 #pragma unroll
                     for (int sb = 0; sb <= tb; sb += 2) {
-                        const T* row = pLane + tb * 16 * S::kStrideP + sb * 16;
-                        const auto p = both(*reinterpret_cast<const vec<T, 4>*>(row), *reinterpret_cast<const vec<T, 4>*>(row + 16));
+                        const LT* row = pLane + tb * 16 * S::kStrideP + sb * 16;
+                        const auto p = both(*reinterpret_cast<const vec<LT, 4>*>(row), *reinterpret_cast<const vec<LT, 4>*>(row + 16));
 #pragma unroll
-                        for (int o = 0; o < kOwn; o++) acc[o][tb] = mma(both(c[o][sb], c[o][sb + 1]), p, acc[o][tb]);
+                        for (int o = 0; o < kOwn; o++)
+                            acc[o][tb] = mma(both(__builtin_convertvector(c[o][sb], vec<LT, 4>), __builtin_convertvector(c[o][sb + 1], vec<LT, 4>)),
+                                             p, acc[o][tb]);
                     }
             }
             if (closed) {
@@ -626,9 +630,10 @@ void launchAttentionShape(const Pass& pass, int firstRole, int roles, hipStream_
 {
     // Chunks of 64 steps (16,384 x 64, 8 heads of 64 in bfloat16, gradients:
     // 4.4 ms, in chunks of 32 4.9 ms); of 32 where no sequence is longer, and
-    // for float32, whose matrix instructions the longer chunks' products within
-    // keep busy (4,096 x 64 with gradients: 2.68 ms, in chunks of 64 3.59 ms).
-    constexpr bool large = sizeof(T) == 4;
+    // where products run in float32, whose matrix instructions the longer
+    // chunks' products within keep busy (4,096 x 64 of float32 with gradients:
+    // 2.68 ms, in chunks of 64 3.59 ms; 16,384 x 64 of float16 9.24 and 10.05).
+    constexpr bool large = std::is_same_v<typename Long<T>::type, float>;
     if constexpr (!kStates && !large) {
         if (pass.segmentSteps > 32) launchAttentionSteps<T, kA, kCd, 64, kStates>(pass, firstRole, roles, stream);
         else launchAttentionSteps<T, kA, kCd, 32, kStates>(pass, firstRole, roles, stream);

@@ -37,9 +37,11 @@ enum { CARL_OP_F32 = 0, CARL_OP_BF16 = 1, CARL_OP_F16 = 2 };
  * Steps of the chunked form run in chunks as products of matrices; long
  * sequences are split over workgroups and joined through the workspace.
  * q, k, v and out hold one element type, the memory is float32.  All sums are
- * float32; with 16-bit elements the weights of steps within a chunk are
- * rounded to that type before they meet v, and with bfloat16 so is the memory
- * where q reads it; the memory itself is kept to float32's precision.
+ * float32.  With bfloat16 the weights of steps within a chunk are rounded to
+ * that type before they meet v, and so is the memory where q reads it; what
+ * enters the memory is kept to float32's precision where the memory is
+ * returned, else to 16 bits.  float16's range would not hold the weights: its
+ * intermediate values are float32.
  * Results do not depend on timing: there are no atomics. */
 typedef struct carl_rows {
     void* data;                 /* a row: the head's contiguous elements */

@@ -323,6 +323,34 @@ def test_windows_that_slide_over_one_row(shared, dtype):
     _check(q, k, v, log_decay, starts, memory, dout, dfinal)
 
 
+def test_float16_weights_past_its_range():
+    """q . k of 80,000 meets values of 0.01: the outputs and gradients are within float16's range."""
+    q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(2, 40, 2, 1, 64, 48, torch.float16)
+    _check((100 + 0.1 * q).half(), (100 + 0.1 * k).half(), v * 0.01, log_decay, starts, memory * 0.01, dout * 0.001, dfinal * 0.01)
+
+
+@pytest.mark.parametrize("T", [30, 600])
+def test_float16_weights_below_its_range(T):
+    """Weights about 2^-20, whose roundings in float16 would be a few hundredths of them: outputs and the queries'
+    gradients (weights from small gradients of the outputs) are off by their own rounding and float32 sums alone."""
+    q, k, v, log_decay, starts, _, dout, _ = _inputs(2, T, 2, 1, 64, 48, torch.float16)
+    q, k, v = q * 2.0 ** -10, k * 2.0 ** -10, v * 32
+    out, _ = _ops().linear_attention(q, k, v, log_decay, starts=starts)
+    want, _ = ref.attention(q, k, v, log_decay, starts)
+    size, _ = ref.magnitudes(ref.attention, q, k, v, log_decay, starts)
+
+    def bound(value, size):
+        return 2.0 ** -11 * value.abs() + (T + 64 + 64) * ref.EPS * size + 2.0 ** -24
+
+    ref.assert_within(out, want, bound(want, size), "out")
+    leaf, k, v, dout = q.requires_grad_(), k * 2.0 ** 15, v * 2.0 ** -11, dout * 2.0 ** -14
+    out, _ = _ops().linear_attention(leaf, k, v, log_decay, starts=starts)
+    (got,) = torch.autograd.grad(out, [leaf], dout)
+    args = (leaf.detach(), k, v, log_decay, dout, starts)
+    want, size = ref.attention_gradients(*args)[0], ref.magnitudes(ref.attention_gradients, *args)[0]
+    ref.assert_within(got, want, bound(want, size), "dq")
+
+
 # ------------------------------------------------------------------ streams and graphs
 
 def test_another_stream_and_a_graph():
