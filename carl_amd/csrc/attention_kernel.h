@@ -203,9 +203,14 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
     const int64_t aStep = r.a.step, bStep = r.b.step, cStep = r.c.step;
     const int aGrain = r.aGrain, bGrain = r.bGrain, cGrain = r.cGrain;
 
-    // -infinity times zero steps is no NaN
-    const float decay2 = fmaxf(pass.logDecay[head] * 1.44269504088896341f, -1e30f);
-    const auto power = [&](float steps) { return __builtin_amdgcn_exp2f(decay2 * steps); };
+    // Of a decay that is zero or not a number, no steps are still a weight of
+    // one: this product with zero is zero, whatever the other factor.
+    const float decay2 = pass.logDecay[head] * 1.44269504088896341f;
+    const auto power = [&](float steps) {
+        float x;
+        asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(x) : "v"(decay2), "v"(steps));
+        return __builtin_amdgcn_exp2f(x);
+    };
 
     // A lane's elements of the memory: rows 16 m + 4 quad + i, column 16 (wave's
     // tile) + col.  Through a descriptor, past whose end lies what the padding
@@ -460,7 +465,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         }
 
         const float keep = closed ? 0.0f : power((float)have);
-        factor *= keep;
+        factor = closed ? 0.0f : factor * keep;
         if (!careful) {
             vec<T, 4> c[kOwn][kBlocks];
 #pragma unroll

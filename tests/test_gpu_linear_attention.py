@@ -202,6 +202,41 @@ def test_nothing_of_an_earlier_episode_is_seen(T, bad, dtype):
                       2 * ref.attention_bound(dtype, wants[0], sizes[0], T, 48)[0, cut:late], "dq")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("T", [70, 600])
+def test_a_decay_that_is_not_a_number(T, dtype):
+    """Its head gives NaN wherever a step before is seen, in both forms, and finite values at steps that begin an episode
+    (at the ends of chunks and of segments among them); gradients likewise; other heads are as without it."""
+    ops = _ops()
+    q, k, v, log_decay, _, memory, dout, dfinal = _inputs(2, T, 3, 3, 32, 48, dtype, starts=None)
+    starts = torch.zeros(2, T, dtype=torch.bool, device="cuda")
+    starts[0, [20, 21, 31, 63, T - 1]] = starts[1, 0] = True
+    if T > 256:
+        starts[0, 255] = starts[1, 512] = True
+    broken = log_decay.clone()
+    broken[1] = math.nan
+    results = []
+    for decays in (log_decay, broken):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, memory)]
+        out, final = ops.linear_attention(*leaves[:3], decays, starts=starts, initial_state=leaves[3])
+        results.append([out.detach(), final.detach(), *torch.autograd.grad([out, final], leaves, [dout, dfinal])])
+    heads = (2, 1, 2, 2, 2, 1)
+    for want, got, dim in zip(*results, heads):
+        assert torch.equal(want.select(dim, 0), got.select(dim, 0)) and torch.equal(want.select(dim, 2), got.select(dim, 2))
+    isnan = [torch.isnan(x.select(dim, 1)) for x, dim in zip(results[1], heads)]
+    # forwards all but a start sees a step before; backwards all but the step before a start, and the last, is seen by one after
+    before = ~starts
+    after = torch.cat((~starts[:, 1:], torch.zeros_like(starts[:, :1])), 1)
+    for got, want in zip(isnan, (before, before[:, -1], before, after, after, ~starts[:, 0])):
+        assert torch.equal(got.flatten(want.dim()).all(-1), want) and torch.equal(got.flatten(want.dim()).any(-1), want)
+    # the recurrent form agrees
+    state = memory.clone()
+    for t in range(T):
+        out = ops.linear_attention_step(q[:, t], k[:, t], v[:, t], broken, state, starts=starts[:, t])
+        assert torch.equal(torch.isnan(out[:, 1]), isnan[0][:, t])
+    assert torch.equal(torch.isnan(state[:, 1]), isnan[1])
+
+
 def test_no_steps_and_no_sequences():
     ops = _ops()
     q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(3, 0, 2, 2, 16, 24, torch.float32)
