@@ -215,6 +215,17 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
                     }
                 }
             }
+        // the padding of rows is zero whatever a row holds (an infinity meets
+        // the zeros past the weights' last row)
+        if (kKind != kProductPlain && n0 + kBN > args.n) {
+            const int n = n0 + wn * kTN * 16 + quad * kRun;
+#pragma unroll
+            for (int e = 0; e < kRun; e++) {
+                if (n + e < args.n) continue;
+                first[e] = 0.0f;
+                if constexpr (kKind == kProductGrad) second[e] = third[e] = 0.0f;
+            }
+        }
         store(args.out[0], row, first);
         if constexpr (kKind == kProductGrad) {
             store(args.out[1], row, second);

@@ -160,13 +160,27 @@ def test_an_inner_value_between_bfloat16s_and_float32s_largest():
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("N,F", [(1, 24), (16, 24), (16, 683), (40, 24), (40, 683)])
-def test_an_infinity_of_few_rows_is_no_nan(N, F, dtype):
+@pytest.mark.parametrize("N,F", [(1, 24), (16, 24), (16, 683), (40, 24), (40, 683), (200, 24), (200, 683), (9000, 681)])
+def test_an_infinity_is_no_nan(N, F, dtype):
     """With weights above zero an infinite input makes its row's outputs infinite, and no other's."""
     x, w_gate, w_up, w_down, _ = _inputs(N, 40, F, dtype)
     x[N - 1, 3] = math.inf
     y = _ops().gated_ffn(x, w_gate.abs(), w_up.abs(), w_down.abs())
     assert torch.isposinf(y[N - 1]).all() and torch.isfinite(y[: N - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N,F", [(16, 24), (16, 683), (200, 683), (9000, 681)])
+def test_an_infinite_gradient_is_no_nan(N, F, dtype):
+    """With weights and rows above zero: infinite gradients of its row and of every weight of both projections."""
+    *tensors, dy = _inputs(N, 40, F, dtype)
+    dy[N - 1, 3] = math.inf
+    leaves = [t.abs().requires_grad_() for t in tensors]
+    dx, dg, du, dd = torch.autograd.grad(_ops().gated_ffn(*leaves), leaves, dy)
+    assert torch.isposinf(dx[N - 1]).all() and torch.isfinite(dx[: N - 1]).all()
+    assert torch.isposinf(dg).all() and torch.isposinf(du).all()
+    rest = [i for i in range(40) if i != 3]
+    assert torch.isposinf(dd[3]).all() and torch.isfinite(dd[rest]).all()
 
 
 def test_gradients_against_differences():
