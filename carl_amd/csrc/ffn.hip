@@ -14,6 +14,18 @@ namespace {
 int elementBytes(int type) { return type == CARL_OP_F32 ? 4 : 2; }
 int64_t upTo(int64_t x, int64_t multiple) { return (x + multiple - 1) / multiple * multiple; }
 
+constexpr int64_t kMostRows = (int64_t)1 << 28;
+
+// Of a product's launch, at most, where it is a large one: launchProduct()
+// then takes tiles of at least 128 x 64 (float32, 256 threads) or 128 x 128
+// (16 bits, 512 threads), a multiple of 8 of them across the rows.
+int64_t threadsOf(const carl_ffn& f)
+{
+    const bool wide = f.type == CARL_OP_F32;
+    const int64_t columns = std::max(f.width, f.inner), tile = wide ? 64 : 128;
+    return upTo((f.rows + 127) / 128, 8) * ((columns + tile - 1) / tile) * (wide ? 256 : 512);
+}
+
 int checkFfn(const carl_ffn* f, bool backward)
 {
     if (!f) return fail(CARL_ERR_VALUE, "null feed-forward argument");
@@ -21,10 +33,7 @@ int checkFfn(const carl_ffn* f, bool backward)
     if (f->activation != CARL_SILU && f->activation != CARL_GELU) return fail(CARL_ERR_VALUE, "unknown activation");
     if (f->width < 1 || f->width > CARL_FFN_MAX_DIM) return fail(CARL_ERR_VALUE, "width must be in [1, 65536]");
     if (f->inner < 1 || f->inner > CARL_FFN_MAX_DIM) return fail(CARL_ERR_VALUE, "inner must be in [1, 65536]");
-    // workgroups of a launch (2^31 threads), the smallest tiles
-    if (f->rows < 0 || f->rows > (int64_t)1 << 28
-        || upTo(f->rows, 512) / 64 * (std::max(f->width, f->inner) / 32 + 1) > (int64_t)1 << 22)
-        return fail(CARL_ERR_VALUE, "rows are out of range");
+    if (f->rows < 0 || f->rows > kMostRows || threadsOf(*f) > (int64_t)1 << 31) return fail(CARL_ERR_VALUE, "rows are out of range");
     if (!f->w_gate || !f->w_up || !f->w_down) return fail(CARL_ERR_VALUE, "null weights");
     if (f->rows == 0) return CARL_OK;
     if (!f->x || (!backward && !f->y) || (backward && !f->dy)) return fail(CARL_ERR_VALUE, "null feed-forward tensor");

@@ -61,7 +61,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     w_down          [width, inner]
     activation      "silu", or "gelu" in its tanh form
 
-    All of one type; products are summed in float32.  Gradients reach x and the
+    All of one type; products are summed in float32.  Widths are at most 65,536,
+    rows 2^28, and rows times the larger width about 2^36.  Gradients reach x and the
     weights, once; the backward pass computes both projections again instead of
     keeping them.
     """

@@ -85,7 +85,8 @@ int carl_linear_attention_step(const carl_attention* a, float* state, void* stre
 enum { CARL_SILU = 0, CARL_GELU = 1 };  /* GELU in its tanh form */
 
 typedef struct carl_ffn {
-    int64_t rows;
+    int64_t rows;               /* at most 2^28; times the larger of width and inner, in tiles of
+                                 * 128 x 128 (float32: 128 x 64), at most 2^36 elements */
     int32_t width, inner;       /* 1 to CARL_FFN_MAX_DIM */
     int32_t type, activation;
     const void* x;              /* [rows, width], rows x_row elements apart */

@@ -216,6 +216,17 @@ def test_rows_past_two_to_the_31():
     ref.assert_within(y[-100:], value["y"], bound["y"], "y")
 
 
+def test_more_elements_than_small_tiles_reach():
+    """2^33 elements of x and of y, more than 2^22 small tiles of 64 x 32: the last rows are what they are by themselves."""
+    N, D, F = 1 << 20, 8192, 16
+    _, w_gate, w_up, w_down, _ = _inputs(1, D, F, torch.bfloat16)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(N, D, generator=gen, device="cuda", dtype=torch.bfloat16)
+    y = _ops().gated_ffn(x, w_gate, w_up, w_down)
+    value, bound = ref.ffn(x[-100:].clone(), w_gate, w_up, w_down, "silu")
+    ref.assert_within(y[-100:], value["y"], bound["y"], "y")
+
+
 def test_another_stream_and_a_graph():
     x, w_gate, w_up, w_down, dy = _inputs(5000, 64, 105, torch.bfloat16)
     leaves = [t.requires_grad_() for t in (x, w_gate, w_up, w_down)]

@@ -168,6 +168,24 @@ def test_ffn_refuses(lib, changes, code, message):
     assert lib.carl_gated_ffn(None, None) == VALUE
 
 
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_ffn_takes_what_its_tiles_reach(lib, kind, backward):
+    """2^36 elements in tiles of 128 x 128 (float32: 128 x 64), 2^28 rows."""
+    size = I64(-1)
+
+    def rc(**changes):
+        return lib.carl_gated_ffn_workspace(C.byref(_ffn(type=kind, **changes)), backward, C.byref(size))
+
+    assert rc(rows=1 << 20, width=8192, x_row=8192, dy_row=8192) == OK
+    assert rc(rows=1 << 20, width=65536, inner=65536, x_row=65536, dy_row=65536) == OK
+    assert size.value >= (1 << 36) * (4 if kind == 0 else 2)
+    assert rc(rows=1 << 28) == OK
+    for changes in ({"rows": (1 << 20) + 1, "width": 65536}, {"rows": (1 << 28) + 1}, {"rows": 1 << 28, "inner": 257}):
+        assert rc(**changes) == VALUE
+        assert lib.carl_last_error() == b"rows are out of range"
+
+
 @pytest.mark.parametrize("changes,message", [
     ({"bits": 16}, b"moments must have 8 or 32 bits"),
     ({"step": 0}, b"step must be at least 1"),
