@@ -7,6 +7,9 @@
 // operation; outputs and scratch memory come from torch's allocator.
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/forward_grad.h>
+
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -51,11 +54,21 @@ template <typename... Parts> void requireType(bool ok, const Parts&... parts)
     if (!ok) throw py::type_error(message(parts...));
 }
 
-void onDevice(const Tensor& t, const char* name)
-{
-    require(t.defined() && t.is_cuda() && t.get_device() == 0, name, " must be on cuda:0");
-    require(t.layout() == at::kStrided, name, " must be a dense tensor");
-}
+// The check of every tensor of a call.  A forward-mode tangent is refused: the
+// results, made without autograd, would lose it.  (Whether there can be one is
+// asked once a call: of a step's 210 tensors one by one it took 0.7 us.)
+class OnDevice {
+    const bool tangents_ = torch::autograd::ForwardADLevel::try_get_by_idx(0) && c10::AutogradState::get_tls_state().get_fw_grad_mode();
+
+public:
+    void operator()(const Tensor& t, const char* name) const
+    {
+        require(t.defined(), name, " must be a tensor");
+        require(!tangents_ || !t._fw_grad(0).defined(), name, " has a forward-mode tangent: the operators have no forward-mode derivatives");
+        require(t.is_cuda() && t.get_device() == 0, name, " must be on cuda:0");
+        require(t.layout() == at::kStrided, name, " must be a dense tensor");
+    }
+};
 
 int elementType(const Tensor& t, const char* name)
 {
@@ -79,6 +92,7 @@ carl_rows rowsOf(const Tensor& t, bool steps = true)
 carl_attention attentionOf(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& logDecay,
                            const OptTensor& starts, const OptTensor& memory, double scale, bool steps)
 {
+    const OnDevice onDevice;
     const int dims = steps ? 4 : 3;
     const char* lead = steps ? "[batch, steps, " : "[batch, ";
     for (const auto& [t, name] : { std::pair{ &q, "q" }, { &k, "k" }, { &v, "v" } }) {
@@ -257,6 +271,7 @@ Tensor asRows(const Tensor& x)
 
 carl_ffn ffnOf(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t activation)
 {
+    const OnDevice onDevice;
     for (const auto& [t, name] : { std::pair{ &x, "x" }, { &gate, "w_gate" }, { &up, "w_up" }, { &down, "w_down" } }) {
         onDevice(*t, name);
         requireType(t->scalar_type() == x.scalar_type(), "x and the weights must have the same dtype");
@@ -385,6 +400,7 @@ void adamwStep(const py::object& paramList, const py::object& gradList, const py
     const bool eight = n > 0 && first[0].scalar_type() == at::kChar;
     if (eight) require(firstScale.size() == n && secondScale.size() == n, "8-bit moments need exp_avg_scale and exp_avg_sq_scale");
     else require(firstScale.size() == 0 && secondScale.size() == 0, "float32 moments have no scales");
+    const OnDevice onDevice;
     std::vector<carl_adamw_tensor> list(n);
     for (size_t i = 0; i < n; i++) {
         const Tensor &p = params[i], &g = grads[i], &m = first[i], &v = second[i];
@@ -429,6 +445,7 @@ int64_t momentBlocks(const Tensor& m) { return (m.numel() + CARL_ADAMW_BLOCK - 1
 
 std::tuple<Tensor, Tensor> decodeMoments(const Tensor& m, const Tensor& ms, const Tensor& v, const Tensor& vs)
 {
+    const OnDevice onDevice;
     for (const Tensor* t : { &m, &ms, &v, &vs }) {
         onDevice(*t, "moments");
         require(t->is_contiguous(), "moments must be contiguous");
@@ -445,6 +462,7 @@ std::tuple<Tensor, Tensor> decodeMoments(const Tensor& m, const Tensor& ms, cons
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> encodeMoments(const Tensor& m, const Tensor& v)
 {
+    const OnDevice onDevice;
     for (const Tensor* t : { &m, &v }) {
         onDevice(*t, "moments");
         require(t->is_contiguous(), "moments must be contiguous");

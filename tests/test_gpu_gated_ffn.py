@@ -116,6 +116,17 @@ def test_some_gradients(wanted):
         assert torch.equal(g, full[i])
 
 
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_tangents_are_refused(which):
+    from torch.autograd import forward_ad
+
+    tensors = _inputs(8, 40, 24, torch.float32)[:4]
+    with forward_ad.dual_level():
+        tensors[which] = forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        with pytest.raises(ValueError, match="has a forward-mode tangent"):
+            _ops().gated_ffn(*tensors)
+
+
 def test_no_rows():
     x, w_gate, w_up, w_down, dy = _inputs(0, 32, 48, torch.float32)
     leaves = [t.requires_grad_() for t in (x, w_gate, w_up, w_down)]

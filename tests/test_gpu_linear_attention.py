@@ -237,6 +237,21 @@ def test_a_decay_that_is_not_a_number(T, dtype):
     assert torch.equal(torch.isnan(state[:, 1]), isnan[1])
 
 
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 5])
+def test_forward_mode_tangents_are_refused(which):
+    from torch.autograd import forward_ad
+
+    ops = _ops()
+    args = list(_inputs(2, 5, 2, 2, 16, 24, torch.float32)[:6])
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        q, k, v, log_decay, _, memory = args
+        with pytest.raises(ValueError, match="has a forward-mode tangent"):
+            ops.linear_attention(q, k, v, log_decay, initial_state=memory)
+        with pytest.raises(ValueError, match="has a forward-mode tangent"):
+            ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], log_decay, memory)
+
+
 def test_no_steps_and_no_sequences():
     ops = _ops()
     q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(3, 0, 2, 2, 16, 24, torch.float32)

@@ -250,6 +250,28 @@ def test_host_tensors_are_refused():
         optim.encode_moments(one[0], one[0])
 
 
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor needs no gradient, so a call would run, and its result would have no tangent."""
+    from torch.autograd import forward_ad
+
+    x, w, w_down, decay, state = torch.zeros(2, 3, 2, 16), torch.zeros(4, 16), torch.zeros(16, 4), torch.zeros(2), torch.zeros(2, 2, 16, 16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: ops.gated_ffn(dual(x), w, w, w_down), lambda: ops.linear_attention(dual(x), x, x, decay),
+                 lambda: ops.linear_attention_step(dual(x[:, 0]), x[:, 0], x[:, 0], decay, state),
+                 lambda: optim.adamw_step([dual(decay)], [decay], [decay], [decay], step=1, lr=1e-3),
+                 lambda: optim.encode_moments(dual(decay), decay)]
+        for call in calls:
+            with pytest.raises(ValueError, match="has a forward-mode tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="has a forward-mode tangent"):
+                call()
+        with torch.inference_mode(), pytest.raises(ValueError, match="must be on cuda:0"):
+            ops.gated_ffn(x, w, w, w_down)
+
+
 @pytest.mark.parametrize("changes", [{"bits": 4}, {"lr": -1.0}, {"betas": (1.0, 0.9)}, {"eps": -1.0}, {"weight_decay": -1.0}])
 def test_optimizer_refuses(changes):
     with pytest.raises(ValueError):
