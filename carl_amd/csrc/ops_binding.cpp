@@ -122,7 +122,7 @@ carl_attention attentionOf(const Tensor& q, const Tensor& k, const Tensor& v, co
     requireType(logDecay.scalar_type() == at::kFloat, "log_decay must have dtype float32");
     require(logDecay.dim() == 1 && logDecay.size(0) == a.heads, "log_decay must have shape [heads]");
     require(logDecay.is_contiguous(), "log_decay must be contiguous");
-    require(!logDecay.requires_grad(), "log_decay has no gradient: detach it");
+    require(!at::GradMode::is_enabled() || !logDecay.requires_grad(), "log_decay has no gradient: detach it");
     a.log_decay = logDecay.data_ptr<float>();
     if (starts) {
         onDevice(*starts, "starts");

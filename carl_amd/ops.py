@@ -29,7 +29,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     q               [batch, steps, heads, key width], float32, bfloat16 or float16
     k, v            [batch, steps, key heads, key or value width]; query head h
                     reads key head h // (heads / key heads)
-    log_decay       float32 [heads], at most 0; it has no gradient
+    log_decay       float32 [heads], at most 0; it has no gradient, and may ask
+                    for one only where gradients are off
     starts          bool [batch, steps]: steps that begin an episode and see
                     nothing before them (the `done` of the step before)
     initial_state   float32 [batch, heads, key width, value width]; zero without

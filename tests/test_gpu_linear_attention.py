@@ -252,6 +252,29 @@ def test_forward_mode_tangents_are_refused(which):
             ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], log_decay, memory)
 
 
+def test_a_decay_that_is_a_parameter():
+    """Without gradients (acting, scoring) it is a tensor like any other; with them its own is missing, and refused."""
+    ops = _ops()
+    q, k, v, log_decay, starts, memory, _, _ = _inputs(2, 30, 2, 2, 16, 24, torch.float32)
+    weight = torch.nn.Parameter(log_decay.clone())
+    step = [x[:, 0] for x in (q, k, v)]
+    states = [memory.clone() for _ in range(2)]
+    with torch.no_grad():
+        for a, b in zip(ops.linear_attention(q, k, v, weight, starts=starts), ops.linear_attention(q, k, v, log_decay, starts=starts)):
+            assert torch.equal(a, b)
+        a, b = (ops.linear_attention_step(*step, w, s) for w, s in zip((weight, log_decay), states))
+    assert torch.equal(a, b) and torch.equal(*states)
+    with pytest.raises(ValueError, match="log_decay has no gradient"):
+        ops.linear_attention(q, k, v, weight)
+    with pytest.raises(ValueError, match="log_decay has no gradient"):
+        ops.linear_attention_step(*step, weight, states[0])
+    # asked for after it was passed, it is no reason to refuse the backward pass
+    late = log_decay.clone()
+    out, _ = ops.linear_attention(q.requires_grad_(), k, v, late)
+    late.requires_grad_()
+    out.sum().backward()
+
+
 def test_no_steps_and_no_sequences():
     ops = _ops()
     q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(3, 0, 2, 2, 16, 24, torch.float32)
