@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/forward_grad.h>
 
 #include <c10/core/AutogradState.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -34,7 +35,15 @@ void check(int rc)
     throw std::runtime_error(msg);
 }
 
-void* currentStream() { return c10::hip::getCurrentHIPStream(0).stream(); }
+// The current stream of device 0, where all tensors are: that device is made
+// current too while a call launches (the default stream's handle is null,
+// which is any current device's).
+class Queue {
+    const c10::DeviceGuard guard_{ at::Device(at::kCUDA, 0) };
+
+public:
+    operator void*() const { return c10::hip::getCurrentHIPStream(0).stream(); }
+};
 
 // The message is made of its parts only where it is thrown.
 template <typename... Parts> std::string message(const Parts&... parts)
@@ -180,7 +189,7 @@ std::tuple<Tensor, Tensor> linearAttentionForward(const Tensor& q, const Tensor&
     a.final_state = last.data_ptr<float>();
     const Tensor work = workspaceOf(a, false, q);
     a.workspace = work.defined() ? work.data_ptr() : nullptr;
-    check(carl_linear_attention(&a, currentStream()));
+    check(carl_linear_attention(&a, Queue()));
     return { out, last };
 }
 
@@ -230,7 +239,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         a.d_initial_state = dFirst.defined() ? dFirst.data_ptr<float>() : nullptr;
         const Tensor work = workspaceOf(a, true, q);
         a.workspace = work.defined() ? work.data_ptr() : nullptr;
-        check(carl_linear_attention_backward(&a, currentStream()));
+        check(carl_linear_attention_backward(&a, Queue()));
         return { dq, dk, dv, {}, {}, dFirst, {} };
     }
 };
@@ -254,7 +263,7 @@ Tensor linearAttentionStep(const Tensor& q, const Tensor& k, const Tensor& v, co
     carl_attention a = attentionOf(q, k, v, logDecay, starts, state, s, false);
     Tensor out = at::empty({ a.batch, a.heads, a.value_dim }, q.options());
     a.out = rowsOf(out, false);
-    check(carl_linear_attention_step(&a, state.data_ptr<float>(), currentStream()));
+    check(carl_linear_attention_step(&a, state.data_ptr<float>(), Queue()));
     state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
@@ -307,7 +316,7 @@ Tensor gatedFfnForward(const Tensor& x, const Tensor& gate, const Tensor& up, co
     check(carl_gated_ffn_workspace(&f, 0, &bytes));
     const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
     f.workspace = work.data_ptr();
-    check(carl_gated_ffn(&f, currentStream()));
+    check(carl_gated_ffn(&f, Queue()));
     return y;
 }
 
@@ -349,7 +358,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
         check(carl_gated_ffn_workspace(&f, 1, &bytes));
         const Tensor work = at::empty({ bytes }, x.options().dtype(at::kByte));
         f.workspace = work.data_ptr();
-        check(carl_gated_ffn_backward(&f, currentStream()));
+        check(carl_gated_ffn_backward(&f, Queue()));
         return { dx, dg, du, dd, {} };
     }
 };
@@ -436,7 +445,7 @@ void adamwStep(const py::object& paramList, const py::object& gradList, const py
         require(gradScale->numel() == 1, "grad_scale must hold one value");
         h.grad_scale = gradScale->data_ptr<float>();
     }
-    check(carl_adamw_step(list.data(), (int)n, &h, currentStream()));
+    check(carl_adamw_step(list.data(), (int)n, &h, Queue()));
     for (const TensorList* tensors : { &params, &first, &second, &firstScale, &secondScale })
         for (size_t i = 0; i < tensors->size(); i++) (*tensors)[i].unsafeGetTensorImpl()->bump_version();
 }
@@ -456,7 +465,7 @@ std::tuple<Tensor, Tensor> decodeMoments(const Tensor& m, const Tensor& ms, cons
     require(ms.numel() == momentBlocks(m) && vs.numel() == momentBlocks(m), "scales must have one value for each 256 elements");
     Tensor mOut = at::empty(m.sizes(), ms.options()), vOut = at::empty(m.sizes(), ms.options());
     check(carl_adamw_decode(m.data_ptr<int8_t>(), ms.data_ptr<float>(), v.data_ptr<uint8_t>(), vs.data_ptr<float>(),
-                            m.numel(), mOut.data_ptr<float>(), vOut.data_ptr<float>(), currentStream()));
+                            m.numel(), mOut.data_ptr<float>(), vOut.data_ptr<float>(), Queue()));
     return { mOut, vOut };
 }
 
@@ -472,7 +481,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> encodeMoments(const Tensor& m, const 
     Tensor mOut = at::empty(m.sizes(), m.options().dtype(at::kChar)), vOut = at::empty(m.sizes(), m.options().dtype(at::kByte));
     Tensor ms = at::empty({ momentBlocks(m) }, m.options()), vs = at::empty({ momentBlocks(m) }, m.options());
     check(carl_adamw_encode(m.data_ptr<float>(), v.data_ptr<float>(), m.numel(), mOut.data_ptr<int8_t>(),
-                            ms.data_ptr<float>(), vOut.data_ptr<uint8_t>(), vs.data_ptr<float>(), currentStream()));
+                            ms.data_ptr<float>(), vOut.data_ptr<uint8_t>(), vs.data_ptr<float>(), Queue()));
     return { mOut, ms, vOut, vs };
 }
 
