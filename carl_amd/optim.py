@@ -32,7 +32,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     params, grads   float32, bfloat16 or float16, contiguous, each of its own type
     exp_avg, exp_avg_sq   both float32; or int8 and uint8 codes with their
                     scales, one float32 for each 256 elements of a tensor
-    step            the number of this update, 1 for the first
+    step            the number of this update, 1 for the first; a captured call
+                    keeps this and the other numbers in every replay
     grad_scale      a float32 tensor of one value on the GPU, multiplied onto
                     every gradient (a clipping factor that never reaches the host)
     """
@@ -55,7 +56,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with the fused step; bits=8 keeps both moments in 8 bits.
 
     `step(grad_scale=...)` takes a clipping factor as `adamw_step` does.
-    Gradients must be dense; parameters without one are passed over.
+    Parameters must be contiguous and their gradients dense; parameters without
+    a gradient are passed over.  Steps are counted on the host, so `step` is
+    refused while a graph is captured.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -99,6 +102,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step counts its steps on the host: a graph would repeat one step's bias correction")
         loss = None
         if closure is not None:
             with torch.enable_grad():

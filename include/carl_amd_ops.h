@@ -8,7 +8,8 @@
  * carl_last_error().  Every call checks its arguments on the host, queues its
  * kernels on `stream` (a hipStream_t; NULL is the default stream) of the
  * current device and returns; nothing is allocated, copied to the host or
- * kept between calls, so calls can be captured into a HIP graph.  Device
+ * kept between calls, so calls can be captured into a HIP graph (replays keep
+ * the capture's numbers, AdamW's step and rate among them).  Device
  * pointers must be valid on that device; where a call needs scratch memory,
  * a *_workspace function says how many bytes, and the caller's buffer must be
  * 256-byte aligned and unused by other streams until the call's work is done.

@@ -260,3 +260,21 @@ def test_a_graph_of_the_step(bits):
         for n, xs in lists.items():
             for x, y in zip(xs, want[n]):
                 assert torch.equal(x, y)
+
+
+def test_the_optimizer_refuses_to_be_captured():
+    """A captured step would repeat its bias correction; the same optimizer then steps eagerly."""
+    p, q = (torch.nn.Parameter(torch.ones(10, device="cuda")) for _ in range(2))
+    p.grad, q.grad = torch.full_like(p, 0.5), torch.full_like(q, 0.5)
+    opt, other = (_optim().AdamW([x]) for x in (p, q))
+    torch.cuda.synchronize()
+    graph, kept = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    with torch.cuda.graph(graph):
+        kept += 1
+        with pytest.raises(RuntimeError, match="counts its steps on the host"):
+            opt.step()
+    assert not opt.state
+    graph.replay()
+    opt.step()
+    other.step()
+    assert torch.equal(p, q) and kept.item() == 1.0

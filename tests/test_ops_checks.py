@@ -278,6 +278,18 @@ def test_optimizer_refuses(changes):
         optim.AdamW([torch.nn.Parameter(torch.zeros(2))], **changes)
 
 
+def test_the_optimizer_refuses_to_be_captured(monkeypatch):
+    """Before anything is done: no state is made, the closure is not called."""
+    p = torch.nn.Parameter(torch.zeros(2))
+    p.grad = torch.ones(2)
+    opt = optim.AdamW([p])
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="counts its steps on the host"):
+        opt.step(lambda: pytest.fail("called"))
+    assert not opt.state
+
+
 def test_aliases():
     import carl.ops
     import carl.optim
