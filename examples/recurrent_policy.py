@@ -124,6 +124,8 @@ class Rollout:
             self.next_start = terminated | truncated
         batch = {name: torch.stack(x) for name, x in rows.items()}
         batch["ends"] = torch.cat((batch["starts"][1:], self.next_start[None]))
+        # what the episodes that go on are worth after the last step
+        _, batch["next_values"], _ = self.policy(self.next_obs, [m.clone() for m in self.memories], self.next_start)
         return batch | {"memories": first}
 
 
@@ -137,7 +139,7 @@ def returns(rewards: torch.Tensor, ends: torch.Tensor, last: torch.Tensor, disco
 
 def update(policy: RecurrentPolicy, optimizer: AdamW, batch: dict, discount: float = 0.99, clip: float = 1.0) -> float:
     logits, values, _ = policy(batch["obs"], batch["memories"], batch["starts"])
-    target = returns(batch["rewards"], batch["ends"], values[-1].detach(), discount)
+    target = returns(batch["rewards"], batch["ends"], batch["next_values"], discount)
     advantage = target - values.detach()
     loss = -(log_prob(logits, batch["actions"]) * advantage).mean() + 0.5 * (values - target).square().mean()
     optimizer.zero_grad()

@@ -91,3 +91,41 @@ def test_policy_gradient_updates_run(example):
     assert all(bool(torch.isfinite(p).all()) for p in policy.parameters())
     assert any(not torch.equal(a, b) for a, b in zip(before, policy.parameters()))
     env.close()
+
+
+def test_the_loss_is_that_of_the_returns(example):
+    """Returns by hand, in 64 bits: rewards to the episode's end, or to the rollout's and then the value of the
+    observation after it, which a pass over one step more gives."""
+    env, policy, rollout = _setting(example, 24, no_touch_timeout_ticks=8 * 15)
+    with torch.no_grad():
+        policy.value.weight.mul_(30.0)
+    batch = rollout.collect()
+    assert bool(batch["ends"].any()) and not bool(batch["ends"][-1].all())
+    obs = torch.cat((batch["obs"], rollout.next_obs[None]))
+    starts = torch.cat((batch["starts"], rollout.next_start[None]))
+    with torch.no_grad():
+        logits, values, _ = policy(obs, batch["memories"], starts)
+    rewards, ends, values = batch["rewards"].double().cpu(), batch["ends"].cpu(), values.double().cpu()
+    log_probs = example.log_prob(logits[:-1], batch["actions"]).double().cpu()
+
+    def loss(after):
+        total = 0.0
+        for agent in range(rewards.shape[1]):
+            for t in range(24):
+                target, weight = 0.0, 1.0
+                for s in range(t, 24):
+                    target += weight * float(rewards[s, agent])
+                    weight *= 0.99
+                    if ends[s, agent]:
+                        break
+                else:
+                    target += weight * float(after[agent])
+                advantage = target - float(values[t, agent])
+                total += -float(log_probs[t, agent]) * advantage + 0.5 * advantage ** 2
+        return total / rewards.numel()
+
+    # float32 values and log-probabilities of order 1 to 30, good to 1e-4 as the passes agree
+    want, last = loss(values[24]), loss(values[23])
+    assert abs(want - last) > 2e-2 * abs(want)
+    assert example.update(policy, example.AdamW(policy.parameters(), lr=0.0), batch) == pytest.approx(want, rel=2e-3)
+    env.close()
