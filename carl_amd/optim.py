@@ -28,6 +28,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                eps: float = 1e-8, weight_decay: float = 0.01, exp_avg_scale: Sequence[torch.Tensor] | None = None,
                exp_avg_sq_scale: Sequence[torch.Tensor] | None = None, grad_scale: torch.Tensor | None = None) -> None:
     """One AdamW step of every tensor in place, in one launch for 60 tensors.
+    No two of them may overlap.
 
     params, grads   float32, bfloat16 or float16, contiguous, each of its own type
     exp_avg, exp_avg_sq   both float32; or int8 and uint8 codes with their
@@ -74,6 +75,14 @@ class AdamW(torch.optim.Optimizer):
         if not 0.0 <= weight_decay:
             raise ValueError("weight_decay must be non-negative")
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay, "bits": bits})
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        twice = len(set(group["params"])) != len(group["params"])     # one launch would step it by two threads at once
+        if twice or group["bits"] not in (8, 32):
+            self.param_groups.pop()
+            raise ValueError("a parameter is in the group twice" if twice else "bits must be 8 or 32")
 
     def _moments(self, p: torch.Tensor, bits: int) -> dict:
         state = self.state[p]

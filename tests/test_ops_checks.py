@@ -278,6 +278,23 @@ def test_optimizer_refuses(changes):
         optim.AdamW([torch.nn.Parameter(torch.zeros(2))], **changes)
 
 
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
+def test_the_optimizer_refuses_groups():
+    """A parameter that is listed twice (two threads of a launch would step it at once), and other bits in a group."""
+    p, q = (torch.nn.Parameter(torch.zeros(2)) for _ in range(2))
+    with pytest.raises(ValueError, match="in the group twice"):
+        optim.AdamW([p, q, p])
+    with pytest.raises(ValueError, match="bits must be 8 or 32"):
+        optim.AdamW([{"params": [p], "bits": 16}])
+    opt = optim.AdamW([p], bits=8)
+    for group in ({"params": [q, q]}, {"params": [q], "bits": 4}):
+        with pytest.raises(ValueError):
+            opt.add_param_group(group)
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [q], "bits": 32})
+    assert [g["bits"] for g in opt.param_groups] == [8, 32]
+
+
 def test_the_optimizer_refuses_to_be_captured(monkeypatch):
     """Before anything is done: no state is made, the closure is not called."""
     p = torch.nn.Parameter(torch.zeros(2))
