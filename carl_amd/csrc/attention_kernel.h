@@ -559,10 +559,13 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
 #pragma unroll 1
                 for (int s = leave; s < have; s++) {
                     const float x = TileC::element(sC, s, tile + col) * (power((float)(have - inShift - s)) * r.scaleOut);
+                    int past = dimA - quad * 4;         // rows from here stay zero: theirs would be no number with an infinite x
+                    asm volatile("" : "+v"(past));
 #pragma unroll
                     for (int m = 0; m < kTilesA; m++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) memory[o][m][i] += TileA::element(sB, s, m * 16 + quad * 4 + i) * x;
+                        for (int i = 0; i < 4; i++)
+                            memory[o][m][i] += TileA::element(sB, s, m * 16 + quad * 4 + i) * (m * 16 + i < past ? x : 0.0f);
                 }
             }
         }

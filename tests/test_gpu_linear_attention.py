@@ -275,6 +275,21 @@ def test_a_decay_that_is_a_parameter():
     out.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("dk", [3, 40, 64, 100])
+def test_an_infinite_value_is_no_nan(dk, dtype):
+    """With queries and keys above zero it makes its column of the memory, and the outputs from it on, infinite: whether
+    the keys' width fills a tile or not."""
+    q, k, v, log_decay, _, _, _, _ = _inputs(2, 200, 2, 2, dk, 48, dtype, starts=None)
+    q, k = q.abs() + 0.125, k.abs() + 0.125
+    v[0, 10, 1, 5] = math.inf
+    out, final = _ops().linear_attention(q, k, v, torch.full_like(log_decay, -0.01))
+    seen = torch.zeros(200, 48, dtype=torch.bool, device="cuda")
+    seen[10:, 5] = True
+    assert torch.equal(torch.isposinf(out[0, :, 1]), seen) and torch.equal(~torch.isfinite(out[0, :, 1]), seen)
+    assert torch.isposinf(final[0, 1, :, 5]).all() and torch.isfinite(out[1]).all() and torch.isfinite(out[0, :, 0]).all()
+
+
 def test_no_steps_and_no_sequences():
     ops = _ops()
     q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(3, 0, 2, 2, 16, 24, torch.float32)
