@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void joinKernel(const Pass pass)
                 const int i = i0 + j;
                 if (i >= pass.segments) break;
                 r.parts[((r.backwards ? pass.segments - 1 - i : i) * units + unit) * size + e] = m;
-                m = f[j] == 0.0f ? own[j] : m * f[j] + own[j];        // nothing of a memory that an episode's start clears
+                m = signbit(f[j]) ? own[j] : m * f[j] + own[j];       // nothing of a memory that an episode's start clears
             }
         }
         if (r.last) r.last[unit * size + (r.lastSwapped ? swapped : e)] = m;

@@ -344,7 +344,9 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
 
     // the memory after the last chunk goes to the caller (or to the sums that do)
     const bool handed = r.last && (kStates || pass.segments == 1);
-    float factor = 1.0f;      // of the memory over the whole segment
+    // of the memory over the whole segment; with its sign set where a start closes
+    // it (a weight that is zero in float32 closes nothing: a NaN stays)
+    float factor = 1.0f;
 #pragma unroll 1
     for (int n = 0; n < chunks; n++) {
         const int64_t t0 = chunkStart(n);
@@ -465,7 +467,7 @@ void attentionKernel(const Pass pass, const int firstRole, const int roles)
         }
 
         const float keep = closed ? 0.0f : power((float)have);
-        factor = closed ? 0.0f : factor * keep;
+        factor = closed ? -1.0f : factor * keep;
         if (!careful) {
             vec<T, 4> c[kOwn][kBlocks];
 #pragma unroll

@@ -290,6 +290,21 @@ def test_an_infinite_value_is_no_nan(dk, dtype):
     assert torch.isposinf(final[0, 1, :, 5]).all() and torch.isfinite(out[1]).all() and torch.isfinite(out[0, :, 0]).all()
 
 
+@pytest.mark.parametrize("T", [100, 600])
+def test_a_memory_that_is_not_a_number_is_never_forgotten(T):
+    """Without a start its column is NaN to the end, though its weight is zero in float32 after some steps: whether the
+    sequence is split or not, and in the gradients of a NaN after the last step."""
+    ops = _ops()
+    q, k, v, log_decay, _, memory, dout, dfinal = _inputs(2, T, 2, 2, 32, 48, torch.float32, starts=None)
+    memory[0, 1, 3, 5], dfinal[0, 1, 3, 5] = math.nan, math.nan
+    leaves = [x.requires_grad_() for x in (q, k, v, memory)]
+    out, final = ops.linear_attention(*leaves[:3], torch.full_like(log_decay, -2.0), initial_state=leaves[3])
+    assert torch.isnan(out[0, :, 1, 5]).all() and torch.isnan(final[0, 1, 3, 5]) and torch.isfinite(out[1]).all()
+    dq, dk, dv, first = torch.autograd.grad([out, final], leaves, [dout, dfinal])
+    assert torch.isnan(dk[0, :, 1, 3]).all() and torch.isnan(dv[0, :, 1, 5]).all() and torch.isnan(first[0, 1, 3, 5])
+    assert torch.isnan(dq[0, :, 1, 3]).all() and all(bool(torch.isfinite(x[1]).all()) for x in (dq, dk, dv, first))
+
+
 def test_no_steps_and_no_sequences():
     ops = _ops()
     q, k, v, log_decay, starts, memory, dout, dfinal = _inputs(3, 0, 2, 2, 16, 24, torch.float32)
