@@ -263,8 +263,8 @@ Tensor linearAttentionStep(const Tensor& q, const Tensor& k, const Tensor& v, co
     carl_attention a = attentionOf(q, k, v, logDecay, starts, state, s, false);
     Tensor out = at::empty({ a.batch, a.heads, a.value_dim }, q.options());
     a.out = rowsOf(out, false);
+    state.unsafeGetTensorImpl()->bump_version();        // refuses what may not be changed in place
     check(carl_linear_attention_step(&a, state.data_ptr<float>(), Queue()));
-    state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 
@@ -445,9 +445,10 @@ void adamwStep(const py::object& paramList, const py::object& gradList, const py
         require(gradScale->numel() == 1, "grad_scale must hold one value");
         h.grad_scale = gradScale->data_ptr<float>();
     }
-    check(carl_adamw_step(list.data(), (int)n, &h, Queue()));
+    // refuses what may not be changed in place
     for (const TensorList* tensors : { &params, &first, &second, &firstScale, &secondScale })
         for (size_t i = 0; i < tensors->size(); i++) (*tensors)[i].unsafeGetTensorImpl()->bump_version();
+    check(carl_adamw_step(list.data(), (int)n, &h, Queue()));
 }
 
 int64_t momentBlocks(const Tensor& m) { return (m.numel() + CARL_ADAMW_BLOCK - 1) / CARL_ADAMW_BLOCK; }

@@ -278,3 +278,12 @@ def test_the_optimizer_refuses_to_be_captured():
     opt.step()
     other.step()
     assert torch.equal(p, q) and kept.item() == 1.0
+
+
+def test_inference_tensors_are_refused_before_they_are_changed():
+    lists = [torch.ones(10, device="cuda") for _ in range(4)]
+    with torch.inference_mode():
+        lists[3] = torch.ones(10, device="cuda")
+    with pytest.raises(RuntimeError, match="inference tensor"):
+        _optim().adamw_step(*([x] for x in lists), step=1, lr=1e-3)
+    assert all(bool((x == 1).all()) for x in lists)

@@ -362,6 +362,21 @@ def test_a_step_that_starts_forgets(bad):
     assert not torch.isfinite(out[1]).any()
 
 
+def test_an_inference_state_is_refused_before_it_is_changed():
+    """As torch's own changes in place are: outside inference mode, with the memory as it was."""
+    ops = _ops()
+    q, k, v, log_decay, _, memory, _, _ = _inputs(2, 1, 2, 2, 40, 48, torch.float32)
+    q, k, v = q[:, 0], k[:, 0], v[:, 0]
+    with torch.inference_mode():
+        state = memory.clone()
+    with pytest.raises(RuntimeError, match="inference tensor"):
+        ops.linear_attention_step(q, k, v, log_decay, state)
+    assert torch.equal(state, memory)
+    with torch.inference_mode():
+        ops.linear_attention_step(q, k, v, log_decay, state)
+    assert not torch.equal(state, memory)
+
+
 def test_a_state_at_an_odd_address():
     ops = _ops()
     q, k, v, log_decay, starts, memory, _, _ = _inputs(3, 1, 2, 2, 16, 32, torch.float32)
