@@ -45,7 +45,7 @@ __device__ inline float activate(float g, int activation, float* slopeOut = null
     if (activation == CARL_GELU) {
         const float c = 1.5957691216057308f, g2 = g * g;       // 2 sqrt(2 / pi)
         z = c * (g + 0.044715f * g2 * g);
-        slope = c * (1.0f + 0.134145f * g2);
+        slope = c * (1.0f + 0.134145f * fminf(g2, 1e30f));     // finite: it meets zeros in the tails
     }
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
     const float act = g * s;

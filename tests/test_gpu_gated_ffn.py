@@ -76,6 +76,14 @@ def test_large_activations(dtype):
         _check(x, w_gate * 40, w_up, w_down, dy, activation)
 
 
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gates_whose_square_is_past_float32(dtype, activation):
+    """Gates about 10^20: flat tails, whose slopes are 0 and 1."""
+    x, w_gate, w_up, w_down, dy = _inputs(40, 32, 48, dtype)
+    _check(x, w_gate * 1e20, w_up, w_down * 1e-20, dy, activation)
+
+
 def test_leading_dimensions_strides_and_odd_addresses():
     ops = _ops()
     x, w_gate, w_up, w_down, dy = _inputs(60, 32, 48, torch.bfloat16)
