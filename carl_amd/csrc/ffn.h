@@ -12,6 +12,16 @@
 // kept from the forward pass in 16 bits they would be rounded twice, in 32
 // bits they would cost more traffic than the products take.
 //
+// float16's range holds neither any h, dg and du nor the bits of small ones:
+// they are written times a power of two, the same for all rows, and the
+// products that read them undo it.  |act(g)| <= |g| and norms bound what they
+// can be:
+//   |h| <= |x| |Wg| |x| |Wu|      |dg|, |du| <= 1.13 |dy| |Wd| |x| max(|Wg|, |Wu|)
+// with the largest norm of a row of x and dy, of a row of Wg and Wu and of a
+// column of Wd each (rows that are not finite aside: what they give is not
+// either).  The bound goes to 2^15 at most, so that nothing overflows and 29
+// powers of two below keep all their bits.
+//
 // Two kernels do all products.  `product` multiplies rows by rows (both
 // operands contiguous along the sum); `outer` sums over rows (both operands
 // contiguous across it), for the weights' gradients.  Both copy panels of 128
@@ -43,13 +53,14 @@ struct ProductArgs {
     int64_t outStride;
     int32_t outWidth;      // columns that are written (gate, grad: to the end of the padding)
     int32_t outWide;       // rows are 16-byte aligned
+    const float* scale[2]; // float16: factors of out[0] and of the others
 };
 
 // The forward pass of a few rows: operands as they lie, whatever their addresses.
 struct ThinArgs {
     const void* a;                // [m, k], rows aStride apart: x, or h
     const void *b0, *b1;          // [n, k]; b1 for gate
-    void* out;                    // [m, n], rows outStride apart: h (of up to 16 rows in float32), or y
+    void* out;                    // [m, n], rows outStride apart: h (of up to 16 rows, or of float16, in float32), or y
     int64_t aStride, outStride;
     int32_t m, n, k, activation;
 };
@@ -79,12 +90,26 @@ struct SumJob {
     const float* part;
     void* out;
     int64_t count;
+    const float* scale;    // float16: a factor of the sum, or NULL for none
 };
 
 struct SumArgs {
     SumJob job[3];
     int32_t splits, jobs;
 };
+
+// The largest rows by their norm, of x, w_gate, w_up and, backwards, of dy and
+// of w_down's transpose, and from them the factors of h and of dg and du.
+struct ScaleArgs {
+    Panel rows[5];
+    float* part;           // [5][kScaleBlocks]
+    float* scale;          // of h, of dg and du, and what undoes each
+    int32_t panels;        // 3 or 5
+};
+constexpr int kScaleBlocks = 512;
+enum { kScaleH = 0, kScaleD = 1, kUnscaleH = 2, kUnscaleD = 3 };
+
+int launchScale(const ScaleArgs& args, hipStream_t stream);      // float16
 
 template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream);
 template <typename T> int launchThin(bool gate, const ThinArgs& args, hipStream_t stream);

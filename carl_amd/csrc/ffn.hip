@@ -91,11 +91,24 @@ private:
     PackArgs packs_{};
 };
 
+// float16: where the factors of h, dg and du are.
+ScaleArgs scalesOf(const carl_ffn& f, Plan& plan)
+{
+    ScaleArgs a{};
+    if (f.type != CARL_OP_F16) return a;
+    a.part = static_cast<float*>(plan.take(5 * kScaleBlocks * 4));
+    a.scale = static_cast<float*>(plan.take(4 * 4));
+    return a;
+}
+
+const float* factor(const ScaleArgs& a, int which) { return a.scale ? a.scale + which : nullptr; }
+
 // Up to so many rows the forward pass is a matter of latency.
 constexpr int kThinRows = 128;
 
 struct Forward {
     Panel x{}, gate{}, up{}, down{}, h;
+    ScaleArgs scales{};
     explicit Forward(const carl_ffn& f, Plan& plan)
     {
         if (f.rows <= kThinRows) {
@@ -108,11 +121,17 @@ struct Forward {
         up = plan.rows(f.w_up, f.inner, f.width, f.width);
         down = plan.rows(f.w_down, f.width, f.inner, f.inner);
         h = plan.scratch(f.rows, f.inner);
+        scales = scalesOf(f, plan);
+        scales.panels = 3;
+        scales.rows[0] = x;
+        scales.rows[1] = gate;
+        scales.rows[2] = up;
     }
 };
 
 struct Backward {
     Panel x, dy, gate, up, downT, gateT{}, upT{}, h, dg, du;
+    ScaleArgs scales{};
     OuterArgs outer{};
     int tile = 256;
     explicit Backward(const carl_ffn& f, Plan& plan)
@@ -127,6 +146,10 @@ struct Backward {
         h = plan.scratch(f.rows, f.inner);
         dg = plan.scratch(f.rows, f.inner);
         du = plan.scratch(f.rows, f.inner);
+        scales = scalesOf(f, plan);
+        scales.panels = 5;
+        const Panel normed[5] = { x, gate, up, dy, downT };
+        std::copy(normed, normed + 5, scales.rows);
 
         // the three weights' gradients in one launch, rows split until the
         // tiles fill the compute units
@@ -180,6 +203,8 @@ int outerProducts(int type, const OuterArgs& a, int tile, hipStream_t s)
     return launchOuter<f16>(a, tile, s);
 }
 
+int scale(int type, const ScaleArgs& a, hipStream_t s) { return type == CARL_OP_F16 ? launchScale(a, s) : (int)CARL_OK; }
+
 int sums(int type, const SumArgs& a, hipStream_t s)
 {
     if (type == CARL_OP_F32) return launchSum<float>(a, s);
@@ -232,7 +257,9 @@ int carl_gated_ffn(const carl_ffn* f, void* stream)
         return thin(f->type, false, down, s);
     }
     if (int rc = pack(f->type, plan.packs(), s)) return rc;
+    if (int rc = scale(f->type, p.scales, s)) return rc;
     ProductArgs a{};
+    a.scale[0] = factor(p.scales, kScaleH);
     a.a[0] = p.x;
     a.b[0] = p.gate;
     a.b[1] = p.up;
@@ -248,6 +275,7 @@ int carl_gated_ffn(const carl_ffn* f, void* stream)
     y.a[0] = p.h;
     y.b[0] = p.down;
     y.terms = 1;
+    y.scale[0] = factor(p.scales, kUnscaleH);
     return product(f->type, kProductPlain, y, s);
 }
 
@@ -259,14 +287,17 @@ int carl_gated_ffn_backward(const carl_ffn* f, void* stream)
     void* const weights[3] = { f->dw_gate, f->dw_up, f->dw_down };
     if (f->rows == 0) {
         for (void* w : weights)
-            if (w) sum.job[sum.jobs++] = { nullptr, w, (int64_t)f->width * f->inner };
+            if (w) sum.job[sum.jobs++] = { nullptr, w, (int64_t)f->width * f->inner, nullptr };
         return sum.jobs ? sums(f->type, sum, s) : CARL_OK;
     }
     if (!f->workspace) return fail(CARL_ERR_VALUE, "null workspace");
     Plan plan(f->type, static_cast<char*>(f->workspace));
     const Backward p(*f, plan);
     if (int rc = pack(f->type, plan.packs(), s)) return rc;
+    if (int rc = scale(f->type, p.scales, s)) return rc;
     ProductArgs a{};
+    a.scale[0] = factor(p.scales, kScaleH);
+    a.scale[1] = factor(p.scales, kScaleD);
     a.a[0] = p.x;
     a.a[1] = p.dy;
     a.b[0] = p.gate;
@@ -289,6 +320,7 @@ int carl_gated_ffn_backward(const carl_ffn* f, void* stream)
         d.b[0] = p.gateT;
         d.b[1] = p.upT;
         d.terms = 2;
+        d.scale[0] = factor(p.scales, kUnscaleD);
         if (int rc = product(f->type, kProductPlain, d, s)) return rc;
     }
     OuterArgs outer = p.outer;
@@ -301,7 +333,7 @@ int carl_gated_ffn_backward(const carl_ffn* f, void* stream)
         outer.part[k] = p.outer.part[j];
         outer.m[k] = p.outer.m[j];
         outer.n[k] = p.outer.n[j];
-        sum.job[k] = { p.outer.part[j], weights[j], (int64_t)f->width * f->inner };
+        sum.job[k] = { p.outer.part[j], weights[j], (int64_t)f->width * f->inner, factor(p.scales, j < 2 ? kUnscaleD : kUnscaleH) };
     }
     if (outer.jobs == 0) return CARL_OK;
     if (int rc = outerProducts(f->type, outer, p.tile, s)) return rc;

@@ -192,6 +192,11 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
                 if (n + e < args.outWidth) to[e] = (T)x[e];
         }
     };
+    float scaleFirst = 1.0f, scaleRest = 1.0f;
+    if constexpr (std::is_same_v<T, f16>) {
+        scaleFirst = *args.scale[0];
+        if constexpr (kKind == kProductGrad) scaleRest = *args.scale[1];
+    }
 #pragma unroll
     for (int i = 0; i < kTM; i++) {
         const int64_t row = m0 + (wm * kTM + i) * 16 + col;
@@ -215,6 +220,16 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
                     }
                 }
             }
+        if constexpr (std::is_same_v<T, f16>) {
+#pragma unroll
+            for (int e = 0; e < kRun; e++) {
+                first[e] *= scaleFirst;
+                if constexpr (kKind == kProductGrad) {
+                    second[e] *= scaleRest;
+                    third[e] *= scaleRest;
+                }
+            }
+        }
         // the padding of rows is zero whatever a row holds (an infinity meets
         // the zeros past the weights' last row)
         if (kKind != kProductPlain && n0 + kBN > args.n) {
@@ -244,9 +259,9 @@ __global__ __launch_bounds__((ProductShape<T, kKind, kBM, kBN, kWM, kWN, kRowByt
 // 256 by 683: the block's two launches 14.0 us before, laid out and in tiles
 // of 64 rows, now 9.5 us.  Up to 16 rows h goes from one launch to the other
 // in float32 and meets w_down as two terms of bfloat16 (8.0 us for 16 rows
-// either way; for 34 it would be 12.3 us); float16, whose range does not hold
-// such terms, runs that product in float32.  h's rows are padded with zeros to
-// multiples of 64.
+// either way; for 34 it would be 12.3 us); float16, whose range holds neither h
+// nor such terms, runs that product in float32 whatever the rows.  h's rows are
+// padded with zeros to multiples of 64.
 constexpr float kMostBf16 = 0x1.fep127f;
 
 template <typename T> __device__ inline uint4 loadAny(const T* p, int have)
@@ -268,7 +283,7 @@ template <typename T, bool kGate, int kTM> __global__ __launch_bounds__(512) voi
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * kTM;
     // rows past the end are the last one again; their results are not stored
     const int n = n0 + col < args.n ? n0 + col : args.n - 1;
-    using H = std::conditional_t<kTM == 1, float, T>;
+    using H = std::conditional_t<kTM == 1 || std::is_same_v<T, f16>, float, T>;
     using A = std::conditional_t<kGate, T, H>;
     const T* b[kNB];
     b[0] = static_cast<const T*>(args.b0) + (int64_t)n * args.k;
@@ -465,10 +480,11 @@ __global__ __launch_bounds__(kWM* kWN * 64) void outerKernel(const OuterArgs arg
 template <typename T> __global__ __launch_bounds__(256) void sumKernel(const SumArgs args)
 {
     const SumJob& job = args.job[blockIdx.y];
+    const float scale = std::is_same_v<T, f16> && job.scale ? *job.scale : 1.0f;
     for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < job.count; e += (int64_t)gridDim.x * 256) {
         float x = 0.0f;
         for (int s = 0; s < args.splits; s++) x += job.part[s * job.count + e];
-        static_cast<T*>(job.out)[e] = (T)x;
+        static_cast<T*>(job.out)[e] = (T)(std::is_same_v<T, f16> ? x * scale : x);
     }
 }
 

@@ -81,8 +81,10 @@ int carl_linear_attention_step(const carl_attention* a, float* state, void* stre
  *   h = act(x w_gate^T) * (x w_up^T)        y = h w_down^T
  * and its gradients.  All matrices hold one element type; products are summed
  * in float32, and h (of more than 16 rows) and the gradients of both
- * projections are rounded to that type once, where the next product reads them.  The backward pass needs only
- * the inputs: it computes both projections again. */
+ * projections are rounded to that type once, where the next product reads them
+ * (float16's times a power of two that the largest possible one fits, so that
+ * they do not leave its range; its h of up to 128 rows is not rounded).  The
+ * backward pass needs only the inputs: it computes both projections again. */
 enum { CARL_SILU = 0, CARL_GELU = 1 };  /* GELU in its tanh form */
 
 typedef struct carl_ffn {

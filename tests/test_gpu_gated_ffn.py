@@ -76,6 +76,35 @@ def test_large_activations(dtype):
         _check(x, w_gate * 40, w_up, w_down, dy, activation)
 
 
+@pytest.mark.parametrize("what,factors", [
+    ("inner values of 100,000 and more", (1.0, 400.0, 400.0, 0.01, 0.001)),
+    ("inner values below float16's normal numbers", (1.0, 0.002, 0.002, 64.0, 0.01)),
+    ("gradients of outputs below them", (1.0, 30.0, 1.0, 1.0, 2.0 ** -18)),
+    ("gradients of projections past its largest", (0.002, 0.002, 640.0, 256.0, 512.0))])
+@pytest.mark.parametrize("N", [20, 100, 200, 5000])
+def test_float16_keeps_what_its_range_does_not_hold(N, what, factors, monkeypatch):
+    """Inputs and results are within float16's range, values on the way are not: each is off by one rounding all the same."""
+    tensors = [t * f for t, f in zip(_inputs(N, 40, 56, torch.float16), factors)]
+    if "below float16's normal" in what:
+        tensors[0][N // 2] *= 32.0        # a row that stands out
+    x, w_gate, w_up, w_down, dy = tensors
+    leaves = [t.detach().requires_grad_() for t in tensors[:4]]
+    y = _ops().gated_ffn(*leaves)
+    got = dict(zip(("y", *GRADS), (y, *torch.autograd.grad(y, leaves, dy))))
+    monkeypatch.setitem(ref.TINY, torch.float16, 0.0)
+    value, bound = ref.ffn(*tensors[:4], "silu", dy)
+    # 2^-25 of values that are written times what takes the product of the largest norms to at least 2^14
+    xs, gs, us, ds, ys = (ref.wide(t).abs() for t in tensors)
+    norm = [t.square().sum(d).sqrt().max() for t, d in ((xs, 1), (gs, 1), (us, 1), (ds, 0), (ys, 1))]
+    h = 2.0 ** -39 * norm[0] ** 2 * norm[1] * norm[2]
+    d = 2.0 ** -39 * norm[4] * norm[3] * norm[0] * torch.maximum(norm[1], norm[2])
+    more = {"y": h * ds.sum(1), "dx": d * (gs.sum(0) + us.sum(0)), "dw_gate": d * xs.sum(0), "dw_up": d * xs.sum(0),
+            "dw_down": h * ys.sum(0)[:, None]}
+    for name, result in got.items():
+        assert float(value[name].abs().max()) < 65504
+        ref.assert_within(result, value[name], bound[name] + more[name] + 2.0 ** -24, name)
+
+
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_gates_whose_square_is_past_float32(dtype, activation):
