@@ -13,13 +13,9 @@ using bf16 = __bf16;
 using f16 = _Float16;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
 template <typename T, int N> using vec = typename VecOf<T, N>::type;
