@@ -106,7 +106,7 @@ struct ScaleArgs {
     float* scale;          // of h, of dg and du, and what undoes each
     int32_t panels;        // 3 or 5
 };
-constexpr int kScaleBlocks = 512;
+constexpr int kScaleBlocks = 2048;
 enum { kScaleH = 0, kScaleD = 1, kUnscaleH = 2, kUnscaleD = 3 };
 
 int launchScale(const ScaleArgs& args, hipStream_t stream);      // float16

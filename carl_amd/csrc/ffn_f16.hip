@@ -55,6 +55,8 @@ __global__ __launch_bounds__(256) void normKernel(const ScaleArgs args)
     if (threadIdx.x == 0) args.part[blockIdx.y * kScaleBlocks + blockIdx.x] = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
 }
 
+constexpr int kScaleThreads = 512;
+
 // A power of two that takes `bound` to [2^14, 2^15], and its inverse.
 __device__ inline void factorOf(float bound, float& scale, float& unscale)
 {
@@ -64,11 +66,13 @@ __device__ inline void factorOf(float bound, float& scale, float& unscale)
     unscale = ldexpf(1.0f, exponent - 15);
 }
 
-__global__ __launch_bounds__(kScaleBlocks) void scaleKernel(const ScaleArgs args)
+__global__ __launch_bounds__(kScaleThreads) void scaleKernel(const ScaleArgs args)
 {
-    __shared__ float parts[5][kScaleBlocks / 64];
+    __shared__ float parts[5][kScaleThreads / 64];
     for (int j = 0; j < args.panels; j++) {
-        float most = args.part[j * kScaleBlocks + threadIdx.x];
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kScaleBlocks; i += kScaleThreads) most = fmaxf(most, args.part[j * kScaleBlocks + i + threadIdx.x]);
         for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
         if ((threadIdx.x & 63) == 0) parts[j][threadIdx.x >> 6] = most;
     }
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(kScaleBlocks) void scaleKernel(const ScaleArgs args
     if (threadIdx.x != 0) return;
     float norm[5] = {};
     for (int j = 0; j < args.panels; j++) {
-        for (int i = 0; i < kScaleBlocks / 64; i++) norm[j] = fmaxf(norm[j], parts[j][i]);
+        for (int i = 0; i < kScaleThreads / 64; i++) norm[j] = fmaxf(norm[j], parts[j][i]);
         norm[j] = sqrtf(norm[j]);
     }
     const float x = norm[0], gate = norm[1], up = norm[2], dy = norm[3], down = norm[4];
@@ -90,7 +94,7 @@ int launchScale(const ScaleArgs& args, hipStream_t stream)
 {
     normKernel<<<dim3(kScaleBlocks, (unsigned)args.panels), 256, 0, stream>>>(args);
     if (int rc = launched("norms of rows")) return rc;
-    scaleKernel<<<dim3(1), kScaleBlocks, 0, stream>>>(args);
+    scaleKernel<<<dim3(1), kScaleThreads, 0, stream>>>(args);
     return launched("factors of float16 values");
 }
 
