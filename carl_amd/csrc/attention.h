@@ -30,9 +30,10 @@
 // What bounds it: no unit throughout, but the chain from a chunk's copies over
 // P to its outputs, which only other workgroups of the compute unit hide.
 // 16,384 x 64 steps, 8 heads of 64 in bfloat16: forward 2.26 ms (8.6 GB, 3.8
-// TB/s), gradients 4.2 ms (11.8 GB, 2.8 TB/s), four workgroups a compute unit.
-// 6 x 4,603 steps, 8 heads of 128 on 4: 85 and 308 us for the outputs' and the
-// gradients' launch, two workgroups a compute unit, matrix cores busy 10%.
+// TB/s), gradients 4.2 ms (11.8 GB, 2.8 TB/s), four workgroups a compute unit;
+// in float16, most of whose products run on the float32 instructions, 2.47 and
+// 6.4 ms.  6 x 4,603 steps, 8 heads of 128 on 4: 88 and 316 us for the outputs'
+// and the gradients' launch, two workgroups a compute unit, matrix cores busy 10%.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -219,18 +219,22 @@ Rows rowsOf(const carl_rows& r) { return Rows{ r.data, r.batch, r.step, r.head }
 
 // How a sequence is split.  One workgroup walks a whole sequence of one head
 // where those and the pass's directions fill the GPU; with fewer, segments of
-// at least 256 steps, as many as run at once (two workgroups a compute unit
-// with the widest rows, three or four with others).  They need the memories
-// before each segment, which a first launch sums up (reading keys and values
-// once more) and a second joins.  6 sequences of 4,603 steps, 8 heads of 128:
-// 18 segments both ways, as 1,024 workgroups would have them, 855 us with
-// gradients.
+// about 256 steps or more (never under 192, in whole 64s), as many as run at once
+// (two workgroups a compute unit with the widest rows, three or four with
+// others).  Backwards that counts all three directions, as they run where the
+// widths of keys and values are equal; where they differ run() launches them
+// one after the other, and each has fewer workgroups than would fit.  Segments
+// need the memories before them, which a first launch sums up (reading keys and
+// values once more) and a second joins.  6 sequences of 4,603 steps, 8 heads of
+// 128: 18 segments both ways, as 1,024 workgroups would have them, 855 us with
+// gradients; as here 617.
 //
 // Backwards fewer directions are summed up than run, and the first launch would
 // leave compute units with one workgroup: it takes the segments in two halves
 // where all of them run at once (three workgroups a compute unit, or as many
-// as of the others): 6 x 4,603 with gradients 636 us with whole segments, 601
-// with halves.
+// as of the others) and their length allows it, a multiple of 128: 6 x 4,603
+// (segments of 1,536) with gradients 636 us with whole segments, 601 with
+// halves, when that was measured.
 struct Split {
     int segments;
     int64_t steps;

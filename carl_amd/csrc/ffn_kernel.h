@@ -375,7 +375,8 @@ __global__ __launch_bounds__(kWM* kWN * 64) void outerKernel(const OuterArgs arg
     __shared__ __align__(1024) char stages[2 * kStage];
 
     const int job = blockIdx.y;
-    // splits in turn over the 8 dies: a split's rows are read through one cache
+    // a tile's splits next to each other (with 8 of them, or a multiple, a
+    // split's rows go through one die's cache; other counts spread them)
     const int split = (int)(blockIdx.x % args.splits), tile = (int)(blockIdx.x / args.splits);
     const int m = args.m[job], n = args.n[job], tilesN = (n + kB - 1) / kB;
     if (tile >= tilesN * ((m + kB - 1) / kB)) return;
@@ -539,12 +540,13 @@ int launchProductShape(const ProductArgs& args, hipStream_t stream)
 //            grad   2,048 x 512 x 1,408   64 x 64 84   128 x 64 107       32,768 x 512 x 1,408   1,153 and 1,102
 //            plain  2,048 x 1,408 to 512   64 x 64 36.9   128 x 64 56.9     8,192 x 2,816 to 1,024   402 and 379
 //                   62,000 x 684 to 256   128 x 128 188   256 x 256 194
-// At 262,144 rows of 512 by 1,408 in bfloat16 gate runs at 830 TFLOP/s, grad at
-// 630 and plain at 1,010 to 1,100 (a large library product: 1,300; one of
-// gate's sizes: 770).  gate and grad are bound by their tiles' short sums
-// (512), under which the copies' latency and the stores of h, dg and du (2.2
-// GB: 440 us of grad's 1,790) do not disappear; float32 by its matrix
-// instructions (110 to 117 TFLOP/s; the library's product 154).
+// At 262,144 rows of 512 by 1,408 in bfloat16 gate runs at 860 TFLOP/s, grad at
+// 590 and plain at 940 to 1,070 (the library's products of the same operands'
+// layout: 1,320 to 1,580 for large ones, 875 and 1,260 for gate's and plain's
+// sizes).  gate and grad are bound by their tiles' short sums (512), under which
+// the copies' latency and the stores of h, dg and du (2.2 GB: 470 us of grad's
+// 1,920) do not disappear; float32 by its matrix instructions (102 to 110
+// TFLOP/s; the library's product 154).
 template <typename T> int launchProduct(int kind, const ProductArgs& args, hipStream_t stream)
 {
     constexpr bool wide = sizeof(T) == 4;
