@@ -33,13 +33,14 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
                     for one only where gradients are off
     starts          bool [batch, steps]: steps that begin an episode and see
                     nothing before them (the `done` of the step before)
-    initial_state   float32 [batch, heads, key width, value width]; zero without
+    initial_state   float32 [batch, heads, key width, value width], contiguous;
+                    zero without
     scale           key width ** -0.5 without
 
-    Widths are at most 128.  Batch, step and head strides are free (a rollout
-    kept as [steps, batch, ...] is passed transposed, and its outputs and
-    gradients come in the same order); the last dimension is contiguous.
-    Gradients reach q, k, v and initial_state, once.
+    Widths are at most 128, batch times heads 4,194,304.  Batch, step and head
+    strides are free (a rollout kept as [steps, batch, ...] is passed
+    transposed, and its outputs and gradients come in the same order); the last
+    dimension is contiguous.  Gradients reach q, k, v and initial_state, once.
     """
     return _ops.linear_attention(q, k, v, log_decay, starts, initial_state, scale)
 
@@ -48,8 +49,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                           state: torch.Tensor, *, starts: torch.Tensor | None = None,
                           scale: float | None = None) -> torch.Tensor:
     """One step of `linear_attention` for every agent: q, k and v without the
-    steps' dimension, starts [batch], and the memory `state` updated in place.
-    For acting; it has no gradient."""
+    steps' dimension, starts [batch], and the contiguous memory `state` updated
+    in place.  For acting; it has no gradient."""
     return _ops.linear_attention_step(q, k, v, log_decay, state, starts, scale)
 
 
@@ -62,10 +63,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     w_down          [width, inner]
     activation      "silu", or "gelu" in its tanh form
 
-    All of one type; products are summed in float32.  Widths are at most 65,536,
-    rows 2^28, and rows times the larger width about 2^36.  Gradients reach x and the
-    weights, once; the backward pass computes both projections again instead of
-    keeping them.
+    All of one type; products are summed in float32.  Widths are at most
+    65,536, rows 2^28, and rows times the larger width about 2^36.  Gradients
+    reach x and the weights, once; the backward pass computes both projections
+    again instead of keeping them.
     """
     return _ops.gated_ffn(x, w_gate, w_up, w_down, activation)
 
