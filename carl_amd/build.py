@@ -38,7 +38,7 @@ HIP_FLAGS = [
 
 ENGINE_SOURCES = ["engine.hip", "arena.cpp", "adamw.hip", "attention.hip", "attention_f32.hip",
                   "attention_bf16.hip", "attention_f16.hip",
-                  "ffn.hip", "ffn_f32.hip", "ffn_bf16.hip", "ffn_f16.hip"]
+                  "ffn.hip", "ffn_f32.hip", "ffn_bf16.hip", "ffn_f16.hip", "actions.hip", "norm.hip", "int8.hip"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -1,0 +1,419 @@
+// norm.hip - root-mean-square norm with the addition before it, its gradients,
+// and rows in 8 bits.
+//
+//   s = x + residual          u = s / sqrt(mean(s^2) + eps)          y = u w
+//   d = r (g - u mean(g u)) + dsum     with g = dy w, r = 1 / sqrt(mean(s^2) + eps)
+//   dw = sum over rows of dy u
+//   codes of t = s w: m = max |t|, code = rint(t (127 / m)), scale = (m / 127) r
+// The factor r cancels in the codes, so they come from s and w alone, with one
+// rounding a step: whatever the order of the sum of squares, the same codes.
+//
+// What bounds it: memory.  A row's elements stay in registers between the
+// reduction and the output, so each is read and written once; the lanes that
+// share a row are as few as hold it in one to four pieces of 16 bytes each.
+// The sum s is rounded to the elements' type once, as it is kept, and the norm
+// is that of the rounded sum: the backward pass reads it and needs nothing else.
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/carl_amd_ops.h"
+#include "elem.h"
+#include "reduce.h"
+#include "status.h"
+
+using namespace carl;
+
+namespace {
+
+enum { kPlain = 0, kNormCodes = 1, kRowCodes = 2 };
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    int64_t xRow, residualRow, rows;
+    int32_t width;
+    float eps;
+    void *sum, *y;
+    int8_t* codes;
+    int64_t codesRow;
+    float* scale;
+};
+
+struct NormGradArgs {
+    const void *s, *dy, *dsum, *weight;
+    int64_t sRow, dyRow, dsumRow, rows;
+    int32_t width;
+    float eps;
+    void* dx;
+    void* dw;          // written by a launch of one workgroup
+    float* part;       // [workgroups, width], of a launch of more
+};
+
+// Squares of values this large add up to less than float32's largest; of rows
+// whose do not, and of none else, the squares are those of 2^-80 times the values.
+constexpr float kMostSquares = 0x1p120f, kSmaller = 0x1p-80f;
+constexpr float kLeast = 0x1p-100f;       // a row's largest magnitude counts as this much at least
+
+// 16 bytes of a row from any address; zeros past the row's end.
+template <typename T> __device__ inline vec<T, 16 / sizeof(T)> loadPiece(const T* p, int have)
+{
+    constexpr int kE = 16 / sizeof(T);
+    vec<T, kE> r;
+    if (have >= kE) __builtin_memcpy(&r, p, 16);
+    else
+#pragma unroll
+        for (int j = 0; j < kE; j++) r[j] = j < have ? p[j] : T(0);
+    return r;
+}
+
+template <typename T> __device__ inline void storePiece(T* p, int have, vec<T, 16 / sizeof(T)> r)
+{
+    constexpr int kE = 16 / sizeof(T);
+    if (have >= kE) __builtin_memcpy(p, &r, 16);
+    else
+#pragma unroll
+        for (int j = 0; j < kE; j++)
+            if (j < have) p[j] = r[j];
+}
+
+// Over the lanes of a row: kLanes of a wave, or a workgroup.
+template <typename Op, int kLanes, typename X> __device__ inline X overRow(X x, X* slots)
+{
+    if constexpr (kLanes <= 64) return overLanes<Op, kLanes>(x);
+    else return overWorkgroup<Op, kLanes>(x, slots);
+}
+
+template <typename T, int kKind, int kLanes, int kPieces>
+__global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(const NormArgs a)
+{
+    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 256 ? 256 : kLanes, kGroups = kThreads / kLanes;
+    __shared__ float slots[kThreads / 64];
+    __shared__ uint32_t bits[kThreads / 64];
+    const int lane = threadIdx.x % kLanes;
+    vec<float, kE> w[kPieces];
+    if constexpr (kKind != kRowCodes)
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE;
+            w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight) + at, a.width - at));
+        }
+    for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+        vec<float, kE> s[kPieces];
+        vec<T, kE> in[kPieces], more[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE;
+            in[p] = loadPiece(static_cast<const T*>(a.x) + row * a.xRow + at, a.width - at);
+            if (kKind != kRowCodes && a.residual) more[p] = loadPiece(static_cast<const T*>(a.residual) + row * a.residualRow + at, a.width - at);
+        }
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            s[p] = toFloat<T, kE>(in[p]);
+            if (kKind != kRowCodes && a.residual) {
+                const int at = (p * kLanes + lane) * kE;
+                const auto kept = fromFloat<T, kE>(s[p] + toFloat<T, kE>(more[p]));
+                storePiece(static_cast<T*>(a.sum) + row * a.width + at, a.width - at, kept);
+                s[p] = toFloat<T, kE>(kept);
+            }
+        }
+        float r = 1.0f;
+        if constexpr (kKind != kRowCodes) {
+            float squares = 0.0f, factor = 1.0f;
+#pragma unroll
+            for (int p = 0; p < kPieces; p++)
+#pragma unroll
+                for (int j = 0; j < kE; j++) squares += s[p][j] * s[p][j];
+            squares = overRow<Add, kLanes>(squares, slots);
+            if (!(squares < kMostSquares)) {
+                factor = kSmaller;
+                squares = 0.0f;
+#pragma unroll
+                for (int p = 0; p < kPieces; p++) {
+                    s[p] *= factor;
+#pragma unroll
+                    for (int j = 0; j < kE; j++) squares += s[p][j] * s[p][j];
+                }
+                squares = overRow<Add, kLanes>(squares, slots);
+            }
+            r = 1.0f / sqrtf(squares / (float)a.width + a.eps * factor * factor);
+        }
+        if constexpr (kKind == kPlain) {
+#pragma unroll
+            for (int p = 0; p < kPieces; p++) {
+                const int at = (p * kLanes + lane) * kE;
+                storePiece(static_cast<T*>(a.y) + row * a.width + at, a.width - at, fromFloat<T, kE>(s[p] * r * w[p]));
+            }
+        } else {
+            // bit patterns of magnitudes order as unsigned numbers, infinity and NaN last
+            uint32_t most = 0;
+#pragma unroll
+            for (int p = 0; p < kPieces; p++) {
+                if constexpr (kKind == kNormCodes) s[p] *= w[p];
+#pragma unroll
+                for (int j = 0; j < kE; j++) most = Most::of(most, __float_as_uint(s[p][j]) & 0x7fffffffu);
+            }
+            most = overRow<Most, kLanes>(most, bits);
+            const bool finite = most < 0x7f800000u;
+            const float m = fmaxf(__uint_as_float(most), kLeast), inverse = finite ? 127.0f / m : 0.0f;
+            if (lane == 0) a.scale[row] = finite ? m / 127.0f * r : __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int p = 0; p < kPieces; p++) {
+                const int at = (p * kLanes + lane) * kE, have = a.width - at;
+                vec<int8_t, kE> code;
+#pragma unroll
+                for (int j = 0; j < kE; j++) code[j] = finite ? (int8_t)(int)rintf(s[p][j] * inverse) : (int8_t)0;
+                int8_t* to = a.codes + row * a.codesRow + at;
+                if (have >= kE) __builtin_memcpy(to, &code, kE);
+                else
+#pragma unroll
+                    for (int j = 0; j < kE; j++)
+                        if (j < have) to[j] = code[j];
+            }
+        }
+    }
+}
+
+template <typename T, int kLanes, int kPieces>
+__global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(const NormGradArgs a)
+{
+    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 256 ? 256 : kLanes, kGroups = kThreads / kLanes;
+    constexpr int kColumns = kLanes * kPieces * kE;
+    __shared__ __align__(32) float sums[kGroups > 1 ? kGroups * kColumns : kThreads / 64];
+    float* const slots = sums;            // a row of a whole workgroup has no columns to add up
+    const int lane = threadIdx.x % kLanes;
+    vec<float, kE> w[kPieces], dw[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; p++) {
+        const int at = (p * kLanes + lane) * kE;
+        w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight) + at, a.width - at));
+        dw[p] = vec<float, kE>(0.0f);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+        vec<T, kE> in[kPieces], out[kPieces], on[kPieces];
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE;
+            in[p] = loadPiece(static_cast<const T*>(a.s) + row * a.sRow + at, a.width - at);
+            out[p] = loadPiece(static_cast<const T*>(a.dy) + row * a.dyRow + at, a.width - at);
+            if (a.dsum) on[p] = loadPiece(static_cast<const T*>(a.dsum) + row * a.dsumRow + at, a.width - at);
+        }
+        // sums of s^2 and of g s in one pass, with s times a power of two where its squares need one
+        float squares, inner, factor = 1.0f;
+        const auto sumUp = [&]() {
+            squares = inner = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kPieces; p++) {
+                const auto s = toFloat<T, kE>(in[p]) * factor, g = toFloat<T, kE>(out[p]) * w[p];
+#pragma unroll
+                for (int j = 0; j < kE; j++) {
+                    squares += s[j] * s[j];
+                    inner += g[j] * s[j];
+                }
+            }
+            squares = overRow<Add, kLanes>(squares, slots);
+            inner = overRow<Add, kLanes>(inner, slots);
+        };
+        sumUp();
+        if (!(squares < kMostSquares)) {
+            factor = kSmaller;
+            sumUp();
+        }
+        const float r = 1.0f / sqrtf(squares / (float)a.width + a.eps * factor * factor);
+        const float mean = inner / (float)a.width * r, own = r * factor;
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE;
+            const auto u = toFloat<T, kE>(in[p]) * factor * r, dy = toFloat<T, kE>(out[p]);
+            dw[p] += dy * u;
+            if (!a.dx) continue;
+            auto d = (dy * w[p] - u * mean) * own;
+            if (a.dsum) d += toFloat<T, kE>(on[p]);
+            storePiece(static_cast<T*>(a.dx) + row * a.width + at, a.width - at, fromFloat<T, kE>(d));
+        }
+    }
+    if (!a.part && !a.dw) return;
+    const auto write = [&](int column, float x) {
+        if (column >= a.width) return;
+        if (a.part) a.part[(int64_t)blockIdx.x * a.width + column] = x;
+        else static_cast<T*>(a.dw)[column] = (T)x;
+    };
+    if constexpr (kGroups > 1) {
+        float* const mine = sums + threadIdx.x / kLanes * kColumns;
+#pragma unroll
+        for (int p = 0; p < kPieces; p++) *reinterpret_cast<vec<float, kE>*>(mine + (p * kLanes + lane) * kE) = dw[p];
+        __syncthreads();
+        for (int c = threadIdx.x; c < kColumns; c += kThreads) {
+            float x = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kGroups; g++) x += sums[g * kColumns + c];
+            write(c, x);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < kPieces; p++)
+#pragma unroll
+            for (int j = 0; j < kE; j++) write((p * kLanes + lane) * kE + j, dw[p][j]);
+    }
+}
+
+// Workgroups' parts of dw: 64 columns a workgroup, the parts dealt to its 16 waves.
+template <typename T> __global__ __launch_bounds__(1024) void partsKernel(const float* part, int parts, int width, T* dw)
+{
+    __shared__ float sums[16][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = blockIdx.x * 64 + lane;
+    float x = 0.0f;
+    if (column < width)
+        for (int i = wave; i < parts; i += 16) x += part[(int64_t)i * width + column];
+    sums[wave][lane] = x;
+    __syncthreads();
+    if (wave != 0 || column >= width) return;
+    for (int i = 1; i < 16; i++) x += sums[i][lane];
+    dw[column] = (T)x;
+}
+
+constexpr int64_t kMostRows = (int64_t)1 << 40;
+
+// The lanes that share a row, and the pieces that each takes of it: as few
+// lanes as hold the row in one piece each up to a wave, then more pieces, then
+// more waves.
+template <typename T, typename F> void withShape(int width, F&& run)
+{
+    const int pieces = (int)((width * sizeof(T) + 15) / 16);
+    const auto lanes = [&](auto l, auto p) { run(l, p); };
+    using std::integral_constant;
+    if (pieces <= 16) lanes(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else if (pieces <= 32) lanes(integral_constant<int, 32>(), integral_constant<int, 1>());
+    else if (pieces <= 64) lanes(integral_constant<int, 64>(), integral_constant<int, 1>());
+    else if (pieces <= 128) lanes(integral_constant<int, 64>(), integral_constant<int, 2>());
+    else if (pieces <= 256) lanes(integral_constant<int, 64>(), integral_constant<int, 4>());
+    else if (pieces <= 1024) lanes(integral_constant<int, 256>(), integral_constant<int, 4>());
+    else lanes(integral_constant<int, 1024>(), integral_constant<int, 4>());
+}
+
+constexpr int groupsOf(int lanes) { return lanes < 256 ? 256 / lanes : 1; }
+constexpr int threadsOf(int lanes) { return lanes < 256 ? 256 : lanes; }
+
+// Enough workgroups to fill the GPU; each goes on with rows further down.
+int blocksOf(int64_t rows, int lanes, int most)
+{
+    const int64_t groups = groupsOf(lanes);
+    return (int)std::min<int64_t>((rows + groups - 1) / groups, lanes <= 256 ? most : most / 4);
+}
+
+constexpr int kForwardBlocks = 2048, kGradBlocks = 1024;
+
+template <typename T, int kKind> void launchNorm(const NormArgs& a, hipStream_t stream)
+{
+    withShape<T>(a.width, [&](auto lanes, auto pieces) {
+        normKernel<T, kKind, lanes(), pieces()><<<dim3(blocksOf(a.rows, lanes(), kForwardBlocks)), threadsOf(lanes()), 0, stream>>>(a);
+    });
+}
+
+template <int kKind> int norm(int type, const NormArgs& a, hipStream_t stream)
+{
+    if (type == CARL_OP_F32) launchNorm<float, kKind>(a, stream);
+    else if (type == CARL_OP_BF16) launchNorm<bf16, kKind>(a, stream);
+    else launchNorm<f16, kKind>(a, stream);
+    return launched("norm");
+}
+
+template <typename T> int gradBlocks(const carl_norm& n)
+{
+    int blocks = 0;
+    withShape<T>(n.width, [&](auto lanes, auto) { blocks = blocksOf(n.rows, lanes(), kGradBlocks); });
+    return blocks;
+}
+
+int gradBlocks(const carl_norm& n) { return n.type == CARL_OP_F32 ? gradBlocks<float>(n) : gradBlocks<bf16>(n); }
+
+template <typename T> int normBackward(const carl_norm& n, hipStream_t stream)
+{
+    const int blocks = gradBlocks<T>(n);
+    NormGradArgs a{ n.sum, n.dy, n.d_sum, n.weight, n.sum_row, n.dy_row, n.d_sum_row, n.rows, n.width, n.eps, n.d_x, nullptr, nullptr };
+    if (n.d_weight && blocks > 1) a.part = static_cast<float*>(n.workspace);
+    else a.dw = n.d_weight;
+    withShape<T>(n.width, [&](auto lanes, auto pieces) {
+        normGradKernel<T, lanes(), pieces()><<<dim3(blocks), threadsOf(lanes()), 0, stream>>>(a);
+    });
+    if (int rc = launched("norm's gradients")) return rc;
+    if (!a.part) return CARL_OK;
+    partsKernel<T><<<dim3((n.width + 63) / 64), 1024, 0, stream>>>(a.part, blocks, n.width, static_cast<T*>(n.d_weight));
+    return launched("norm's weight gradient");
+}
+
+int checkNorm(const carl_norm* n, bool normed)
+{
+    if (!n) return fail(CARL_ERR_VALUE, "null norm argument");
+    if (n->type != CARL_OP_F32 && n->type != CARL_OP_BF16 && n->type != CARL_OP_F16) return fail(CARL_ERR_TYPE, "unknown element type");
+    if (n->width < 1 || n->width > CARL_NORM_MAX_DIM) return fail(CARL_ERR_VALUE, "width must be in [1, 16384]");
+    if (n->rows < 0 || n->rows > kMostRows) return fail(CARL_ERR_VALUE, "rows are out of range");
+    if (!normed) return CARL_OK;
+    if (!(n->eps >= CARL_NORM_MIN_EPS) || !std::isfinite(n->eps)) return fail(CARL_ERR_VALUE, "eps must be finite and at least 1e-30");
+    if (!n->weight) return fail(CARL_ERR_VALUE, "null weight");
+    return CARL_OK;
+}
+
+NormArgs argsOf(const carl_norm& n)
+{
+    return { n.x, n.residual, n.weight, n.x_row, n.residual_row, n.rows, n.width, n.eps, n.sum, n.y, n.codes, n.codes_row, n.scale };
+}
+
+}  // namespace
+
+extern "C" {
+
+int carl_rms_norm(const carl_norm* n, void* stream)
+{
+    if (int rc = checkNorm(n, true)) return rc;
+    if (n->rows == 0) return CARL_OK;
+    if (!n->x || !n->y || (n->residual && !n->sum)) return fail(CARL_ERR_VALUE, "null norm tensor");
+    return norm<kPlain>(n->type, argsOf(*n), (hipStream_t)stream);
+}
+
+int carl_rms_norm_int8(const carl_norm* n, void* stream)
+{
+    if (int rc = checkNorm(n, true)) return rc;
+    if (n->rows == 0) return CARL_OK;
+    if (!n->x || !n->codes || !n->scale || (n->residual && !n->sum)) return fail(CARL_ERR_VALUE, "null norm tensor");
+    if (n->codes_row < n->width) return fail(CARL_ERR_VALUE, "rows of codes overlap");
+    return norm<kNormCodes>(n->type, argsOf(*n), (hipStream_t)stream);
+}
+
+int carl_quantize_int8(const carl_norm* n, void* stream)
+{
+    if (int rc = checkNorm(n, false)) return rc;
+    if (n->rows == 0) return CARL_OK;
+    if (!n->x || !n->codes || !n->scale) return fail(CARL_ERR_VALUE, "null tensor of rows");
+    if (n->codes_row < n->width) return fail(CARL_ERR_VALUE, "rows of codes overlap");
+    return norm<kRowCodes>(n->type, argsOf(*n), (hipStream_t)stream);
+}
+
+int carl_rms_norm_workspace(const carl_norm* n, int64_t* bytes)
+{
+    if (!bytes) return fail(CARL_ERR_VALUE, "null norm argument");
+    if (int rc = checkNorm(n, false)) return rc;
+    const int blocks = gradBlocks(*n);
+    *bytes = blocks > 1 ? (int64_t)blocks * n->width * 4 : 0;
+    return CARL_OK;
+}
+
+int carl_rms_norm_backward(const carl_norm* n, void* stream)
+{
+    if (int rc = checkNorm(n, true)) return rc;
+    if (!n->d_x && !n->d_weight) return CARL_OK;
+    if (n->rows > 0 && (!n->sum || !n->dy)) return fail(CARL_ERR_VALUE, "null norm tensor");
+    const hipStream_t s = (hipStream_t)stream;
+    if (n->rows == 0) {
+        if (!n->d_weight) return CARL_OK;
+        const dim3 grid((n->width + 63) / 64);
+        if (n->type == CARL_OP_F32) partsKernel<float><<<grid, 1024, 0, s>>>(nullptr, 0, n->width, static_cast<float*>(n->d_weight));
+        else if (n->type == CARL_OP_BF16) partsKernel<bf16><<<grid, 1024, 0, s>>>(nullptr, 0, n->width, static_cast<bf16*>(n->d_weight));
+        else partsKernel<f16><<<grid, 1024, 0, s>>>(nullptr, 0, n->width, static_cast<f16*>(n->d_weight));
+        return launched("norm's weight gradient");
+    }
+    if (n->d_weight && !n->workspace && gradBlocks(*n) > 1) return fail(CARL_ERR_VALUE, "null workspace");
+    if (n->type == CARL_OP_F32) return normBackward<float>(*n, s);
+    if (n->type == CARL_OP_BF16) return normBackward<bf16>(*n, s);
+    return normBackward<f16>(*n, s);
+}
+
+}  // extern "C"

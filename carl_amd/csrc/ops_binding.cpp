@@ -7,6 +7,7 @@
 // operation; outputs and scratch memory come from torch's allocator.
 #include <torch/extension.h>
 
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/forward_grad.h>
 
 #include <c10/core/AutogradState.h>
@@ -371,6 +372,391 @@ Tensor gatedFfn(const Tensor& x, const Tensor& gate, const Tensor& up, const Ten
     return GatedFfn::apply(x, gate, up, down, which);
 }
 
+// ----------------------------------------------------------------- actions
+
+// The checks of logits, heads and mask; the sizes of the call.
+carl_actions actionsOf(const Tensor& logits, const std::vector<int64_t>& heads, const OptTensor& mask, std::vector<int32_t>& sizes)
+{
+    const OnDevice onDevice;
+    onDevice(logits, "logits");
+    carl_actions a{};
+    a.type = elementType(logits, "logits");
+    require(!heads.empty() && heads.size() <= CARL_ACTIONS_MAX_HEADS, "heads must have 1 to 64 sizes");
+    int64_t total = 0;
+    for (const int64_t n : heads) {
+        require(n >= 1 && n <= CARL_ACTIONS_MAX_LOGITS, "head sizes must be at least 1, and 16,384 in all at most");
+        sizes.push_back((int32_t)n);
+        total += n;
+    }
+    require(total <= CARL_ACTIONS_MAX_LOGITS, "head sizes must be at least 1, and 16,384 in all at most");
+    require(logits.dim() >= 1 && logits.size(-1) == total, "logits must have shape [..., sum of heads]");
+    a.rows = logits.numel() / total;
+    a.heads = (int32_t)heads.size();
+    a.sizes = sizes.data();
+    if (mask) {
+        onDevice(*mask, "mask");
+        requireType(mask->scalar_type() == at::kBool, "mask must have dtype bool");
+        require(mask->sizes() == logits.sizes(), "mask must have the logits' shape");
+    }
+    return a;
+}
+
+// The tensors of a call, alive until it is queued.
+struct ActionRows {
+    Tensor logits, mask, actions;
+
+    ActionRows(carl_actions& a, const Tensor& l, const OptTensor& m, const Tensor& given) : logits(asRows(l))
+    {
+        a.logits = logits.data_ptr();
+        a.logits_row = logits.stride(0);
+        if (m) {
+            mask = asRows(*m);
+            a.mask = static_cast<const uint8_t*>(mask.data_ptr());
+            a.mask_row = mask.stride(0);
+        }
+        if (!given.defined()) return;
+        const OnDevice onDevice;
+        onDevice(given, "actions");
+        requireType(given.scalar_type() == at::kInt || given.scalar_type() == at::kLong, "actions must have dtype int32 or int64");
+        require(given.dim() == l.dim() && given.size(-1) == a.heads && given.sizes().slice(0, l.dim() - 1) == l.sizes().slice(0, l.dim() - 1),
+                "actions must have shape [..., heads]");
+        actions = asRows(given);
+        a.actions = actions.data_ptr();
+        a.actions_row = actions.stride(0);
+        a.actions_wide = given.scalar_type() == at::kLong;
+    }
+};
+
+std::tuple<Tensor, Tensor> actionLogProbForward(const Tensor& logits, const Tensor& actions, const std::vector<int64_t>& heads,
+                                                const OptTensor& mask)
+{
+    std::vector<int32_t> sizes;
+    carl_actions a = actionsOf(logits, heads, mask, sizes);
+    const ActionRows rows(a, logits, mask, actions);
+    const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+    Tensor logProb = at::empty(lead, logits.options().dtype(at::kFloat)), entropy = at::empty(lead, logits.options().dtype(at::kFloat));
+    a.log_prob = logProb.data_ptr<float>();
+    a.entropy = entropy.data_ptr<float>();
+    check(carl_action_log_prob(&a, Queue()));
+    return { logProb, entropy };
+}
+
+struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& actions,
+                                                  const std::vector<int64_t>& heads, const OptTensor& mask)
+    {
+        auto [logProb, entropy] = actionLogProbForward(logits, actions, heads, mask);
+        ctx->save_for_backward({ logits, actions, mask ? *mask : Tensor() });
+        ctx->saved_data["heads"] = heads;
+        ctx->set_materialize_grads(false);
+        return { logProb, entropy };
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        if (at::GradMode::is_enabled()) throw std::runtime_error("action_log_prob has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined() && !grads[1].defined()) return { {}, {}, {}, {} };
+        const OptTensor mask = saved[2].defined() ? OptTensor(saved[2]) : std::nullopt;
+        const Tensor logits = saved[0].detach();
+        std::vector<int32_t> sizes;
+        carl_actions a = actionsOf(logits, ctx->saved_data["heads"].toIntVector(), mask, sizes);
+        const ActionRows rows(a, logits, mask, saved[1]);
+        // one value for all rows (the gradient of a mean, say) is read as it is
+        Tensor held[2];
+        const auto column = [&](int i, const float*& at, int64_t& step) {
+            if (!grads[i].defined()) return;
+            const bool one = std::all_of(grads[i].strides().begin(), grads[i].strides().end(), [](int64_t s) { return s == 0; });
+            held[i] = one ? grads[i] : grads[i].contiguous();
+            at = held[i].data_ptr<float>();
+            step = one ? 0 : 1;
+        };
+        column(0, a.d_log_prob, a.d_log_prob_step);
+        column(1, a.d_entropy, a.d_entropy_step);
+        Tensor d = at::empty(logits.sizes(), logits.options());
+        a.d_logits = d.data_ptr();
+        check(carl_action_log_prob_backward(&a, Queue()));
+        return { d, {}, {}, {} };
+    }
+};
+
+std::tuple<Tensor, Tensor> actionLogProb(const Tensor& logits, const Tensor& actions, const std::vector<int64_t>& heads, const OptTensor& mask)
+{
+    if (!wantsGradient({ &logits })) return actionLogProbForward(logits, actions, heads, mask);
+    auto out = ActionLogProb::apply(logits, actions, heads, mask);
+    return { out[0], out[1] };
+}
+
+// Operators that have no gradient say so where one is asked for.
+void requireNoGradient(std::initializer_list<const Tensor*> tensors, const char* name)
+{
+    require(!wantsGradient(tensors), name, " has no gradient: call it under torch.no_grad()");
+}
+
+std::tuple<Tensor, Tensor> topActions(const Tensor& logits, const std::vector<int64_t>& heads, int64_t k, const OptTensor& mask, const OptTensor& noise)
+{
+    requireNoGradient({ &logits, noise ? &*noise : &logits }, "top_actions");
+    require(k >= 1 && k <= CARL_ACTIONS_MAX_K, "k must be in [1, 64]");
+    std::vector<int32_t> sizes;
+    carl_actions a = actionsOf(logits, heads, mask, sizes);
+    Tensor noiseRows;
+    if (noise) {
+        const OnDevice onDevice;
+        onDevice(*noise, "noise");
+        requireType(noise->scalar_type() == at::kFloat, "noise must have dtype float32");
+        require(noise->sizes() == logits.sizes(), "noise must have the logits' shape");
+        noiseRows = asRows(*noise);
+        a.noise = noiseRows.data_ptr<float>();
+        a.noise_row = noiseRows.stride(0);
+    }
+    const ActionRows rows(a, logits, mask, Tensor());
+    std::vector<int64_t> shape = logits.sizes().slice(0, logits.dim() - 1).vec();
+    shape.push_back(a.heads);
+    shape.push_back(k);
+    Tensor best = at::empty(shape, logits.options().dtype(at::kInt)), logProb = at::empty(shape, logits.options().dtype(at::kFloat));
+    a.k = (int32_t)k;
+    a.best = best.data_ptr<int32_t>();
+    a.log_prob = logProb.data_ptr<float>();
+    check(carl_top_actions(&a, Queue()));
+    return { best, logProb };
+}
+
+// ------------------------------------------- root-mean-square norm, 8 bits
+
+carl_norm normOf(const Tensor& x, const Tensor* weight, const Tensor* residual, double eps)
+{
+    const OnDevice onDevice;
+    onDevice(x, "x");
+    carl_norm n{};
+    n.type = elementType(x, "x");
+    require(x.dim() >= 1, "x must have shape [..., width]");
+    const int64_t width = x.size(-1);
+    require(width >= 1 && width <= CARL_NORM_MAX_DIM, "width must be in [1, 16384]");
+    n.rows = x.numel() / width;
+    n.width = (int32_t)width;
+    n.eps = (float)eps;
+    if (weight) {
+        onDevice(*weight, "weight");
+        requireType(weight->scalar_type() == x.scalar_type(), "x and weight must have the same dtype");
+        require(weight->dim() == 1 && weight->size(0) == width, "weight must have shape [width]");
+    }
+    if (residual) {
+        onDevice(*residual, "residual");
+        requireType(residual->scalar_type() == x.scalar_type(), "x and residual must have the same dtype");
+        require(residual->sizes() == x.sizes(), "residual must have x's shape");
+    }
+    return n;
+}
+
+// The tensors of a call, alive until it is queued; x's, the weight's and the residual's places.
+struct NormRows {
+    Tensor x, weight, residual, sum;
+
+    NormRows(carl_norm& n, const Tensor& in, const Tensor* w, const Tensor* r) : x(asRows(in))
+    {
+        n.x = x.data_ptr();
+        n.x_row = x.stride(0);
+        if (w) {
+            weight = w->contiguous();
+            n.weight = weight.data_ptr();
+        }
+        if (!r) return;
+        residual = asRows(*r);
+        n.residual = residual.data_ptr();
+        n.residual_row = residual.stride(0);
+        sum = at::empty(in.sizes(), in.options());
+        n.sum = sum.data_ptr();
+    }
+};
+
+std::tuple<Tensor, Tensor> rmsNormForward(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps)
+{
+    const Tensor* r = residual ? &*residual : nullptr;
+    carl_norm n = normOf(x, &weight, r, eps);
+    const NormRows rows(n, x, &weight, r);
+    Tensor y = at::empty(x.sizes(), x.options());
+    n.y = y.data_ptr();
+    check(carl_rms_norm(&n, Queue()));
+    return { y, rows.sum };
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                                  const OptTensor& residual, double eps)
+    {
+        auto [y, sum] = rmsNormForward(x, weight, residual, eps);
+        ctx->save_for_backward({ residual ? sum : x, weight });
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["added"] = residual.has_value();
+        ctx->set_materialize_grads(false);
+        if (!residual) return { y };
+        return { y, sum };
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        if (at::GradMode::is_enabled()) throw std::runtime_error("rms_norm has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const bool added = ctx->saved_data["added"].toBool();
+        const Tensor dSum = added ? grads[1] : Tensor();
+        if (!grads[0].defined()) return { dSum, {}, dSum, {} };      // the sum alone was used
+        const Tensor s = saved[0].detach(), weight = saved[1].detach();
+        carl_norm n = normOf(s, &weight, nullptr, ctx->saved_data["eps"].toDouble());
+        const Tensor rows = asRows(s), w = weight.contiguous(), dy = asRows(grads[0]), on = dSum.defined() ? asRows(dSum) : Tensor();
+        n.weight = w.data_ptr();
+        n.sum = rows.data_ptr();
+        n.sum_row = rows.stride(0);
+        n.dy = dy.data_ptr();
+        n.dy_row = dy.stride(0);
+        if (on.defined()) {
+            n.d_sum = on.data_ptr();
+            n.d_sum_row = on.stride(0);
+        }
+        const bool stream = ctx->needs_input_grad(0) || (added && ctx->needs_input_grad(2));
+        const Tensor dx = stream ? at::empty(s.sizes(), s.options()) : Tensor();
+        const Tensor dw = ctx->needs_input_grad(1) ? at::empty(weight.sizes(), weight.options()) : Tensor();
+        n.d_x = dx.defined() ? dx.data_ptr() : nullptr;
+        n.d_weight = dw.defined() ? dw.data_ptr() : nullptr;
+        int64_t bytes = 0;
+        check(carl_rms_norm_workspace(&n, &bytes));
+        const Tensor work = dw.defined() && bytes ? at::empty({ bytes }, s.options().dtype(at::kByte)) : Tensor();
+        n.workspace = work.defined() ? work.data_ptr() : nullptr;
+        check(carl_rms_norm_backward(&n, Queue()));
+        return { ctx->needs_input_grad(0) ? dx : Tensor(), dw, added && ctx->needs_input_grad(2) ? dx : Tensor(), {} };
+    }
+};
+
+py::object rmsNorm(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps)
+{
+    if (!wantsGradient({ &x, &weight, residual ? &*residual : &x })) {
+        auto [y, sum] = rmsNormForward(x, weight, residual, eps);
+        return residual ? py::object(py::make_tuple(y, sum)) : py::cast(y);
+    }
+    auto out = RmsNorm::apply(x, weight, residual, eps);
+    return residual ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+}
+
+// Codes in rows that begin every 16 bytes.
+Tensor codesLike(const Tensor& x, int64_t width)
+{
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = (width + 15) / 16 * 16;
+    const Tensor rows = at::empty(shape, x.options().dtype(at::kChar));
+    return rows.narrow(-1, 0, width);
+}
+
+py::tuple normCodes(const Tensor& x, const Tensor* weight, const OptTensor& residual, double eps)
+{
+    const Tensor* r = residual ? &*residual : nullptr;
+    carl_norm n = normOf(x, weight, r, eps);
+    const NormRows rows(n, x, weight, r);
+    const Tensor codes = codesLike(x, n.width), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    n.codes = codes.data_ptr<int8_t>();
+    n.codes_row = (n.width + 15) / 16 * 16;
+    n.scale = scale.data_ptr<float>();
+    check(weight ? carl_rms_norm_int8(&n, Queue()) : carl_quantize_int8(&n, Queue()));
+    return residual ? py::make_tuple(codes, scale, rows.sum) : py::make_tuple(codes, scale);
+}
+
+py::tuple rmsNormInt8(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps)
+{
+    requireNoGradient({ &x, &weight, residual ? &*residual : &x }, "rms_norm_int8");
+    return normCodes(x, &weight, residual, eps);
+}
+
+py::tuple quantizeInt8(const Tensor& x)
+{
+    requireNoGradient({ &x }, "quantize_int8");
+    return normCodes(x, nullptr, std::nullopt, 0.0);
+}
+
+// ------------------------------------------------------ products in 8 bits
+
+void weightsOf(const Tensor& w, const Tensor& scale, int64_t width, int64_t columns, const char* name, const char* scaleName)
+{
+    const OnDevice onDevice;
+    onDevice(w, name);
+    requireType(w.scalar_type() == at::kChar, name, " must have dtype int8");
+    require(w.dim() == 2 && w.size(0) == columns && w.size(1) == width, name, " must have shape [columns, width]");
+    onDevice(scale, scaleName);
+    requireType(scale.scalar_type() == at::kFloat, scaleName, " must have dtype float32");
+    require(scale.dim() == 1 && scale.size(0) == columns, scaleName, " must have shape [columns]");
+}
+
+Tensor int8Product(const Tensor& x, const Tensor& xScale, const Tensor& w, const Tensor& wScale, const Tensor* up, const Tensor* upScale,
+                   const OptTensor& bias, int64_t activation, at::ScalarType dtype)
+{
+    const OnDevice onDevice;
+    onDevice(x, "x");
+    requireType(x.scalar_type() == at::kChar, "x must have dtype int8");
+    require(x.dim() >= 1, "x must have shape [..., width]");
+    onDevice(xScale, "x_scale");
+    requireType(xScale.scalar_type() == at::kFloat, "x_scale must have dtype float32");
+    require(xScale.sizes() == x.sizes().slice(0, x.dim() - 1), "x_scale must have a value for each row of x");
+    require(w.defined() && w.dim() == 2, up ? "w_gate" : "weight", " must have shape [columns, width]");
+    const int64_t width = x.size(-1), columns = w.size(0);
+    weightsOf(w, wScale, width, columns, up ? "w_gate" : "weight", up ? "gate_scale" : "weight_scale");
+    if (up) weightsOf(*up, *upScale, width, columns, "w_up", "up_scale");
+    require(width >= 1 && width <= CARL_INT8_MAX_DIM, "width must be in [1, 65536]");
+    require(columns >= 1 && columns <= CARL_INT8_MAX_DIM, "columns must be in [1, 65536]");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = columns;
+    carl_int8_linear p{};
+    const Tensor rows = asRows(x), scale = xScale.contiguous(), weight = asRows(w), weightScale = wScale.contiguous();
+    Tensor upRows, upScales, biases;
+    p.rows = x.numel() / width;
+    p.width = (int32_t)width;
+    p.columns = (int32_t)columns;
+    p.activation = (int32_t)activation;
+    p.x = rows.data_ptr<int8_t>();
+    p.x_row = rows.stride(0);
+    p.x_scale = scale.data_ptr<float>();
+    p.w = weight.data_ptr<int8_t>();
+    p.w_row = weight.stride(0);
+    p.w_scale = weightScale.data_ptr<float>();
+    if (up) {
+        upRows = asRows(*up);
+        upScales = upScale->contiguous();
+        p.w_up = upRows.data_ptr<int8_t>();
+        p.w_up_row = upRows.stride(0);
+        p.w_up_scale = upScales.data_ptr<float>();
+    }
+    if (bias) {
+        onDevice(*bias, "bias");
+        requireType(bias->scalar_type() == dtype, "bias must have the result's dtype");
+        require(bias->dim() == 1 && bias->size(0) == columns, "bias must have shape [columns]");
+        biases = bias->contiguous();
+        p.bias = biases.data_ptr();
+    }
+    Tensor y = at::empty(shape, x.options().dtype(dtype));
+    p.type = elementType(y, "the result");
+    p.y = y.data_ptr();
+    check(carl_int8_linear_forward(&p, Queue()));
+    return y;
+}
+
+at::ScalarType resultType(const py::object& dtype)
+{
+    requireType(THPDtype_Check(dtype.ptr()), "dtype must be float32, bfloat16 or float16");
+    const at::ScalarType t = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+    requireType(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "dtype must be float32, bfloat16 or float16");
+    return t;
+}
+
+Tensor int8Linear(const Tensor& x, const Tensor& xScale, const Tensor& w, const Tensor& wScale, const OptTensor& bias, const py::object& dtype)
+{
+    requireNoGradient({ &xScale, &wScale, bias ? &*bias : &xScale }, "int8_linear");
+    return int8Product(x, xScale, w, wScale, nullptr, nullptr, bias, 0, resultType(dtype));
+}
+
+Tensor int8GatedLinear(const Tensor& x, const Tensor& xScale, const Tensor& gate, const Tensor& gateScale, const Tensor& up,
+                       const Tensor& upScale, const std::string& activation, const py::object& dtype)
+{
+    require(activation == "silu" || activation == "gelu", "activation must be 'silu' or 'gelu'");
+    requireNoGradient({ &xScale, &gateScale, &upScale }, "int8_gated_linear");
+    return int8Product(x, xScale, gate, gateScale, &up, &upScale, std::nullopt, activation == "silu" ? CARL_SILU : CARL_GELU, resultType(dtype));
+}
+
 // ------------------------------------------------------------------- AdamW
 
 // A sequence of tensors, looked at in place: a step's six lists of a policy's
@@ -497,4 +883,11 @@ PYBIND11_MODULE(_ops, m)
     m.def("adamw_step", &adamwStep);
     m.def("decode_moments", &decodeMoments);
     m.def("encode_moments", &encodeMoments);
+    m.def("action_log_prob", &actionLogProb);
+    m.def("top_actions", &topActions);
+    m.def("rms_norm", &rmsNorm);
+    m.def("rms_norm_int8", &rmsNormInt8);
+    m.def("quantize_int8", &quantizeInt8);
+    m.def("int8_linear", &int8Linear);
+    m.def("int8_gated_linear", &int8GatedLinear);
 }

@@ -4,12 +4,26 @@
                          rollouts and replays, with gradients
   linear_attention_step  its recurrent form: one step of every agent
   gated_ffn              a gated feed-forward block, with gradients
+  rms_norm               root-mean-square norm with the addition before it,
+                         with gradients
+  action_log_prob        log-probability and entropy of actions over several
+                         heads, with gradients
+  top_actions            the best actions of each head, or a sample
+
+and, for acting with weights in 8 bits:
+
+  quantize_int8          rows as 8-bit codes with a scale for each
+  rms_norm_int8          rms_norm with such an output
+  int8_linear            a projection of codes by codes
+  int8_gated_linear      the gate and up projections of a gated block
 
 Formulas are those of include/carl_amd_ops.h.  Tensors must be on cuda:0; work
 is queued on torch's current stream.  Unfitting arguments raise ValueError or
 TypeError before anything is queued.
 """
 from __future__ import annotations
+
+from collections.abc import Sequence
 
 import torch
 
@@ -71,4 +85,100 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return _ops.gated_ffn(x, w_gate, w_up, w_down, activation)
 
 
-__all__ = ["gated_ffn", "linear_attention", "linear_attention_step"]
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
+             eps: float = 1e-6) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """s / sqrt(mean(s^2) + eps) * weight with s = x + residual; with a
+    residual (result, s).
+
+    x, residual     [..., width], float32, bfloat16 or float16
+    weight          [width]
+    eps             at least 1e-30
+
+    All of one type; s is rounded to it once and the norm is that of the
+    rounded s.  Widths are at most 16,384.  Gradients reach x, residual and
+    weight, once, from both results.
+    """
+    return _ops.rms_norm(x, weight, residual, eps)
+
+
+def action_log_prob(logits: torch.Tensor, actions: torch.Tensor, heads: Sequence[int], *,
+                    mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(log-probability, entropy) of the actions of all heads, float32 [...].
+
+    logits          [..., sum of heads], float32, bfloat16 or float16: the
+                    heads' logits next to each other
+    actions         [..., len(heads)], int32 or int64
+    heads           the heads' sizes (carl.ACTION_NVECS): 1 to 64 of them,
+                    16,384 logits in all at most
+    mask            bool, of the logits' shape: True where an action can be taken
+
+    A masked logit, or one of -infinity, weighs nothing whatever it holds and
+    gets the gradient 0; its action's log-probability is -infinity.  A head
+    with nothing to take has entropy 0.  An action below 0 is none: its head
+    adds nothing to the log-probability; an action past its head's last gives
+    NaN.  Gradients of both results reach logits, once.
+    """
+    return _ops.action_log_prob(logits, actions, list(heads), mask)
+
+
+def top_actions(logits: torch.Tensor, heads: Sequence[int], k: int = 1, *, mask: torch.Tensor | None = None,
+                noise: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The k best actions of each head, int32 [..., len(heads), k], and their
+    log-probabilities, float32.
+
+    noise           float32, of the logits' shape, added to them before they
+                    are compared (not to the log-probabilities): with
+                    -log(-log(u)), u uniform in (0, 1), the best action is a
+                    sample of the policy
+
+    Logits, heads and mask are those of `action_log_prob`.  Equal ones go by
+    their index.  Where fewer than k can be taken the rest are -1, with the
+    log-probability -infinity; k is at most 64.  For acting; it has no gradient.
+    """
+    return _ops.top_actions(logits, list(heads), k, mask, noise)
+
+
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes (int8 [..., width]) and scales (float32 [...]) of rows: a code c of
+    a row stands for c times the row's scale, its largest magnitude / 127.
+
+    Codes lie in rows that begin every 16 bytes, as `int8_linear` reads them
+    best.  Widths are at most 16,384.  A row with a NaN or an infinity has the
+    scale NaN.  For weights, and for rows that no norm has made; it has no
+    gradient.
+    """
+    return _ops.quantize_int8(x)
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
+                  eps: float = 1e-6) -> tuple[torch.Tensor, ...]:
+    """`rms_norm` with its result as codes and scales, as `quantize_int8` gives
+    them: (codes, scales), and with a residual (codes, scales, s)."""
+    return _ops.rms_norm_int8(x, weight, residual, eps)
+
+
+def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
+                bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(x weight^T) x_scale weight_scale + bias
+
+    x               int8 [..., width], x_scale float32 [...]
+    weight          int8 [columns, width], weight_scale float32 [columns]
+    bias            [columns], of the result's type
+    dtype           of the result: float32, bfloat16 or float16
+
+    The sum of products is exact; it is scaled in float32 and rounded once.
+    Widths and columns are at most 65,536.  It has no gradient.
+    """
+    return _ops.int8_linear(x, x_scale, weight, weight_scale, bias, dtype)
+
+
+def int8_gated_linear(x: torch.Tensor, x_scale: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                      up_scale: torch.Tensor, *, activation: str = "silu", dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """act(gate) * up of two products as `int8_linear` makes them: the inner
+    values of `gated_ffn`, in one pass over x."""
+    return _ops.int8_gated_linear(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, dtype)
+
+
+__all__ = ["action_log_prob", "gated_ffn", "int8_gated_linear", "int8_linear", "linear_attention", "linear_attention_step",
+           "quantize_int8", "rms_norm", "rms_norm_int8", "top_actions"]

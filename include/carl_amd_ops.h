@@ -1,7 +1,8 @@
 /*
  * carl_amd_ops.h - C-ABI of the learner's operators beside the step engine:
  * linear attention with a decay for each head (chunked and recurrent forms),
- * the gated feed-forward block, and AdamW over many tensors.
+ * the gated feed-forward block, AdamW over many tensors, log-probabilities and
+ * choices of actions, the root-mean-square norm, and products in 8 bits.
  *
  * Same conventions as carl_amd.h: plain pointers and sizes, CARL_OK or a
  * negative status, the message of the calling thread's last failure in
@@ -163,6 +164,128 @@ int carl_adamw_decode(const int8_t* exp_avg, const float* exp_avg_scale, const u
 /* The codes and scales of n float32 moments, as carl_adamw_step writes them. */
 int carl_adamw_encode(const float* exp_avg, const float* exp_avg_sq, int64_t n, int8_t* exp_avg_out,
                       float* exp_avg_scale, uint8_t* exp_avg_sq_out, float* exp_avg_sq_scale, void* stream);
+
+/* ---- actions ----------------------------------------------------------------
+ * A row holds the logits of all action heads, one head after another.  A logit
+ * is available where it is not masked and not -infinity; with x_j a head's
+ * available logits
+ *   log p_j = x_j - log(sum_i exp x_i)      H = -sum_j p_j log p_j
+ * and a row's log-probability and entropy are its heads' sums, in order.  What
+ * is not available weighs nothing whatever it holds, has the log-probability
+ * -infinity and the gradient 0.  A head with nothing available has entropy 0.
+ * An action below 0 is none: its head adds 0 to the log-probability (and takes
+ * part in the entropy).  An action past its head's last gives NaN.  A NaN or
+ * +infinity among the available logits makes its head's results NaN.
+ *
+ * The best actions of a head are those with the largest keys, the available
+ * logits plus noise (one float32 addition; without noise the logits), equal
+ * ones by their index, a NaN before all others; with noise -log(-log u), u
+ * uniform in (0, 1), the best one is a sample.  Where fewer than k are
+ * available the rest have the action -1 and the log-probability -infinity. */
+typedef struct carl_actions {
+    int64_t rows;               /* at most 2^40 */
+    int32_t type;               /* of logits and their gradients */
+    int32_t heads;              /* 1 to CARL_ACTIONS_MAX_HEADS */
+    const int32_t* sizes;       /* on the host, [heads]: at least 1, CARL_ACTIONS_MAX_LOGITS in all */
+    const void* logits;         /* [rows, logits], rows logits_row elements apart */
+    int64_t logits_row;
+    const uint8_t* mask;        /* likewise: 1 where available, 0 where masked; or NULL */
+    int64_t mask_row;
+    /* log-probabilities */
+    const void* actions;        /* [rows, heads], rows actions_row apart: int32_t, or int64_t */
+    int64_t actions_row;
+    int32_t actions_wide;       /* 1 for int64_t */
+    float *log_prob, *entropy;  /* [rows], of the choice log_prob is [rows, heads, k] */
+    /* backward: gradients of both outputs, row_step apart (0: one value for all rows), NULL for zero */
+    const float *d_log_prob, *d_entropy;
+    int64_t d_log_prob_step, d_entropy_step;
+    void* d_logits;             /* [rows, logits] */
+    /* the best actions */
+    const float* noise;         /* [rows, logits], rows noise_row apart, or NULL */
+    int64_t noise_row;
+    int32_t k;                  /* 1 to CARL_ACTIONS_MAX_K */
+    int32_t* best;              /* [rows, heads, k] */
+} carl_actions;
+
+enum { CARL_ACTIONS_MAX_HEADS = 64, CARL_ACTIONS_MAX_LOGITS = 16384, CARL_ACTIONS_MAX_K = 64 };
+
+int carl_action_log_prob(const carl_actions* a, void* stream);
+int carl_action_log_prob_backward(const carl_actions* a, void* stream);
+int carl_top_actions(const carl_actions* a, void* stream);
+
+/* ---- root-mean-square norm, rows in 8 bits -------------------------------------
+ *   s = x + residual        y = s / sqrt(mean(s^2) + eps) w
+ * All matrices hold one element type; s is rounded to it once, as it is kept,
+ * and the norm is that of the rounded s.  Sums are float32; of rows whose
+ * squares add up to 2^120 or more s is first multiplied by 2^-80.
+ *
+ * Codes of a row, every step one IEEE binary32 operation:
+ *   t = s w (of rows without a norm t = x)      m = max(max |t|, 2^-100)
+ *   code = rint(t (127 / m))                    scale = (m / 127) / sqrt(mean(s^2) + eps)
+ * (without a norm scale = m / 127).  A row with a NaN or an infinity in t has
+ * the codes 0 and the scale NaN. */
+typedef struct carl_norm {
+    int64_t rows;               /* at most 2^40 */
+    int32_t width;              /* 1 to CARL_NORM_MAX_DIM */
+    int32_t type;
+    float eps;                  /* at least CARL_NORM_MIN_EPS */
+    const void* x;              /* [rows, width], rows x_row elements apart */
+    int64_t x_row;
+    const void* residual;       /* likewise, or NULL */
+    int64_t residual_row;
+    const void* weight;         /* [width] */
+    void* sum;                  /* written where there is a residual: [rows, width] */
+    void* y;                    /* [rows, width] */
+    int8_t* codes;              /* [rows, width], rows codes_row apart */
+    int64_t codes_row;
+    float* scale;               /* [rows] */
+    /* backward: s (x where there is no residual) is read from `sum`, rows sum_row apart */
+    int64_t sum_row;
+    const void* dy;
+    int64_t dy_row;
+    const void* d_sum;          /* gradient of s from elsewhere, or NULL */
+    int64_t d_sum_row;
+    void* d_x;                  /* of x and of the residual alike, or NULL */
+    void* d_weight;             /* or NULL */
+    void* workspace;            /* carl_rms_norm_workspace bytes, or NULL for 0 */
+} carl_norm;
+
+enum { CARL_NORM_MAX_DIM = 16384 };
+#define CARL_NORM_MIN_EPS 1e-30f
+
+int carl_rms_norm(const carl_norm* n, void* stream);
+int carl_rms_norm_workspace(const carl_norm* n, int64_t* bytes);        /* of the backward pass */
+int carl_rms_norm_backward(const carl_norm* n, void* stream);
+int carl_rms_norm_int8(const carl_norm* n, void* stream);
+int carl_quantize_int8(const carl_norm* n, void* stream);               /* of x: no weight, no eps */
+
+/* ---- products in 8 bits ----------------------------------------------------------
+ *   acc = sum over k of x[row][k] w[column][k], exact
+ *   y = (acc x_scale[row]) w_scale[column] + bias[column]
+ *   gated: y = act(gate) up, both of them such products
+ * in float32, rounded to y's type once.  All int8 values are allowed, -128
+ * among them. */
+typedef struct carl_int8_linear {
+    int64_t rows;               /* at most 2^28; times columns, in tiles of 128 x 128, at most 2^36 */
+    int32_t width, columns;     /* 1 to CARL_INT8_MAX_DIM */
+    int32_t type;               /* of y and the bias */
+    int32_t activation;         /* of the gated form: CARL_SILU or CARL_GELU */
+    const int8_t* x;            /* [rows, width], rows x_row apart */
+    int64_t x_row;
+    const float* x_scale;       /* [rows] */
+    const int8_t* w;            /* [columns, width], rows w_row apart */
+    int64_t w_row;
+    const float* w_scale;       /* [columns] */
+    const int8_t* w_up;         /* gated: w is the gate's; or NULL */
+    int64_t w_up_row;
+    const float* w_up_scale;
+    const void* bias;           /* [columns], or NULL (gated: NULL) */
+    void* y;                    /* [rows, columns] */
+} carl_int8_linear;
+
+enum { CARL_INT8_MAX_DIM = 65536 };
+
+int carl_int8_linear_forward(const carl_int8_linear* p, void* stream);
 
 #ifdef __cplusplus
 }
