@@ -5,11 +5,10 @@
 // A product of two codes is at most 2^14 and a sum has at most 2^16 of them.
 // Sums are whole numbers, so neither tiles nor the order change a result.
 //
-// `product` copies panels of both operands straight into LDS, two stages of 128
-// bytes a row, one barrier a stage; rows that do not lie in whole 16-byte pieces
-// go there through registers.  A row's last piece may hold bytes that are not
-// its own: they are zeros in one of the operands.  `thin` is the product of a
-// few rows, from memory to registers.
+// `product` multiplies panels that it copies straight into LDS; rows that do not
+// lie in whole 16-byte pieces go there through registers.  A row's last piece
+// may hold bytes that are not its own: they are zeros in one of the operands.
+// `thin` is the product of a few rows, from memory to registers.
 #include <algorithm>
 
 #include "../../include/carl_amd_ops.h"
@@ -25,7 +24,7 @@ struct Args {
     const float *xScale, *wScale[2];
     const void* bias;
     void* y;
-    int32_t width, columns, type, activation;
+    int32_t width, columns, activation;
 };
 
 __device__ inline i32x4 mma(uint4 a, uint4 b, i32x4 c)
@@ -58,175 +57,364 @@ __device__ inline uint4 loadBytes(const int8_t* p, int have)
     return r;
 }
 
-__device__ inline float biasOf(const Args& a, int n)
+// kActivation: of the gated form, or kNone.
+constexpr int kNone = -1;
+
+template <int kActivation> __device__ inline float valueOf(int acc, int up, float xScale, float scale, float upScale)
 {
-    if (a.type == CARL_OP_F32) return static_cast<const float*>(a.bias)[n];
-    if (a.type == CARL_OP_BF16) return (float)static_cast<const bf16*>(a.bias)[n];
-    return (float)static_cast<const f16*>(a.bias)[n];
+    const float y = (float)acc * xScale * scale;
+    if constexpr (kActivation == kNone) return y;
+    else return activate(y, kActivation) * ((float)up * xScale * upScale);
 }
 
-template <bool kGated> __device__ inline float valueOf(const Args& a, int acc, int up, float xScale, const float (&scale)[2], float bias)
-{
-    const float y = (float)acc * xScale * scale[0];
-    if constexpr (kGated) return activate(y, a.activation) * ((float)up * xScale * scale[1]);
-    return a.bias ? y + bias : y;
-}
-
-// kRun neighbouring values of a row from column n on.
-template <typename T, int kRun> __device__ inline void storeRun(const Args& a, int64_t row, int n, const float (&x)[kRun])
+// kRun neighbouring values of a row, of which `have` are the result's.
+template <typename T, int kRun> __device__ inline void storeRun(T* to, const float (&x)[kRun], int have)
 {
     constexpr int kE = 16 / sizeof(T), kPiece = kRun < kE ? kRun : kE;
-    T* const to = static_cast<T*>(a.y) + row * a.columns + n;
-    if (n + kRun <= a.columns) {
+    if (have >= kRun) {
 #pragma unroll
         for (int e = 0; e < kRun; e += kPiece) {
-            vec<T, kPiece> v;
+            vec<float, kPiece> v;
 #pragma unroll
-            for (int i = 0; i < kPiece; i++) v[i] = (T)x[e + i];
-            __builtin_memcpy(to + e, &v, sizeof(v));
+            for (int i = 0; i < kPiece; i++) v[i] = x[e + i];
+            const auto r = fromFloat<T, kPiece>(v);
+            __builtin_memcpy(to + e, &r, sizeof(r));
         }
     } else {
 #pragma unroll
         for (int e = 0; e < kRun; e++)
-            if (n + e < a.columns) to[e] = (T)x[e];
+            if (e < have) to[e] = (T)x[e];
     }
 }
 
 // ---- product -------------------------------------------------------------------
 
-constexpr int kRowBytes = 128, kPieces = kRowBytes / 16;
+constexpr int kRowBytes = 128, kPieces = kRowBytes / 16;     // of a row in a stage
 
-// Rows in LDS have their pieces permuted by the number of the lane that reads
-// them, as in the block's products: a's rows by the row mod 8, b's by what
-// bReader() says.
-template <bool kGated, bool kDirect, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(kWM* kWN * 64) void int8ProductKernel(const Args args)
+// 4 bytes a lane from memory to 4 x lane bytes past `lds`, as copyToLds.
+__device__ inline void copyWordToLds(i32x4 from, int offset, uint32_t lds)
 {
-    constexpr int kNB = kGated ? 2 : 1, kThreads = kWM * kWN * 64;
-    constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16, kRun = 4 * kTN;
-    constexpr int kStage = (kBM + kNB * kBN) * kRowBytes, kCopyRows = kThreads / kPieces;
-    static_assert(kBM % kCopyRows == 0 && kBN % kCopyRows == 0, "whole copies");
-    static_assert(kCopyRows % 8 == 0 && kCopyRows % (2 * kRun) == 0, "one permutation for a thread's pieces");
-    __shared__ __align__(1024) char stages[2 * kStage];
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds), "v"(offset), "s"(from) : "memory");
+}
 
-    // the tiles of one row of tiles run next to each other on one of the 8 dies
-    const int tilesN = (args.columns + kBN - 1) / kBN;
-    const int64_t tilesM = (args.rows + kBM - 1) / kBM;
-    const int die = blockIdx.x % 8;
-    const int64_t local = blockIdx.x / 8;
-    const int64_t tm = local / tilesN * 8 + die;
-    const int tn = (int)(local % tilesN);
-    if (tm >= tilesM) return;
-    const int64_t m0 = tm * kBM;
-    const int n0 = tn * kBN;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    const int wm = wave / kWN, wn = wave % kWN;
+template <int kYounger> __device__ inline void waitAllBut()
+{
+    static_assert(kYounger < 64, "what vmcnt counts");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kYounger) : "memory");
+}
+
+// What is computed from it is computed where it is used: the largest tiles have
+// no register left to keep it in.
+__device__ inline int anew(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// A tile of kBM rows by kBN columns (of the gated form: of both weights) that
+// kWM x kWN waves compute from stages of 128 bytes of every row in LDS.
+//
+// The tiles of b that a wave multiplies are dealt to the columns so that a
+// lane's results are runs of 8 neighbours, and the four quads' runs lie next to
+// each other: element e of tile j and quad q is column 32 (j / 2) + 8 q +
+// 4 (j % 2) + e.  Rows in LDS have their eight 16-byte pieces permuted by the
+// number, mod 8, of the lane that reads them, so that eight lanes meet all
+// banks: x's by the row's, w's by what wReader says.
+template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN> struct Tile {
+    static constexpr int kNB = kGated ? 2 : 1, kThreads = kWM * kWN * 64, kWaves = kWM * kWN;
+    static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16, kRun = 8;
+    static constexpr int kRows = kBM + kNB * kBN, kStage = kRows * kRowBytes;
+    static constexpr int kCopyRows = kThreads / kPieces, kCopies = kRows / kCopyRows;
+    // words of scales: of the rows, of the columns, and the bias
+    static constexpr int kBiasWords = kGated ? 0 : (kBN * (int)sizeof(T) / 4 + 63) / 64 * 64, kWords = kBM + kNB * kBN + kBiasWords;
+    static constexpr int kWordCopies = (kWords + kThreads - 1) / kThreads, kScales = kWords * 4;
+    static constexpr int kStores = kTM * (kTN / 2) * (int)sizeof(T) / 2;       // of a whole tile
+    static_assert(kBM % kCopyRows == 0 && kBN % kCopyRows == 0, "whole copies");
+    static_assert(kCopyRows % 16 == 0 && kTN % 2 == 0, "one permutation for a thread's pieces, runs of two tiles");
+    static_assert(kBM % 64 == 0 && kBN % 64 == 0, "a wave's words are of one kind");
 
     i32x4 acc[kNB][kTN][kTM];
-#pragma unroll
-    for (int b = 0; b < kNB; b++)
-#pragma unroll
-        for (int j = 0; j < kTN; j++)
-#pragma unroll
-            for (int i = 0; i < kTM; i++) acc[b][j][i] = i32x4{ 0, 0, 0, 0 };
+    int wm, wn;
 
-    // Rows past the operand's end lie past the descriptor's, pieces past a
-    // row's width are sent there: both arrive as zeros.  (A piece with a byte
-    // of a row in it is read whole: it lies in one page with that byte.)
-    const int copyRow = threadIdx.x / kPieces;
-    const auto copyPanel = [&](const int8_t* data, int64_t all, int64_t stride, int64_t row0, int rows, int k0, int at, bool weights) {
-        const int8_t* base = data + row0 * stride;
-        const int have = (int)(all - row0 < rows ? all - row0 : rows);
-        const int c = (threadIdx.x % kPieces ^ (weights ? bReader<kRun>(copyRow) : copyRow & 7)) * 16;
-        if constexpr (kDirect) {
-            const i32x4 from = descriptor(base, have * (int)stride);
-            const bool within = k0 + c < args.width;
-#pragma unroll
-            for (int i = 0; i < rows / kCopyRows; i++)
-                copyToLds(from, within ? (copyRow + i * kCopyRows) * (int)stride + c : kOutside, k0,
-                          ldsAddress(stages) + at + (i * kThreads + wave * 64) * 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < rows / kCopyRows; i++) {
-                const int row = copyRow + i * kCopyRows;
-                const uint4 piece = loadBytes(base + row * stride + k0 + c, row < have ? args.width - k0 - c : 0);
-                *reinterpret_cast<uint4*>(stages + at + (i * kThreads + threadIdx.x) * 16) = piece;
-            }
-        }
-    };
-    const auto copyStage = [&](int step, int at) {
-        copyPanel(args.x, args.rows, args.xRow, m0, kBM, step * kRowBytes, at, false);
+    __device__ Tile()
+    {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wm = wave / kWN;
+        wn = wave % kWN;
+    }
+
+    __device__ void clear()
+    {
 #pragma unroll
         for (int b = 0; b < kNB; b++)
-            copyPanel(args.w[b], args.columns, args.wRow[b], n0, kBN, step * kRowBytes, at + (kBM + b * kBN) * kRowBytes, true);
+#pragma unroll
+            for (int j = 0; j < kTN; j++)
+#pragma unroll
+                for (int i = 0; i < kTM; i++) acc[b][j][i] = i32x4{ 0, 0, 0, 0 };
+    }
+
+    // What a thread copies of x's rows (or w's): a piece of every kCopyRows-th, at this byte of their 128.
+    static __device__ int wReader(int row) { return (row & 3) | (row >> 3 & 1) << 2; }
+    static __device__ int pieceOf(int thread, bool weights)
+    {
+        const int row = thread / kPieces;
+        return (thread % kPieces ^ (weights ? wReader(row) : row & 7)) * 16;
+    }
+
+    // What a wave multiplies of half a stage.
+    struct Fragments {
+        uint4 x[kTM], w[kNB][kTN];
     };
-    const int aRow = (wm * kTM * 16 + col) * kRowBytes, piece0 = (quad ^ (col & 7)) * 16;
-    const int bRow = (wn * kTN * 16 + (col >> 2) * kRun + (col & 3)) * kRowBytes;
-    const int steps = (args.width + kRowBytes - 1) / kRowBytes;
-    const auto multiply = [&](const char* lds, int step) {
-        const bool cut = kDirect && step == steps - 1 && args.width % 16 != 0;
+
+    __device__ void load(Fragments& f, const char* lds, int half) const
+    {
+        const int lane = anew(threadIdx.x) & 63, col = lane & 15, quad = lane >> 4, piece = (half * 4 + quad ^ col & 7) * 16;
+        const char* const x = lds + (wm * kTM * 16 + col) * kRowBytes + piece;
+        const char* const w = lds + (kBM + wn * kTN * 16 + (col >> 2) * 8 + (col & 3)) * kRowBytes + piece;
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            __builtin_amdgcn_sched_barrier(0);      // the fragments of one half at a time
-            const char* aAt = lds + (aRow + (piece0 ^ half * 64));
-            const char* bAt = lds + kBM * kRowBytes + (bRow + (piece0 ^ half * 64));
-            uint4 a[kTM];
+        for (int i = 0; i < kTM; i++) f.x[i] = *reinterpret_cast<const uint4*>(x + i * 16 * kRowBytes);
 #pragma unroll
-            for (int i = 0; i < kTM; i++) a[i] = *reinterpret_cast<const uint4*>(aAt + i * 16 * kRowBytes);
-            if (cut) {
-                const int have = args.width - step * kRowBytes - half * 64 - quad * 16;
+        for (int b = 0; b < kNB; b++)
 #pragma unroll
-                for (int i = 0; i < kTM; i++) a[i] = firstBytes(a[i], have);
-            }
+            for (int j = 0; j < kTN; j++) f.w[b][j] = *reinterpret_cast<const uint4*>(w + (b * kBN + j / 2 * 32 + j % 2 * 4) * kRowBytes);
+    }
+
+    // have: bytes of the rows from this half on; what lies past them counts as zeros.
+    __device__ void multiply(Fragments& f, int have)
+    {
+        if (have < 64) {
+            const int quad = (anew(threadIdx.x) & 63) >> 4;
 #pragma unroll
-            for (int p = 0; p < kNB; p++)
+            for (int i = 0; i < kTM; i++) f.x[i] = firstBytes(f.x[i], have - quad * 16);
+        }
 #pragma unroll
-                for (int j = 0; j < kTN; j++) {
-                    const uint4 b = *reinterpret_cast<const uint4*>(bAt + (p * kBN + j * 4) * kRowBytes);
+        for (int b = 0; b < kNB; b++)
 #pragma unroll
-                    for (int i = 0; i < kTM; i++) acc[p][j][i] = mma(b, a[i], acc[p][j][i]);
+            for (int j = 0; j < kTN; j++)
+#pragma unroll
+                for (int i = 0; i < kTM; i++) acc[b][j][i] = mma(f.w[b][j], f.x[i], acc[b][j][i]);
+    }
+
+    template <int kActivation, bool kWhole> __device__ void finish(const Args& args, const float* scales, int64_t m0, int n0) const
+    {
+        const int lane = anew(threadIdx.x) & 63, n = wn * kTN * 16 + (lane >> 4) * 8, m = wm * kTM * 16 + (lane & 15);
+        T* const y = static_cast<T*>(args.y) + (m0 + m) * args.columns + n0 + n;
+        float xScale[kTM];
+#pragma unroll
+        for (int i = 0; i < kTM; i++) xScale[i] = scales[m + i * 16];
+#pragma unroll
+        for (int r = 0; r < kTN / 2; r++) {
+            f32x4 scale[kNB][2];
+            vec<T, kRun> bias;
+#pragma unroll
+            for (int b = 0; b < kNB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) scale[b][h] = *reinterpret_cast<const f32x4*>(scales + kBM + b * kBN + n + r * 32 + h * 4);
+            if (!kGated && args.bias) bias = *reinterpret_cast<const vec<T, kRun>*>(reinterpret_cast<const T*>(scales + kBM + kBN) + n + r * 32);
+#pragma unroll
+            for (int i = 0; i < kTM; i++) {
+                if (!kWhole && m0 + m + i * 16 >= args.rows) continue;
+                float value[kRun];
+#pragma unroll
+                for (int e = 0; e < kRun; e++) {
+                    const int j = r * 2 + e / 4;
+                    value[e] = valueOf<kActivation>(acc[0][j][i][e % 4], acc[kNB - 1][j][i][e % 4], xScale[i], scale[0][e / 4][e % 4],
+                                                    scale[kNB - 1][e / 4][e % 4]);
+                    if (!kGated && args.bias) value[e] += (float)bias[e];
                 }
+                storeRun<T, kRun>(y + (int64_t)i * 16 * args.columns + r * 32, value, kWhole ? kRun : args.columns - n0 - n - r * 32);
+            }
+        }
+    }
+
+    // Whether all of the tile was stored, with kStores stores.
+    __device__ bool finish(const Args& args, const float* scales, int64_t m0, int n0) const
+    {
+        const bool whole = m0 + kBM <= args.rows && n0 + kBN <= args.columns;
+        const auto with = [&](auto activation) {
+            if (whole) finish<activation(), true>(args, scales, m0, n0);
+            else finish<activation(), false>(args, scales, m0, n0);
+        };
+        if constexpr (!kGated) with(std::integral_constant<int, kNone>());
+        else if (args.activation == CARL_SILU) with(std::integral_constant<int, CARL_SILU>());
+        else with(std::integral_constant<int, CARL_GELU>());
+        return whole;
+    }
+};
+
+// Tiles of one row of tiles run next to each other on one of the 8 dies (blocks
+// are dealt to them in turn), so that x's rows are read from memory once.
+struct Places {
+    int die, tilesN, count;        // of the die's tiles, in order
+
+    __device__ Places(const Args& args, int bm, int bn) : die(blockIdx.x % 8), tilesN((args.columns + bn - 1) / bn)
+    {
+        const int tilesM = (int)((args.rows + bm - 1) / bm);
+        count = (tilesM - die + 7) / 8 * tilesN;
+    }
+};
+
+// Workgroups stay and take every so-many-th tile of their die.  While half a
+// stage is multiplied from registers, the next half is read from LDS, and the
+// stages after it are on their way there, across the ends of tiles, so that the
+// next tile's first ones (and its scales) arrive while a tile's results are
+// computed and written.  Between the halves a step waits for the next stage's
+// copies, the younger ones (and the last results' stores) stay outstanding; the
+// one barrier after it hands that stage over and frees this one, which is in
+// registers by then.
+template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN, int kStages, int kBlocks>
+__global__ __launch_bounds__(kWM* kWN * 64, kWM* kWN * kBlocks / 4) void int8ProductKernel(const Args args)
+{
+    using Tile = Tile<T, kGated, kBM, kBN, kWM, kWN>;
+    constexpr int kNB = Tile::kNB, kThreads = Tile::kThreads, kStage = Tile::kStage, kCopyRows = Tile::kCopyRows;
+    constexpr int kCopies = Tile::kCopies, kYounger = kCopies * (kStages - 2);
+    // stages, the scales of a tile and of those that copies may be ahead by
+    __shared__ __align__(1024) char stages[kStages * kStage + (kStages + 1) * Tile::kScales];
+    const Places places(args, kBM, kBN);
+    const int stride = gridDim.x / 8, first = blockIdx.x / 8;
+    if (first >= places.count) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int steps = (args.width + kRowBytes - 1) / kRowBytes;
+    const uint32_t lds = ldsAddress(stages);
+
+    // Rows past an operand's end lie past its descriptor's, pieces past a row's
+    // width are sent there: both arrive as zeros.  (A piece with a byte of a
+    // row in it is read whole: it lies in one page with that byte.)
+    i32x4 from[1 + kNB];
+    int at[1 + kNB];
+    at[0] = (int)threadIdx.x / kPieces * (int)args.xRow + Tile::pieceOf(threadIdx.x, false);
+#pragma unroll
+    for (int b = 0; b < kNB; b++) at[1 + b] = (int)threadIdx.x / kPieces * (int)args.wRow[b] + Tile::pieceOf(threadIdx.x, true);
+    int copyPlace = first, copyStep = 0, copyScales = 0;
+    const auto copyNext = [&](int slot) {
+        if (copyStep == 0) {        // another tile: its rows, and its scales
+            const bool any = copyPlace < places.count;
+            const int64_t m0 = (int64_t)(copyPlace / places.tilesN * 8 + places.die) * kBM;
+            const int n0 = copyPlace % places.tilesN * kBN;
+            const int rows = !any ? 0 : args.rows - m0 < kBM ? (int)(args.rows - m0) : kBM;
+            const int columns = !any ? 0 : args.columns - n0 < kBN ? args.columns - n0 : kBN;
+            from[0] = descriptor(args.x + m0 * args.xRow, rows * (int)args.xRow);
+#pragma unroll
+            for (int b = 0; b < kNB; b++) from[1 + b] = descriptor(args.w[b] + n0 * args.wRow[b], columns * (int)args.wRow[b]);
+            for (int word = wave * 64; word < Tile::kWords; word += kThreads) {
+                const void* of = args.xScale + m0 + word;
+                int bytes = (rows - word) * 4;
+                if (word >= kBM + kNB * kBN) {
+                    // (a last column's odd half is read with the one before it)
+                    const int c = (word - kBM - kNB * kBN) * 4 / (int)sizeof(T);
+                    of = static_cast<const T*>(args.bias) + n0 + c;
+                    bytes = args.bias ? ((columns - c) * (int)sizeof(T) + 3) / 4 * 4 : 0;
+                } else if (word >= kBM) {
+                    const int b = (word - kBM) / kBN, c = (word - kBM) % kBN;
+                    of = args.wScale[b] + n0 + c;
+                    bytes = (columns - c) * 4;
+                }
+                copyWordToLds(descriptor(of, bytes > 0 ? bytes : 0), (int)(threadIdx.x & 63) * 4,
+                              lds + kStages * kStage + copyScales * Tile::kScales + word * 4);
+            }
+            copyScales = copyScales == kStages ? 0 : copyScales + 1;
+            copyPlace += stride;
+        }
+        const int k0 = copyStep * kRowBytes, thread = anew(threadIdx.x);
+#pragma unroll
+        for (int p = 0; p < 1 + kNB; p++) {
+            const bool within = k0 + Tile::pieceOf(thread, p > 0) < args.width;
+            const int apart = kCopyRows * (int)(p == 0 ? args.xRow : args.wRow[p == 2 ? 1 : 0]);
+#pragma unroll
+            for (int i = 0; i < (p == 0 ? kBM : kBN) / kCopyRows; i++)
+                copyToLds(from[p], within ? at[p] + i * apart : kOutside, k0,
+                          lds + slot * kStage + (p == 0 ? 0 : kBM + (p - 1) * kBN) * kRowBytes + i * kThreads * 16 + wave * 1024);
+        }
+        copyStep = copyStep + 1 == steps ? 0 : copyStep + 1;
+    };
+
+#pragma unroll
+    for (int i = 0; i < kStages; i++) copyNext(i);
+    Tile tile;
+    typename Tile::Fragments even, odd;
+    waitAllBut<kCopies*(kStages - 1)>();
+    __syncthreads();
+    tile.load(even, stages, 0);
+    int slot = 0, scales = 0, storesLeft = 0;
+    for (int place = first; place < places.count; place += stride) {
+        tile.clear();
+        for (int i = 0; i < steps; i++) {
+            const int have = args.width - i * kRowBytes;
+            tile.load(odd, stages + slot * kStage, 1);
+            tile.multiply(even, have);
+            if (storesLeft > 0) {
+                waitAllBut<kYounger + Tile::kStores>();
+                storesLeft--;
+            } else waitAllBut<kYounger>();
+            __syncthreads();
+            copyNext(slot);
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            tile.load(even, stages + slot * kStage, 0);
+            if (have > 64) tile.multiply(odd, have - 64);
+        }
+        const float* const own = reinterpret_cast<const float*>(stages + kStages * kStage + scales * Tile::kScales);
+        const bool whole = tile.finish(args, own, (int64_t)(place / places.tilesN * 8 + places.die) * kBM, place % places.tilesN * kBN);
+        scales = scales == kStages ? 0 : scales + 1;
+        // the stores are younger than the copies of the next kStages stages; a part of a tile has fewer, so that they are waited for
+        if (!whole) waitCopies();
+        storesLeft = whole ? kStages - 1 : 0;
+    }
+    waitCopies();          // none outlives its workgroup's LDS
+}
+
+// The same of rows that do not lie in whole pieces, or scales and biases that
+// do not begin at words: through registers, a tile a workgroup.
+template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__(kWM* kWN * 64) void int8LooseKernel(const Args args)
+{
+    using Tile = Tile<T, kGated, kBM, kBN, kWM, kWN>;
+    constexpr int kNB = Tile::kNB, kThreads = Tile::kThreads, kStage = Tile::kStage, kCopyRows = Tile::kCopyRows;
+    __shared__ __align__(1024) char stages[2 * kStage + Tile::kScales];
+    const Places places(args, kBM, kBN);
+    const int place = blockIdx.x / 8;
+    if (place >= places.count) return;
+    const int64_t m0 = (int64_t)(place / places.tilesN * 8 + places.die) * kBM;
+    const int n0 = place % places.tilesN * kBN;
+
+    float* const scales = reinterpret_cast<float*>(stages + 2 * kStage);
+    for (int i = threadIdx.x; i < kBM; i += kThreads) scales[i] = m0 + i < args.rows ? args.xScale[m0 + i] : 0.0f;
+    for (int i = threadIdx.x; i < kNB * kBN; i += kThreads) scales[kBM + i] = n0 + i % kBN < args.columns ? args.wScale[i / kBN][n0 + i % kBN] : 0.0f;
+    if (!kGated && args.bias)
+        for (int i = threadIdx.x; i < kBN; i += kThreads)
+            reinterpret_cast<T*>(scales + kBM + kBN)[i] = n0 + i < args.columns ? static_cast<const T*>(args.bias)[n0 + i] : T(0);
+
+    uint4 held[Tile::kCopies];
+    const auto load = [&](int k0) {
+#pragma unroll
+        for (int n = 0; n < Tile::kCopies; n++) {
+            const int panel = n * kCopyRows < kBM ? 0 : (n * kCopyRows - kBM) / kBN + 1;
+            const int row = n * kCopyRows - (panel == 0 ? 0 : kBM + (panel - 1) * kBN) + (int)threadIdx.x / kPieces, c = k0 + Tile::pieceOf(threadIdx.x, panel > 0);
+            const int64_t at = (panel == 0 ? m0 : n0) + row, stride = panel == 0 ? args.xRow : args.wRow[panel - 1];
+            const bool have = at < (panel == 0 ? args.rows : args.columns);
+            held[n] = loadBytes((panel == 0 ? args.x : args.w[panel - 1]) + at * stride + c, have ? args.width - c : 0);
         }
     };
-
-    copyStage(0, 0);
-    waitCopies();
-    __syncthreads();
-    for (int step = 0; step < steps; step++) {
-        if (step + 1 < steps) copyStage(step + 1, ((step + 1) & 1) * kStage);
-        multiply(stages + (step & 1) * kStage, step);
-        waitCopies();
+    const auto put = [&](int slot) {
+#pragma unroll
+        for (int n = 0; n < Tile::kCopies; n++) *reinterpret_cast<uint4*>(stages + slot * kStage + (n * kThreads + threadIdx.x) * 16) = held[n];
+    };
+    Tile tile;
+    tile.clear();
+    load(0);
+    put(0);
+    const int steps = (args.width + kRowBytes - 1) / kRowBytes;
+    for (int i = 0; i < steps; i++) {
         __syncthreads();
+        if (i + 1 < steps) load((i + 1) * kRowBytes);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            typename Tile::Fragments now;
+            tile.load(now, stages + (i & 1) * kStage, half);
+            tile.multiply(now, args.width - i * kRowBytes - half * 64);
+        }
+        if (i + 1 < steps) put((i + 1) & 1);
     }
-
-    // a lane's columns: kRun neighbours from n on, of row `col` of each tile
-    const int n = n0 + wn * kTN * 16 + quad * kRun;
-    float scale[kNB][kRun], bias[kRun];
-#pragma unroll
-    for (int e = 0; e < kRun; e++) {
-        const int at = n + e < args.columns ? n + e : args.columns - 1;
-#pragma unroll
-        for (int b = 0; b < kNB; b++) scale[b][e] = args.wScale[b][at];
-        bias[e] = args.bias ? biasOf(args, at) : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < kTM; i++) {
-        const int64_t row = m0 + (wm * kTM + i) * 16 + col;
-        if (row >= args.rows) continue;
-        const float xScale = args.xScale[row];
-        float y[kRun];
-#pragma unroll
-        for (int j = 0; j < kTN; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int at = j * 4 + e;
-                const float both[2] = { scale[0][at], scale[kNB - 1][at] };
-                y[at] = valueOf<kGated>(args, acc[0][j][i][e], acc[kNB - 1][j][i][e], xScale, both, bias[at]);
-            }
-        if (args.type == CARL_OP_F32) storeRun<float, kRun>(args, row, n, y);
-        else if (args.type == CARL_OP_BF16) storeRun<bf16, kRun>(args, row, n, y);
-        else storeRun<f16, kRun>(args, row, n, y);
-    }
+    tile.finish(args, scales, m0, n0);
 }
 
 // ---- thin ----------------------------------------------------------------------
@@ -235,7 +423,7 @@ __global__ __launch_bounds__(kWM* kWN * 64) void int8ProductKernel(const Args ar
 // columns a workgroup, its eight waves taking the sum's blocks in turn,
 // fragments straight from memory, whatever its alignment, to registers, one
 // exchange at the end.
-template <bool kGated, int kTM> __global__ __launch_bounds__(512) void int8ThinKernel(const Args args)
+template <typename T, bool kGated, int kTM> __global__ __launch_bounds__(512) void int8ThinKernel(const Args args)
 {
     constexpr int kWaves = 8, kNB = kGated ? 2 : 1;
     __shared__ i32x4 parts[kWaves][kNB][kTM][64];
@@ -285,26 +473,31 @@ template <bool kGated, int kTM> __global__ __launch_bounds__(512) void int8ThinK
     const int64_t m = m0 + wave * 16 + col;
     if (m >= args.rows) return;
     const int n = n0 + quad * 4;
+    const float xScale = args.xScale[m];
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const int at = n + e < args.columns ? n + e : args.columns - 1;
-        const float scale[2] = { args.wScale[0][at], kGated ? args.wScale[1][at] : 0.0f };
-        y[e] = valueOf<kGated>(args, sum[0][e], sum[kNB - 1][e], args.xScale[m], scale, args.bias ? biasOf(args, at) : 0.0f);
+        const float scale = args.wScale[0][at], upScale = kGated ? args.wScale[1][at] : 0.0f;
+        if constexpr (!kGated) {
+            y[e] = valueOf<kNone>(sum[0][e], 0, xScale, scale, 0.0f);
+            if (args.bias) y[e] += (float)static_cast<const T*>(args.bias)[at];
+        } else if (args.activation == CARL_SILU) y[e] = valueOf<CARL_SILU>(sum[0][e], sum[1][e], xScale, scale, upScale);
+        else y[e] = valueOf<CARL_GELU>(sum[0][e], sum[1][e], xScale, scale, upScale);
     }
-    if (args.type == CARL_OP_F32) storeRun<float, 4>(args, m, n, y);
-    else if (args.type == CARL_OP_BF16) storeRun<bf16, 4>(args, m, n, y);
-    else storeRun<f16, 4>(args, m, n, y);
+    storeRun<T, 4>(static_cast<T*>(args.y) + m * args.columns + n, y, args.columns - n);
 }
 
 // ---- launches ------------------------------------------------------------------
 
 constexpr int64_t kMostRows = (int64_t)1 << 28, kThinRows = 128;
 
-template <bool kGated, bool kDirect, int kBM, int kBN, int kWM, int kWN> void launchTile(const Args& a, hipStream_t stream)
+// kBlocks workgroups a compute unit.
+template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN, int kStages, int kBlocks> void launchTile(const Args& a, hipStream_t stream)
 {
     const int64_t tilesM = (a.rows + kBM - 1) / kBM, tilesN = (a.columns + kBN - 1) / kBN;
-    int8ProductKernel<kGated, kDirect, kBM, kBN, kWM, kWN><<<dim3((unsigned)((tilesM + 7) / 8 * 8 * tilesN)), kWM * kWN * 64, 0, stream>>>(a);
+    const dim3 grid((unsigned)std::min<int64_t>((tilesM + 7) / 8 * 8 * tilesN, 256 * kBlocks));
+    int8ProductKernel<T, kGated, kBM, kBN, kWM, kWN, kStages, kBlocks><<<grid, kWM * kWN * 64, 0, stream>>>(a);
 }
 
 // Rows that a descriptor can take: whole 16-byte pieces, one row after another.
@@ -313,26 +506,39 @@ bool inPieces(const void* p, int64_t stride, int width)
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0 && stride >= width && stride <= (int64_t)1 << 22;
 }
 
-template <bool kGated, bool kDirect> void launchProduct(const Args& a, hipStream_t stream)
-{
-    const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
-    if (tiles(128, 128) >= 256) launchTile<kGated, kDirect, 128, 128, 2, 2>(a, stream);
-    else launchTile<kGated, kDirect, 64, 64, 2, 2>(a, stream);
-}
+bool inWords(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
-template <bool kGated> void launchAll(const Args& a, hipStream_t stream)
+template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t stream)
 {
     if (a.rows <= kThinRows) {
         const unsigned columns = (unsigned)((a.columns + 15) / 16);
-        if (a.rows <= 16) int8ThinKernel<kGated, 1><<<dim3(columns), 512, 0, stream>>>(a);
-        else if (a.rows <= 32) int8ThinKernel<kGated, 2><<<dim3(columns), 512, 0, stream>>>(a);
-        else int8ThinKernel<kGated, 4><<<dim3(columns, (unsigned)((a.rows + 63) / 64)), 512, 0, stream>>>(a);
+        if (a.rows <= 16) int8ThinKernel<T, kGated, 1><<<dim3(columns), 512, 0, stream>>>(a);
+        else if (a.rows <= 32) int8ThinKernel<T, kGated, 2><<<dim3(columns), 512, 0, stream>>>(a);
+        else int8ThinKernel<T, kGated, 4><<<dim3(columns, (unsigned)((a.rows + 63) / 64)), 512, 0, stream>>>(a);
         return;
     }
+    const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
     const bool direct = inPieces(a.x, a.xRow, a.width) && inPieces(a.w[0], a.wRow[0], a.width)
-                     && (!kGated || inPieces(a.w[1], a.wRow[1], a.width));
-    if (direct) launchProduct<kGated, true>(a, stream);
-    else launchProduct<kGated, false>(a, stream);
+                     && (!kGated || inPieces(a.w[1], a.wRow[1], a.width)) && inWords(a.bias);
+    if (!direct) {
+        constexpr int kBN = kGated ? 64 : 128;
+        const dim3 grid((unsigned)((tiles(128, a.columns) + 7) / 8 * 8 * tiles(a.rows, kBN)));
+        int8LooseKernel<T, kGated, 128, kBN, 2, 2><<<grid, 256, 0, stream>>>(a);
+    } else if constexpr (kGated) {
+        if (tiles(256, 128) >= 256) launchTile<T, kGated, 256, 128, 4, 2, 2, 1>(a, stream);
+        else if (tiles(128, 64) >= 256) launchTile<T, kGated, 128, 64, 2, 2, 2, 2>(a, stream);
+        else launchTile<T, kGated, 64, 64, 2, 2, 3, 2>(a, stream);
+    } else {
+        if (tiles(256, 256) >= 256) launchTile<T, kGated, 256, 256, 4, 2, 2, 1>(a, stream);
+        else if (tiles(128, 128) >= 256) launchTile<T, kGated, 128, 128, 2, 2, 2, 2>(a, stream);
+        else launchTile<T, kGated, 64, 64, 2, 2, 4, 2>(a, stream);
+    }
+}
+
+template <typename T> void launchFor(const Args& a, hipStream_t stream)
+{
+    if (a.w[1]) launchAll<T, true>(a, stream);
+    else launchAll<T, false>(a, stream);
 }
 
 }  // namespace
@@ -351,8 +557,9 @@ extern "C" int carl_int8_linear_forward(const carl_int8_linear* p, void* stream)
     if (p->rows == 0) return CARL_OK;
     if (!p->x || !p->x_scale || !p->w || !p->w_scale || (gated && !p->w_up_scale) || !p->y) return fail(CARL_ERR_VALUE, "null product tensor");
     const Args a{ p->x, { p->w, p->w_up }, p->x_row, { p->w_row, p->w_up_row }, p->rows, p->x_scale, { p->w_scale, p->w_up_scale },
-                  p->bias, p->y, p->width, p->columns, p->type, p->activation };
-    if (gated) launchAll<true>(a, (hipStream_t)stream);
-    else launchAll<false>(a, (hipStream_t)stream);
+                  p->bias, p->y, p->width, p->columns, p->activation };
+    if (p->type == CARL_OP_F32) launchFor<float>(a, (hipStream_t)stream);
+    else if (p->type == CARL_OP_BF16) launchFor<bf16>(a, (hipStream_t)stream);
+    else launchFor<f16>(a, (hipStream_t)stream);
     return launched("8-bit product");
 }

@@ -261,8 +261,18 @@ template <typename T> __global__ __launch_bounds__(1024) void partsKernel(const 
     __shared__ float sums[16][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = blockIdx.x * 64 + lane;
     float x = 0.0f;
-    if (column < width)
-        for (int i = wave; i < parts; i += 16) x += part[(int64_t)i * width + column];
+    if (column < width) {
+        // eight loads on their way at once
+        int i = wave;
+        for (; i + 7 * 16 < parts; i += 8 * 16) {
+            float own[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) own[j] = part[(int64_t)(i + j * 16) * width + column];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x += own[j];
+        }
+        for (; i < parts; i += 16) x += part[(int64_t)i * width + column];
+    }
     sums[wave][lane] = x;
     __syncthreads();
     if (wave != 0 || column >= width) return;
