@@ -294,6 +294,7 @@ template <typename T, typename F> void withShape(int width, F&& run)
     else if (pieces <= 32) lanes(integral_constant<int, 32>(), integral_constant<int, 1>());
     else if (pieces <= 64) lanes(integral_constant<int, 64>(), integral_constant<int, 1>());
     else if (pieces <= 128) lanes(integral_constant<int, 64>(), integral_constant<int, 2>());
+    else if (pieces <= 192) lanes(integral_constant<int, 64>(), integral_constant<int, 3>());
     else if (pieces <= 256) lanes(integral_constant<int, 64>(), integral_constant<int, 4>());
     else if (pieces <= 1024) lanes(integral_constant<int, 256>(), integral_constant<int, 4>());
     else lanes(integral_constant<int, 1024>(), integral_constant<int, 4>());
@@ -309,7 +310,7 @@ int blocksOf(int64_t rows, int lanes, int most)
     return (int)std::min<int64_t>((rows + groups - 1) / groups, lanes <= 256 ? most : most / 4);
 }
 
-constexpr int kForwardBlocks = 2048, kGradBlocks = 1024;
+constexpr int kForwardBlocks = 65536, kGradBlocks = 1024;
 
 template <typename T, int kKind> void launchNorm(const NormArgs& a, hipStream_t stream)
 {

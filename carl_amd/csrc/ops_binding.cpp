@@ -637,12 +637,16 @@ py::object rmsNorm(const Tensor& x, const Tensor& weight, const OptTensor& resid
 }
 
 // Codes in rows that begin every 16 bytes.
-Tensor codesLike(const Tensor& x, int64_t width)
+Tensor codesLike(const Tensor& x)
 {
-    std::vector<int64_t> shape = x.sizes().vec();
-    shape.back() = (width + 15) / 16 * 16;
-    const Tensor rows = at::empty(shape, x.options().dtype(at::kChar));
-    return rows.narrow(-1, 0, width);
+    const std::vector<int64_t> shape = x.sizes().vec();
+    std::vector<int64_t> strides(shape.size(), 1);
+    int64_t apart = (shape.back() + 15) / 16 * 16;
+    for (int64_t i = (int64_t)shape.size() - 2; i >= 0; i--) {
+        strides[i] = apart;
+        apart *= std::max<int64_t>(shape[i], 1);
+    }
+    return at::empty_strided(shape, strides, x.options().dtype(at::kChar));
 }
 
 py::tuple normCodes(const Tensor& x, const Tensor* weight, const OptTensor& residual, double eps)
@@ -650,7 +654,7 @@ py::tuple normCodes(const Tensor& x, const Tensor* weight, const OptTensor& resi
     const Tensor* r = residual ? &*residual : nullptr;
     carl_norm n = normOf(x, weight, r, eps);
     const NormRows rows(n, x, weight, r);
-    const Tensor codes = codesLike(x, n.width), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    const Tensor codes = codesLike(x), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
     n.codes = codes.data_ptr<int8_t>();
     n.codes_row = (n.width + 15) / 16 * 16;
     n.scale = scale.data_ptr<float>();
