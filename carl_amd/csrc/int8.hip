@@ -524,30 +524,44 @@ bool inPieces(const void* p, int64_t stride, int width)
 
 bool inWords(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
+// By a sweep from 129 to 131,072 rows (us):
+//   few rows      1,408 to 512, 512 rows   thin 5.6   64 x 64 7.1     1,024 rows  9.0 and 7.4     (thin: 16 columns, 64 rows)
+//   small tiles   1,024 to 2,816, 512 rows   64 x 64 7.5   128 x 128 9.3     1,024 rows  9.7 and 9.4     8,192 rows  44.8 and 34.0
+//                 gated, 512 rows   64 x 64 9.4   128 x 64 12.5      2,001 rows  20.6 and 18.8
+//   large tiles   1,408 to 512, 32,768 rows (256 tiles)   128 x 128 29.9   256 x 256 28.7      131,072 rows  139 and 107
+//                 512 to 1,408, 16,384 rows (384 tiles, a round and a half)  22.8 and 26.5
+// so the largest tiles are taken where they leave no more than a fifth of
+// their rounds empty.  Of whole matrices at 8,192 cubed they reach 2,330 TOP/s
+// (the library's 8-bit product, without scales: 2,420; 131,072 x 1,408 to 512
+// 1,730 against 940).  They are bound by their copies into LDS (which alone
+// take 0.6 of the time, in stages of 64 bytes a row 0.75) beside the matrix
+// instructions (0.75); the gated form then by the operations on its results:
+// 107 of 250 us of 131,072 x 512 to 1,408, which no other tile's products hide.
 template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t stream)
 {
-    if (a.rows <= kThinRows) {
+    const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
+    if (a.rows <= kThinRows || tiles(64, 16) <= 256) {
         const unsigned columns = (unsigned)((a.columns + 15) / 16);
         if (a.rows <= 16) int8ThinKernel<T, kGated, 1><<<dim3(columns), 512, 0, stream>>>(a);
         else if (a.rows <= 32) int8ThinKernel<T, kGated, 2><<<dim3(columns), 512, 0, stream>>>(a);
         else int8ThinKernel<T, kGated, 4><<<dim3(columns, (unsigned)((a.rows + 63) / 64)), 512, 0, stream>>>(a);
         return;
     }
-    const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
     const bool direct = inPieces(a.x, a.xRow, a.width) && inPieces(a.w[0], a.wRow[0], a.width)
                      && (!kGated || inPieces(a.w[1], a.wRow[1], a.width)) && inWords(a.bias);
+    const auto fills = [](int64_t tiles) { return 5 * tiles >= 4 * ((tiles + 255) / 256 * 256); };
     if (!direct) {
         constexpr int kBN = kGated ? 64 : 128;
-        const dim3 grid((unsigned)((tiles(128, a.columns) + 7) / 8 * 8 * tiles(a.rows, kBN)));
+        const dim3 grid((unsigned)((tiles(128, a.columns) + 7) / 8 * 8 * tiles((int)a.rows, kBN)));
         int8LooseKernel<T, kGated, 128, kBN, 2, 2><<<grid, 256, 0, stream>>>(a);
     } else if constexpr (kGated) {
-        if (tiles(256, 128) >= 256) launchTile<T, kGated, 256, 128, 4, 2, 2, 1>(a, stream);
+        if (fills(tiles(256, 128))) launchTile<T, kGated, 256, 128, 4, 2, 2, 1>(a, stream);
         else if (tiles(128, 64) >= 256) launchTile<T, kGated, 128, 64, 2, 2, 2, 2>(a, stream);
-        else launchTile<T, kGated, 64, 64, 2, 2, 3, 2>(a, stream);
+        else launchTile<T, kGated, 64, 64, 2, 2, 2, 3>(a, stream);
     } else {
-        if (tiles(256, 256) >= 256) launchTile<T, kGated, 256, 256, 4, 2, 2, 1>(a, stream);
-        else if (tiles(128, 128) >= 256) launchTile<T, kGated, 128, 128, 2, 2, 2, 2>(a, stream);
-        else launchTile<T, kGated, 64, 64, 2, 2, 4, 2>(a, stream);
+        if (fills(tiles(256, 256))) launchTile<T, kGated, 256, 256, 4, 2, 2, 1>(a, stream);
+        else if (tiles(128, 128) >= 176) launchTile<T, kGated, 128, 128, 4, 2, 2, 2>(a, stream);
+        else launchTile<T, kGated, 64, 64, 2, 2, 3, 3>(a, stream);
     }
 }
 

@@ -70,10 +70,29 @@ def test_many_tiles(N, D, F, padded):
         _check(*_inputs(N, D, F, dtype, seed=N, padded=padded))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("D", [16, 70, 128, 129, 200, 257, 400])
+def test_large_tiles(D, dtype):
+    """One to four stages of the largest tiles, whole ones and parts of them, one and two of them a workgroup."""
+    for N in (27_001, 65_000):
+        _check(*_inputs(N, D, 500, dtype, seed=D), gated=False)
+    for N in (14_001, 32_600):
+        x, x_scale, w, w_scale, up, up_scale, _ = _inputs(N, D, 500, dtype, seed=D)
+        y = _ops().int8_gated_linear(x, x_scale, w, w_scale, up, up_scale, dtype=dtype)
+        ref.assert_within(y, *policy.gated(x, x_scale, w, w_scale, up, up_scale, "silu", dtype), "silu")
+
+
+@pytest.mark.parametrize("N,D,F,gated", [(1000, 60, 1000, True), (3000, 150, 700, True), (2000, 300, 1500, False), (700, 129, 500, False),
+                                         (130, 40, 2100, True), (130, 40, 2100, False)])
+def test_other_tiles(N, D, F, gated):
+    for dtype in DTYPES:
+        _check(*_inputs(N, D, F, dtype, seed=N), gated=gated)
+
+
 @pytest.mark.parametrize("value", [-128, 127])
 def test_the_largest_sums(value):
     """65,536 products of -128 by -128 add up to 2^30."""
-    for N in (3, 200):
+    for N in (3, 200, 2000):
         x = torch.full((N, 65536), value, dtype=torch.int8, device="cuda")
         w = torch.full((20, 65536), value, dtype=torch.int8, device="cuda")
         w[3] = 127
