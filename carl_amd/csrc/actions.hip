@@ -12,8 +12,8 @@
 //   own     rows of up to 64 logits in heads of up to 32.  A lane takes a row,
 //           in pieces of 16 bytes (masked logits as -infinity), and keeps it
 //           in LDS, where heads of any size can be found by an index.
-//   shared  16 or 64 lanes take a row together, straight from memory, eight
-//           logits of a head a lane in registers; of longer heads the rest is
+//   shared  8 to 64 lanes, or a workgroup, take a head together, straight from
+//           memory, eight logits a lane in registers; of longer heads the rest is
 //           read again for each step.
 #include <cmath>
 
@@ -395,72 +395,126 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
 
 // ---- shared ----------------------------------------------------------------------
 
-template <typename T, int kWhat, int kLanes> __global__ __launch_bounds__(256) void sharedKernel(const Args a)
+constexpr int kSharedThreads = 256, kHeld = 8;
+
+// A group of lanes for each head of a row; a workgroup has whole rows, and adds
+// up their heads' results in order.
+template <typename T, int kWhat, bool kMasked, bool kNoisy, int kLanes>
+__global__ __launch_bounds__(kSharedThreads) void sharedKernel(const Args a, int rowsOf, int longest)
 {
-    constexpr int kHeld = 8, kGroups = 256 / kLanes;
-    const int lane = threadIdx.x % kLanes;
-    for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
-        float logProb = 0.0f, entropy = 0.0f, dLogProb = 0.0f, dEntropy = 0.0f;
-        if constexpr (kWhat == kGradient) {
-            if (a.dLogProb) dLogProb = a.dLogProb[row * a.dLogProbStep];
-            if (a.dEntropy) dEntropy = a.dEntropy[row * a.dEntropyStep];
-        }
-        const RowActions actions(a, row);
-        for (int h = 0; h < a.heads; h++) {
-            const int first = a.first[h], n = a.first[h + 1] - first;
+    constexpr int kGroups = kSharedThreads / kLanes;
+    __shared__ float results[2][kGroups > kMostHeads ? kGroups : kMostHeads], slots[kSharedThreads / 64];
+    __shared__ uint32_t bits[kSharedThreads / 64];
+    __shared__ int firsts[kMostHeads + 1];
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    if ((int)threadIdx.x <= a.heads) firsts[threadIdx.x] = a.first[threadIdx.x];
+    __syncthreads();
+    const float inHeads = 1.0f / (float)a.heads;
+    for (int64_t row0 = (int64_t)blockIdx.x * rowsOf; row0 < a.rows; row0 += (int64_t)gridDim.x * rowsOf) {
+        const int rows = a.rows - row0 < rowsOf ? (int)(a.rows - row0) : rowsOf;
+        for (int unit = group; unit < rows * a.heads; unit += kGroups) {
+            const int r = (int)(((float)unit + 0.5f) * inHeads), h = unit - r * a.heads;       // (units are fewer than 128)
+            const int64_t row = row0 + r;
+            const int first = firsts[h], n = firsts[h + 1] - first;
             const T* const from = static_cast<const T*>(a.logits) + row * a.logitsRow + first;
-            const uint8_t* const mask = a.mask ? a.mask + row * a.maskRow + first : nullptr;
-            const auto load = [&](int j) { return j < n && (!mask || mask[j]) ? (float)from[j] : kNone; };
-            float held[kHeld];
+            const uint8_t* const mask = kMasked ? a.mask + row * a.maskRow + first : nullptr;
+            const float* const noise = kNoisy ? a.noise + row * a.noiseRow + first : nullptr;
+            // eight logits a lane in registers, all on their way at once
+            T in[kHeld];
+            uint8_t there[kHeld];
+            float more[kHeld], held[kHeld];
 #pragma unroll
-            for (int i = 0; i < kHeld; i++) held[i] = load(i * kLanes + lane);
+            for (int i = 0; i < kHeld; i++) {
+                const int j = i * kLanes + lane;
+                if (i * kLanes < longest && j < n) {
+                    in[i] = from[j];
+                    if constexpr (kMasked) there[i] = mask[j];
+                    if constexpr (kNoisy) more[i] = noise[j];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) {
+                held[i] = i * kLanes + lane < n ? (float)in[i] : kNone;
+                if constexpr (kMasked) held[i] = there[i] ? held[i] : kNone;
+                if constexpr (kNoisy) more[i] += held[i];
+            }
+            const auto load = [&](int j) {
+                const float x = (float)from[j];
+                return !kMasked || mask[j] ? x : kNone;
+            };
+            // f(j, logit, key): the conditions on `longest` are the same for all lanes
             const auto each = [&](auto&& f) {
 #pragma unroll
-                for (int i = 0; i < kHeld; i++) f(i * kLanes + lane, held[i]);
-                for (int j = kHeld * kLanes + lane; j < n; j += kLanes) f(j, load(j));
+                for (int i = 0; i < kHeld; i++)
+                    if (i * kLanes < longest) f(i * kLanes + lane, held[i], kNoisy ? more[i] : held[i]);
+                for (int j = kHeld * kLanes + lane; j < n; j += kLanes) {
+                    const float x = load(j);
+                    f(j, x, kNoisy ? x + noise[j] : x);
+                }
             };
             float most = kNone, z = 0.0f, sum = 0.0f;
-            each([&](int, float x) { most = fmaxf(most, x); });
-            const float base = baseOf(overLanes<Most, kLanes>(most));
-            each([&](int, float x) { addTo(z, sum, x - base, exponential(x - base)); });
-            const Sums s(base, overLanes<Add, kLanes>(z), overLanes<Add, kLanes>(sum));
+            each([&](int, float x, float) { most = fmaxf(most, x); });
+            const float base = baseOf(overRow<Most, kLanes>(most, slots));
+            each([&](int, float x, float) { addTo(z, sum, x - base, exponential(x - base)); });
+            const float zAll = overRow<Add, kLanes>(z, slots), sumAll = overRow<Add, kLanes>(sum, slots);
+            const Sums s(base, zAll, sumAll);
             if constexpr (kWhat == kBest) {
-                const float* const noise = a.noise ? a.noise + row * a.noiseRow + first : nullptr;
                 const int64_t at = (row * a.heads + h) * a.k;
-                uint64_t last = 0;
+                uint32_t lastKey = 0xffffffffu;
+                int last = -1;
                 for (int i = 0; i < a.k; i++) {
-                    // key, then the lower index; 0 for none
-                    uint64_t best = 0;
-                    each([&](int j, float x) {
-                        const uint64_t u = keyOf(noise && x != kNone ? x + noise[j] : x, x);
-                        const uint64_t own = u << 32 | (uint32_t)~j;
-                        if (u && (i == 0 || own < last) && own > best) best = own;
+                    uint32_t largest = 0;
+                    int best = INT32_MAX;
+                    float picked = kNone;
+                    each([&](int j, float x, float key) {
+                        const uint32_t u = keyOf(key, x);
+                        if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
+                            largest = u;
+                            best = j;
+                            picked = x;
+                        }
                     });
-                    for (int d = 1; d < kLanes; d *= 2) best = Most::of(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
-                    if (lane == 0) {
-                        const int j = (int)~(uint32_t)best;
-                        a.best[at + i] = best ? j : -1;
-                        a.logProb[at + i] = best ? s.logProb(load(j)) : kNone;
+                    lastKey = overRow<Most, kLanes>(largest, bits);
+                    last = (int)overRow<Least, kLanes>((uint32_t)(largest == lastKey ? best : INT32_MAX), bits);
+                    // (of nothing that is left, the group's first lane)
+                    if (last == INT32_MAX ? lane == 0 : best == last) {
+                        a.best[at + i] = last == INT32_MAX ? -1 : best;
+                        a.logProb[at + i] = s.logProb(picked);
                     }
-                    last = best;
                 }
             } else {
-                const int action = actions[h];
+                const int action = RowActions(a, row)[h];
                 if constexpr (kWhat == kLogProb) {
-                    logProb += s.taken(action, n, action >= 0 && action < n ? load(action) : 0.0f);
-                    entropy += s.entropy;
+                    const float own = s.taken(action, n, action >= 0 && action < n ? load(action) : 0.0f);
+                    if (lane == 0 && a.heads == 1) {
+                        a.logProb[row] = own;
+                        a.entropy[row] = s.entropy;
+                    } else if (lane == 0) {
+                        results[0][unit] = own;
+                        results[1][unit] = s.entropy;
+                    }
                 } else {
-                    const float share = shareOf(action, n, dLogProb);
+                    const float share = shareOf(action, n, a.dLogProb ? a.dLogProb[row * a.dLogProbStep] : 0.0f);
+                    const float dEntropy = a.dEntropy ? a.dEntropy[row * a.dEntropyStep] : 0.0f;
                     T* const to = static_cast<T*>(a.dLogits) + row * a.first[a.heads] + first;
-                    each([&](int j, float x) {
+                    each([&](int j, float x, float) {
                         if (j < n) to[j] = (T)gradient(s, x, x - base, exponential(x - base), j == action, share, dEntropy);
                     });
                 }
             }
         }
-        if (kWhat == kLogProb && lane == 0) {
-            a.logProb[row] = logProb;
-            a.entropy[row] = entropy;
+        if (kWhat == kLogProb && a.heads > 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < rows) {
+                float logProb = 0.0f, entropy = 0.0f;
+                for (int h = 0; h < a.heads; h++) {
+                    logProb += results[0][threadIdx.x * a.heads + h];
+                    entropy += results[1][threadIdx.x * a.heads + h];
+                }
+                a.logProb[row0 + threadIdx.x] = logProb;
+                a.entropy[row0 + threadIdx.x] = entropy;
+            }
+            __syncthreads();
         }
     }
 }
@@ -476,25 +530,35 @@ template <typename T, int kWhat> void launch(const Args& a, hipStream_t stream)
         const int64_t n = (a.rows + rows - 1) / rows;
         return dim3((unsigned)(n < kMostBlocks ? n : kMostBlocks));
     };
-    if (logits <= kOwnLogits && longest <= kOwnHead) {
-        const int bytes = (64 * (logits | 1) + kAhead) * 4 * (kWhat == kBest ? 2 : 1);
-        // A lane for each head where a lane for each row leaves the GPU empty, and heads are so short that a wave does not wait
-        // for its longest (us for best actions, log-probabilities, gradients: 34 rows of the simulator's heads own 7.2, 4.6, 5.7
-        // and head 3.6, 3.8, 3.5; 62,000 own 9.4, 6.8, 8.1 and head 7.3, 7.2, 7.0; 131,072 own 11.5, 7.1, 8.9 and head 12.9, 12.9,
-        // 12.3; one head of 20, 62,000 rows: own 8.3, 5.3, 7.5 and head 17.8, 9.8, 16.4)
-        const bool few = a.rows <= 65536 && longest <= 8;
-        const auto with = [&](auto masked, auto noisy) {
-            if (few) headKernel<T, kWhat, masked(), noisy()><<<blocks(64 / a.heads * 4), 256, 0, stream>>>(a, longest);
-            else ownKernel<T, kWhat, masked(), noisy()><<<blocks(64), 64, bytes, stream>>>(a);
+    using std::false_type, std::integral_constant, std::true_type;
+    const bool small = logits <= kOwnLogits && longest <= kOwnHead;
+    // A lane for each head where a lane for each row leaves the GPU empty, and heads are so short that a wave does not wait
+    // for its longest (us for best actions, log-probabilities, gradients: 34 rows of the simulator's heads own 7.2, 4.6, 5.7
+    // and head 3.6, 3.8, 3.5; 62,000 own 9.4, 6.8, 8.1 and head 7.3, 7.2, 7.0; 131,072 own 11.5, 7.1, 8.9 and head 12.9, 12.9,
+    // 12.3; one head of 20, 62,000 rows: own 8.3, 5.3, 7.5 and head 17.8, 9.8, 16.4)
+    const bool few = small && a.rows <= 65536 && longest <= 8;
+    // Lanes of a head by a sweep over 20 M logits (us, log-probabilities): heads of 33 8 lanes 40, 16 lanes 69; of 90 16 lanes 34;
+    // of 200 32 lanes 34, 64 lanes 56; of 513 64 lanes 35, a workgroup 80; of 2,000 64 lanes 40, a workgroup 33 (34 rows: 9 and 5).
+    const auto with = [&](auto masked, auto noisy) {
+        const auto shared = [&](auto lanes) {
+            const int groups = kSharedThreads / lanes(), rows = groups > a.heads ? groups / a.heads : 1;
+            sharedKernel<T, kWhat, masked(), noisy(), lanes()><<<blocks(rows), kSharedThreads, 0, stream>>>(a, rows, longest);
         };
-        using std::false_type, std::true_type;
-        if constexpr (kWhat == kBest) {
-            if (a.noise) return a.mask ? with(true_type(), true_type()) : with(false_type(), true_type());
-        }
-        if (a.mask) with(true_type(), false_type());
-        else with(false_type(), false_type());
-    } else if (longest <= 128) sharedKernel<T, kWhat, 16><<<blocks(16), 256, 0, stream>>>(a);
-    else sharedKernel<T, kWhat, 64><<<blocks(4), 256, 0, stream>>>(a);
+        if (few) headKernel<T, kWhat, masked(), noisy()><<<blocks(64 / a.heads * 4), 256, 0, stream>>>(a, longest);
+        else if (small) {
+            const int bytes = (64 * (logits | 1) + kAhead) * 4 * (kWhat == kBest ? 2 : 1);
+            ownKernel<T, kWhat, masked(), noisy()><<<blocks(64), 64, bytes, stream>>>(a);
+        } else if (longest <= 64) shared(integral_constant<int, 8>());
+        else if (longest <= 128) shared(integral_constant<int, 16>());
+        else if (longest <= 256) shared(integral_constant<int, 32>());
+        else if (longest <= 1024) shared(integral_constant<int, 64>());
+        else shared(integral_constant<int, kSharedThreads>());
+    };
+    if constexpr (kWhat == kBest) {
+        if (a.noise) return a.mask ? with(true_type(), true_type()) : with(false_type(), true_type());
+    }
+    if (a.mask) with(true_type(), false_type());
+    else with(false_type(), false_type());
 }
 
 template <int kWhat> int launch(int type, const Args& a, hipStream_t stream)

@@ -75,13 +75,6 @@ template <typename T> __device__ inline void storePiece(T* p, int have, vec<T, 1
             if (j < have) p[j] = r[j];
 }
 
-// Over the lanes of a row: kLanes of a wave, or a workgroup.
-template <typename Op, int kLanes, typename X> __device__ inline X overRow(X x, X* slots)
-{
-    if constexpr (kLanes <= 64) return overLanes<Op, kLanes>(x);
-    else return overWorkgroup<Op, kLanes>(x, slots);
-}
-
 template <typename T, int kKind, int kLanes, int kPieces>
 __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(const NormArgs a)
 {
