@@ -9,9 +9,10 @@
 //
 // What bounds it: memory, and for short heads the exponentials and the chain of
 // one head's steps.  Two forms:
-//   own     rows of up to 64 logits in heads of up to 32.  A lane takes a row,
-//           in pieces of 16 bytes (masked logits as -infinity), and keeps it
-//           in LDS, where heads of any size can be found by an index.
+//   own     heads of up to 32.  A lane takes a row, in pieces of 16 bytes (masked
+//           logits as -infinity), and keeps it in LDS, where heads of any size
+//           can be found by an index; up to four waves take the same rows and
+//           share their heads.
 //   shared  8 to 64 lanes, or a workgroup, take a head together, straight from
 //           memory, eight logits a lane in registers; of longer heads the rest is
 //           read again for each step.
@@ -129,28 +130,28 @@ __device__ inline float shareOf(int action, int size, float dLogProb)
 
 // ---- own -------------------------------------------------------------------------
 
-constexpr int kOwnLogits = 64, kOwnHead = 32;
+constexpr int kOwnHead = 32;
 
-// A row's elements in pieces of kE, 32 elements on their way at once: each(first
-// element, piece).  A last piece that is not whole begins earlier, and its first
+// Every kShare-th of a row's pieces of kE elements from the one numbered `part`
+// on, 32 elements on their way at once: each(first element, piece).  A last piece that is not whole begins earlier, and its first
 // elements come twice; rows shorter than a piece come one by one.
-template <int kE, typename Load, typename Each> __device__ inline void inPieces(int n, Load&& load, Each&& each)
+template <int kE, int kShare, typename Load, typename Each> __device__ inline void inPieces(int n, int part, Load&& load, Each&& each)
 {
     if (n < kE) {
-        for (int j = 0; j < n; j++) each(j, load(j, std::integral_constant<int, 1>()));
+        for (int j = part; j < n; j += kShare) each(j, load(j, std::integral_constant<int, 1>()));
         return;
     }
     constexpr int kAtOnce = 32 / kE;
-    for (int j0 = 0; j0 < n; j0 += kAtOnce * kE) {
+    for (int j0 = part * kE; j0 < n; j0 += kAtOnce * kShare * kE) {
         decltype(load(0, std::integral_constant<int, kE>())) piece[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
-            const int j = j0 + i * kE;
+            const int j = j0 + i * kShare * kE;
             if (j < n) piece[i] = load(j + kE <= n ? j : n - kE, std::integral_constant<int, kE>());
         }
 #pragma unroll
         for (int i = 0; i < kAtOnce; i++) {
-            const int j = j0 + i * kE;
+            const int j = j0 + i * kShare * kE;
             if (j < n) each(j + kE <= n ? j : n - kE, piece[i]);
         }
     }
@@ -176,14 +177,23 @@ struct Ahead {
     int action;
 };
 
-template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_bounds__(64) void ownKernel(const Args a)
+// kShare waves take the same 64 rows, each every kShare-th head of them.
+template <typename T, int kWhat, bool kMasked, bool kNoisy, int kShare> __global__ __launch_bounds__(64 * kShare) void ownKernel(const Args a)
 {
     constexpr int kE = 16 / sizeof(T);
     extern __shared__ float rows[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int logits = a.first[a.heads], across = logits | 1;      // odd: the lanes' rows begin in different banks
-    float* const own = rows + threadIdx.x * across;
-    uint32_t* const keys = reinterpret_cast<uint32_t*>(rows + 64 * across + kAhead + threadIdx.x * across);
-    for (int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 64) {
+    float* const own = rows + lane * across;
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(rows + 64 * across + kAhead + lane * across);
+    float* const results = rows + 64 * across + kAhead + lane;      // of a head, log-probability and entropy, 64 apart
+    const auto handOver = [&]() {
+        if constexpr (kShare > 1) __syncthreads();
+    };
+    for (int64_t row0 = (int64_t)blockIdx.x * 64; row0 < a.rows; row0 += (int64_t)gridDim.x * 64) {
+        // (rows past the last are the last one again; their results are not stored)
+        const bool mine = row0 + lane < a.rows;
+        const int64_t row = mine ? row0 + lane : a.rows - 1;
         const T* const from = static_cast<const T*>(a.logits) + row * a.logitsRow;
         const auto load = [&](int j, auto n) {
             Piece<T, n()> p;
@@ -192,7 +202,7 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
             if constexpr (kNoisy) p.noise = loadVec<float, n()>(a.noise + row * a.noiseRow + j);
             return p;
         };
-        inPieces<kE>(logits, load, [&](int j, const auto& p) {
+        inPieces<kE, kShare>(logits, wave, load, [&](int j, const auto& p) {
             constexpr int n = sizeof(p.x) / sizeof(T);
 #pragma unroll
             for (int i = 0; i < n; i++) {
@@ -208,6 +218,7 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
             if (a.dLogProb) dLogProb = a.dLogProb[row * a.dLogProbStep];
             if (a.dEntropy) dEntropy = a.dEntropy[row * a.dEntropyStep];
         }
+        handOver();
         const RowActions actions(a, row);
         // a head's first logits (and keys) and its action are read while the head before it is computed
         Ahead ahead;
@@ -221,10 +232,10 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
             }
             if constexpr (kWhat != kBest) ahead.action = actions[h];
         };
-        read(0);
-        for (int h = 0; h < a.heads; h++) {
+        if (wave < a.heads) read(wave);
+        for (int h = wave; h < a.heads; h += kShare) {
             const Ahead now = ahead;
-            if (h + 1 < a.heads) read(h + 1);
+            if (h + kShare < a.heads) read(h + kShare);
             float* const x = own + a.first[h];
             const int n = a.first[h + 1] - a.first[h];
             // (the conditions are the same for all lanes)
@@ -263,15 +274,23 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
                     for (int j = 0; j < kAhead; j++)
                         if (j < n) consider(j, now.key[j], now.x[j]);
                     for (int j = kAhead; j < n; j++) consider(j, key[j], x[j]);
-                    a.best[at + i] = best;
-                    a.logProb[at + i] = s.logProb(picked);
+                    if (mine) {
+                        a.best[at + i] = best;
+                        a.logProb[at + i] = s.logProb(picked);
+                    }
                     lastKey = largest;
                     last = best < 0 ? n : best;
                 }
             } else if constexpr (kWhat == kLogProb) {
                 const int action = now.action;
-                logProb += s.taken(action, n, x[action >= 0 && action < n ? action : 0]);
-                entropy += s.entropy;
+                const float taken = s.taken(action, n, x[action >= 0 && action < n ? action : 0]);
+                if constexpr (kShare == 1) {
+                    logProb += taken;
+                    entropy += s.entropy;
+                } else {
+                    results[h * 128] = taken;
+                    results[h * 128 + 64] = s.entropy;
+                }
             } else {
                 const float share = shareOf(now.action, n, dLogProb);
 #pragma unroll
@@ -280,9 +299,17 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
                 for (int j = kAhead; j < n; j++) x[j] = gradient(s, x[j], x[j] - base, exponential(x[j] - base), j == now.action, share, dEntropy);
             }
         }
+        handOver();
         if constexpr (kWhat == kLogProb) {
-            a.logProb[row] = logProb;
-            a.entropy[row] = entropy;
+            if (wave == 0 && mine) {
+                if constexpr (kShare > 1)
+                    for (int h = 0; h < a.heads; h++) {
+                        logProb += results[h * 128];
+                        entropy += results[h * 128 + 64];
+                    }
+                a.logProb[row] = logProb;
+                a.entropy[row] = entropy;
+            }
         } else if constexpr (kWhat == kGradient) {
             T* const to = static_cast<T*>(a.dLogits) + row * logits;
             const auto read = [&](int j, auto n) {
@@ -291,105 +318,9 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_
                 for (int i = 0; i < n(); i++) r[i] = (T)own[j + i];
                 return r;
             };
-            inPieces<kE>(logits, read, [&](int j, const auto& r) { __builtin_memcpy(to + j, &r, sizeof(r)); });
+            if (mine) inPieces<kE, kShare>(logits, wave, read, [&](int j, const auto& r) { __builtin_memcpy(to + j, &r, sizeof(r)); });
         }
-    }
-}
-
-// ---- head ------------------------------------------------------------------------
-
-// A lane for each head: as many rows a wave as fit.  The same operations in the
-// same order as of a row's own lane, so the results are the same.
-template <typename T, int kWhat, bool kMasked, bool kNoisy> __global__ __launch_bounds__(256) void headKernel(const Args a, int longest)
-{
-    const int lane = threadIdx.x & 63, r = lane / a.heads, h = lane - r * a.heads, each = 64 / a.heads;
-    int first = 0, n = 0;
-    for (int i = 0; i < a.heads; i++)
-        if (i == h) {
-            first = a.first[i];
-            n = a.first[i + 1] - first;
-        }
-    for (int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * each; row0 < a.rows; row0 += (int64_t)gridDim.x * 4 * each) {
-        const int64_t row = row0 + r;
-        const bool mine = r < each && row < a.rows;
-        const int size = mine ? n : 0;
-        const T* const from = static_cast<const T*>(a.logits) + row * a.logitsRow + first;
-        const uint8_t* const mask = kMasked ? a.mask + row * a.maskRow + first : nullptr;
-        const float* const noise = kNoisy ? a.noise + row * a.noiseRow + first : nullptr;
-        float dLogProb = 0.0f, dEntropy = 0.0f, held[kAhead], more[kAhead];
-        uint8_t there[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; i++)
-            if (i < size) {
-                held[i] = (float)from[i];
-                if constexpr (kMasked) there[i] = mask[i];
-                if constexpr (kNoisy) more[i] = noise[i];
-            }
-        int action = -1;
-        if (kWhat != kBest && mine) action = RowActions(a, row)[h];
-        if constexpr (kWhat == kGradient) {
-            if (mine && a.dLogProb) dLogProb = a.dLogProb[row * a.dLogProbStep];
-            if (mine && a.dEntropy) dEntropy = a.dEntropy[row * a.dEntropyStep];
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            if constexpr (kMasked) held[i] = i < size && there[i] ? held[i] : kNone;
-            else held[i] = i < size ? held[i] : kNone;
-        }
-        const auto load = [&](int j) { return j < size && (!kMasked || mask[j]) ? (float)from[j] : kNone; };
-        const auto all = [&](auto&& f) {
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) f(i, held[i], i);
-            for (int j = kAhead; j < longest; j++) f(j, load(j), kAhead);
-        };
-        float most = kNone, z = 0.0f, sum = 0.0f;
-        all([&](int, float x, int) { most = fmaxf(most, x); });
-        const float base = baseOf(most);
-        all([&](int, float x, int) { addTo(z, sum, x - base, exponential(x - base)); });
-        const Sums s(base, z, sum);
-        if constexpr (kWhat == kBest) {
-            const int64_t at = (row * a.heads + h) * a.k;
-            uint32_t lastKey = 0xffffffffu;
-            int last = -1;
-            for (int i = 0; i < a.k; i++) {
-                uint32_t largest = 0;
-                int best = -1;
-                float picked = kNone;
-                all([&](int j, float x, int reg) {
-                    float key = x;
-                    if constexpr (kNoisy) key = x == kNone ? x : x + (reg < kAhead ? more[reg < kAhead ? reg : 0] : noise[j]);
-                    const uint32_t u = keyOf(key, x);
-                    if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
-                        largest = u;
-                        best = j;
-                        picked = x;
-                    }
-                });
-                if (mine) {
-                    a.best[at + i] = best;
-                    a.logProb[at + i] = s.logProb(picked);
-                }
-                lastKey = largest;
-                last = best < 0 ? size : best;
-            }
-        } else if constexpr (kWhat == kLogProb) {
-            const float own = s.taken(action, size, load(action >= 0 && action < size ? action : size));
-            float logProb = 0.0f, entropy = 0.0f;
-            for (int i = 0; i < a.heads; i++) {
-                logProb += __shfl(own, r * a.heads + i);
-                entropy += __shfl(s.entropy, r * a.heads + i);
-            }
-            if (mine && h == 0) {
-                a.logProb[row] = logProb;
-                a.entropy[row] = entropy;
-            }
-        } else {
-            const float share = shareOf(action, size, dLogProb);
-            T* const to = static_cast<T*>(a.dLogits) + row * a.first[a.heads] + first;
-            all([&](int j, float x, int) {
-                if (j < size) to[j] = (T)gradient(s, x, x - base, exponential(x - base), j == action, share, dEntropy);
-            });
-        }
+        handOver();
     }
 }
 
@@ -531,12 +462,15 @@ template <typename T, int kWhat> void launch(const Args& a, hipStream_t stream)
         return dim3((unsigned)(n < kMostBlocks ? n : kMostBlocks));
     };
     using std::false_type, std::integral_constant, std::true_type;
-    const bool small = logits <= kOwnLogits && longest <= kOwnHead;
-    // A lane for each head where a lane for each row leaves the GPU empty, and heads are so short that a wave does not wait
-    // for its longest (us for best actions, log-probabilities, gradients: 34 rows of the simulator's heads own 7.2, 4.6, 5.7
-    // and head 3.6, 3.8, 3.5; 62,000 own 9.4, 6.8, 8.1 and head 7.3, 7.2, 7.0; 131,072 own 11.5, 7.1, 8.9 and head 12.9, 12.9,
-    // 12.3; one head of 20, 62,000 rows: own 8.3, 5.3, 7.5 and head 17.8, 9.8, 16.4)
-    const bool few = small && a.rows <= 65536 && longest <= 8;
+    // A lane for each row of short heads where the rows fit LDS and are many, or short themselves (us, best actions and
+    // log-probabilities, a lane for each row and lanes for each head: 5 heads of 16, 250,000 rows 61, 20 and 121, 82; 16,384 rows
+    // 10.3, 6.4 and 9.8, 8.2; 34 rows 9.0, 5.2 and 3.9, 4.1).
+    const int ownArray = 64 * (logits | 1) + kAhead;
+    const int ownBytes = (ownArray + (kWhat == kBest ? ownArray : kWhat == kLogProb ? a.heads * 128 : 0)) * 4;
+    const bool own = longest <= kOwnHead && ownBytes <= 65536 && (logits <= 32 || a.rows >= 16384);
+    // Waves for its 64 rows (the simulator's heads, one, two and four waves: 34 rows 7.5, 5.3, 4.0 and 4.7, 3.9, 3.1; 131,072
+    // 11.4, 10.0, 10.2 and 7.4, 6.5, 7.3; 1,048,576 59, 53, 53 and 22, 24, 28; 8 heads of 8, 262,144 rows 84, 53, 35 and 27, 21, 16).
+    const int share = a.rows <= 65536 || logits > 32 ? 4 : a.heads > 1 && (kWhat == kBest || a.rows <= 200000) ? 2 : 1;
     // Lanes of a head by a sweep over 20 M logits (us, log-probabilities): heads of 33 8 lanes 40, 16 lanes 69; of 90 16 lanes 34;
     // of 200 32 lanes 34, 64 lanes 56; of 513 64 lanes 35, a workgroup 80; of 2,000 64 lanes 40, a workgroup 33 (34 rows: 9 and 5).
     const auto with = [&](auto masked, auto noisy) {
@@ -544,10 +478,13 @@ template <typename T, int kWhat> void launch(const Args& a, hipStream_t stream)
             const int groups = kSharedThreads / lanes(), rows = groups > a.heads ? groups / a.heads : 1;
             sharedKernel<T, kWhat, masked(), noisy(), lanes()><<<blocks(rows), kSharedThreads, 0, stream>>>(a, rows, longest);
         };
-        if (few) headKernel<T, kWhat, masked(), noisy()><<<blocks(64 / a.heads * 4), 256, 0, stream>>>(a, longest);
-        else if (small) {
-            const int bytes = (64 * (logits | 1) + kAhead) * 4 * (kWhat == kBest ? 2 : 1);
-            ownKernel<T, kWhat, masked(), noisy()><<<blocks(64), 64, bytes, stream>>>(a);
+        if (own) {
+            const auto with = [&](auto share) {
+                ownKernel<T, kWhat, masked(), noisy(), share()><<<blocks(64), 64 * share(), ownBytes, stream>>>(a);
+            };
+            if (share == 4) with(integral_constant<int, 4>());
+            else if (share == 2) with(integral_constant<int, 2>());
+            else with(integral_constant<int, 1>());
         } else if (longest <= 64) shared(integral_constant<int, 8>());
         else if (longest <= 128) shared(integral_constant<int, 16>());
         else if (longest <= 256) shared(integral_constant<int, 32>());

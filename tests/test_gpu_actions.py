@@ -14,9 +14,9 @@ pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 CAR = (3, 3, 3, 2, 2, 3, 2)
-# both forms, their borders (64 logits, heads of 32; heads of 128), lanes with nothing, several reads a lane
+# both forms, their borders (heads of 32; of 64, 128, 256, 1,024), lanes with nothing, several reads a lane
 HEADS = [CAR, (1,), (2,), (1, 1), (32, 32), (31, 33), (32, 31, 1), (33,), (64,), (65,), (90,), (16,) * 5, (127, 2), (128,), (129,),
-         (130, 1, 140), (513,), (1, 1200, 3), (3,) * 21, (2,) * 64]
+         (130, 1, 140), (256,), (257, 2), (513,), (1, 1024), (1, 1200, 3), (2100,), (3,) * 21, (2,) * 64]
 
 
 def _ops():
@@ -77,6 +77,28 @@ def test_rows(rows, dtype):
     for heads in (CAR, (90,), (300, 2)):
         logits, actions, there = _rows((rows,), heads, dtype, seed=rows)
         _check(logits, actions, heads, there)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows,heads", [(16_385, (32, 32)), (16_390, (16,) * 5), (17_000, (3,) * 21), (16_400, (2,) * 64), (16_500, (30,) * 7),
+                                        (70_001, CAR), (70_000, (20,)), (210_003, CAR), (210_000, (4,) * 5), (70_000, (5,) * 9)], ids=str)
+def test_many_rows(rows, heads, dtype):
+    """Every number of waves that share rows, and rows of more logits than few rows of that form have."""
+    logits, actions, there = _rows((rows,), heads, dtype, seed=rows)
+    _check(logits, actions, heads, there)
+    noise = torch.randn(logits.shape, generator=torch.Generator().manual_seed(rows)).cuda()
+    for k in (1, 2):
+        best, log_prob = _ops().top_actions(logits, heads, k, mask=there, noise=noise)
+        keys = (logits.float() + noise).masked_fill(~there, -math.inf).cpu()
+        first = 0
+        for h, n in enumerate(heads):
+            order = torch.sort(keys[:, first:first + n], dim=1, descending=True, stable=True)
+            want = torch.where(order[0][:, :k] == -math.inf, -1, order[1][:, :k])
+            assert torch.equal(best[:, h, :min(k, n)].cpu().long(), want)
+            head = policy.Head(logits[:, first:first + n].cpu().double(), there[:, first:first + n].cpu())
+            at = want.clamp(min=0)
+            _same(log_prob[:, h, :min(k, n)], torch.where(want < 0, policy.NONE, head.logs.gather(1, at)), head.logs_off.gather(1, at), "log-probability")
+            first += n
 
 
 @pytest.mark.parametrize("heads", [CAR, (70, 3), (2,) * 9, (400,)], ids=str)
@@ -280,7 +302,7 @@ def test_no_rows(heads):
 
 @pytest.mark.parametrize("heads", [(30, 30), (120,)], ids=str)
 def test_rows_past_two_to_the_31(heads):
-    """More than 2^31 logits: the last rows are what they are by themselves."""
+    """More than 2^31 logits: the last rows' results."""
     L = sum(heads)
     N = (1 << 31) // L + 1000
     gen = torch.Generator(device="cuda").manual_seed(0)
@@ -290,13 +312,14 @@ def test_rows_past_two_to_the_31(heads):
     log_prob, entropy = _ops().action_log_prob(leaf, actions, heads)
     (grad,) = torch.autograd.grad(log_prob.sum() + entropy.sum(), [leaf])
     best, logs = _ops().top_actions(logits.detach(), heads)
-    tail = logits[-70:].detach().clone().requires_grad_()
-    own = _ops().action_log_prob(tail, actions[-70:], heads)
-    (own_grad,) = torch.autograd.grad(own[0].sum() + own[1].sum(), [tail])
-    own_best = _ops().top_actions(tail.detach(), heads)
-    for a, b in zip((log_prob, entropy, grad, best, logs), (*own, own_grad, *own_best)):
-        assert torch.equal(a[-70:], b)
-    _check(tail, actions[-70:], heads)
+    tail, taken, one = logits[-70:].detach(), actions[-70:], torch.ones(())
+    (want, off), (want_entropy, entropy_off) = policy.log_prob(tail, taken, heads)
+    _same(log_prob[-70:], want, off, "log-probability")
+    _same(entropy[-70:], want_entropy, entropy_off, "entropy")
+    _same(grad[-70:], *policy.log_prob_gradient(tail, taken, heads, one, one), "gradient")
+    want, want_logs, off = policy.top(tail, heads, 1)
+    assert torch.equal(best[-70:].cpu(), want)
+    _same(logs[-70:], want_logs, off, "best log-probability")
 
 
 def test_another_stream_and_a_graph():
