@@ -6,10 +6,13 @@ The policy acts one step at a time with `linear_attention_step` (the memories
 of all agents stay on the GPU), and is trained on whole rollouts with
 `linear_attention`: the rollout's buffers are [steps, agents, ...], the memory
 it began with is its initial state, and an episode that ended restarts the
-memory at the next step.  Between the two lie `gated_ffn` blocks; `AdamW` takes
-all tensors in one step, its clipping factor computed and applied on the GPU.
-The loss is a plain policy gradient with a learned baseline: an example of the
-operators together, not a training recipe.
+memory at the next step.  Around the two lie `rms_norm`, which adds to the
+residual stream as it norms it, and `gated_ffn`; `top_actions` samples and
+`action_log_prob` scores all action heads at once; `AdamW` takes all tensors in
+one step, its clipping factor computed and applied on the GPU.  With
+`--act-bits 8` the policy acts on 8-bit codes of its weights, made anew for each
+rollout.  The loss is a plain policy gradient with a learned baseline: an
+example of the operators together, not a training recipe.
 """
 from __future__ import annotations
 
@@ -26,8 +29,12 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 import carl  # noqa: E402
 from carl.gymnasium import ACTION_NVECS, CARLActionCodec  # noqa: E402
 from carl.gymnasium.torch import CARLTorchVectorEnv  # noqa: E402
-from carl.ops import gated_ffn, linear_attention, linear_attention_step  # noqa: E402
+from carl.ops import (action_log_prob, gated_ffn, int8_gated_linear, int8_linear, linear_attention, linear_attention_step,  # noqa: E402
+                      quantize_int8, rms_norm, rms_norm_int8, top_actions)
 from carl.optim import AdamW  # noqa: E402
+
+
+EPS = torch.finfo(torch.float32).eps
 
 
 class Block(nn.Module):
@@ -44,20 +51,39 @@ class Block(nn.Module):
         # memories of 8 to 512 steps
         self.register_buffer("log_decay", torch.log1p(-torch.exp2(-torch.linspace(3.0, 9.0, heads))))
 
-    def _norm(self, x: torch.Tensor, i: int) -> torch.Tensor:
-        return nn.functional.rms_norm(x, x.shape[-1:], self.norms[i])
+    def quantized(self) -> dict:
+        """Codes and scales of the weights, to act with."""
+        return {name: quantize_int8(getattr(self, name).weight.detach()) for name in ("qkv", "out", "gate", "up", "down")}
 
-    def forward(self, x: torch.Tensor, memory: torch.Tensor, starts: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
-        """x [agents, width] and the memory in place, or [steps, agents, width] and a new memory."""
-        q, k, v = (t.unflatten(-1, (self.heads, -1)) for t in self.qkv(self._norm(x, 0)).chunk(3, dim=-1))
+    def _split(self, qkv: torch.Tensor) -> list[torch.Tensor]:
+        return [t.unflatten(-1, (self.heads, -1)) for t in qkv.chunk(3, dim=-1)]
+
+    def forward(self, x: torch.Tensor, stream: torch.Tensor, memory: torch.Tensor,
+                starts: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """x is added to the stream first, and what comes back is yet to be added to the stream that comes with it:
+        [agents, width] and the memory in place, or [steps, agents, width] and a new memory."""
+        y, stream = rms_norm(x, self.norms[0], residual=stream, eps=EPS)
+        q, k, v = self._split(self.qkv(y))
         if x.dim() == 2:
             mixed = linear_attention_step(q, k, v, self.log_decay, memory, starts=starts)
         else:
             mixed, memory = linear_attention(q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1), self.log_decay,
                                              starts=None if starts is None else starts.t(), initial_state=memory)
             mixed = mixed.transpose(0, 1)
-        x = x + self.out(mixed.flatten(-2))
-        return x + gated_ffn(self._norm(x, 1), self.gate.weight, self.up.weight, self.down.weight), memory
+        y, stream = rms_norm(self.out(mixed.flatten(-2)), self.norms[1], residual=stream, eps=EPS)
+        return gated_ffn(y, self.gate.weight, self.up.weight, self.down.weight), stream, memory
+
+    def act(self, x: torch.Tensor, stream: torch.Tensor, memory: torch.Tensor, starts: torch.Tensor | None,
+            codes: dict) -> tuple[torch.Tensor, torch.Tensor]:
+        """A step of `forward` with the weights' codes."""
+        dtype = x.dtype
+        y, scale, stream = rms_norm_int8(x, self.norms[0], residual=stream, eps=EPS)
+        q, k, v = self._split(int8_linear(y, scale, *codes["qkv"], dtype=dtype))
+        mixed = linear_attention_step(q, k, v, self.log_decay, memory, starts=starts)
+        x = int8_linear(*quantize_int8(mixed.flatten(-2)), *codes["out"], dtype=dtype)
+        y, scale, stream = rms_norm_int8(x, self.norms[1], residual=stream, eps=EPS)
+        inner = int8_gated_linear(y, scale, *codes["gate"], *codes["up"], dtype=dtype)
+        return int8_linear(*quantize_int8(inner), *codes["down"], dtype=dtype), stream
 
 
 class RecurrentPolicy(nn.Module):
@@ -78,31 +104,43 @@ class RecurrentPolicy(nn.Module):
     def forward(self, obs: torch.Tensor, memories: list[torch.Tensor], starts: torch.Tensor | None = None):
         """obs [agents, obs_dim] (memories are updated in place) or [steps, agents, obs_dim] (new ones are returned)."""
         x = self.encode(obs)
+        stream = torch.zeros_like(x)
         after = []
         for block, memory in zip(self.blocks, memories):
-            x, memory = block(x, memory, starts)
+            x, stream, memory = block(x, stream, memory, starts)
             after.append(memory)
-        logits = self.act(x).masked_fill(~self.codec.mask(obs), -math.inf)
-        return logits, self.value(x).squeeze(-1), after
+        return *self._heads(x + stream, obs), after
+
+    def quantized(self) -> list[dict]:
+        return [block.quantized() for block in self.blocks]
+
+    def step(self, obs: torch.Tensor, memories: list[torch.Tensor], starts: torch.Tensor, codes: list[dict]):
+        """Logits and values of one step of every agent, the blocks' products in 8 bits."""
+        x = self.encode(obs)
+        stream = torch.zeros_like(x)
+        for block, memory, weights in zip(self.blocks, memories, codes):
+            x, stream = block.act(x, stream, memory, starts, weights)
+        return self._heads(x + stream, obs)
+
+    def _heads(self, x: torch.Tensor, obs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.act(x).masked_fill(~self.codec.mask(obs), -math.inf), self.value(x).squeeze(-1)
 
 
 def sample(logits: torch.Tensor) -> torch.Tensor:
-    heads = logits.split(ACTION_NVECS, dim=-1)
-    return torch.stack([torch.distributions.Categorical(logits=h).sample() for h in heads], dim=-1).int()
+    noise = torch.empty(logits.shape, device=logits.device).exponential_().log_().neg_()
+    return top_actions(logits, ACTION_NVECS, noise=noise)[0].squeeze(-1)
 
 
 def log_prob(logits: torch.Tensor, actions: torch.Tensor) -> torch.Tensor:
-    heads = logits.split(ACTION_NVECS, dim=-1)
-    picked = [h.log_softmax(-1).gather(-1, actions[..., i:i + 1].long()) for i, h in enumerate(heads)]
-    return torch.cat(picked, dim=-1).sum(-1)
+    return action_log_prob(logits, actions, ACTION_NVECS)[0]
 
 
 class Rollout:
     """Steps of every agent, [steps, agents, ...], and the memories they began with."""
 
-    def __init__(self, policy: RecurrentPolicy, env: CARLTorchVectorEnv, steps: int):
+    def __init__(self, policy: RecurrentPolicy, env: CARLTorchVectorEnv, steps: int, act_bits: int = 32):
         n = env.n_envs
-        self.policy, self.env, self.steps = policy, env, steps
+        self.policy, self.env, self.steps, self.act_bits = policy, env, steps, act_bits
         self.memories = policy.memories(n)
         self.next_obs = env.reset().as_subclass(torch.Tensor).clone()
         self.next_start = torch.ones(n, dtype=torch.bool, device="cuda")
@@ -111,8 +149,12 @@ class Rollout:
     def collect(self) -> dict:
         first = [m.clone() for m in self.memories]
         rows = {name: [] for name in ("obs", "starts", "actions", "logits", "rewards")}
+        codes = self.policy.quantized() if self.act_bits == 8 else None
         for _ in range(self.steps):
-            logits, _, _ = self.policy(self.next_obs, self.memories, self.next_start)
+            if codes is None:
+                logits, _, _ = self.policy(self.next_obs, self.memories, self.next_start)
+            else:
+                logits, _ = self.policy.step(self.next_obs, self.memories, self.next_start, codes)
             actions = sample(logits)
             rows["obs"].append(self.next_obs)
             rows["starts"].append(self.next_start)
@@ -155,12 +197,13 @@ def main() -> None:
     args.add_argument("--steps", type=int, default=32)
     args.add_argument("--updates", type=int, default=20)
     args.add_argument("--bits", type=int, default=8, choices=(8, 32), help="of the optimizer's moments")
+    args.add_argument("--act-bits", type=int, default=32, choices=(8, 32), help="of the weights while acting")
     a = args.parse_args()
     torch.manual_seed(0)
     env = CARLTorchVectorEnv(a.n_sim, 1, 1, normalize=True, discrete_actions=True)
     policy = RecurrentPolicy(env.single_observation_space.shape[0]).cuda()
     optimizer = AdamW(policy.parameters(), lr=3e-4, bits=a.bits)
-    rollout = Rollout(policy, env, a.steps)
+    rollout = Rollout(policy, env, a.steps, a.act_bits)
     for i in range(a.updates):
         print(f"update {i}: loss {update(policy, optimizer, rollout.collect()):.5f}", flush=True)
     env.close()
