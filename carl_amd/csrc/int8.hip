@@ -458,7 +458,7 @@ template <typename T, bool kGated, int kTM> __global__ __launch_bounds__(512) vo
     for (int p = 0; p < kNB; p++)
 #pragma unroll
         for (int i = 0; i < kTM; i++) acc[p][i] = i32x4{ 0, 0, 0, 0 };
-#pragma unroll 2
+#pragma unroll(kTM == 4 ? 2 : 4)
     for (int k = wave * 64 + quad * 16; k - quad * 16 < args.width; k += kWaves * 64) {
         const int have = args.width - k;
         uint4 b[kNB];
@@ -542,9 +542,14 @@ template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t str
     const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
     if (a.rows <= kThinRows || tiles(64, 16) <= 256) {
         const unsigned columns = (unsigned)((a.columns + 15) / 16);
-        if (a.rows <= 16) int8ThinKernel<T, kGated, 1><<<dim3(columns), 512, 0, stream>>>(a);
-        else if (a.rows <= 32) int8ThinKernel<T, kGated, 2><<<dim3(columns), 512, 0, stream>>>(a);
-        else int8ThinKernel<T, kGated, 4><<<dim3(columns, (unsigned)((a.rows + 63) / 64)), 512, 0, stream>>>(a);
+        const auto thin = [&](auto tiles) {
+            int8ThinKernel<T, kGated, tiles()><<<dim3(columns, (unsigned)((a.rows + 16 * tiles() - 1) / (16 * tiles()))), 512, 0, stream>>>(a);
+        };
+        // as few rows a workgroup as keep the GPU from more than one round or so (4,096 to 64, 1,006 rows: 16 rows 5.8 us, 64 rows
+        // 11.0; 1,408 to 512, 512 rows: 7.4 and 5.7)
+        if (tiles(16, 16) <= 256) thin(std::integral_constant<int, 1>());
+        else if (tiles(32, 16) <= 384) thin(std::integral_constant<int, 2>());
+        else thin(std::integral_constant<int, 4>());
         return;
     }
     const bool direct = inPieces(a.x, a.xRow, a.width) && inPieces(a.w[0], a.wRow[0], a.width)

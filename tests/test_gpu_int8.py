@@ -14,7 +14,7 @@ import policy_reference as policy
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
-SIZES = [(1, 1), (1, 300), (300, 1), (7, 13), (15, 16), (16, 15), (17, 33), (63, 64), (64, 65), (65, 129), (127, 100), (128, 128), (129, 257),
+SIZES = [(3767, 21), (1, 1), (1, 300), (300, 1), (7, 13), (15, 16), (16, 15), (17, 33), (63, 64), (64, 65), (65, 129), (127, 100), (128, 128), (129, 257),
          (256, 683), (683, 256), (1000, 70), (2049, 40)]
 
 
