@@ -9,8 +9,9 @@
 // rounding a step: whatever the order of the sum of squares, the same codes.
 //
 // What bounds it: memory.  A row's elements stay in registers between the
-// reduction and the output, so each is read and written once; the lanes that
-// share a row are as few as hold it in one to four pieces of 16 bytes each.
+// reduction and the output, so each is read and written once, in pieces of 16
+// bytes.  48,828 bf16 rows of 2,048: 69 us (5.8 TB/s), with the addition 135
+// (5.9), backward 163 (4.9), to codes 46 (6.6).
 // The sum s is rounded to the elements' type once, as it is kept, and the norm
 // is that of the rounded sum: the backward pass reads it and needs nothing else.
 #include <algorithm>
@@ -53,41 +54,54 @@ struct NormGradArgs {
 constexpr float kMostSquares = 0x1p120f, kSmaller = 0x1p-80f;
 constexpr float kLeast = 0x1p-100f;       // a row's largest magnitude counts as this much at least
 
-// 16 bytes of a row from any address; zeros past the row's end.
-template <typename T> __device__ inline vec<T, 16 / sizeof(T)> loadPiece(const T* p, int have)
+// A row's piece of 16 bytes at element `at`, from any address.  The last one
+// begins earlier where it would not be whole, at the row's end minus a piece:
+// its first elements are the piece's before it, too, which get the same values
+// from both, and which dupOf() keeps out of the sums.  Rows shorter than a piece
+// are filled up with zeros.
+template <typename T> constexpr int kOf = 16 / sizeof(T);
+
+template <typename T> __device__ inline int dupOf(int at, int width)
 {
-    constexpr int kE = 16 / sizeof(T);
-    vec<T, kE> r;
-    if (have >= kE) __builtin_memcpy(&r, p, 16);
+    const int have = width - at;
+    return have > 0 && have < kOf<T> && width >= kOf<T> ? kOf<T> - have : 0;
+}
+
+template <typename T> __device__ inline vec<T, kOf<T>> loadPiece(const T* row, int at, int width)
+{
+    vec<T, kOf<T>> r = {};
+    if (at >= width) return r;
+    if (width >= kOf<T>) __builtin_memcpy(&r, row + (at + kOf<T> <= width ? at : width - kOf<T>), 16);
     else
 #pragma unroll
-        for (int j = 0; j < kE; j++) r[j] = j < have ? p[j] : T(0);
+        for (int j = 0; j < kOf<T>; j++) r[j] = j < width ? row[j] : T(0);
     return r;
 }
 
-template <typename T> __device__ inline void storePiece(T* p, int have, vec<T, 16 / sizeof(T)> r)
+template <typename X, int kN> __device__ inline void storePiece(X* row, int at, int width, vec<X, kN> r)
 {
-    constexpr int kE = 16 / sizeof(T);
-    if (have >= kE) __builtin_memcpy(p, &r, 16);
+    if (at >= width) return;
+    if (width >= kN) __builtin_memcpy(row + (at + kN <= width ? at : width - kN), &r, sizeof(X) * kN);
     else
 #pragma unroll
-        for (int j = 0; j < kE; j++)
-            if (j < have) p[j] = r[j];
+        for (int j = 0; j < kN; j++)
+            if (j < width) row[j] = r[j];
 }
 
 template <typename T, int kKind, int kLanes, int kPieces>
-__global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(const NormArgs a)
+__global__ __launch_bounds__((kLanes < 128 ? 256 : kLanes)) void normKernel(const NormArgs a)
 {
-    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 256 ? 256 : kLanes, kGroups = kThreads / kLanes;
+    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 128 ? 256 : kLanes, kGroups = kThreads / kLanes;
     __shared__ float slots[kThreads / 64];
     __shared__ uint32_t bits[kThreads / 64];
     const int lane = threadIdx.x % kLanes;
+    const bool tail = a.width % kE != 0;
     vec<float, kE> w[kPieces];
     if constexpr (kKind != kRowCodes)
 #pragma unroll
         for (int p = 0; p < kPieces; p++) {
             const int at = (p * kLanes + lane) * kE;
-            w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight) + at, a.width - at));
+            w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight), at, a.width));
         }
     for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
         vec<float, kE> s[kPieces];
@@ -95,8 +109,8 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(cons
 #pragma unroll
         for (int p = 0; p < kPieces; p++) {
             const int at = (p * kLanes + lane) * kE;
-            in[p] = loadPiece(static_cast<const T*>(a.x) + row * a.xRow + at, a.width - at);
-            if (kKind != kRowCodes && a.residual) more[p] = loadPiece(static_cast<const T*>(a.residual) + row * a.residualRow + at, a.width - at);
+            in[p] = loadPiece(static_cast<const T*>(a.x) + row * a.xRow, at, a.width);
+            if (kKind != kRowCodes && a.residual) more[p] = loadPiece(static_cast<const T*>(a.residual) + row * a.residualRow, at, a.width);
         }
 #pragma unroll
         for (int p = 0; p < kPieces; p++) {
@@ -104,28 +118,29 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(cons
             if (kKind != kRowCodes && a.residual) {
                 const int at = (p * kLanes + lane) * kE;
                 const auto kept = fromFloat<T, kE>(s[p] + toFloat<T, kE>(more[p]));
-                storePiece(static_cast<T*>(a.sum) + row * a.width + at, a.width - at, kept);
+                storePiece<T, kE>(static_cast<T*>(a.sum) + row * a.width, at, a.width, kept);
                 s[p] = toFloat<T, kE>(kept);
             }
         }
         float r = 1.0f;
         if constexpr (kKind != kRowCodes) {
-            float squares = 0.0f, factor = 1.0f;
-#pragma unroll
-            for (int p = 0; p < kPieces; p++)
-#pragma unroll
-                for (int j = 0; j < kE; j++) squares += s[p][j] * s[p][j];
-            squares = overRow<Add, kLanes>(squares, slots);
-            if (!(squares < kMostSquares)) {
-                factor = kSmaller;
+            float squares, factor = 1.0f;
+            const auto sumUp = [&]() {
                 squares = 0.0f;
 #pragma unroll
                 for (int p = 0; p < kPieces; p++) {
-                    s[p] *= factor;
+                    const int dup = tail ? dupOf<T>((p * kLanes + lane) * kE, a.width) : 0;
 #pragma unroll
-                    for (int j = 0; j < kE; j++) squares += s[p][j] * s[p][j];
+                    for (int j = 0; j < kE; j++) squares += j < dup ? 0.0f : s[p][j] * s[p][j];
                 }
                 squares = overRow<Add, kLanes>(squares, slots);
+            };
+            sumUp();
+            if (!(squares < kMostSquares)) {
+                factor = kSmaller;
+#pragma unroll
+                for (int p = 0; p < kPieces; p++) s[p] *= factor;
+                sumUp();
             }
             r = 1.0f / sqrtf(squares / (float)a.width + a.eps * factor * factor);
         }
@@ -133,7 +148,7 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(cons
 #pragma unroll
             for (int p = 0; p < kPieces; p++) {
                 const int at = (p * kLanes + lane) * kE;
-                storePiece(static_cast<T*>(a.y) + row * a.width + at, a.width - at, fromFloat<T, kE>(s[p] * r * w[p]));
+                storePiece<T, kE>(static_cast<T*>(a.y) + row * a.width, at, a.width, fromFloat<T, kE>(s[p] * r * w[p]));
             }
         } else {
             // bit patterns of magnitudes order as unsigned numbers, infinity and NaN last
@@ -150,34 +165,29 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normKernel(cons
             if (lane == 0) a.scale[row] = finite ? m / 127.0f * r : __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int p = 0; p < kPieces; p++) {
-                const int at = (p * kLanes + lane) * kE, have = a.width - at;
                 vec<int8_t, kE> code;
 #pragma unroll
                 for (int j = 0; j < kE; j++) code[j] = finite ? (int8_t)(int)rintf(s[p][j] * inverse) : (int8_t)0;
-                int8_t* to = a.codes + row * a.codesRow + at;
-                if (have >= kE) __builtin_memcpy(to, &code, kE);
-                else
-#pragma unroll
-                    for (int j = 0; j < kE; j++)
-                        if (j < have) to[j] = code[j];
+                storePiece<int8_t, kE>(a.codes + row * a.codesRow, (p * kLanes + lane) * kE, a.width, code);
             }
         }
     }
 }
 
 template <typename T, int kLanes, int kPieces>
-__global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(const NormGradArgs a)
+__global__ __launch_bounds__((kLanes < 128 ? 256 : kLanes)) void normGradKernel(const NormGradArgs a)
 {
-    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 256 ? 256 : kLanes, kGroups = kThreads / kLanes;
+    constexpr int kE = 16 / sizeof(T), kThreads = kLanes < 128 ? 256 : kLanes, kGroups = kThreads / kLanes;
     constexpr int kColumns = kLanes * kPieces * kE;
     __shared__ __align__(32) float sums[kGroups > 1 ? kGroups * kColumns : kThreads / 64];
     float* const slots = sums;            // a row of a whole workgroup has no columns to add up
     const int lane = threadIdx.x % kLanes;
+    const bool tail = a.width % kE != 0;
     vec<float, kE> w[kPieces], dw[kPieces];
 #pragma unroll
     for (int p = 0; p < kPieces; p++) {
         const int at = (p * kLanes + lane) * kE;
-        w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight) + at, a.width - at));
+        w[p] = toFloat<T, kE>(loadPiece(static_cast<const T*>(a.weight), at, a.width));
         dw[p] = vec<float, kE>(0.0f);
     }
     for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
@@ -185,9 +195,9 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(
 #pragma unroll
         for (int p = 0; p < kPieces; p++) {
             const int at = (p * kLanes + lane) * kE;
-            in[p] = loadPiece(static_cast<const T*>(a.s) + row * a.sRow + at, a.width - at);
-            out[p] = loadPiece(static_cast<const T*>(a.dy) + row * a.dyRow + at, a.width - at);
-            if (a.dsum) on[p] = loadPiece(static_cast<const T*>(a.dsum) + row * a.dsumRow + at, a.width - at);
+            in[p] = loadPiece(static_cast<const T*>(a.s) + row * a.sRow, at, a.width);
+            out[p] = loadPiece(static_cast<const T*>(a.dy) + row * a.dyRow, at, a.width);
+            if (a.dsum) on[p] = loadPiece(static_cast<const T*>(a.dsum) + row * a.dsumRow, at, a.width);
         }
         // sums of s^2 and of g s in one pass, with s times a power of two where its squares need one
         float squares, inner, factor = 1.0f;
@@ -196,10 +206,11 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(
 #pragma unroll
             for (int p = 0; p < kPieces; p++) {
                 const auto s = toFloat<T, kE>(in[p]) * factor, g = toFloat<T, kE>(out[p]) * w[p];
+                const int dup = tail ? dupOf<T>((p * kLanes + lane) * kE, a.width) : 0;
 #pragma unroll
                 for (int j = 0; j < kE; j++) {
-                    squares += s[j] * s[j];
-                    inner += g[j] * s[j];
+                    squares += j < dup ? 0.0f : s[j] * s[j];
+                    inner += j < dup ? 0.0f : g[j] * s[j];
                 }
             }
             squares = overRow<Add, kLanes>(squares, slots);
@@ -220,7 +231,7 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(
             if (!a.dx) continue;
             auto d = (dy * w[p] - u * mean) * own;
             if (a.dsum) d += toFloat<T, kE>(on[p]);
-            storePiece(static_cast<T*>(a.dx) + row * a.width + at, a.width - at, fromFloat<T, kE>(d));
+            storePiece<T, kE>(static_cast<T*>(a.dx) + row * a.width, at, a.width, fromFloat<T, kE>(d));
         }
     }
     if (!a.part && !a.dw) return;
@@ -232,7 +243,14 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(
     if constexpr (kGroups > 1) {
         float* const mine = sums + threadIdx.x / kLanes * kColumns;
 #pragma unroll
-        for (int p = 0; p < kPieces; p++) *reinterpret_cast<vec<float, kE>*>(mine + (p * kLanes + lane) * kE) = dw[p];
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE, dup = tail ? dupOf<T>(at, a.width) : 0;
+            if (dup == 0) *reinterpret_cast<vec<float, kE>*>(mine + at) = dw[p];
+            else
+#pragma unroll
+                for (int j = 0; j < kE; j++)
+                    if (j >= dup) mine[at - dup + j] = dw[p][j];
+        }
         __syncthreads();
         for (int c = threadIdx.x; c < kColumns; c += kThreads) {
             float x = 0.0f;
@@ -242,9 +260,12 @@ __global__ __launch_bounds__((kLanes < 256 ? 256 : kLanes)) void normGradKernel(
         }
     } else {
 #pragma unroll
-        for (int p = 0; p < kPieces; p++)
+        for (int p = 0; p < kPieces; p++) {
+            const int at = (p * kLanes + lane) * kE, dup = tail ? dupOf<T>(at, a.width) : 0;
 #pragma unroll
-            for (int j = 0; j < kE; j++) write((p * kLanes + lane) * kE + j, dw[p][j]);
+            for (int j = 0; j < kE; j++)
+                if (j >= dup) write(at - dup + j, dw[p][j]);
+        }
     }
 }
 
@@ -275,26 +296,45 @@ template <typename T> __global__ __launch_bounds__(1024) void partsKernel(const 
 
 constexpr int64_t kMostRows = (int64_t)1 << 40;
 
-// The lanes that share a row, and the pieces that each takes of it: as few
-// lanes as hold the row in one piece each up to a wave, then more pieces, then
-// more waves.
-template <typename T, typename F> void withShape(int width, F&& run)
+// The lanes that share a row, and the pieces that each takes of it.  Up to 256
+// pieces lanes of a wave do, so that it holds several rows: most of what a row
+// costs beside its bytes are a reduction's steps, which a wave takes for all its
+// rows at once, and lanes without a piece (262,144 bf16 rows of 257: 54 us with 16
+// lanes of three pieces, 96 with 64 of one).  Beyond it a workgroup does, of as
+// few waves as keep its registers low and its lanes filled (42,140 bf16 rows of
+// 2,373, 297 pieces, backward: 193 us with 128 lanes of three, 257 with 256 of
+// two; of 1,408 in f32, 352 pieces, 325 with 192 of two and 394 with 128 of three).
+// `wide` calls read two or three rows at once for each that the others read, and
+// take more lanes at two borders (195,312 bf16 rows of 512: codes 46 us with 32
+// lanes of two and 55 with 64 of one, norm with an addition 131 and 127).
+template <typename T, typename F> void withShape(int width, bool wide, F&& run)
 {
     const int pieces = (int)((width * sizeof(T) + 15) / 16);
-    const auto lanes = [&](auto l, auto p) { run(l, p); };
+    const auto shape = [&](auto lanes, auto each) { run(lanes, each); };
     using std::integral_constant;
-    if (pieces <= 16) lanes(integral_constant<int, 16>(), integral_constant<int, 1>());
-    else if (pieces <= 32) lanes(integral_constant<int, 32>(), integral_constant<int, 1>());
-    else if (pieces <= 64) lanes(integral_constant<int, 64>(), integral_constant<int, 1>());
-    else if (pieces <= 128) lanes(integral_constant<int, 64>(), integral_constant<int, 2>());
-    else if (pieces <= 192) lanes(integral_constant<int, 64>(), integral_constant<int, 3>());
-    else if (pieces <= 256) lanes(integral_constant<int, 64>(), integral_constant<int, 4>());
-    else if (pieces <= 1024) lanes(integral_constant<int, 256>(), integral_constant<int, 4>());
-    else lanes(integral_constant<int, 1024>(), integral_constant<int, 4>());
+#define SHAPE(lanes, each) shape(integral_constant<int, lanes>(), integral_constant<int, each>())
+    if (pieces <= 8) SHAPE(8, 1);
+    else if (pieces <= 16) SHAPE(16, 1);
+    else if (pieces <= 32) SHAPE(32, 1);
+    else if (pieces <= 48) SHAPE(16, 3);
+    else if (pieces <= 64 && !wide) SHAPE(32, 2);
+    else if (pieces <= 64) SHAPE(64, 1);
+    else if (pieces <= 96) SHAPE(32, 3);
+    else if (pieces <= 128) SHAPE(64, 2);
+    else if (pieces <= 192) SHAPE(64, 3);
+    else if (pieces <= 256) SHAPE(64, 4);
+    else if (pieces <= 384) SHAPE((sizeof(T) == 4 ? 192 : 128), (sizeof(T) == 4 ? 2 : 3));
+    else if (pieces <= 512) SHAPE(256, 2);
+    else if (pieces <= 768) SHAPE(256, 3);
+    else if (pieces <= 1024) SHAPE(512, 2);
+    else if (pieces <= 1536 && !wide) SHAPE(512, 3);
+    else if (sizeof(T) == 2 || pieces <= 2048) SHAPE(1024, 2);
+    else if constexpr (sizeof(T) == 4) SHAPE(1024, 4);
+#undef SHAPE
 }
 
-constexpr int groupsOf(int lanes) { return lanes < 256 ? 256 / lanes : 1; }
-constexpr int threadsOf(int lanes) { return lanes < 256 ? 256 : lanes; }
+constexpr int groupsOf(int lanes) { return lanes < 128 ? 256 / lanes : 1; }
+constexpr int threadsOf(int lanes) { return lanes < 128 ? 256 : lanes; }
 
 // Enough workgroups to fill the GPU; each goes on with rows further down.
 int blocksOf(int64_t rows, int lanes, int most)
@@ -307,7 +347,7 @@ constexpr int kForwardBlocks = 65536, kGradBlocks = 1024;
 
 template <typename T, int kKind> void launchNorm(const NormArgs& a, hipStream_t stream)
 {
-    withShape<T>(a.width, [&](auto lanes, auto pieces) {
+    withShape<T>(a.width, kKind != kRowCodes && a.residual, [&](auto lanes, auto pieces) {
         normKernel<T, kKind, lanes(), pieces()><<<dim3(blocksOf(a.rows, lanes(), kForwardBlocks)), threadsOf(lanes()), 0, stream>>>(a);
     });
 }
@@ -323,7 +363,7 @@ template <int kKind> int norm(int type, const NormArgs& a, hipStream_t stream)
 template <typename T> int gradBlocks(const carl_norm& n)
 {
     int blocks = 0;
-    withShape<T>(n.width, [&](auto lanes, auto) { blocks = blocksOf(n.rows, lanes(), kGradBlocks); });
+    withShape<T>(n.width, true, [&](auto lanes, auto) { blocks = blocksOf(n.rows, lanes(), kGradBlocks); });
     return blocks;
 }
 
@@ -335,7 +375,7 @@ template <typename T> int normBackward(const carl_norm& n, hipStream_t stream)
     NormGradArgs a{ n.sum, n.dy, n.d_sum, n.weight, n.sum_row, n.dy_row, n.d_sum_row, n.rows, n.width, n.eps, n.d_x, nullptr, nullptr };
     if (n.d_weight && blocks > 1) a.part = static_cast<float*>(n.workspace);
     else a.dw = n.d_weight;
-    withShape<T>(n.width, [&](auto lanes, auto pieces) {
+    withShape<T>(n.width, true, [&](auto lanes, auto pieces) {
         normGradKernel<T, lanes(), pieces()><<<dim3(blocks), threadsOf(lanes()), 0, stream>>>(a);
     });
     if (int rc = launched("norm's gradients")) return rc;

@@ -223,7 +223,7 @@ int carl_top_actions(const carl_actions* a, void* stream);
  *   t = s w (of rows without a norm t = x)      m = max(max |t|, 2^-100)
  *   code = rint(t (127 / m))                    scale = (m / 127) / sqrt(mean(s^2) + eps)
  * (without a norm scale = m / 127).  A row with a NaN or an infinity in t has
- * the codes 0 and the scale NaN. */
+ * the codes 0 and the scale NaN.  No output overlaps an input. */
 typedef struct carl_norm {
     int64_t rows;               /* at most 2^40 */
     int32_t width;              /* 1 to CARL_NORM_MAX_DIM */

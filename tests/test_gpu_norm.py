@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # every number of lanes and pieces a row takes, at its borders in both element sizes
 WIDTHS = [1, 2, 7, 8, 9, 16, 31, 63, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 511, 512, 513, 683, 1000, 1024, 1025, 2047, 2048, 2049,
-          4095, 4096, 4097, 8191, 8192, 8193, 16383, 16384]
+          4095, 4096, 4097, 8191, 8192, 8193, 16383, 16384, 32, 33, 192, 193, 384, 385, 768, 769, 1408, 1536, 1537, 2373, 3100, 5000, 6144, 6145,
+          12288, 12289]
 
 
 def _ops():
