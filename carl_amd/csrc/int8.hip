@@ -72,7 +72,8 @@ template <int kActivation> __device__ inline float valueOf(int acc, int up, floa
     const float y = (float)acc * xScale * scale;
     if constexpr (kActivation == kNone) return y;
     const float u = (float)up * xScale * upScale;
-    if constexpr (kActivation == CARL_SILU) return y * u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y));
+    // (the gate first: of a large negative one it is 0 whatever u is, where y u may be an infinity)
+    if constexpr (kActivation == CARL_SILU) return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y)) * u;
     else return activate(y, CARL_GELU) * u;
 }
 

@@ -157,6 +157,16 @@ def test_gates_far_into_both_tails():
             ref.assert_within(y, *policy.gated(x, x_scale, w, w_scale * factor, up, up_scale, name, torch.float32), name)
 
 
+@pytest.mark.parametrize("N", [60, 2500])
+def test_gates_of_values_whose_product_float32_does_not_hold(N):
+    x, x_scale, w, w_scale, up, up_scale, _ = _inputs(N, 48, 400, torch.float32)
+    g, u = policy.product(x, x_scale, w, w_scale * 1e22), policy.product(x, x_scale, up, up_scale * 1e22)
+    for name in ("silu", "gelu"):
+        y = _ops().int8_gated_linear(x, x_scale, w, w_scale * 1e22, up, up_scale * 1e22, activation=name, dtype=torch.float32).cpu()
+        assert not torch.isnan(y).any()
+        assert (y[g < 0] == 0).all() and (y[(g > 1e20) & (u > 1e20)] == math.inf).all()
+
+
 def test_no_rows():
     x, w = torch.zeros(0, 3, 32, dtype=torch.int8, device="cuda"), torch.zeros(8, 32, dtype=torch.int8, device="cuda")
     assert _ops().int8_linear(x, torch.ones(0, 3, device="cuda"), w, torch.ones(8, device="cuda")).shape == (0, 3, 8)
