@@ -256,16 +256,24 @@ template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN> struct Ti
     }
 };
 
-// Tiles of one row of tiles run next to each other on one of the 8 dies (blocks
-// are dealt to them in turn), so that x's rows are read from memory once.
+// Each of the 8 dies (blocks are dealt to them in turn) takes every eighth row of
+// tiles, so that x's rows are read from memory once, and an eighth of the tiles of
+// the rows that are left (512 rows of 4,096 to 8,192, four rows of tiles, 29 us;
+// by four dies alone 43).  Rows far apart for each die would not do: 131,072 x 512
+// to 1,408, where they lie 2^23 bytes apart, 174 us, so 168.
 struct Places {
-    int die, tilesN, count;        // of the die's tiles, in order
+    int die, tilesN, own, rest, restBegin, count;        // of the die's tiles, in order
 
     __device__ Places(const Args& args, int bm, int bn) : die(blockIdx.x % 8), tilesN((args.columns + bn - 1) / bn)
     {
-        const int tilesM = (int)((args.rows + bm - 1) / bm);
-        count = (tilesM - die + 7) / 8 * tilesN;
+        const int tilesM = (int)((args.rows + bm - 1) / bm), left = tilesM % 8 * tilesN;
+        own = tilesM / 8 * tilesN;
+        rest = tilesM / 8 * 8;
+        restBegin = left * die / 8;
+        count = own + left * (die + 1) / 8 - restBegin;
     }
+    __device__ int row(int place) const { return place < own ? place / tilesN * 8 + die : rest + (restBegin + place - own) / tilesN; }
+    __device__ int column(int place) const { return (place < own ? place : restBegin + place - own) % tilesN; }
 };
 
 // Workgroups stay and take every so-many-th tile of their die.  While half a
@@ -303,8 +311,8 @@ __global__ __launch_bounds__(kWM* kWN * 64, kWM* kWN * kBlocks / 4) void int8Pro
     const auto copyNext = [&](int slot) {
         if (copyStep == 0) {        // another tile: its rows, and its scales
             const bool any = copyPlace < places.count;
-            const int64_t m0 = (int64_t)(copyPlace / places.tilesN * 8 + places.die) * kBM;
-            const int n0 = copyPlace % places.tilesN * kBN;
+            const int64_t m0 = (int64_t)places.row(copyPlace) * kBM;
+            const int n0 = places.column(copyPlace) * kBN;
             const int rows = !any ? 0 : args.rows - m0 < kBM ? (int)(args.rows - m0) : kBM;
             const int columns = !any ? 0 : args.columns - n0 < kBN ? args.columns - n0 : kBN;
             from[0] = descriptor(args.x + m0 * args.xRow, rows * (int)args.xRow);
@@ -367,7 +375,7 @@ __global__ __launch_bounds__(kWM* kWN * 64, kWM* kWN * kBlocks / 4) void int8Pro
             if (have > 64) tile.multiply(odd, have - 64);
         }
         const float* const own = reinterpret_cast<const float*>(stages + kStages * kStage + scales * Tile::kScales);
-        const bool whole = tile.finish(args, own, (int64_t)(place / places.tilesN * 8 + places.die) * kBM, place % places.tilesN * kBN);
+        const bool whole = tile.finish(args, own, (int64_t)places.row(place) * kBM, places.column(place) * kBN);
         scales = scales == kStages ? 0 : scales + 1;
         // the stores are younger than the copies of the next kStages stages; a part of a tile has fewer, so that they are waited for
         if (!whole) waitCopies();
@@ -387,8 +395,8 @@ __global__ __launch_bounds__(kWM* kWN * 64) void int8LooseKernel(const Args args
     const Places places(args, kBM, kBN);
     const int place = blockIdx.x / 8;
     if (place >= places.count) return;
-    const int64_t m0 = (int64_t)(place / places.tilesN * 8 + places.die) * kBM;
-    const int n0 = place % places.tilesN * kBN;
+    const int64_t m0 = (int64_t)places.row(place) * kBM;
+    const int n0 = places.column(place) * kBN;
 
     float* const scales = reinterpret_cast<float*>(stages + 2 * kStage);
     for (int i = threadIdx.x; i < kBM; i += kThreads) scales[i] = m0 + i < args.rows ? args.xScale[m0 + i] : 0.0f;
@@ -512,8 +520,8 @@ constexpr int64_t kMostRows = (int64_t)1 << 28, kThinRows = 128;
 // kBlocks workgroups a compute unit.
 template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN, int kStages, int kBlocks> void launchTile(const Args& a, hipStream_t stream)
 {
-    const int64_t tilesM = (a.rows + kBM - 1) / kBM, tilesN = (a.columns + kBN - 1) / kBN;
-    const dim3 grid((unsigned)std::min<int64_t>((tilesM + 7) / 8 * 8 * tilesN, 256 * kBlocks));
+    const int64_t tiles = (a.rows + kBM - 1) / kBM * ((a.columns + kBN - 1) / kBN);
+    const dim3 grid((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, 256 * kBlocks));
     int8ProductKernel<T, kGated, kBM, kBN, kWM, kWN, kStages, kBlocks><<<grid, kWM * kWN * 64, 0, stream>>>(a);
 }
 
@@ -558,7 +566,7 @@ template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t str
     const auto fills = [](int64_t tiles) { return 5 * tiles >= 4 * ((tiles + 255) / 256 * 256); };
     if (!direct) {
         constexpr int kBN = kGated ? 64 : 128;
-        const dim3 grid((unsigned)((tiles(128, a.columns) + 7) / 8 * 8 * tiles((int)a.rows, kBN)));
+        const dim3 grid((unsigned)((tiles(128, kBN) + 7) / 8 * 8));
         int8LooseKernel<T, kGated, 128, kBN, 2, 2><<<grid, 256, 0, stream>>>(a);
     } else if constexpr (kGated) {
         if (fills(tiles(256, 128))) launchTile<T, kGated, 256, 128, 4, 2, 2, 1>(a, stream);
