@@ -224,6 +224,16 @@ def test_some_gradients():
     assert torch.equal(dx, dres)
 
 
+def test_one_tensor_as_input_and_residual():
+    x, weight, _, dy, dsum = _rows(300, 72, torch.float32)
+    leaf, w = x.detach().requires_grad_(), weight.detach().requires_grad_()
+    y, total = _ops().rms_norm(leaf, w, residual=leaf)
+    torch.autograd.backward([y, total], [dy, dsum])
+    value, bound = policy.norm(x, weight, x, 1e-6, dy, dsum)
+    ref.assert_within(leaf.grad, 2 * value["dx"], 2 * bound["dx"], "dx")        # doubling rounds nothing
+    ref.assert_within(w.grad, value["dweight"], bound["dweight"], "dweight")
+
+
 def test_gradients_add_up_over_a_stream():
     """Two norms on one residual stream, as blocks use them, against the chain in 64 bits."""
     x, weight, residual, dy, dsum = _rows(20, 48, torch.float32)
