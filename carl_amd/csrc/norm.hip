@@ -340,7 +340,7 @@ constexpr int threadsOf(int lanes) { return lanes < 128 ? 256 : lanes; }
 int blocksOf(int64_t rows, int lanes, int most)
 {
     const int64_t groups = groupsOf(lanes);
-    return (int)std::min<int64_t>((rows + groups - 1) / groups, lanes <= 256 ? most : most / 4);
+    return (int)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)most * 256 / std::max(lanes, 256));
 }
 
 constexpr int kForwardBlocks = 65536, kGradBlocks = 1024;
