@@ -9,8 +9,8 @@
 //
 // What bounds it: memory, and for short heads the exponentials and the chain of
 // one head's steps (the simulator's 7 heads of 18 logits in bf16, masked: 1,048,576
-// log-probabilities 27 us, 3.6 TB/s, and gradients 32, 4.2 TB/s; 131,072 best
-// actions with noise 10.0, 2.4 TB/s; 62,000 rows of 90 in f32 9.3 and 12.8).  Two
+// log-probabilities 24 us, 3.9 TB/s, and gradients 30, 4.3 TB/s; 131,072 best
+// actions with noise 9.6, 2.5 TB/s; 62,000 rows of 90 in f32 9.3 and 12.8).  Two
 // forms:
 //   own     heads of up to 32.  A lane takes a row, in pieces of 16 bytes (masked
 //           logits as -infinity), and keeps it in LDS, where heads of any size
@@ -86,6 +86,16 @@ __device__ inline uint32_t keyOf(float key, float logit)
 // the last place each; Z is at least 1 where anything is available.
 __device__ inline float exponential(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
+// The larger number; of a number and a (quiet) NaN the number.  fmaxf takes two
+// instructions where it does not see what its argument is, the first to make
+// signalling NaN quiet; here they stay NaN.
+__device__ inline float larger(float a, float b)
+{
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 // The largest of a head's logits as the others are taken from: 0 where nothing
 // is available (or all of it is NaN, which Z then tells).
 __device__ inline float baseOf(float most) { return most == kNone ? 0.0f : most; }
@@ -95,7 +105,7 @@ __device__ inline float baseOf(float most) { return most == kNone ? 0.0f : most;
 __device__ inline void addTo(float& z, float& a, float d, float e)
 {
     z += e;
-    a += e * fmaxf(d, -1e30f);
+    a = __builtin_fmaf(e, fmaxf(d, -1e30f), a);
 }
 
 // What follows from a head's m, Z and A.
@@ -242,66 +252,73 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy, int kShare> __global
             if (h + kShare < a.heads) read(h + kShare);
             float* const x = own + a.first[h];
             const int n = a.first[h + 1] - a.first[h];
-            // (the conditions are the same for all lanes)
-            float most = kNone, z = 0.0f, sum = 0.0f, d[kAhead], e[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (i < n) most = fmaxf(most, now.x[i]);
-            for (int j = kAhead; j < n; j++) most = fmaxf(most, x[j]);
-            const float base = baseOf(most);
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (i < n) {
-                    d[i] = now.x[i] - base;
-                    e[i] = exponential(d[i]);
-                    addTo(z, sum, d[i], e[i]);
-                }
-            for (int j = kAhead; j < n; j++) addTo(z, sum, x[j] - base, exponential(x[j] - base));
-            const Sums s(base, z, sum);
-            if constexpr (kWhat == kBest) {
-                const uint32_t* const key = keys + a.first[h];
-                const int64_t at = (row * a.heads + h) * a.k;
-                uint32_t lastKey = 0xffffffffu;
-                int last = -1;
-                for (int i = 0; i < a.k; i++) {
-                    uint32_t largest = 0;
-                    int best = -1;
-                    float picked = kNone;
-                    const auto consider = [&](int j, uint32_t u, float v) {
-                        if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
-                            largest = u;
-                            best = j;
-                            picked = v;
-                        }
-                    };
-#pragma unroll
-                    for (int j = 0; j < kAhead; j++)
-                        if (j < n) consider(j, now.key[j], now.x[j]);
-                    for (int j = kAhead; j < n; j++) consider(j, key[j], x[j]);
-                    if (mine) {
-                        a.best[at + i] = best;
-                        a.logProb[at + i] = s.logProb(picked);
-                    }
-                    lastKey = largest;
-                    last = best < 0 ? n : best;
-                }
-            } else if constexpr (kWhat == kLogProb) {
-                const int action = now.action;
-                const float taken = s.taken(action, n, x[action >= 0 && action < n ? action : 0]);
-                if constexpr (kShare == 1) {
-                    logProb += taken;
-                    entropy += s.entropy;
-                } else {
-                    results[h * 128] = taken;
-                    results[h * 128 + 64] = s.entropy;
-                }
-            } else {
-                const float share = shareOf(now.action, n, dLogProb);
+            // short heads by their length, which is the same for all lanes (a condition for each logit: 26 and 32 us for 24 and 30)
+            const auto compute = [&](auto few) {
+                float most = kNone, z = 0.0f, sum = 0.0f, d[kAhead], e[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; i++)
-                    if (i < n) x[i] = gradient(s, now.x[i], d[i], e[i], i == now.action, share, dEntropy);
-                for (int j = kAhead; j < n; j++) x[j] = gradient(s, x[j], x[j] - base, exponential(x[j] - base), j == now.action, share, dEntropy);
-            }
+                    if (i < few()) most = larger(most, now.x[i]);
+                for (int j = kAhead; few() == kAhead && j < n; j++) most = larger(most, x[j]);
+                const float base = baseOf(most);
+#pragma unroll
+                for (int i = 0; i < kAhead; i++)
+                    if (i < few()) {
+                        d[i] = now.x[i] - base;
+                        e[i] = exponential(d[i]);
+                        addTo(z, sum, d[i], e[i]);
+                    }
+                for (int j = kAhead; few() == kAhead && j < n; j++) addTo(z, sum, x[j] - base, exponential(x[j] - base));
+                const Sums s(base, z, sum);
+                if constexpr (kWhat == kBest) {
+                    const uint32_t* const key = keys + a.first[h];
+                    const int64_t at = (row * a.heads + h) * a.k;
+                    uint32_t lastKey = 0xffffffffu;
+                    int last = -1;
+                    for (int i = 0; i < a.k; i++) {
+                        uint32_t largest = 0;
+                        int best = -1;
+                        float picked = kNone;
+                        const auto consider = [&](int j, uint32_t u, float v) {
+                            if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
+                                largest = u;
+                                best = j;
+                                picked = v;
+                            }
+                        };
+#pragma unroll
+                        for (int j = 0; j < kAhead; j++)
+                            if (j < n) consider(j, now.key[j], now.x[j]);
+                        for (int j = kAhead; few() == kAhead && j < n; j++) consider(j, key[j], x[j]);
+                        if (mine) {
+                            a.best[at + i] = best;
+                            a.logProb[at + i] = s.logProb(picked);
+                        }
+                        lastKey = largest;
+                        last = best < 0 ? n : best;
+                    }
+                } else if constexpr (kWhat == kLogProb) {
+                    const int action = now.action;
+                    const float taken = s.taken(action, n, x[action >= 0 && action < n ? action : 0]);
+                    if constexpr (kShare == 1) {
+                        logProb += taken;
+                        entropy += s.entropy;
+                    } else {
+                        results[h * 128] = taken;
+                        results[h * 128 + 64] = s.entropy;
+                    }
+                } else {
+                    const float share = shareOf(now.action, n, dLogProb);
+#pragma unroll
+                    for (int i = 0; i < kAhead; i++)
+                        if (i < few()) x[i] = gradient(s, now.x[i], d[i], e[i], i == now.action, share, dEntropy);
+                    for (int j = kAhead; few() == kAhead && j < n; j++)
+                        x[j] = gradient(s, x[j], x[j] - base, exponential(x[j] - base), j == now.action, share, dEntropy);
+                }
+            };
+            if (n == 1) compute(std::integral_constant<int, 1>());
+            else if (n == 2) compute(std::integral_constant<int, 2>());
+            else if (n == 3) compute(std::integral_constant<int, 3>());
+            else compute(std::integral_constant<int, kAhead>());
         }
         handOver();
         if constexpr (kWhat == kLogProb) {
