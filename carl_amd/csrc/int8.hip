@@ -565,9 +565,13 @@ template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t str
                      && (!kGated || inPieces(a.w[1], a.wRow[1], a.width)) && inWords(a.bias);
     const auto fills = [](int64_t tiles) { return 5 * tiles >= 4 * ((tiles + 255) / 256 * 256); };
     if (!direct) {
+        // (683 to 257, 2,001 rows: tiles of 128 x 128 24.8 us, of 64 x 64 15.6; 257 to 512, 16,384 rows: 14.4 and 19.0)
         constexpr int kBN = kGated ? 64 : 128;
-        const dim3 grid((unsigned)((tiles(128, kBN) + 7) / 8 * 8));
-        int8LooseKernel<T, kGated, 128, kBN, 2, 2><<<grid, 256, 0, stream>>>(a);
+        const auto loose = [&](auto bm, auto bn) {
+            int8LooseKernel<T, kGated, bm(), bn(), 2, 2><<<dim3((unsigned)((tiles(bm(), bn()) + 7) / 8 * 8)), 256, 0, stream>>>(a);
+        };
+        if (tiles(128, kBN) >= 256) loose(std::integral_constant<int, 128>(), std::integral_constant<int, kBN>());
+        else loose(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
     } else if constexpr (kGated) {
         if (fills(tiles(256, 128))) launchTile<T, kGated, 256, 128, 4, 2, 2, 1>(a, stream);
         else if (tiles(128, 64) >= 256) launchTile<T, kGated, 128, 64, 2, 2, 2, 2>(a, stream);
