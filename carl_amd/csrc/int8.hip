@@ -131,13 +131,13 @@ __device__ inline int anew(int x)
 // number, mod 8, of the lane that reads them, so that eight lanes meet all
 // banks: x's by the row's, w's by what wReader says.
 template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN> struct Tile {
-    static constexpr int kNB = kGated ? 2 : 1, kThreads = kWM * kWN * 64, kWaves = kWM * kWN;
+    static constexpr int kNB = kGated ? 2 : 1, kThreads = kWM * kWN * 64;
     static constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16, kRun = 8;
     static constexpr int kRows = kBM + kNB * kBN, kStage = kRows * kRowBytes;
     static constexpr int kCopyRows = kThreads / kPieces, kCopies = kRows / kCopyRows;
     // words of scales: of the rows, of the columns, and the bias
     static constexpr int kBiasWords = kGated ? 0 : (kBN * (int)sizeof(T) / 4 + 63) / 64 * 64, kWords = kBM + kNB * kBN + kBiasWords;
-    static constexpr int kWordCopies = (kWords + kThreads - 1) / kThreads, kScales = kWords * 4;
+    static constexpr int kScales = kWords * 4;
     static constexpr int kStores = kTM * (kTN / 2) * (int)sizeof(T) / 2;       // of a whole tile
     static_assert(kBM % kCopyRows == 0 && kBN % kCopyRows == 0, "whole copies");
     static_assert(kCopyRows % 16 == 0 && kTN % 2 == 0, "one permutation for a thread's pieces, runs of two tiles");
@@ -515,7 +515,7 @@ template <typename T, bool kGated, int kTM> __global__ __launch_bounds__(512) vo
 
 // ---- launches ------------------------------------------------------------------
 
-constexpr int64_t kMostRows = (int64_t)1 << 28, kThinRows = 128;
+constexpr int64_t kMostRows = (int64_t)1 << 28, kThinRows = 16;
 
 // kBlocks workgroups a compute unit.
 template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN, int kStages, int kBlocks> void launchTile(const Args& a, hipStream_t stream)
@@ -533,8 +533,11 @@ bool inPieces(const void* p, int64_t stride, int width)
 
 bool inWords(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
-// By a sweep from 129 to 131,072 rows (us):
-//   few rows      1,408 to 512, 512 rows   thin 5.6   64 x 64 7.1     1,024 rows  9.0 and 7.4     (thin: 16 columns, 64 rows)
+// By sweeps from 1 to 131,072 rows (us):
+//   few rows      1,408 to 512, 512 rows   thin 5.6   64 x 64 7.1     1,024 rows  9.0 and 7.4
+//                 4,096 to 8,192, 1 row   7.0 and 16.2     32 rows  13.4 and 16.4     64 rows  21.2 and 16.5
+//                 1,024 to 20,000, 16 rows   7.0 and 7.5     32 rows  9.5 and 7.8     128 rows  32.4 and 11.6
+//                 (one row of 4,096 to 65,536 53 us: 5.0 TB/s of weights)
 //   small tiles   1,024 to 2,816, 512 rows   64 x 64 7.5   128 x 128 9.3     1,024 rows  9.7 and 9.4     8,192 rows  44.8 and 34.0
 //                 gated, 512 rows   64 x 64 9.4   128 x 64 12.5      2,001 rows  20.6 and 18.8
 //   large tiles   1,408 to 512, 32,768 rows (256 tiles)   128 x 128 29.9   256 x 256 28.7      131,072 rows  139 and 107
@@ -549,15 +552,15 @@ bool inWords(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t stream)
 {
     const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
-    if (a.rows <= kThinRows || tiles(64, 16) <= 256) {
+    if (a.rows <= kThinRows || tiles(16, 16) <= 1024) {
         const unsigned columns = (unsigned)((a.columns + 15) / 16);
         const auto thin = [&](auto tiles) {
             int8ThinKernel<T, kGated, tiles()><<<dim3(columns, (unsigned)((a.rows + 16 * tiles() - 1) / (16 * tiles()))), 512, 0, stream>>>(a);
         };
-        // as few rows a workgroup as keep the GPU from more than one round or so (4,096 to 64, 1,006 rows: 16 rows 5.8 us, 64 rows
-        // 11.0; 1,408 to 512, 512 rows: 7.4 and 5.7)
-        if (tiles(16, 16) <= 256) thin(std::integral_constant<int, 1>());
-        else if (tiles(32, 16) <= 384) thin(std::integral_constant<int, 2>());
+        // as few rows a workgroup as there are, or as keep the GPU from more than one round or so (4,096 to 64, 1,006 rows: 16 rows
+        // 5.8 us, 64 rows 11.0; 1,408 to 512, 512 rows: 7.4 and 5.7; 4,096 to 8,192, one row: 7.0 and 11.8)
+        if (a.rows <= 16 || tiles(16, 16) <= 256) thin(std::integral_constant<int, 1>());
+        else if (a.rows <= 32 || tiles(32, 16) <= 384) thin(std::integral_constant<int, 2>());
         else thin(std::integral_constant<int, 4>());
         return;
     }

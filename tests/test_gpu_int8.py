@@ -168,7 +168,8 @@ def test_gates_of_values_whose_product_float32_does_not_hold(N):
 
 
 @pytest.mark.parametrize("N,D,F,gated", [(400, 64, 20_000, False), (250, 200, 9001, False), (300, 130, 9000, True), (2300, 64, 3000, False),
-                                         (140, 20, 65_536, True), (3, 20, 65_536, True)])
+                                         (140, 20, 65_536, True), (3, 20, 65_536, True), (16, 300, 17_000, False), (17, 100, 17_000, True),
+                                         (32, 77, 9000, False), (33, 77, 9000, True), (64, 64, 9000, False), (90, 140, 5000, True)])
 def test_more_columns_than_rows(N, D, F, gated):
     for padded in (True, False):
         _check(*_inputs(N, D, F, torch.bfloat16, seed=F, padded=padded), gated=gated)
