@@ -412,26 +412,61 @@ __global__ __launch_bounds__(kSharedThreads) void sharedKernel(const Args a, int
             const Sums s(base, zAll, sumAll);
             if constexpr (kWhat == kBest) {
                 const int64_t at = (row * a.heads + h) * a.k;
-                uint32_t lastKey = 0xffffffffu;
-                int last = -1;
-                for (int i = 0; i < a.k; i++) {
+                if (kLanes == kSharedThreads && a.k > 1) {
+                    // a lane's keys lie in LDS and its best one in registers, and only the lane whose key was taken looks for its
+                    // next one
+                    extern __shared__ uint32_t keys[];
+                    each([&](int j, float x, float key) {
+                        if (j < n) keys[j] = keyOf(key, x);
+                    });
                     uint32_t largest = 0;
                     int best = INT32_MAX;
-                    float picked = kNone;
-                    each([&](int j, float x, float key) {
-                        const uint32_t u = keyOf(key, x);
-                        if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
-                            largest = u;
-                            best = j;
-                            picked = x;
+                    const auto look = [&]() {
+                        largest = 0;
+                        best = INT32_MAX;
+#pragma unroll 8
+                        for (int j = lane; j < n; j += kLanes) {
+                            const uint32_t u = keys[j];
+                            best = u > largest ? j : best;
+                            largest = u > largest ? u : largest;
                         }
-                    });
-                    lastKey = overRow<Most, kLanes>(largest, bits);
-                    last = (int)overRow<Least, kLanes>((uint32_t)(largest == lastKey ? best : INT32_MAX), bits);
-                    // (of nothing that is left, the group's first lane)
-                    if (last == INT32_MAX ? lane == 0 : best == last) {
-                        a.best[at + i] = last == INT32_MAX ? -1 : best;
-                        a.logProb[at + i] = s.logProb(picked);
+                    };
+                    look();
+                    for (int i = 0; i < a.k; i++) {
+                        const uint32_t most = overRow<Most, kLanes>(largest, bits);
+                        const int taken = (int)overRow<Least, kLanes>((uint32_t)(largest == most ? best : INT32_MAX), bits);
+                        // (of nothing that is left, the first lane)
+                        if (taken == INT32_MAX ? lane == 0 : best == taken) {
+                            a.best[at + i] = taken == INT32_MAX ? -1 : taken;
+                            a.logProb[at + i] = s.logProb(taken == INT32_MAX ? kNone : load(taken));
+                            if (taken != INT32_MAX) {
+                                keys[taken] = 0;
+                                look();
+                            }
+                        }
+                    }
+                } else {
+                    uint32_t lastKey = 0xffffffffu;
+                    int last = -1;
+                    for (int i = 0; i < a.k; i++) {
+                        uint32_t largest = 0;
+                        int best = INT32_MAX;
+                        float picked = kNone;
+                        each([&](int j, float x, float key) {
+                            const uint32_t u = keyOf(key, x);
+                            if (u > largest && (u < lastKey || (u == lastKey && j > last))) {
+                                largest = u;
+                                best = j;
+                                picked = x;
+                            }
+                        });
+                        lastKey = overRow<Most, kLanes>(largest, bits);
+                        last = (int)overRow<Least, kLanes>((uint32_t)(largest == lastKey ? best : INT32_MAX), bits);
+                        // (of nothing that is left, the group's first lane)
+                        if (last == INT32_MAX ? lane == 0 : best == last) {
+                            a.best[at + i] = last == INT32_MAX ? -1 : best;
+                            a.logProb[at + i] = s.logProb(picked);
+                        }
                     }
                 }
             } else {
@@ -494,10 +529,15 @@ template <typename T, int kWhat> void launch(const Args& a, hipStream_t stream)
     const int share = a.rows <= 65536 || logits > 32 ? 4 : a.heads > 1 && (kWhat == kBest || a.rows <= 200000) ? 2 : 1;
     // Lanes of a head by a sweep over 20 M logits (us, log-probabilities): heads of 33 8 lanes 40, 16 lanes 69; of 90 16 lanes 34;
     // of 200 32 lanes 34, 64 lanes 56; of 513 64 lanes 35, a workgroup 80; of 2,000 64 lanes 40, a workgroup 33 (34 rows: 9 and 5).
+    // A workgroup's choice of several (its keys in LDS, 16,384 logits, 1 row, the best 64: 119 us, read again for each 1,099) is
+    // quicker from 769 logits on, and from 513 for few heads (5 best, a workgroup and 64 lanes: 1,000 heads of 700 9.1 and 11.9,
+    // 10,000 51 and 36; of 1,000 56 and 70).
+    const bool together = kWhat == kBest && a.k > 1 && (longest > 768 || a.rows * a.heads <= 2048);
     const auto with = [&](auto masked, auto noisy) {
         const auto shared = [&](auto lanes) {
             const int groups = kSharedThreads / lanes(), rows = groups > a.heads ? groups / a.heads : 1;
-            sharedKernel<T, kWhat, masked(), noisy(), lanes()><<<blocks(rows), kSharedThreads, 0, stream>>>(a, rows, longest);
+            const int bytes = kWhat == kBest && lanes() == kSharedThreads && a.k > 1 ? longest * 4 : 0;
+            sharedKernel<T, kWhat, masked(), noisy(), lanes()><<<blocks(rows), kSharedThreads, bytes, stream>>>(a, rows, longest);
         };
         if (own) {
             const auto with = [&](auto share) {
@@ -509,7 +549,7 @@ template <typename T, int kWhat> void launch(const Args& a, hipStream_t stream)
         } else if (longest <= 64) shared(integral_constant<int, 8>());
         else if (longest <= 128) shared(integral_constant<int, 16>());
         else if (longest <= 256) shared(integral_constant<int, 32>());
-        else if (longest <= 1024) shared(integral_constant<int, 64>());
+        else if (longest <= (together ? 512 : 1024)) shared(integral_constant<int, 64>());
         else shared(integral_constant<int, kSharedThreads>());
     };
     if constexpr (kWhat == kBest) {

@@ -241,7 +241,32 @@ def test_all_of_a_heads_actions_in_order(heads):
     _check_top(logits.masked_fill(~there, -math.inf), heads, 10)
 
 
-@pytest.mark.parametrize("heads", [(8,), (40, 30), (600,)], ids=str)
+@pytest.mark.parametrize("heads", [(513,), (769,), (900, 3), (1025, 2, 800), (5000,), (16_384,)], ids=str)
+def test_many_actions_of_long_heads(heads):
+    logits, _, there = _rows((5,), heads, torch.bfloat16, mask=True)
+    noise = torch.randn(logits.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    there[2], there[3, 7:] = False, False           # nothing to take, and fewer than are asked for
+    logits[4, ::3] = 1.0                            # many equal ones
+    for k in (2, 64):
+        _check_top(logits, heads, k, there)
+        best, _ = _ops().top_actions(logits, heads, k, mask=there, noise=noise)
+        want, _, _ = policy.top(logits, heads, k, there, noise)
+        assert torch.equal(best.cpu(), want)
+
+
+@pytest.mark.parametrize("heads", [(700,), (800,), (1100, 5)], ids=str)
+def test_many_rows_of_several_actions(heads):
+    """As many as are taken by lanes, and by workgroups: the same as of a few rows."""
+    logits, _, there = _rows((2100,), heads, torch.float32)
+    best, logs = _ops().top_actions(logits, heads, 6, mask=there)
+    few = [_ops().top_actions(logits[i:i + 300], heads, 6, mask=there[i:i + 300]) for i in range(0, 2100, 300)]
+    assert torch.equal(best, torch.cat([b for b, _ in few]))
+    # sums of a thousand terms in another order, at logarithms of order 10
+    assert torch.allclose(logs, torch.cat([v for _, v in few]), rtol=0, atol=1e-4)
+    _check_top(logits[:3], heads, 6, there[:3])
+
+
+@pytest.mark.parametrize("heads", [(8,), (40, 30), (600,), (1200,)], ids=str)
 def test_equal_keys_go_by_their_index(heads):
     logits = torch.randint(-1, 2, (12, sum(heads)), generator=torch.Generator().manual_seed(0)).float().cuda()
     logits = torch.where((logits == 0) & (torch.arange(sum(heads), device="cuda") % 2 == 1), -0.0, logits)      # both zeros
@@ -252,7 +277,7 @@ def test_equal_keys_go_by_their_index(heads):
     _check_top(logits, heads, 5, None, noise)
 
 
-@pytest.mark.parametrize("heads", [(8,), (70,), (300,)], ids=str)
+@pytest.mark.parametrize("heads", [(8,), (70,), (300,), (1030,)], ids=str)
 def test_keys_that_are_not_finite(heads):
     """A NaN among the logits goes first and makes the log-probabilities NaN; noise may be infinite or NaN, and counts
     only where an action is available."""
