@@ -60,21 +60,14 @@ __device__ inline uint4 loadBytes(const int8_t* p, int have)
 // kActivation: of the gated form, or kNone.
 constexpr int kNone = -1;
 
-// What columns' scales are multiplied with, once for all rows.  SiLU's gate and
-// up go together as (log2(e) g) (u / log2(e)) / (1 + 2^-(log2(e) g)): a product
-// less for each value, and the values are what bounds the gated form's last step.
-constexpr float kLog2e = 1.44269504088896341f;
-template <int kActivation> __device__ inline float gateScale(float w) { return kActivation == CARL_SILU ? w * kLog2e : w; }
-template <int kActivation> __device__ inline float upScale(float w) { return kActivation == CARL_SILU ? w * (1.0f / kLog2e) : w; }
-
+// The gate is not multiplied by log2(e) in its column's scale, which is a product less for each value (131,072 x 512 to two of
+// 1,408 255 us, so 261): past 2.36e38 that would leave float32's range, to an infinity or, of a negative gate, a NaN.
 template <int kActivation> __device__ inline float valueOf(int acc, int up, float xScale, float scale, float upScale)
 {
     const float y = (float)acc * xScale * scale;
     if constexpr (kActivation == kNone) return y;
-    const float u = (float)up * xScale * upScale;
     // (the gate first: of a large negative one it is 0 whatever u is, where y u may be an infinity)
-    if constexpr (kActivation == CARL_SILU) return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y)) * u;
-    else return activate(y, CARL_GELU) * u;
+    return activate(y, kActivation) * ((float)up * xScale * upScale);
 }
 
 // kRun neighbouring values of a row, of which `have` are the result's.
@@ -219,11 +212,7 @@ template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN> struct Ti
 #pragma unroll
             for (int b = 0; b < kNB; b++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    scale[b][h] = *reinterpret_cast<const f32x4*>(scales + kBM + b * kBN + n + r * 32 + h * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) scale[b][h][e] = b == 0 ? gateScale<kActivation>(scale[b][h][e]) : upScale<kActivation>(scale[b][h][e]);
-                }
+                for (int h = 0; h < 2; h++) scale[b][h] = *reinterpret_cast<const f32x4*>(scales + kBM + b * kBN + n + r * 32 + h * 4);
             if (!kGated && args.bias) bias = *reinterpret_cast<const vec<T, kRun>*>(reinterpret_cast<const T*>(scales + kBM + kBN) + n + r * 32);
 #pragma unroll
             for (int i = 0; i < kTM; i++) {
@@ -502,7 +491,7 @@ template <typename T, bool kGated, int kTM> __global__ __launch_bounds__(512) vo
         const int at = n + e < args.columns ? n + e : args.columns - 1;
         const float scale = args.wScale[0][at], second = kGated ? args.wScale[1][at] : 0.0f;
         const auto value = [&](auto activation) {
-            return valueOf<activation()>(sum[0][e], sum[kNB - 1][e], xScale, gateScale<activation()>(scale), upScale<activation()>(second));
+            return valueOf<activation()>(sum[0][e], sum[kNB - 1][e], xScale, scale, second);
         };
         if constexpr (!kGated) {
             y[e] = value(std::integral_constant<int, kNone>());

@@ -167,6 +167,19 @@ def test_gates_of_values_whose_product_float32_does_not_hold(N):
         assert (y[g < 0] == 0).all() and (y[(g > 1e20) & (u > 1e20)] == math.inf).all()
 
 
+@pytest.mark.parametrize("N,F,padded", [(20, 40, True), (150, 3000, True), (2500, 400, True), (2500, 400, False), (14_001, 500, True)])
+def test_gates_at_the_end_of_float32(N, F, padded):
+    """Gates near float32's largest number, whose product with log2(e) it does not hold, in every form of the product."""
+    x, w, up = (_codes(n, 40, torch.Generator().manual_seed(0), padded).zero_() for n in (N, F, F))
+    x[:, 3], w[::2, 3], w[1::2, 3], up[:, 3] = 1, 1, -1, 1
+    for value in (0.5, 2.0 ** -30):
+        scales = [torch.full((n,), c, device="cuda") for n, c in ((N, 1.0), (F, 3e38), (F, value))]
+        for name in ("silu", "gelu"):
+            y = _ops().int8_gated_linear(x, scales[0], w, scales[1], up, scales[2], activation=name, dtype=torch.float32).cpu()
+            # a gate's act is the gate itself, or 0; the reciprocal is good to a unit in the last place, products to half of one
+            assert ((y[:, ::2] / value - 3e38).abs() <= 4 * 2.0 ** -24 * 3e38).all() and (y[:, 1::2] == 0).all()
+
+
 @pytest.mark.parametrize("N,D,F,gated", [(400, 64, 20_000, False), (250, 200, 9001, False), (300, 130, 9000, True), (2300, 64, 3000, False),
                                          (140, 20, 65_536, True), (3, 20, 65_536, True), (16, 300, 17_000, False), (17, 100, 17_000, True),
                                          (32, 77, 9000, False), (33, 77, 9000, True), (64, 64, 9000, False), (90, 140, 5000, True)])
