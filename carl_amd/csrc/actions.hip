@@ -135,10 +135,10 @@ __device__ inline float gradient(const Sums& s, float x, float d, float e, bool 
     return x == kNone ? 0.0f : g;
 }
 
-// What an action leaves of its log-probability's gradient.
-__device__ inline float shareOf(int action, int size, float dLogProb)
+// What an action leaves of its log-probability's gradient; nothing where there is none.
+__device__ inline float shareOf(int action, int size, const float* given, float dLogProb)
 {
-    return action < 0 ? 0.0f : action >= size ? __builtin_nanf("") : dLogProb;
+    return !given || action < 0 ? 0.0f : action >= size ? __builtin_nanf("") : dLogProb;
 }
 
 // ---- own -------------------------------------------------------------------------
@@ -307,7 +307,7 @@ template <typename T, int kWhat, bool kMasked, bool kNoisy, int kShare> __global
                         results[h * 128 + 64] = s.entropy;
                     }
                 } else {
-                    const float share = shareOf(now.action, n, dLogProb);
+                    const float share = shareOf(now.action, n, a.dLogProb, dLogProb);
 #pragma unroll
                     for (int i = 0; i < kAhead; i++)
                         if (i < few()) x[i] = gradient(s, now.x[i], d[i], e[i], i == now.action, share, dEntropy);
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(kSharedThreads) void sharedKernel(const Args a, int
                         results[1][unit] = s.entropy;
                     }
                 } else {
-                    const float share = shareOf(action, n, a.dLogProb ? a.dLogProb[row * a.dLogProbStep] : 0.0f);
+                    const float share = shareOf(action, n, a.dLogProb, a.dLogProb ? a.dLogProb[row * a.dLogProbStep] : 0.0f);
                     const float dEntropy = a.dEntropy ? a.dEntropy[row * a.dEntropyStep] : 0.0f;
                     T* const to = static_cast<T*>(a.dLogits) + row * a.first[a.heads] + first;
                     each([&](int j, float x, float) {

@@ -115,8 +115,9 @@ def action_log_prob(logits: torch.Tensor, actions: torch.Tensor, heads: Sequence
     A masked logit, or one of -infinity, weighs nothing whatever it holds and
     gets the gradient 0; its action's log-probability is -infinity.  A head
     with nothing to take has entropy 0.  An action below 0 is none: its head
-    adds nothing to the log-probability; an action past its head's last gives
-    NaN.  Gradients of both results reach logits, once.
+    adds nothing to the log-probability; an action past its head's last makes
+    it NaN, and its head's gradients by it.  Gradients of both results reach
+    logits, once.
     """
     return _ops.action_log_prob(logits, actions, list(heads), mask)
 

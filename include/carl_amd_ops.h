@@ -174,8 +174,10 @@ int carl_adamw_encode(const float* exp_avg, const float* exp_avg_sq, int64_t n, 
  * is not available weighs nothing whatever it holds, has the log-probability
  * -infinity and the gradient 0.  A head with nothing available has entropy 0.
  * An action below 0 is none: its head adds 0 to the log-probability (and takes
- * part in the entropy).  An action past its head's last gives NaN.  A NaN or
- * +infinity among the available logits makes its head's results NaN.
+ * part in the entropy).  An action past its head's last makes the
+ * log-probability NaN, and its head's gradients where there are some by the
+ * log-probability.  A NaN or +infinity among the available logits makes its
+ * head's results NaN.
  *
  * The best actions of a head are those with the largest keys, the available
  * logits plus noise (one float32 addition; without noise the logits), equal

@@ -194,6 +194,20 @@ def test_gradients_of_one_result_and_of_a_mean():
         _same(grad, *policy.log_prob_gradient(logits, actions, CAR, *weights, there), "gradient")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("heads", [CAR, (70, 30), (300, 2)], ids=str)
+def test_an_entropys_gradient_has_nothing_to_do_with_the_actions(heads, dtype):
+    """An action past its head's last makes log-probabilities NaN, and gradients by them: not those of the entropy alone."""
+    logits, actions, there = _rows((70,), heads, dtype)
+    wrong = actions.clone()
+    wrong[::2, 0], wrong[1::3, -1] = heads[0], 2 ** 31 - 1
+    for mask in (None, there):
+        leaf = logits.clone().requires_grad_()
+        grads = [torch.autograd.grad(_ops().action_log_prob(leaf, a, heads, mask=mask)[1].sum(), [leaf])[0] for a in (wrong, actions)]
+        _same(grads[0], *policy.log_prob_gradient(logits, actions * 0, heads, torch.zeros(()), torch.ones(()), mask), "gradient")
+        assert torch.equal(*grads)
+
+
 def test_gradients_against_differences():
     heads, gen = (5, 3, 40), torch.Generator().manual_seed(1)
     logits, actions, there = _rows((8,), heads, torch.float32)
