@@ -504,7 +504,7 @@ template <typename T, bool kGated, int kTM> __global__ __launch_bounds__(512) vo
 
 // ---- launches ------------------------------------------------------------------
 
-constexpr int64_t kMostRows = (int64_t)1 << 28, kThinRows = 16;
+constexpr int64_t kThinRows = 16;
 
 // kBlocks workgroups a compute unit.
 template <typename T, bool kGated, int kBM, int kBN, int kWM, int kWN, int kStages, int kBlocks> void launchTile(const Args& a, hipStream_t stream)
@@ -592,7 +592,7 @@ extern "C" int carl_int8_linear_forward(const carl_int8_linear* p, void* stream)
     if (p->width < 1 || p->width > CARL_INT8_MAX_DIM) return fail(CARL_ERR_VALUE, "width must be in [1, 65536]");
     if (p->columns < 1 || p->columns > CARL_INT8_MAX_DIM) return fail(CARL_ERR_VALUE, "columns must be in [1, 65536]");
     const int64_t tiles = (p->rows + 127) / 128 * ((p->columns + 127) / 128);
-    if (p->rows < 0 || p->rows > kMostRows || tiles > (int64_t)1 << 22) return fail(CARL_ERR_VALUE, "rows are out of range");
+    if (p->rows < 0 || p->rows > CARL_INT8_MAX_ROWS || tiles > CARL_INT8_MAX_TILES) return fail(CARL_ERR_VALUE, "rows are out of range");
     if (gated && p->bias) return fail(CARL_ERR_VALUE, "the gated product has no bias");
     if (p->rows == 0) return CARL_OK;
     if (!p->x || !p->x_scale || !p->w || !p->w_scale || (gated && !p->w_up_scale) || !p->y) return fail(CARL_ERR_VALUE, "null product tensor");

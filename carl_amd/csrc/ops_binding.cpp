@@ -401,7 +401,17 @@ carl_actions actionsOf(const Tensor& logits, const std::vector<int64_t>& heads, 
     return a;
 }
 
-// The tensors of a call, alive until it is queued.
+void actionsFit(const Tensor& actions, const Tensor& logits, int32_t heads)
+{
+    const OnDevice onDevice;
+    onDevice(actions, "actions");
+    requireType(actions.scalar_type() == at::kInt || actions.scalar_type() == at::kLong, "actions must have dtype int32 or int64");
+    require(actions.dim() == logits.dim() && actions.size(-1) == heads
+                && actions.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+            "actions must have shape [..., heads]");
+}
+
+// The tensors of a call that all checks are done with, alive until it is queued.
 struct ActionRows {
     Tensor logits, mask, actions;
 
@@ -415,11 +425,6 @@ struct ActionRows {
             a.mask_row = mask.stride(0);
         }
         if (!given.defined()) return;
-        const OnDevice onDevice;
-        onDevice(given, "actions");
-        requireType(given.scalar_type() == at::kInt || given.scalar_type() == at::kLong, "actions must have dtype int32 or int64");
-        require(given.dim() == l.dim() && given.size(-1) == a.heads && given.sizes().slice(0, l.dim() - 1) == l.sizes().slice(0, l.dim() - 1),
-                "actions must have shape [..., heads]");
         actions = asRows(given);
         a.actions = actions.data_ptr();
         a.actions_row = actions.stride(0);
@@ -432,6 +437,7 @@ std::tuple<Tensor, Tensor> actionLogProbForward(const Tensor& logits, const Tens
 {
     std::vector<int32_t> sizes;
     carl_actions a = actionsOf(logits, heads, mask, sizes);
+    actionsFit(actions, logits, a.heads);
     const ActionRows rows(a, logits, mask, actions);
     const auto lead = logits.sizes().slice(0, logits.dim() - 1);
     Tensor logProb = at::empty(lead, logits.options().dtype(at::kFloat)), entropy = at::empty(lead, logits.options().dtype(at::kFloat));
@@ -536,6 +542,7 @@ carl_norm normOf(const Tensor& x, const Tensor* weight, const Tensor* residual, 
     n.width = (int32_t)width;
     n.eps = (float)eps;
     if (weight) {
+        require(n.eps >= CARL_NORM_MIN_EPS && std::isfinite(n.eps), "eps must be finite and at least 1e-30");
         onDevice(*weight, "weight");
         requireType(weight->scalar_type() == x.scalar_type(), "x and weight must have the same dtype");
         require(weight->dim() == 1 && weight->size(0) == width, "weight must have shape [width]");
@@ -703,12 +710,19 @@ Tensor int8Product(const Tensor& x, const Tensor& xScale, const Tensor& w, const
     if (up) weightsOf(*up, *upScale, width, columns, "w_up", "up_scale");
     require(width >= 1 && width <= CARL_INT8_MAX_DIM, "width must be in [1, 65536]");
     require(columns >= 1 && columns <= CARL_INT8_MAX_DIM, "columns must be in [1, 65536]");
+    const int64_t count = x.numel() / width;
+    require(count <= CARL_INT8_MAX_ROWS && (count + 127) / 128 * ((columns + 127) / 128) <= CARL_INT8_MAX_TILES, "rows are out of range");
+    if (bias) {
+        onDevice(*bias, "bias");
+        requireType(bias->scalar_type() == dtype, "bias must have the result's dtype");
+        require(bias->dim() == 1 && bias->size(0) == columns, "bias must have shape [columns]");
+    }
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = columns;
     carl_int8_linear p{};
     const Tensor rows = asRows(x), scale = xScale.contiguous(), weight = asRows(w), weightScale = wScale.contiguous();
     Tensor upRows, upScales, biases;
-    p.rows = x.numel() / width;
+    p.rows = count;
     p.width = (int32_t)width;
     p.columns = (int32_t)columns;
     p.activation = (int32_t)activation;
@@ -726,9 +740,6 @@ Tensor int8Product(const Tensor& x, const Tensor& xScale, const Tensor& w, const
         p.w_up_scale = upScales.data_ptr<float>();
     }
     if (bias) {
-        onDevice(*bias, "bias");
-        requireType(bias->scalar_type() == dtype, "bias must have the result's dtype");
-        require(bias->dim() == 1 && bias->size(0) == columns, "bias must have shape [columns]");
         biases = bias->contiguous();
         p.bias = biases.data_ptr();
     }

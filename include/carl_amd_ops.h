@@ -268,7 +268,7 @@ int carl_quantize_int8(const carl_norm* n, void* stream);               /* of x:
  * in float32, rounded to y's type once.  All int8 values are allowed, -128
  * among them. */
 typedef struct carl_int8_linear {
-    int64_t rows;               /* at most 2^28; times columns, in tiles of 128 x 128, at most 2^36 */
+    int64_t rows;               /* at most CARL_INT8_MAX_ROWS; by columns at most CARL_INT8_MAX_TILES tiles of 128 x 128 */
     int32_t width, columns;     /* 1 to CARL_INT8_MAX_DIM */
     int32_t type;               /* of y and the bias */
     int32_t activation;         /* of the gated form: CARL_SILU or CARL_GELU */
@@ -285,7 +285,7 @@ typedef struct carl_int8_linear {
     void* y;                    /* [rows, columns] */
 } carl_int8_linear;
 
-enum { CARL_INT8_MAX_DIM = 65536 };
+enum { CARL_INT8_MAX_DIM = 65536, CARL_INT8_MAX_ROWS = 1 << 28, CARL_INT8_MAX_TILES = 1 << 22 };
 
 int carl_int8_linear_forward(const carl_int8_linear* p, void* stream);
 
