@@ -80,6 +80,17 @@ public:
     }
 };
 
+// The same of all tensors of a call (null for none) whose types and shapes were
+// looked at before: those checks need no GPU.
+void allOnDevice(std::initializer_list<std::pair<const Tensor*, const char*>> tensors)
+{
+    const OnDevice onDevice;
+    for (const auto& [t, name] : tensors)
+        if (t) onDevice(*t, name);
+}
+
+const Tensor* given(const OptTensor& t) { return t ? &*t : nullptr; }
+
 int elementType(const Tensor& t, const char* name)
 {
     switch (t.scalar_type()) {
@@ -374,11 +385,10 @@ Tensor gatedFfn(const Tensor& x, const Tensor& gate, const Tensor& up, const Ten
 
 // ----------------------------------------------------------------- actions
 
-// The checks of logits, heads and mask; the sizes of the call.
-carl_actions actionsOf(const Tensor& logits, const std::vector<int64_t>& heads, const OptTensor& mask, std::vector<int32_t>& sizes)
+// The checks of types and shapes of logits, heads, mask, actions and noise; the sizes of the call.
+carl_actions actionsOf(const Tensor& logits, const std::vector<int64_t>& heads, const Tensor* mask, const Tensor* actions, const Tensor* noise,
+                       std::vector<int32_t>& sizes)
 {
-    const OnDevice onDevice;
-    onDevice(logits, "logits");
     carl_actions a{};
     a.type = elementType(logits, "logits");
     require(!heads.empty() && heads.size() <= CARL_ACTIONS_MAX_HEADS, "heads must have 1 to 64 sizes");
@@ -394,28 +404,28 @@ carl_actions actionsOf(const Tensor& logits, const std::vector<int64_t>& heads, 
     a.heads = (int32_t)heads.size();
     a.sizes = sizes.data();
     if (mask) {
-        onDevice(*mask, "mask");
         requireType(mask->scalar_type() == at::kBool, "mask must have dtype bool");
         require(mask->sizes() == logits.sizes(), "mask must have the logits' shape");
     }
+    if (actions) {
+        requireType(actions->scalar_type() == at::kInt || actions->scalar_type() == at::kLong, "actions must have dtype int32 or int64");
+        require(actions->dim() == logits.dim() && actions->size(-1) == a.heads
+                    && actions->sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+                "actions must have shape [..., heads]");
+    }
+    if (noise) {
+        requireType(noise->scalar_type() == at::kFloat, "noise must have dtype float32");
+        require(noise->sizes() == logits.sizes(), "noise must have the logits' shape");
+    }
+    allOnDevice({ { &logits, "logits" }, { mask, "mask" }, { actions, "actions" }, { noise, "noise" } });
     return a;
-}
-
-void actionsFit(const Tensor& actions, const Tensor& logits, int32_t heads)
-{
-    const OnDevice onDevice;
-    onDevice(actions, "actions");
-    requireType(actions.scalar_type() == at::kInt || actions.scalar_type() == at::kLong, "actions must have dtype int32 or int64");
-    require(actions.dim() == logits.dim() && actions.size(-1) == heads
-                && actions.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
-            "actions must have shape [..., heads]");
 }
 
 // The tensors of a call that all checks are done with, alive until it is queued.
 struct ActionRows {
-    Tensor logits, mask, actions;
+    Tensor logits, mask, actions, noise;
 
-    ActionRows(carl_actions& a, const Tensor& l, const OptTensor& m, const Tensor& given) : logits(asRows(l))
+    ActionRows(carl_actions& a, const Tensor& l, const Tensor* m, const Tensor* chosen, const Tensor* n) : logits(asRows(l))
     {
         a.logits = logits.data_ptr();
         a.logits_row = logits.stride(0);
@@ -424,11 +434,17 @@ struct ActionRows {
             a.mask = static_cast<const uint8_t*>(mask.data_ptr());
             a.mask_row = mask.stride(0);
         }
-        if (!given.defined()) return;
-        actions = asRows(given);
-        a.actions = actions.data_ptr();
-        a.actions_row = actions.stride(0);
-        a.actions_wide = given.scalar_type() == at::kLong;
+        if (chosen) {
+            actions = asRows(*chosen);
+            a.actions = actions.data_ptr();
+            a.actions_row = actions.stride(0);
+            a.actions_wide = actions.scalar_type() == at::kLong;
+        }
+        if (n) {
+            noise = asRows(*n);
+            a.noise = noise.data_ptr<float>();
+            a.noise_row = noise.stride(0);
+        }
     }
 };
 
@@ -436,9 +452,8 @@ std::tuple<Tensor, Tensor> actionLogProbForward(const Tensor& logits, const Tens
                                                 const OptTensor& mask)
 {
     std::vector<int32_t> sizes;
-    carl_actions a = actionsOf(logits, heads, mask, sizes);
-    actionsFit(actions, logits, a.heads);
-    const ActionRows rows(a, logits, mask, actions);
+    carl_actions a = actionsOf(logits, heads, given(mask), &actions, nullptr, sizes);
+    const ActionRows rows(a, logits, given(mask), &actions, nullptr);
     const auto lead = logits.sizes().slice(0, logits.dim() - 1);
     Tensor logProb = at::empty(lead, logits.options().dtype(at::kFloat)), entropy = at::empty(lead, logits.options().dtype(at::kFloat));
     a.log_prob = logProb.data_ptr<float>();
@@ -463,11 +478,10 @@ struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
         if (at::GradMode::is_enabled()) throw std::runtime_error("action_log_prob has no second derivative");
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined() && !grads[1].defined()) return { {}, {}, {}, {} };
-        const OptTensor mask = saved[2].defined() ? OptTensor(saved[2]) : std::nullopt;
-        const Tensor logits = saved[0].detach();
+        const Tensor logits = saved[0].detach(), *mask = saved[2].defined() ? &saved[2] : nullptr;
         std::vector<int32_t> sizes;
-        carl_actions a = actionsOf(logits, ctx->saved_data["heads"].toIntVector(), mask, sizes);
-        const ActionRows rows(a, logits, mask, saved[1]);
+        carl_actions a = actionsOf(logits, ctx->saved_data["heads"].toIntVector(), mask, &saved[1], nullptr, sizes);
+        const ActionRows rows(a, logits, mask, &saved[1], nullptr);
         // one value for all rows (the gradient of a mean, say) is read as it is
         Tensor held[2];
         const auto column = [&](int i, const float*& at, int64_t& step) {
@@ -504,18 +518,8 @@ std::tuple<Tensor, Tensor> topActions(const Tensor& logits, const std::vector<in
     requireNoGradient({ &logits, noise ? &*noise : &logits }, "top_actions");
     require(k >= 1 && k <= CARL_ACTIONS_MAX_K, "k must be in [1, 64]");
     std::vector<int32_t> sizes;
-    carl_actions a = actionsOf(logits, heads, mask, sizes);
-    Tensor noiseRows;
-    if (noise) {
-        const OnDevice onDevice;
-        onDevice(*noise, "noise");
-        requireType(noise->scalar_type() == at::kFloat, "noise must have dtype float32");
-        require(noise->sizes() == logits.sizes(), "noise must have the logits' shape");
-        noiseRows = asRows(*noise);
-        a.noise = noiseRows.data_ptr<float>();
-        a.noise_row = noiseRows.stride(0);
-    }
-    const ActionRows rows(a, logits, mask, Tensor());
+    carl_actions a = actionsOf(logits, heads, given(mask), nullptr, given(noise), sizes);
+    const ActionRows rows(a, logits, given(mask), nullptr, given(noise));
     std::vector<int64_t> shape = logits.sizes().slice(0, logits.dim() - 1).vec();
     shape.push_back(a.heads);
     shape.push_back(k);
@@ -531,8 +535,6 @@ std::tuple<Tensor, Tensor> topActions(const Tensor& logits, const std::vector<in
 
 carl_norm normOf(const Tensor& x, const Tensor* weight, const Tensor* residual, double eps)
 {
-    const OnDevice onDevice;
-    onDevice(x, "x");
     carl_norm n{};
     n.type = elementType(x, "x");
     require(x.dim() >= 1, "x must have shape [..., width]");
@@ -543,15 +545,14 @@ carl_norm normOf(const Tensor& x, const Tensor* weight, const Tensor* residual, 
     n.eps = (float)eps;
     if (weight) {
         require(n.eps >= CARL_NORM_MIN_EPS && std::isfinite(n.eps), "eps must be finite and at least 1e-30");
-        onDevice(*weight, "weight");
         requireType(weight->scalar_type() == x.scalar_type(), "x and weight must have the same dtype");
         require(weight->dim() == 1 && weight->size(0) == width, "weight must have shape [width]");
     }
     if (residual) {
-        onDevice(*residual, "residual");
         requireType(residual->scalar_type() == x.scalar_type(), "x and residual must have the same dtype");
         require(residual->sizes() == x.sizes(), "residual must have x's shape");
     }
+    allOnDevice({ { &x, "x" }, { weight, "weight" }, { residual, "residual" } });
     return n;
 }
 
@@ -578,7 +579,7 @@ struct NormRows {
 
 std::tuple<Tensor, Tensor> rmsNormForward(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps)
 {
-    const Tensor* r = residual ? &*residual : nullptr;
+    const Tensor* r = given(residual);
     carl_norm n = normOf(x, &weight, r, eps);
     const NormRows rows(n, x, &weight, r);
     Tensor y = at::empty(x.sizes(), x.options());
@@ -658,7 +659,7 @@ Tensor codesLike(const Tensor& x)
 
 py::tuple normCodes(const Tensor& x, const Tensor* weight, const OptTensor& residual, double eps)
 {
-    const Tensor* r = residual ? &*residual : nullptr;
+    const Tensor* r = given(residual);
     carl_norm n = normOf(x, weight, r, eps);
     const NormRows rows(n, x, weight, r);
     const Tensor codes = codesLike(x), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
@@ -685,11 +686,8 @@ py::tuple quantizeInt8(const Tensor& x)
 
 void weightsOf(const Tensor& w, const Tensor& scale, int64_t width, int64_t columns, const char* name, const char* scaleName)
 {
-    const OnDevice onDevice;
-    onDevice(w, name);
     requireType(w.scalar_type() == at::kChar, name, " must have dtype int8");
     require(w.dim() == 2 && w.size(0) == columns && w.size(1) == width, name, " must have shape [columns, width]");
-    onDevice(scale, scaleName);
     requireType(scale.scalar_type() == at::kFloat, scaleName, " must have dtype float32");
     require(scale.dim() == 1 && scale.size(0) == columns, scaleName, " must have shape [columns]");
 }
@@ -697,26 +695,25 @@ void weightsOf(const Tensor& w, const Tensor& scale, int64_t width, int64_t colu
 Tensor int8Product(const Tensor& x, const Tensor& xScale, const Tensor& w, const Tensor& wScale, const Tensor* up, const Tensor* upScale,
                    const OptTensor& bias, int64_t activation, at::ScalarType dtype)
 {
-    const OnDevice onDevice;
-    onDevice(x, "x");
+    const char *name = up ? "w_gate" : "weight", *scaleName = up ? "gate_scale" : "weight_scale";
     requireType(x.scalar_type() == at::kChar, "x must have dtype int8");
     require(x.dim() >= 1, "x must have shape [..., width]");
-    onDevice(xScale, "x_scale");
     requireType(xScale.scalar_type() == at::kFloat, "x_scale must have dtype float32");
     require(xScale.sizes() == x.sizes().slice(0, x.dim() - 1), "x_scale must have a value for each row of x");
-    require(w.defined() && w.dim() == 2, up ? "w_gate" : "weight", " must have shape [columns, width]");
+    require(w.dim() == 2, name, " must have shape [columns, width]");
     const int64_t width = x.size(-1), columns = w.size(0);
-    weightsOf(w, wScale, width, columns, up ? "w_gate" : "weight", up ? "gate_scale" : "weight_scale");
+    weightsOf(w, wScale, width, columns, name, scaleName);
     if (up) weightsOf(*up, *upScale, width, columns, "w_up", "up_scale");
     require(width >= 1 && width <= CARL_INT8_MAX_DIM, "width must be in [1, 65536]");
     require(columns >= 1 && columns <= CARL_INT8_MAX_DIM, "columns must be in [1, 65536]");
     const int64_t count = x.numel() / width;
     require(count <= CARL_INT8_MAX_ROWS && (count + 127) / 128 * ((columns + 127) / 128) <= CARL_INT8_MAX_TILES, "rows are out of range");
     if (bias) {
-        onDevice(*bias, "bias");
         requireType(bias->scalar_type() == dtype, "bias must have the result's dtype");
         require(bias->dim() == 1 && bias->size(0) == columns, "bias must have shape [columns]");
     }
+    allOnDevice({ { &x, "x" }, { &xScale, "x_scale" }, { &w, name }, { &wScale, scaleName }, { up, "w_up" }, { upScale, "up_scale" },
+                  { given(bias), "bias" } });
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = columns;
     carl_int8_linear p{};

@@ -1,10 +1,13 @@
-"""Refused calls of the operators around a policy's layers, on tensors of the GPU: nothing is queued for them."""
+"""Refused calls of the operators around a policy's layers, on tensors of the GPU: every check of types and shapes, and
+that nothing is queued for them."""
 from __future__ import annotations
 
 import math
 
 import pytest
 import torch
+
+import policy_refusals as refusals
 
 pytestmark = pytest.mark.gpu
 
@@ -24,6 +27,48 @@ def _refused(call, error, message):
     with pytest.raises(error, match=message):
         call()
     assert allocations() == before
+
+
+@pytest.mark.parametrize("group", refusals.GROUPS)
+def test_types_and_shapes(group):
+    calls = refusals.calls("cuda")
+    for name, changes, error, message in refusals.GROUPS[group]:
+        a = refusals.made(changes, "cuda")
+        with pytest.raises(error, match=message):
+            calls[name](**a)
+
+
+def test_calls_that_fit_are_taken():
+    for call in refusals.calls("cuda").values():
+        call()
+
+
+@pytest.mark.parametrize("name,tensors", [("action_log_prob", ("logits", "mask", "actions")), ("top_actions", ("logits", "mask", "noise")),
+                                          ("rms_norm", ("x", "weight", "residual")), ("rms_norm_int8", ("x", "weight", "residual")),
+                                          ("quantize_int8", ("x",)), ("int8_linear", ("x", "x_scale", "weight", "weight_scale", "bias")),
+                                          ("int8_gated_linear", ("x", "x_scale", "w_gate", "gate_scale", "w_up", "up_scale"))])
+def test_each_tensor_has_to_be_on_the_gpu(name, tensors):
+    shapes = {"logits": (4, 6, 8), "mask": (4, 6, 8), "noise": (4, 6, 8), "actions": (4, 6, 2), "residual": (4, 6, 16), "x_scale": (4, 6),
+              "bias": (12,)}
+    for tensor in tensors:
+        codes = "linear" in name and tensor in ("x", "weight", "w_gate", "w_up")
+        shape = (4, 6, 32) if codes and tensor == "x" else (12, 32) if codes else (4, 6, 16) if tensor == "x" \
+            else (16,) if tensor == "weight" else shapes.get(tensor, (12,))
+        dtype = torch.int8 if codes else {"mask": torch.bool, "actions": torch.int32, "bias": torch.bfloat16}.get(
+            tensor, torch.bfloat16 if "norm" in name else torch.float32)
+        with pytest.raises(ValueError, match=f"{tensor} must be on cuda:0"):
+            refusals.calls("cuda")[name](**{tensor: torch.zeros(*shape, dtype=dtype)})
+
+
+def test_second_derivatives_are_refused():
+    ops = _ops()
+    logits = torch.randn(4, 8, device="cuda", requires_grad=True)
+    actions = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    x, weight = torch.randn(4, 16, device="cuda", requires_grad=True), torch.ones(16, device="cuda", requires_grad=True)
+    for name, out, leaf in (("action_log_prob", ops.action_log_prob(logits, actions, (5, 3))[0], logits), ("rms_norm", ops.rms_norm(x, weight), x),
+                            ("rms_norm", ops.rms_norm(x, weight, residual=x)[0], weight)):
+        with pytest.raises(RuntimeError, match=f"{name} has no second derivative"):
+            torch.autograd.grad(out.sum(), [leaf], create_graph=True)
 
 
 def _turned(*shape, dtype=torch.float32):
