@@ -82,6 +82,15 @@ def test_large_tiles(D, dtype):
         ref.assert_within(y, *policy.gated(x, x_scale, w, w_scale, up, up_scale, "silu", dtype), "silu")
 
 
+@pytest.mark.parametrize("padded", [True, False])
+@pytest.mark.parametrize("F", [1, 7, 18, 40, 100])
+def test_many_rows_and_few_columns(F, padded):
+    """Fewer columns than a tile of any size has, of rows that fill the GPU with the largest ones once and twice, or whose
+    number makes them smaller: a policy's projections to its action heads and to a value."""
+    for N, dtype in ((65_000, torch.bfloat16), (130_001, torch.float32), (80_003, torch.float16)):
+        _check(*_inputs(N, 72, F, dtype, seed=F, padded=padded), gated=F in (1, 18))
+
+
 @pytest.mark.parametrize("N,D,F,gated", [(1000, 60, 1000, True), (3000, 150, 700, True), (2000, 300, 1500, False), (700, 129, 500, False),
                                          (130, 40, 2100, True), (130, 40, 2100, False)])
 def test_other_tiles(N, D, F, gated):
