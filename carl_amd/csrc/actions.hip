@@ -18,7 +18,10 @@
 //           share their heads.
 //   shared  8 to 64 lanes, or a workgroup, take a head together, straight from
 //           memory, eight logits a lane in registers; of longer heads the rest is
-//           read again for each step.
+//           read again for each step.  A lane's loads are of one logit and one
+//           byte of the mask, and bound it: 20 M bf16 logits with a mask in heads
+//           of 33 to 2,000 36 to 41 us, 1.6 to 1.7 TB/s (62,000 rows of 90 in f32
+//           2.4 TB/s, their gradients 3.4).
 #include <cmath>
 
 #include "../../include/carl_amd_ops.h"

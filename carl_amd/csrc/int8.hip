@@ -537,7 +537,9 @@ bool inWords(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 // 1,730 against 940).  They are bound by their copies into LDS (which alone
 // take 0.6 of the time, in stages of 64 bytes a row 0.75) beside the matrix
 // instructions (0.75); the gated form then by the operations on its results:
-// 107 of 250 us of 131,072 x 512 to 1,408, which no other tile's products hide.
+// some 113 of 261 us of 131,072 x 512 to 1,408, which no other tile's products hide.
+// Few columns pay for whole tiles: 131,072 x 512 to 1, 18 and 64 columns 27, 27 and
+// 28 us, 2.5 TB/s of x.
 template <typename T, bool kGated> void launchAll(const Args& a, hipStream_t stream)
 {
     const auto tiles = [&](int rows, int columns) { return (a.rows + rows - 1) / rows * ((a.columns + columns - 1) / columns); };
